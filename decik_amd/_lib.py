@@ -51,6 +51,19 @@ class LoraBranch(ctypes.Structure):
                 ("ldx", c_i64), ("lddy", c_i64), ("n", c_i64), ("scale", c_f32), ("x_fp32", c_i32)]
 
 
+class QkRope(ctypes.Structure):
+    """dk_qk_rope: a norm / rotation call (dk_qk_rope_fwd, dk_qk_rope_bwd)."""
+
+    _fields_ = [("q", c_vp), ("k", c_vp), ("grad_q", c_vp), ("grad_k", c_vp), ("q_out", c_vp), ("k_out", c_vp),
+                ("q_weight", c_vp), ("k_weight", c_vp), ("dw_q", c_vp), ("dw_k", c_vp), ("cos", c_vp), ("sin", c_vp),
+                ("positions", c_vp), ("inv_freq", c_vp), ("ld_q", c_i64), ("ld_k", c_i64), ("ld_q_out", c_i64),
+                ("ld_k_out", c_i64), ("table_batch_stride", c_i64), ("pos_axis_stride", c_i64),
+                ("pos_batch_stride", c_i64), ("batch", c_i64), ("tokens", c_i64), ("n_heads", c_i32),
+                ("n_kv_heads", c_i32), ("head_dim", c_i32), ("dtype", c_i32), ("w_dtype", c_i32), ("n_axes", c_i32),
+                ("sections", c_i32 * 4), ("interleaved", c_i32), ("positions_int64", c_i32), ("eps", c_f32),
+                ("reserved", c_i32)]
+
+
 EXPORTS = {
     "dk_nf4_dequant": ([ctypes.POINTER(NF4Weight), c_vp, c_vp], c_i32),
     "dk_nf4_dequant_batched": ([ctypes.POINTER(NF4Weight), ctypes.POINTER(c_vp), c_i32, c_vp], c_i32),
@@ -90,6 +103,13 @@ EXPORTS = {
                         c_i32, c_vp], c_i32),
     "dk_rope_qk_bwd": ([c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp],
                        c_i32),
+    "dk_dropout_fwd": ([c_vp, c_i32, c_i64, c_vp, ctypes.POINTER(ctypes.c_double), c_i32, ctypes.POINTER(c_vp), c_i32,
+                        ctypes.POINTER(c_i64), c_i64, c_i64, c_vp], c_i32),
+    "dk_dropout_bwd": ([ctypes.POINTER(c_vp), c_i32, ctypes.POINTER(c_i64), c_vp, ctypes.POINTER(ctypes.c_double),
+                        c_i32, c_vp, c_i32, c_i64, c_i64, c_i64, c_vp], c_i32),
+    "dk_qk_rope_fwd": ([ctypes.POINTER(QkRope), c_vp], c_i32),
+    "dk_qk_rope_bwd_workspace": ([ctypes.POINTER(QkRope)], c_i64),
+    "dk_qk_rope_bwd": ([ctypes.POINTER(QkRope), c_vp, c_i64, c_vp], c_i32),
     "dk_swiglu_fwd": ([c_vp, c_vp, c_vp, c_i64, c_vp], c_i32),
     "dk_swiglu_bwd": ([c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp], c_i32),
     "dk_last_error": ([], ctypes.c_char_p),
@@ -135,6 +155,37 @@ def raw_stream(device):
 
 def stream_of(device):
     return ctypes.c_void_p(raw_stream(device))
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device):
+    """Context of a launch on `device`: the current device where it is that one already."""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def gpu_tensors(what, device, **tensors):
+    """Each given tensor (None: absent) must be a GPU tensor on `device`."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what}: {name} must be a tensor")
+        if not t.is_cuda or t.device != device:
+            raise ValueError(f"{what}: {name} must be on the GPU of the input ({device}), not on {t.device}")
+
+
+# element types of the entries that take more than fp16 (include/decik_nf4.h)
+DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
 def ptr(t):

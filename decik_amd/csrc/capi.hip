@@ -637,6 +637,17 @@ hipError_t allow_dynamic_lds(const void* fn, size_t bytes) {
     return e;
 }
 
+int dk_fail(const char* msg) {
+    try {
+        g_error = msg;
+    } catch (...) {
+        g_error.clear();  // no memory for the message
+    }
+    return 1;
+}
+
+void dk_clear_error() { g_error.clear(); }
+
 }  // namespace dk
 
 using namespace dk;

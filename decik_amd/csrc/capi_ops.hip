@@ -1,0 +1,218 @@
+// C ABI (include/decik_nf4.h) of the operators around the frozen projections: seeded dropout, norms
+// and rotation of q and k. Argument checks and launches.
+#include <cmath>
+#include <cstdio>
+
+#include "dk_internal.h"
+
+using namespace dk;
+
+namespace {
+
+int check_launch(hipError_t e, const char* what) {
+    if (e == hipSuccess) return 0;
+    char msg[256];
+    snprintf(msg, sizeof(msg), "%s: %s", what, hipGetErrorString(e));
+    return dk_fail(msg);
+}
+
+bool is_dtype(int d) { return d == DK_FP16 || d == DK_BF16 || d == DK_FP32; }
+
+bool aligned_to(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// everything of a dropout call but its tensors
+int dropout_common(DropoutArgs* a, int in_dtype, int out_dtype, const int64_t* rng, const double* p, int nb,
+                   int64_t rows, int64_t width) {
+    if (nb < 1 || nb > kDropoutMaxBranches) return dk_fail("dk_dropout: 1 to 4 branches");
+    if (!is_dtype(in_dtype) || !is_dtype(out_dtype) ||
+        (in_dtype != out_dtype && in_dtype != DK_FP32 && out_dtype != DK_FP32))
+        return dk_fail("dk_dropout: types must be equal, or one of them fp32");
+    if (rows < 0 || width < 0) return dk_fail("dk_dropout: negative size");
+    if (p == nullptr) return dk_fail("dk_dropout: null pointer");
+    for (int b = 0; b < nb; ++b) {
+        if (!(p[b] >= 0.0 && p[b] <= 1.0)) return dk_fail("dk_dropout: p must be in [0, 1]");
+        a->thr[b] = (uint32_t)std::nearbyint(p[b] * 65536.0);
+        a->scale[b] = a->thr[b] < 65536u ? (float)(65536.0 / (65536.0 - a->thr[b])) : 0.0f;
+    }
+    // columns are 32-bit numbers in the kernel
+    const int64_t limit = int64_t(1) << 31;
+    if (width > 0xFFFFFFF0ll) return dk_fail("dk_dropout: width must be below 2^32 - 16");
+    const int64_t groups = (width + 7) / 8;
+    if (groups > 0 && rows > (limit - 1) / groups)
+        return dk_fail("dk_dropout: rows * ceil(width / 8) must be below 2^31");
+    if (rows * groups > 0 && (rng == nullptr || !aligned_to(rng, 8)))
+        return dk_fail("dk_dropout: rng must be two int64 in device memory");
+    a->rng = rng;
+    a->width = (uint32_t)width;
+    a->groups = (uint32_t)groups;
+    a->items = (uint32_t)(rows * groups);
+    a->nb = nb;
+    return 0;
+}
+
+// everything of a norm / rotation call but the gradients
+int qk_rope_common(const dk_qk_rope* d, QkRopeArgs* a) {
+    if (d == nullptr) return dk_fail("dk_qk_rope: null descriptor");
+    if (d->dtype != DK_FP16 && d->dtype != DK_BF16) return dk_fail("dk_qk_rope: q and k must be fp16 or bf16");
+    if (d->head_dim < 16 || d->head_dim > 512 || d->head_dim % 16 != 0)
+        return dk_fail("dk_qk_rope: head_dim must be a multiple of 16 from 16 to 512");
+    if (d->n_heads < 1 || d->n_kv_heads < 1 || d->n_heads > 65536 || d->n_kv_heads > 65536)
+        return dk_fail("dk_qk_rope: 1 to 65536 heads each");
+    if (d->batch < 0 || d->tokens < 0 || d->tokens >= INT32_MAX || d->batch >= INT32_MAX ||
+        d->batch * d->tokens > (int64_t)INT32_MAX - kQkMaxWaves)
+        return dk_fail("dk_qk_rope: batch * tokens must be non-negative and below 2^31 - 4096");
+    if ((d->q_weight == nullptr) != (d->k_weight == nullptr))
+        return dk_fail("dk_qk_rope: norm weights for both q and k, or for neither");
+    if (d->q_weight != nullptr && !is_dtype(d->w_dtype)) return dk_fail("dk_qk_rope: unknown norm weight type");
+    const bool axes = d->n_axes != 0, empty = d->batch * d->tokens == 0;
+    if (!axes && !empty && (d->cos == nullptr || d->sin == nullptr || !aligned_to(d->cos, 4) || !aligned_to(d->sin, 4)))
+        return dk_fail("dk_qk_rope: without axes cos and sin must be set");
+    if (axes) {
+        if (d->n_axes < 1 || d->n_axes > 4) return dk_fail("dk_qk_rope: 1 to 4 axes");
+        if (!empty && (d->positions == nullptr || d->inv_freq == nullptr))
+            return dk_fail("dk_qk_rope: axes need positions and inv_freq");
+        int sum = 0;
+        for (int i = 0; i < d->n_axes; ++i) {
+            if (d->sections[i] < 0 || d->sections[i] > d->head_dim)
+                return dk_fail("dk_qk_rope: sections must be non-negative and add up to head_dim / 2");
+            sum += d->sections[i];
+        }
+        if (sum != d->head_dim / 2)
+            return dk_fail("dk_qk_rope: sections must be non-negative and add up to head_dim / 2");
+        if (d->interleaved)
+            for (int i = 1; i < d->n_axes; ++i)
+                if (d->sections[i] > 0 && d->n_axes * (d->sections[i] - 1) + i >= sum)
+                    return dk_fail("dk_qk_rope: an interleaved axis has more frequencies than its places");
+    }
+    a->q = d->q;
+    a->k = d->k;
+    a->gq = d->grad_q;
+    a->gk = d->grad_k;
+    a->oq = d->q_out;
+    a->ok = d->k_out;
+    a->ldq = d->ld_q;
+    a->ldk = d->ld_k;
+    a->ldoq = d->ld_q_out;
+    a->ldok = d->ld_k_out;
+    a->qw = d->q_weight;
+    a->kw = d->k_weight;
+    a->cos = d->cos;
+    a->sin = d->sin;
+    a->table_batch = d->table_batch_stride;
+    a->pos = d->positions;
+    a->inv_freq = d->inv_freq;
+    a->pos_axis = d->pos_axis_stride;
+    a->pos_batch = d->pos_batch_stride;
+    for (int i = 0; i < 4; ++i) a->section[i] = i < d->n_axes ? d->sections[i] : 0;
+    a->n_axes = d->n_axes;
+    a->interleaved = d->interleaved;
+    a->pos64 = d->positions_int64;
+    a->w_dtype = d->w_dtype;
+    a->tokens = (uint32_t)d->tokens;
+    a->rows = (uint32_t)(d->batch * d->tokens);
+    a->hq = d->n_heads;
+    a->hk = d->n_kv_heads;
+    a->d = d->head_dim;
+    a->eps = d->eps;
+    a->inv_d = 1.0f / (float)d->head_dim;
+    return 0;
+}
+
+bool rows_fit(int64_t ld, int heads, int d) { return ld >= (int64_t)heads * d; }
+
+}  // namespace
+
+extern "C" {
+
+int dk_dropout_fwd(const void* x, int x_dtype, int64_t ldx, const int64_t* rng, const double* p, int nbranches,
+                   void* const* outs, int out_dtype, const int64_t* ldo, int64_t rows, int64_t width, void* stream) {
+    dk_clear_error();
+    DropoutArgs a{};
+    if (int rc = dropout_common(&a, x_dtype, out_dtype, rng, p, nbranches, rows, width)) return rc;
+    if (a.items == 0) return 0;
+    if (x == nullptr || outs == nullptr || ldo == nullptr) return dk_fail("dk_dropout_fwd: null pointer");
+    if (rows > 1 && ldx < 0) return dk_fail("dk_dropout_fwd: negative row stride");
+    a.in[0] = x;
+    a.ld_in[0] = ldx;
+    for (int b = 0; b < nbranches; ++b) {
+        if (outs[b] == nullptr) return dk_fail("dk_dropout_fwd: null pointer");
+        if (rows > 1 && ldo[b] < width) return dk_fail("dk_dropout_fwd: output rows overlap");
+        a.out[b] = outs[b];
+        a.ld_out[b] = ldo[b];
+    }
+    return check_launch(launch_dropout(a, x_dtype, out_dtype, false, static_cast<hipStream_t>(stream)),
+                        "dk_dropout_fwd launch");
+}
+
+int dk_dropout_bwd(const void* const* grads, int grad_dtype, const int64_t* ldg, const int64_t* rng, const double* p,
+                   int nbranches, void* dx, int dx_dtype, int64_t lddx, int64_t rows, int64_t width, void* stream) {
+    dk_clear_error();
+    DropoutArgs a{};
+    if (int rc = dropout_common(&a, grad_dtype, dx_dtype, rng, p, nbranches, rows, width)) return rc;
+    if (a.items == 0) return 0;
+    if (grads == nullptr || ldg == nullptr || dx == nullptr) return dk_fail("dk_dropout_bwd: null pointer");
+    if (rows > 1 && lddx < width) return dk_fail("dk_dropout_bwd: output rows overlap");
+    for (int b = 0; b < nbranches; ++b) {
+        if (grads[b] != nullptr && rows > 1 && ldg[b] < 0) return dk_fail("dk_dropout_bwd: negative row stride");
+        a.in[b] = grads[b];
+        a.ld_in[b] = ldg[b];
+    }
+    a.out[0] = dx;
+    a.ld_out[0] = lddx;
+    return check_launch(launch_dropout(a, grad_dtype, dx_dtype, true, static_cast<hipStream_t>(stream)),
+                        "dk_dropout_bwd launch");
+}
+
+int dk_qk_rope_fwd(const dk_qk_rope* d, void* stream) {
+    dk_clear_error();
+    QkRopeArgs a{};
+    if (int rc = qk_rope_common(d, &a)) return rc;
+    if (a.rows == 0) return 0;
+    if (a.q == nullptr || a.k == nullptr || a.oq == nullptr || a.ok == nullptr)
+        return dk_fail("dk_qk_rope_fwd: null pointer");
+    if (a.rows > 1 && (!rows_fit(a.ldq, a.hq, a.d) || !rows_fit(a.ldk, a.hk, a.d)))
+        return dk_fail("dk_qk_rope_fwd: row strides must cover the heads");
+    return check_launch(launch_qk_rope(a, d->dtype, d->q_weight != nullptr, d->n_axes != 0, false, nullptr,
+                                       nullptr, static_cast<hipStream_t>(stream)),
+                        "dk_qk_rope_fwd launch");
+}
+
+int64_t dk_qk_rope_bwd_workspace(const dk_qk_rope* d) {
+    dk_clear_error();
+    QkRopeArgs a{};
+    if (qk_rope_common(d, &a) != 0) return -1;
+    if (d->dw_q == nullptr || d->q_weight == nullptr || a.rows == 0) return 0;
+    return (int64_t)qk_rope_groups(a.rows, qk_rope_passes(a.hq, a.hk, a.d)) * 2 * a.d * (int64_t)sizeof(float);
+}
+
+int dk_qk_rope_bwd(const dk_qk_rope* d, void* workspace, int64_t workspace_bytes, void* stream) {
+    dk_clear_error();
+    QkRopeArgs a{};
+    if (int rc = qk_rope_common(d, &a)) return rc;
+    const bool norm = d->q_weight != nullptr;
+    if ((d->dw_q == nullptr) != (d->dw_k == nullptr))
+        return dk_fail("dk_qk_rope_bwd: dw_q and dw_k both, or neither");
+    if (d->dw_q != nullptr && !norm) return dk_fail("dk_qk_rope_bwd: no norm weights to take a gradient of");
+    if (a.rows != 0) {
+        if (a.gq == nullptr || a.gk == nullptr || a.oq == nullptr || a.ok == nullptr)
+            return dk_fail("dk_qk_rope_bwd: null pointer");
+        if (norm && (a.q == nullptr || a.k == nullptr)) return dk_fail("dk_qk_rope_bwd: norms need q and k again");
+        if (a.rows > 1 && norm && (!rows_fit(a.ldq, a.hq, a.d) || !rows_fit(a.ldk, a.hk, a.d)))
+            return dk_fail("dk_qk_rope_bwd: row strides must cover the heads");
+        if (a.rows > 1 && (!rows_fit(a.ldoq, a.hq, a.d) || !rows_fit(a.ldok, a.hk, a.d)))
+            return dk_fail("dk_qk_rope_bwd: row strides must cover the heads");
+        if (d->dw_q != nullptr) {
+            const int64_t need = dk_qk_rope_bwd_workspace(d);
+            if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
+                return dk_fail("dk_qk_rope_bwd: workspace too small (dk_qk_rope_bwd_workspace)");
+            a.slabs = static_cast<float*>(workspace);
+        }
+    } else if (d->dw_q == nullptr) {
+        return 0;
+    }
+    return check_launch(launch_qk_rope(a, d->dtype, norm, d->n_axes != 0, true, d->dw_q, d->dw_k,
+                                       static_cast<hipStream_t>(stream)),
+                        "dk_qk_rope_bwd launch");
+}
+
+}  // extern "C"

@@ -240,6 +240,52 @@ struct RopeArgs {
 };
 hipError_t launch_rope(const RopeArgs& a, bool backward, hipStream_t s);
 
+// Seeded dropout (dropout.hip): forward in[0] -> out[0 .. nb - 1], backward in[0 .. nb - 1] (null: a
+// branch without a gradient) -> out[0].
+constexpr int kDropoutMaxBranches = DK_MAX_GROUPS;
+struct DropoutArgs {
+    const void* in[kDropoutMaxBranches];
+    void* out[kDropoutMaxBranches];
+    int64_t ld_in[kDropoutMaxBranches], ld_out[kDropoutMaxBranches];  // elements
+    uint32_t thr[kDropoutMaxBranches];  // rint(65536 p)
+    float scale[kDropoutMaxBranches];
+    const int64_t* rng;  // device: seed, offset
+    uint32_t width, groups, items;  // groups of eight columns a row, rows * groups
+    int32_t nb;
+};
+hipError_t launch_dropout(const DropoutArgs& a, int in_dtype, int out_dtype, bool backward, hipStream_t s);
+
+// Norms and rotation of q and k heads (qk_rope.hip).
+constexpr int kQkMaxWaves = 4096;
+struct QkRopeArgs {
+    const void *q, *k;    // token-major rows (forward; backward with norms)
+    const void *gq, *gk;  // backward: gradients, head-major
+    void *oq, *ok;        // forward: head-major; backward: token-major rows
+    int64_t ldq, ldk, ldoq, ldok;
+    const void *qw, *kw;  // norm weights
+    float* slabs;         // backward: sums of the norm weights' gradients a work-group, or null
+    const float *cos, *sin;
+    int64_t table_batch;  // elements between the tables of two batch entries (0: shared)
+    const void* pos;
+    const float* inv_freq;
+    int64_t pos_axis, pos_batch;
+    int32_t section[4];
+    int32_t n_axes, interleaved, pos64, w_dtype;
+    uint32_t tokens, rows;  // tokens a batch entry, batch * tokens
+    int32_t hq, hk, d;
+    float eps, inv_d;
+    int32_t passes, streams;
+};
+// work-groups (slabs) of a launch
+int qk_rope_passes(int hq, int hk, int d);
+int qk_rope_groups(int64_t rows, int passes);
+hipError_t launch_qk_rope(QkRopeArgs a, int dtype, bool norm, bool axes, bool backward, float* dwq, float* dwk,
+                          hipStream_t s);
+
+// The calling thread's error (dk_last_error); dk_fail returns 1.
+int dk_fail(const char* msg);
+void dk_clear_error();
+
 // Let `fn` launch with `bytes` of dynamic LDS on the current device (hipFuncSetAttribute once per
 // device and kernel; thread-safe). Needed above 64 KB.
 hipError_t allow_dynamic_lds(const void* fn, size_t bytes);

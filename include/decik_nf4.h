@@ -46,6 +46,8 @@
  *                                               (solution/attn.py:257)
  *   dk_rope_qk_fwd / dk_rope_qk_bwd           <- skc_rope_fwd_kernel / skc_rope_bwd_kernel and
  *                                               FusedQKRope (solution/attn.py:27-126)
+ *   dk_dropout_*, dk_qk_rope_*                no counterpart: seeded LoRA dropout, q/k norms and
+ *                                               multi-axis rotation
  *   dk_swiglu_fwd / dk_swiglu_bwd             <- example_swiglu_fwd/bwd_kernel
  *                                               (solution/swiglu.py:15-37)
  */
@@ -301,6 +303,61 @@ int dk_rope_qk_fwd(const uint16_t* q_base, const uint16_t* q_lora, int64_t ldq, 
 int dk_rope_qk_bwd(const uint16_t* grad_q, const uint16_t* grad_k, const float* cos, const float* sin, uint16_t* dq,
                    int64_t lddq, uint16_t* dk, int64_t lddk, int64_t n_tok, int n_heads, int n_kv_heads, int head_dim,
                    void* stream);
+
+/* Element types of the entries below. */
+#define DK_FP16 0
+#define DK_BF16 1
+#define DK_FP32 2
+
+/* Seeded dropout: the masks come from a counter-based generator (Philox4x32-10) and are never stored.
+ * rng: device, two int64: seed (the key) and offset. Columns 8 g .. 8 g + 7 of row r in branch b take
+ * the eight 16-bit halves of the generator's four words at counter (g, r, low word, high word of
+ * offset + b), low half first; an element is kept when its number is not below rint(65536 p[b]),
+ * and then multiplied by 65536 / (65536 - rint(65536 p[b])). 0 <= p <= 1 (p: host array).
+ * forward: outs[b] = dropped-out x of branch b, 1 to 4 branches from one read of x.
+ * backward: dx = sum over the branches of grads[b] through the same masks (fp32, in branch order); a
+ * NULL gradient counts as zeros. Dropped elements are +0 whatever they held.
+ * Rows of `width` elements with row strides ld* (elements) at any alignment; types DK_FP16, DK_BF16 or
+ * DK_FP32, the two sides equal or one of them fp32. rows * ceil(width / 8) < 2^31. */
+int dk_dropout_fwd(const void* x, int x_dtype, int64_t ldx, const int64_t* rng, const double* p, int nbranches,
+                   void* const* outs, int out_dtype, const int64_t* ldo, int64_t rows, int64_t width, void* stream);
+int dk_dropout_bwd(const void* const* grads, int grad_dtype, const int64_t* ldg, const int64_t* rng, const double* p,
+                   int nbranches, void* dx, int dx_dtype, int64_t lddx, int64_t rows, int64_t width, void* stream);
+
+/* RMS norms of the query and key heads with the rotation of rotary positions, and rotary positions with
+ * several axes. For a head row x, halves a and b of head_dim / 2: y = x / sqrt(mean(x^2) + eps) * weight
+ * (y = x where both weights are NULL), out_a = y_a cos_a - y_b sin_a, out_b = y_b cos_b + y_a sin_b, in
+ * fp32, rounded once. Forward: q, k token-major in, q_out, k_out head-major [batch, heads, tokens,
+ * head_dim]. Backward: grad_q, grad_k head-major in, dq, dk token-major out (the fields q_out, k_out,
+ * ld_q_out, ld_k_out), and with norms q, k are read again and the weights' gradients go to dw_q, dw_k. */
+typedef struct dk_qk_rope {
+    const void *q, *k;           /* [batch * tokens] rows of heads * head_dim, row strides ld_q, ld_k  */
+    const void *grad_q, *grad_k; /* backward: contiguous [batch, heads, tokens, head_dim]              */
+    void *q_out, *k_out;
+    const void *q_weight, *k_weight; /* [head_dim] of w_dtype; both or neither                         */
+    float *dw_q, *dw_k;          /* backward with norms: fp32 [head_dim] each, or both NULL            */
+    const float *cos, *sin;      /* n_axes = 0: tables fp32 [tokens, head_dim]                         */
+    const void* positions;       /* n_axes > 0: int32 or int64 (positions_int64), token t of axis a at */
+    const float* inv_freq;       /*   a * pos_axis_stride + batch * pos_batch_stride + t; head_dim / 2 */
+                                 /*   finite frequencies in radians a position                         */
+    int64_t ld_q, ld_k, ld_q_out, ld_k_out;
+    int64_t table_batch_stride;  /* elements between the tables of two batch entries; 0: shared        */
+    int64_t pos_axis_stride, pos_batch_stride;
+    int64_t batch, tokens;
+    int32_t n_heads, n_kv_heads, head_dim; /* head_dim: a multiple of 16 up to 512                     */
+    int32_t dtype;               /* DK_FP16 or DK_BF16: q, k, gradients and outputs                    */
+    int32_t w_dtype;
+    int32_t n_axes;              /* 0: cos and sin; 1 to 4: positions                                  */
+    int32_t sections[4];         /* frequencies of each axis, together head_dim / 2                    */
+    int32_t interleaved;         /* 0: consecutive sections. 1: frequency j belongs to axis            */
+    int32_t positions_int64;     /*   j % n_axes while j < n_axes * sections of that axis, else to 0   */
+    float eps;
+    int32_t reserved;
+} dk_qk_rope;
+int dk_qk_rope_fwd(const dk_qk_rope* a, void* stream);
+/* workspace: dk_qk_rope_bwd_workspace(a) bytes of device memory (0: none) where dw_q is set */
+int64_t dk_qk_rope_bwd_workspace(const dk_qk_rope* a);
+int dk_qk_rope_bwd(const dk_qk_rope* a, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* out = fp16(silu(gate) * up), computed in fp32 (n elements). */
 int dk_swiglu_fwd(const uint16_t* gate, const uint16_t* up, uint16_t* out, int64_t n,
