@@ -110,6 +110,10 @@ EXPORTS = {
     "dk_qk_rope_fwd": ([ctypes.POINTER(QkRope), c_vp], c_i32),
     "dk_qk_rope_bwd_workspace": ([ctypes.POINTER(QkRope)], c_i64),
     "dk_qk_rope_bwd": ([ctypes.POINTER(QkRope), c_vp, c_i64, c_vp], c_i32),
+    "dk_int8_quantize": ([c_vp, c_i32, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp], c_i32),
+    "dk_int8_linear_workspace": ([c_i32, c_i64, c_i64, c_i64], c_i64),
+    "dk_int8_linear": ([c_i32, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_i64, c_i64, c_i64,
+                        c_i64, c_vp, c_i64, c_vp], c_i32),
     "dk_swiglu_fwd": ([c_vp, c_vp, c_vp, c_i64, c_vp], c_i32),
     "dk_swiglu_bwd": ([c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp], c_i32),
     "dk_last_error": ([], ctypes.c_char_p),

@@ -1,5 +1,5 @@
-// C ABI (include/decik_nf4.h) of the operators around the frozen projections: seeded dropout, norms
-// and rotation of q and k. Argument checks and launches.
+// C ABI (include/decik_nf4.h) of the operators around the NF4 projections: seeded dropout, norms and
+// rotation of q and k, linears in 8-bit integers. Argument checks and launches.
 #include <cmath>
 #include <cstdio>
 
@@ -118,6 +118,16 @@ int qk_rope_common(const dk_qk_rope* d, QkRopeArgs* a) {
     return 0;
 }
 
+constexpr int64_t kInt8MaxK = 131071, kInt8MaxLd = int64_t(1) << 23, kInt8MaxRows = int64_t(1) << 23;
+
+bool int8_sizes(int64_t m, int64_t n, int64_t k) {
+    return m >= 0 && n >= 0 && k >= 1 && k <= kInt8MaxK && m < kInt8MaxRows && n < kInt8MaxRows;
+}
+
+bool int8_rows_ok(const void* p, int64_t ld, int64_t cols) {
+    return aligned_to(p, 16) && ld % 16 == 0 && ld >= (cols + 15) / 16 * 16 && ld < kInt8MaxLd;
+}
+
 bool rows_fit(int64_t ld, int heads, int d) { return ld >= (int64_t)heads * d; }
 
 }  // namespace
@@ -213,6 +223,69 @@ int dk_qk_rope_bwd(const dk_qk_rope* d, void* workspace, int64_t workspace_bytes
     return check_launch(launch_qk_rope(a, d->dtype, norm, d->n_axes != 0, true, d->dw_q, d->dw_k,
                                        static_cast<hipStream_t>(stream)),
                         "dk_qk_rope_bwd launch");
+}
+
+int dk_int8_quantize(const void* x, int x_dtype, int64_t ldx, const float* col_scale, int8_t* q, int64_t ldq,
+                     float* scale, int64_t rows, int64_t k, void* stream) {
+    dk_clear_error();
+    if (!is_dtype(x_dtype)) return dk_fail("dk_int8_quantize: unknown type");
+    if (rows < 0 || rows >= kInt8MaxRows || k < 1 || k > kInt8MaxK)
+        return dk_fail("dk_int8_quantize: 0 <= rows < 2^23, 1 <= k <= 131071");
+    if (rows == 0) return 0;
+    if (x == nullptr || q == nullptr || scale == nullptr) return dk_fail("dk_int8_quantize: null pointer");
+    if (rows > 1 && ldx < 0) return dk_fail("dk_int8_quantize: negative row stride");
+    if (!int8_rows_ok(q, ldq, k))
+        return dk_fail("dk_int8_quantize: q must be 16-byte aligned, its row stride a multiple of 16 that covers k");
+    Int8QuantArgs a{x, col_scale, q, scale, ldx, ldq, rows, (int32_t)k};
+    return check_launch(launch_int8_quantize(a, x_dtype, static_cast<hipStream_t>(stream)), "dk_int8_quantize launch");
+}
+
+int64_t dk_int8_linear_workspace(int transposed, int64_t m, int64_t n, int64_t k) {
+    dk_clear_error();
+    if (!int8_sizes(m, n, k)) {
+        dk_fail("dk_int8_linear: 0 <= m, n < 2^23, 1 <= k <= 131071");
+        return -1;
+    }
+    return int8_plan(m, n, k, transposed != 0).partial_bytes;
+}
+
+int dk_int8_linear(int transposed, const int8_t* xq, int64_t ldx, const float* xs, const int8_t* wq, int64_t ldw,
+                   const float* ws, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t m,
+                   int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, void* stream) {
+    dk_clear_error();
+    if (!int8_sizes(m, n, k)) return dk_fail("dk_int8_linear: 0 <= m, n < 2^23, 1 <= k <= 131071");
+    if (!is_dtype(y_dtype) || (bias != nullptr && !is_dtype(bias_dtype)))
+        return dk_fail("dk_int8_linear: unknown type");
+    if (transposed && (ws != nullptr || bias != nullptr))
+        return dk_fail("dk_int8_linear: the transposed product has neither channel scales nor bias");
+    if (m == 0 || n == 0) return 0;
+    if (xq == nullptr || xs == nullptr || wq == nullptr || y == nullptr || (!transposed && ws == nullptr))
+        return dk_fail("dk_int8_linear: null pointer");
+    if (!int8_rows_ok(xq, ldx, k) || !int8_rows_ok(wq, ldw, transposed ? n : k))
+        return dk_fail("dk_int8_linear: xq and wq must be 16-byte aligned, their row strides multiples of 16 below "
+                       "2^23 that cover their columns");
+    if (m > 1 && ldy < n) return dk_fail("dk_int8_linear: output rows overlap");
+    const Int8Plan p = int8_plan(m, n, k, transposed != 0);
+    if (p.partial_bytes > 0 &&
+        (workspace == nullptr || workspace_bytes < p.partial_bytes || !aligned_to(workspace, 16)))
+        return dk_fail("dk_int8_linear: workspace too small (dk_int8_linear_workspace)");
+    Int8GemmArgs a{};
+    a.x = xq;
+    a.w = wq;
+    a.xs = xs;
+    a.ws = ws;
+    a.bias = bias;
+    a.y = y;
+    a.partials = static_cast<int32_t*>(workspace);
+    a.ldx = ldx;
+    a.ldw = ldw;
+    a.ldy = ldy;
+    a.m = (int32_t)m;
+    a.n = (int32_t)n;
+    a.k = (int32_t)k;
+    a.bias_dtype = bias_dtype;
+    return check_launch(launch_int8_gemm(a, p, y_dtype, transposed != 0, static_cast<hipStream_t>(stream)),
+                        "dk_int8_linear launch");
 }
 
 }  // extern "C"

@@ -282,6 +282,37 @@ int qk_rope_groups(int64_t rows, int passes);
 hipError_t launch_qk_rope(QkRopeArgs a, int dtype, bool norm, bool axes, bool backward, float* dwq, float* dwk,
                           hipStream_t s);
 
+// Products of 8-bit integers (int8_gemm.hip).
+constexpr int kInt8FewM = 32;  // forward launches of so few tokens stream the weight to registers
+struct Int8GemmArgs {
+    const int8_t* x;   // [m, k], row stride ldx, zeros from k to the next multiple of 16
+    const int8_t* w;   // forward [n, k], transposed [k, n], row stride ldw
+    const float* xs;   // [m]
+    const float* ws;   // forward [n]
+    const void* bias;  // [n] or null
+    void* y;
+    int32_t* partials;  // splits > 1
+    int64_t ldx, ldw, ldy, slab;
+    int32_t m, n, k, bias_dtype, ldp;
+    int32_t m_tiles, n_tiles, splits, steps_per_split;
+};
+struct Int8Plan {
+    bool few;
+    int tm, m_tiles, n_tiles, splits, steps_per_split;
+    int64_t partial_bytes;
+};
+struct Int8QuantArgs {
+    const void* x;
+    const float* col_scale;
+    int8_t* q;
+    float* scale;
+    int64_t ldx, ldq, rows;
+    int32_t k;
+};
+Int8Plan int8_plan(int64_t m, int64_t n, int64_t k, bool tr);
+hipError_t launch_int8_gemm(Int8GemmArgs a, const Int8Plan& p, int out_dtype, bool tr, hipStream_t s);
+hipError_t launch_int8_quantize(const Int8QuantArgs& a, int dtype, hipStream_t s);
+
 // The calling thread's error (dk_last_error); dk_fail returns 1.
 int dk_fail(const char* msg);
 void dk_clear_error();

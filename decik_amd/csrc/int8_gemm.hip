@@ -1,0 +1,536 @@
+// Product of 8-bit integer matrices with a scale per token and per channel, on 32x32x32 integer MFMAs:
+//   forward:   y[m, n]  = (sum_k xq[m, k] wq[n, k]) xs[m] ws[n] + bias[n]
+//   TR:        y[m, n]  = (sum_k xq[m, k] wq[k, n]) xs[m]         (the input gradient: xq holds the
+//              gradient times the channel scales, quantized per token; wq as it is stored)
+// Sums are exact in 32-bit integers (k <= 131071), so neither the order nor the split of k changes a
+// result; the scales are applied in fp32 and rounded once.
+//
+// Work-group: 8 waves, tile of TM tokens by 256 channels, steps of 128 along k. Both operands go
+// straight to LDS (16 bytes a lane) through a ring of stages, STAGES - 1 steps ahead; one wait and one
+// barrier a step. Rows of a stage are 128 bytes, their 16-byte chunks permuted by row so that the
+// operand reads (32 rows at one chunk) spread over the banks. TR stages wq as it lies (rows along k,
+// 256 bytes) and turns it through the transposed LDS read of 8-bit elements: in each 16 lanes, lanes
+// 2 r and 2 r + 1 read the 16 bytes of row r, lane i receives byte i of the 8 rows.
+#include "elem.h"
+#include "gemm_common.h"
+
+namespace dk {
+
+typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef int int16v_t __attribute__((ext_vector_type(16)));
+
+constexpr int kI8Threads = 512;
+constexpr int kI8BN = 256;
+constexpr int kI8BK = 128;
+
+__host__ __device__ constexpr int i8_stage_bytes(int tm) { return (kI8BN + tm) * kI8BK; }
+__host__ __device__ constexpr int i8_stages(int tm) { return tm == 256 ? 2 : 3; }
+
+// chunk permutation of a row: tokens are read 32 consecutive rows at a time
+__device__ __forceinline__ int row_key(int r) { return (r >> 1) & 7; }
+
+__device__ __forceinline__ int4_t lds128(const uint8_t* p) { return *(const int4_t*)p; }
+
+__device__ __forceinline__ uint32_t lds_addr(const uint8_t* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
+}
+
+template <int TM, bool TR>
+struct I8Tile {
+    // waves along channels and tokens
+    static constexpr int WN = TM == 256 ? (TR ? 4 : 2) : TM == 128 ? 4 : 8;
+    static constexpr int WM = 8 / WN;
+    static constexpr int TN = kI8BN / WN / 32, TT = TM / WM / 32;  // 32x32 blocks a wave
+    static constexpr int WLOADS = kI8BN * kI8BK / 8192, XLOADS = TM * kI8BK / 8192;  // a wave and step
+    static constexpr int LOADS = WLOADS + XLOADS;
+};
+
+template <int OUT>
+__device__ __forceinline__ void store4(typename Elem<OUT>::type* p, float4_t v, int left) {
+    typedef typename Elem<OUT>::type E;
+    typedef E vec4 __attribute__((ext_vector_type(4)));
+    typedef vec4 loose4 __attribute__((aligned(sizeof(E))));
+    if (left >= 4) {
+        *(loose4*)p = __builtin_convertvector(v, vec4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < left) p[e] = (E)v[e];
+    }
+}
+
+// OUT: an element type, or -1 for the int32 partial sums of a split
+template <int TM, bool TR, int OUT>
+__global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8GemmArgs a) {
+    typedef I8Tile<TM, TR> T;
+    constexpr int S = i8_stages(TM), STAGE = i8_stage_bytes(TM);
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, g = lane >> 5;
+
+    // consecutive tiles on one XCD (work-groups are dealt to the eight in turn), token tiles fastest
+    // within groups of eight, so that the tiles of an XCD at one time share rows of both operands
+    const int per = a.m_tiles * a.n_tiles, nwg = per * a.splits;
+    const int xcd = blockIdx.x & 7, r8 = nwg & 7;
+    const int L = xcd * (nwg >> 3) + min(xcd, r8) + (blockIdx.x >> 3);
+    const int split = L / per, tile = L - split * per;
+    const int band = tile / (8 * a.n_tiles), in = tile - band * 8 * a.n_tiles;
+    const int rows = min(8, a.m_tiles - 8 * band);
+    const int m0 = (8 * band + in % rows) * TM, n0 = (in / rows) * kI8BN;
+    const int k_begin = split * a.steps_per_split * kI8BK;
+    const int steps = min(a.steps_per_split, (a.k + kI8BK - 1) / kI8BK - split * a.steps_per_split);
+    const int kpad = (a.k + 15) & ~15, npad = (a.n + 15) & ~15;
+
+    const int8_t* const xb = a.x + (int64_t)m0 * a.ldx;
+    const uint32_t x_bytes = (uint32_t)((min(TM, a.m - m0) - 1) * a.ldx + kpad);
+    const int8_t* const wb = TR ? a.w + n0 : a.w + (int64_t)n0 * a.ldw;
+    const uint32_t w_bytes = TR ? (uint32_t)min(kI8BN, npad - n0)
+                                : (uint32_t)((min(kI8BN, a.n - n0) - 1) * a.ldw + kpad);
+
+    // this lane's source offsets, and its column along k, of every load of a step
+    uint32_t woff[T::WLOADS], xoff[T::XLOADS];
+    int wcol[T::WLOADS], xcol[T::XLOADS];
+#pragma unroll
+    for (int i = 0; i < T::WLOADS; ++i) {
+        const int q = wave * T::WLOADS + i;
+        if constexpr (TR) {
+            const int r = 4 * q + (lane >> 4);
+            wcol[i] = 0;
+            woff[i] = r * (uint32_t)a.ldw + 16 * ((lane & 15) ^ ((r & 7) << 1));
+        } else {
+            const int r = 8 * q + (lane >> 3);
+            wcol[i] = 16 * ((lane & 7) ^ row_key(r));
+            woff[i] = r * (uint32_t)a.ldw + wcol[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < T::XLOADS; ++i) {
+        const int r = 8 * (wave * T::XLOADS + i) + (lane >> 3);
+        xcol[i] = 16 * ((lane & 7) ^ row_key(r));
+        xoff[i] = r * (uint32_t)a.ldx + xcol[i];
+    }
+
+    // loads of step t into its stage; past the last step they read nothing (and write zeros nobody reads),
+    // which keeps the number of loads in flight the same for every wait
+    const auto fetch = [&](int t) {
+        uint8_t* const st = smem + (t % S) * STAGE;
+        const int k0 = k_begin + t * kI8BK;
+        const bool live = t < steps;
+        const int left = live ? a.k - k0 : 0;
+        const rsrc_t xr = make_rsrc(xb + k0, live ? x_bytes - (uint32_t)k0 : 0u);
+        if constexpr (TR) {
+            const rsrc_t wr = make_rsrc(wb + (int64_t)k0 * a.ldw,
+                                        live ? (uint32_t)(min(kI8BK, left) - 1) * (uint32_t)a.ldw + w_bytes : 0u);
+#pragma unroll
+            for (int i = 0; i < T::WLOADS; ++i)
+                bload128_lds(wr, st + 1024 * (wave * T::WLOADS + i), woff[i]);
+        } else {
+            const rsrc_t wr = make_rsrc(wb + k0, live ? w_bytes - (uint32_t)k0 : 0u);
+#pragma unroll
+            for (int i = 0; i < T::WLOADS; ++i)
+                bload128_lds(wr, st + 1024 * (wave * T::WLOADS + i), off_if(wcol[i] < left, woff[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < T::XLOADS; ++i)
+            bload128_lds(xr, st + kI8BN * kI8BK + 1024 * (wave * T::XLOADS + i), off_if(xcol[i] < left, xoff[i]));
+    };
+
+    int16v_t acc[T::TN][T::TT];
+#pragma unroll
+    for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+        for (int j = 0; j < T::TT; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+
+    const int wn = (wave / T::WM) * 32 * T::TN, wm = (wave % T::WM) * 32 * T::TT;
+    // this lane's operand addresses in a stage, for chunk pair 0 (slice s flips bits of the chunk)
+    uint32_t wat[T::TN], xat[T::TT];
+#pragma unroll
+    for (int i = 0; i < T::TN; ++i) {
+        if constexpr (TR) {
+            const int r = (lane & 15) >> 1, c = (wn + 32 * i) / 16 + ((lane >> 4) & 1);
+            wat[i] = (16 * g + r) * 256 + 16 * (c ^ (r << 1)) + 8 * (lane & 1);
+        } else {
+            const int r = wn + 32 * i + l32;
+            wat[i] = r * 128 + 16 * (g ^ row_key(r));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < T::TT; ++j) {
+        const int r = wm + 32 * j + l32;
+        xat[j] = kI8BN * kI8BK + r * 128 + 16 * (g ^ row_key(r));
+    }
+
+#pragma unroll
+    for (int t = 0; t < S - 1; ++t) fetch(t);
+    for (int t = 0; t < steps; ++t) {
+        wait_vmcnt<T::LOADS * (S - 2)>();
+        lds_barrier();
+        fetch(t + S - 1);
+        const uint8_t* const st = smem + (t % S) * STAGE;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            int4_t wf[T::TN], xf[T::TT];
+#pragma unroll
+            for (int j = 0; j < T::TT; ++j) xf[j] = lds128(st + (xat[j] ^ (32 * s)));
+            if constexpr (TR) {
+                u32x2_t lo[T::TN], hi[T::TN];
+                const uint32_t base = lds_addr(st) + s * 8192;
+                static_assert(T::TN == 1 || T::TN == 2, "blocks of the transposed reads");
+                if constexpr (T::TN == 2)
+                    asm volatile(
+                        "ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %4 offset:2048\n\t"
+                        "ds_read_b64_tr_b8 %2, %5\n\tds_read_b64_tr_b8 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+                        : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[T::TN - 1]), "=&v"(hi[T::TN - 1])
+                        : "v"(base + wat[0]), "v"(base + wat[T::TN - 1])
+                        : "memory");
+                else
+                    asm volatile(
+                        "ds_read_b64_tr_b8 %0, %2\n\tds_read_b64_tr_b8 %1, %2 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+                        : "=&v"(lo[0]), "=&v"(hi[0])
+                        : "v"(base + wat[0])
+                        : "memory");
+#pragma unroll
+                for (int i = 0; i < T::TN; ++i)
+                    wf[i] = int4_t{(int)lo[i].x, (int)lo[i].y, (int)hi[i].x, (int)hi[i].y};
+            } else {
+#pragma unroll
+                for (int i = 0; i < T::TN; ++i) wf[i] = lds128(st + (wat[i] ^ (32 * s)));
+            }
+#pragma unroll
+            for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+                for (int j = 0; j < T::TT; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[i], xf[j], acc[i][j], 0, 0, 0);
+        }
+    }
+    wait_vmcnt<0>();
+
+    // lane: token wm + 32 j + l32, channels wn + 32 i + 8 q + 4 g + 0..3
+#pragma unroll
+    for (int j = 0; j < T::TT; ++j) {
+        const int m = m0 + wm + 32 * j + l32;
+        if (m >= a.m) continue;
+        const float xs = OUT < 0 ? 0.0f : a.xs[m];
+#pragma unroll
+        for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = n0 + wn + 32 * i + 8 * q + 4 * g;
+                const int left = a.n - n;
+                if (left <= 0) continue;
+                const int4_t v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                if constexpr (OUT < 0) {
+                    // slab rows are padded to four channels
+                    *(int4_t*)(a.partials + (int64_t)split * a.slab + (int64_t)m * a.ldp + n) = v;
+                } else {
+                    float4_t f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        f[e] = (float)v[e] * xs;
+                        if (!TR && e < left) {
+                            f[e] *= a.ws[n + e];
+                            if (a.bias != nullptr) f[e] += load_any(a.bias, a.bias_dtype, n + e);
+                        }
+                    }
+                    store4<OUT < 0 ? 0 : OUT>((typename Elem<(OUT < 0 ? 0 : OUT)>::type*)a.y + (int64_t)m * a.ldy + n, f,
+                                              left);
+                }
+            }
+    }
+}
+
+// Split sums added, scaled, rounded: four channels a thread.
+template <int OUT>
+__global__ __launch_bounds__(256) void int8_reduce_kernel(const Int8GemmArgs a) {
+    const int quads = a.ldp / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)a.m * quads) return;
+    const int m = (int)(i / quads), n = 4 * (int)(i - (int64_t)m * quads);
+    int4_t v = {0, 0, 0, 0};
+    for (int s = 0; s < a.splits; ++s) v += *(const int4_t*)(a.partials + s * a.slab + (int64_t)m * a.ldp + n);
+    const float xs = a.xs[m];
+    const int left = a.n - n;
+    float4_t f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f[e] = (float)v[e] * xs;
+        if (a.ws != nullptr && e < left) f[e] *= a.ws[n + e];
+        if (a.bias != nullptr && e < left) f[e] += load_any(a.bias, a.bias_dtype, n + e);
+    }
+    store4<OUT>((typename Elem<OUT>::type*)a.y + (int64_t)m * a.ldy + n, f, left);
+}
+
+// Few tokens: the weight streams from memory once, straight to registers. A work-group of WAVES waves
+// owns 16 channels, the waves take slices of k; 16x16x64 integer MFMAs with MT blocks of 16 tokens (rows
+// past m repeat the last one and are dropped). The exact integer sums of the waves meet in LDS.
+template <int MT, int WAVES, int OUT>
+__global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Int8GemmArgs a) {
+    constexpr int U = 8;  // 64-byte columns of the weight in flight a wave
+    __shared__ int red[WAVES][MT][256];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = 16 * blockIdx.x, l16 = lane & 15, c = 16 * (lane >> 4);
+    const int cols = (a.k + 63) / 64, share = (cols + WAVES - 1) / WAVES;
+    const int begin = wave * share, end = min(cols, begin + share);
+    const int8_t* const w = a.w + (int64_t)min(n0 + l16, a.n - 1) * a.ldw + c;
+    const int8_t* x[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) x[t] = a.x + (int64_t)min(16 * t + l16, a.m - 1) * a.ldx + c;
+    int4_t acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = int4_t{0, 0, 0, 0};
+    for (int b = begin; b < end; b += U) {
+        int4_t wf[U], xf[MT][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = 64 * (b + u);
+            const bool ok = b + u < end && k + c < a.k;
+            wf[u] = ok ? *(const int4_t*)(w + k) : int4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < MT; ++t) xf[t][u] = ok ? *(const int4_t*)(x[t] + k) : int4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], xf[t][u], acc[t], 0, 0, 0);
+    }
+    // lane: channels 4 (lane / 16) + 0..3 of token l16
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) red[wave][t][l16 * 16 + 4 * (lane >> 4) + r] = acc[t][r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256 * MT; i += 64 * WAVES) {
+        const int m = i >> 4, n = n0 + (i & 15);
+        if (m >= a.m || n >= a.n) continue;
+        int v = 0;
+#pragma unroll
+        for (int s = 0; s < WAVES; ++s) v += red[s][m >> 4][i & 255];
+        float f = (float)v * a.xs[m] * a.ws[n];
+        if (a.bias != nullptr) f += load_any(a.bias, a.bias_dtype, n);
+        store1<OUT>((typename Elem<OUT>::type*)a.y + (int64_t)m * a.ldy + n, f);
+    }
+}
+
+// ---- quantization of rows ------------------------------------------------------------------------
+// scale = absmax / 127, q = rint(x * (127 / absmax)) in fp32 (COL: of x times a scale per column). Rows
+// whose largest magnitude is below 2^-120 count as zeros; a row that holds an infinity or NaN gets the
+// scale NaN and zeros, so that its products are NaN. THREADS threads a row, which stays in their registers
+// between its maximum and its rounding (R groups of eight a thread), or is read again (R = 0).
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+template <int DT, bool COL>
+__device__ __forceinline__ float8_t quant_load(const Int8QuantArgs& a, int64_t row, int col) {
+    const typename Elem<DT>::type* p = (const typename Elem<DT>::type*)a.x + row * a.ldx + col;
+    float8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (col + 8 <= a.k) {
+        v = load8<DT>(p);
+        if constexpr (COL) v = v * load8<DK_FP32>(a.col_scale + col);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + e < a.k) v[e] = COL ? (float)p[e] * a.col_scale[col + e] : (float)p[e];
+    }
+    return v;
+}
+
+__device__ __forceinline__ uint32_t top8(float8_t v, uint32_t top) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[e]));
+    return top;
+}
+
+__device__ __forceinline__ u32x2_t quant8(float8_t v, float inv) {
+    u32x2_t o = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e / 4] |= ((uint32_t)(int)__builtin_rintf(v[e] * inv) & 0xFFu) << (8 * (e & 3));
+    return o;
+}
+
+template <int DT, bool COL, int THREADS, int R>
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void int8_quantize_kernel(const Int8QuantArgs a) {
+    constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, ROWS = BLOCK / THREADS, NW = THREADS / 64;
+    __shared__ uint32_t tops[NW];
+    const int tid = threadIdx.x % THREADS;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
+    if (THREADS == 64 && row >= a.rows) return;  // whole waves; larger groups have one row a work-group
+    const int groups = (a.k + 7) / 8, padded = (a.k + 15) / 16 * 2;
+    float8_t v[R > 0 ? R : 1];
+    uint32_t top = 0;
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int q = tid + i * THREADS;
+            if (q < groups) v[i] = quant_load<DT, COL>(a, row, 8 * q);
+            else v[i] = float8_t{0, 0, 0, 0, 0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) top = top8(v[i], top);
+    } else {
+        for (int q = tid; q < groups; q += THREADS) top = top8(quant_load<DT, COL>(a, row, 8 * q), top);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    if constexpr (NW > 1) {
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NW; ++i) top = max(top, tops[i]);
+    }
+    const float most = __uint_as_float(top);
+    const bool bad = top >= 0x7F800000u, none = most < 7.523163845262640e-37f;  // 2^-120
+    const float inv = bad || none ? 0.0f : 127.0f / most;
+    if (tid == 0) a.scale[row] = bad ? __builtin_nanf("") : none ? 0.0f : most / 127.0f;
+    int8_t* const out = a.q + row * a.ldq;
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int q = tid + i * THREADS;
+            if (q < padded) *(u32x2_t*)(out + 8 * q) = bad ? u32x2_t{0, 0} : quant8(v[i], inv);
+        }
+    } else {
+        for (int q = tid; q < padded; q += THREADS) {
+            const float8_t x = q < groups ? quant_load<DT, COL>(a, row, 8 * q) : float8_t{0, 0, 0, 0, 0, 0, 0, 0};
+            *(u32x2_t*)(out + 8 * q) = bad ? u32x2_t{0, 0} : quant8(x, inv);
+        }
+    }
+}
+
+template <int DT, bool COL>
+static void launch_quantize_typed(const Int8QuantArgs& a, hipStream_t s) {
+    const int groups = (a.k + 15) / 16 * 2;
+    const unsigned rows = (unsigned)a.rows;
+    if (groups <= 64 * 4)
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 64, 4>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
+    else if (groups <= 256 * 2)
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 256, 2>), dim3(rows), dim3(256), 0, s, a);
+    else if (groups <= 256 * 4)
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 256, 4>), dim3(rows), dim3(256), 0, s, a);
+    else if (groups <= 512 * 5)
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 512, 5>), dim3(rows), dim3(512), 0, s, a);
+    else
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 512, 0>), dim3(rows), dim3(512), 0, s, a);
+}
+
+hipError_t launch_int8_quantize(const Int8QuantArgs& a, int dtype, hipStream_t s) {
+    if (a.rows == 0) return hipSuccess;
+    const bool col = a.col_scale != nullptr;
+    if (dtype == DK_FP16)
+        col ? launch_quantize_typed<DK_FP16, true>(a, s) : launch_quantize_typed<DK_FP16, false>(a, s);
+    else if (dtype == DK_BF16)
+        col ? launch_quantize_typed<DK_BF16, true>(a, s) : launch_quantize_typed<DK_BF16, false>(a, s);
+    else
+        col ? launch_quantize_typed<DK_FP32, true>(a, s) : launch_quantize_typed<DK_FP32, false>(a, s);
+    return hipGetLastError();
+}
+
+// ---- launches ------------------------------------------------------------------------------------
+
+Int8Plan int8_plan(int64_t m, int64_t n, int64_t k, bool tr) {
+    Int8Plan best{};
+    if (m <= 0 || n <= 0) return best;
+    if (!tr && m <= kInt8FewM) {
+        best.few = true;
+        best.splits = 1;
+        return best;
+    }
+    const int cus = device_cus();
+    const int64_t steps = (k + kI8BK - 1) / kI8BK > 0 ? (k + kI8BK - 1) / kI8BK : 1;
+    double best_us = 0;
+    // microseconds a step of a work-group, by tile height
+    const int tms[3] = {256, 128, 64};
+    const double step_us[3] = {1.15, 0.65, 0.45};
+    for (int v = 0; v < 3; ++v) {
+        const int64_t mt = (m + tms[v] - 1) / tms[v], nt = (n + kI8BN - 1) / kI8BN, tiles = mt * nt;
+        for (int64_t sp = 1; sp <= steps && sp <= 32; ++sp) {
+            const int64_t sps = (steps + sp - 1) / sp;
+            if ((steps + sps - 1) / sps != sp) continue;
+            const int64_t rounds = (tiles * sp + cus - 1) / cus;
+            const int64_t ldp = (n + 3) / 4 * 4;
+            double us = 6.0 + rounds * (sps * step_us[v] + 3.0);
+            if (sp > 1) us += 3.0 + 8.0 * sp * m * ldp / 5.0e6;  // partials written and read back
+            if (sp > 1 && sp * m * ldp * 4 > (int64_t(1) << 30)) continue;
+            if (best_us == 0 || us < best_us) {
+                best_us = us;
+                best.tm = tms[v];
+                best.m_tiles = (int)mt;
+                best.n_tiles = (int)nt;
+                best.splits = (int)sp;
+                best.steps_per_split = (int)sps;
+                best.partial_bytes = sp > 1 ? sp * m * ldp * 4 : 0;
+            }
+        }
+    }
+    return best;
+}
+
+template <int TM, bool TR, int OUT>
+static hipError_t launch_tile(const Int8GemmArgs& a, hipStream_t s) {
+    constexpr size_t lds = (size_t)i8_stages(TM) * i8_stage_bytes(TM);
+    const hipError_t e = allow_dynamic_lds((const void*)int8_gemm_kernel<TM, TR, OUT>, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((int8_gemm_kernel<TM, TR, OUT>), dim3((unsigned)(a.m_tiles * a.n_tiles * a.splits)),
+                       dim3(kI8Threads), lds, s, a);
+    return hipGetLastError();
+}
+
+template <int TM, int OUT>
+static hipError_t launch_way(const Int8GemmArgs& a, bool tr, hipStream_t s) {
+    return tr ? launch_tile<TM, true, OUT>(a, s) : launch_tile<TM, false, OUT>(a, s);
+}
+
+template <int OUT>
+static hipError_t launch_out(const Int8GemmArgs& a, int tm, bool tr, hipStream_t s) {
+    if (tm == 256) return launch_way<256, OUT>(a, tr, s);
+    if (tm == 128) return launch_way<128, OUT>(a, tr, s);
+    return launch_way<64, OUT>(a, tr, s);
+}
+
+template <int MT, int WAVES>
+static void launch_few(const Int8GemmArgs& a, int out, unsigned grid, hipStream_t s) {
+    const dim3 b(64 * WAVES);
+    if (out == DK_FP16)
+        hipLaunchKernelGGL((int8_few_kernel<MT, WAVES, DK_FP16>), dim3(grid), b, 0, s, a);
+    else if (out == DK_BF16)
+        hipLaunchKernelGGL((int8_few_kernel<MT, WAVES, DK_BF16>), dim3(grid), b, 0, s, a);
+    else
+        hipLaunchKernelGGL((int8_few_kernel<MT, WAVES, DK_FP32>), dim3(grid), b, 0, s, a);
+}
+
+hipError_t launch_int8_gemm(Int8GemmArgs a, const Int8Plan& p, int out_dtype, bool tr, hipStream_t s) {
+    if (a.m == 0 || a.n == 0) return hipSuccess;
+    if (p.few) {
+        const unsigned grid = (unsigned)((a.n + 15) / 16);
+        const bool wide = grid < 512;  // few work-groups: more waves of each along k
+        if (a.m <= 16)
+            wide ? launch_few<1, 16>(a, out_dtype, grid, s) : launch_few<1, 4>(a, out_dtype, grid, s);
+        else
+            wide ? launch_few<2, 16>(a, out_dtype, grid, s) : launch_few<2, 4>(a, out_dtype, grid, s);
+        return hipGetLastError();
+    }
+    a.m_tiles = p.m_tiles;
+    a.n_tiles = p.n_tiles;
+    a.splits = p.splits;
+    a.steps_per_split = p.steps_per_split;
+    if (p.splits == 1) {
+        if (out_dtype == DK_FP16) return launch_out<DK_FP16>(a, p.tm, tr, s);
+        if (out_dtype == DK_BF16) return launch_out<DK_BF16>(a, p.tm, tr, s);
+        return launch_out<DK_FP32>(a, p.tm, tr, s);
+    }
+    a.ldp = (a.n + 3) / 4 * 4;
+    a.slab = (int64_t)a.m * a.ldp;
+    const hipError_t e = launch_out<-1>(a, p.tm, tr, s);
+    if (e != hipSuccess) return e;
+    const unsigned grid = (unsigned)((a.slab / 4 + 255) / 256);
+    if (out_dtype == DK_FP16)
+        hipLaunchKernelGGL(int8_reduce_kernel<DK_FP16>, dim3(grid), dim3(256), 0, s, a);
+    else if (out_dtype == DK_BF16)
+        hipLaunchKernelGGL(int8_reduce_kernel<DK_BF16>, dim3(grid), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL(int8_reduce_kernel<DK_FP32>, dim3(grid), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace dk

@@ -46,8 +46,8 @@
  *                                               (solution/attn.py:257)
  *   dk_rope_qk_fwd / dk_rope_qk_bwd           <- skc_rope_fwd_kernel / skc_rope_bwd_kernel and
  *                                               FusedQKRope (solution/attn.py:27-126)
- *   dk_dropout_*, dk_qk_rope_*                no counterpart: seeded LoRA dropout, q/k norms and
- *                                               multi-axis rotation
+ *   dk_dropout_*, dk_qk_rope_*, dk_int8_*     no counterpart: seeded LoRA dropout, q/k norms and
+ *                                               multi-axis rotation, linears in 8-bit integers
  *   dk_swiglu_fwd / dk_swiglu_bwd             <- example_swiglu_fwd/bwd_kernel
  *                                               (solution/swiglu.py:15-37)
  */
@@ -358,6 +358,26 @@ int dk_qk_rope_fwd(const dk_qk_rope* a, void* stream);
 /* workspace: dk_qk_rope_bwd_workspace(a) bytes of device memory (0: none) where dw_q is set */
 int64_t dk_qk_rope_bwd_workspace(const dk_qk_rope* a);
 int dk_qk_rope_bwd(const dk_qk_rope* a, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Linear layers in 8-bit integers: a scale per token (row of x) and per output channel (row of w).
+ * dk_int8_quantize: row r of x [rows, k] (times col_scale[k] in fp32 where given) becomes
+ * q = rint(x * (127 / absmax)), scale[r] = absmax / 127, in fp32. Rows whose absmax is below 2^-120
+ * count as zeros; one that holds an infinity or NaN gets zeros and the scale NaN. q: row stride ldq, a
+ * multiple of 16, 16-byte aligned; columns k to the next multiple of 16 are set to zero. x of x_dtype at
+ * any alignment; 1 <= k <= 131071, rows < 2^23.
+ * dk_int8_linear: y[m, n] = (sum_k xq wq) xs[m] ws[n] + bias[n] with wq [n, k]; transposed: wq is
+ * [k, n], there are neither ws nor bias, y[m, n] = (sum_k xq wq) xs[m] -- the input gradient of a layer
+ * with weight wq, xq and xs quantized from dY with col_scale = ws. The sums are exact, the result is
+ * fp32(sum) * xs * ws + bias rounded once to y_dtype. xq [m, k]: zeros from k to the next multiple of 16;
+ * rows of wq (and xq) are read to the next multiple of 16 of their columns, which must be allocated, with
+ * whatever values. Row strides of xq and wq: multiples of 16 below 2^23, 16-byte aligned starts. bias NULL
+ * or of bias_dtype. workspace: dk_int8_linear_workspace bytes (0: none). */
+int dk_int8_quantize(const void* x, int x_dtype, int64_t ldx, const float* col_scale, int8_t* q, int64_t ldq,
+                     float* scale, int64_t rows, int64_t k, void* stream);
+int64_t dk_int8_linear_workspace(int transposed, int64_t m, int64_t n, int64_t k);
+int dk_int8_linear(int transposed, const int8_t* xq, int64_t ldx, const float* xs, const int8_t* wq, int64_t ldw,
+                   const float* ws, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t m,
+                   int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* out = fp16(silu(gate) * up), computed in fp32 (n elements). */
 int dk_swiglu_fwd(const uint16_t* gate, const uint16_t* up, uint16_t* out, int64_t n,
