@@ -17,6 +17,8 @@
 namespace dk {
 
 typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef int int2v_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) const uint8_t* lds_t;
 typedef int int16v_t __attribute__((ext_vector_type(16)));
 
 constexpr int kI8Threads = 512;
@@ -31,8 +33,27 @@ __device__ __forceinline__ int row_key(int r) { return (r >> 1) & 7; }
 
 __device__ __forceinline__ int4_t lds128(const uint8_t* p) { return *(const int4_t*)p; }
 
-__device__ __forceinline__ uint32_t lds_addr(const uint8_t* p) {
-    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t*)p;
+// Operands from a TR stage: 16 rows of a lane's byte column, two transposed reads of 8 rows each. One asm
+// block with its own wait: the builtin counts as aliasing every load to LDS in flight and would drain the
+// ring at every read.
+__device__ __forceinline__ void lds_tr8(const uint8_t* p, int4_t (&o)[1]) {
+    int2v_t a, b;
+    asm volatile("ds_read_b64_tr_b8 %0, %2\n\tds_read_b64_tr_b8 %1, %2 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(a), "=&v"(b)
+                 : "v"((lds_t)p)
+                 : "memory");
+    o[0] = int4_t{a.x, a.y, b.x, b.y};
+}
+__device__ __forceinline__ void lds_tr8(const uint8_t* p, const uint8_t* q, int4_t (&o)[2]) {
+    int2v_t a, b, c, d;
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %4 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %2, %5\n\tds_read_b64_tr_b8 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
+        : "v"((lds_t)p), "v"((lds_t)q)
+        : "memory");
+    o[0] = int4_t{a.x, a.y, b.x, b.y};
+    o[1] = int4_t{c.x, c.y, d.x, d.y};
 }
 
 template <int TM, bool TR>
@@ -57,6 +78,21 @@ __device__ __forceinline__ void store4(typename Elem<OUT>::type* p, float4_t v, 
         for (int e = 0; e < 4; ++e)
             if (e < left) p[e] = (E)v[e];
     }
+}
+
+__device__ __forceinline__ int4_t quad(const int16v_t& v, int q) {
+    return int4_t{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+}
+
+// four sums times the token's scale and (not TR) the channels' scales, plus their biases (256 on)
+template <bool TR>
+__device__ __forceinline__ float4_t scaled(int4_t v, float xs, const float* chan) {
+    float4_t f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = (float)v[e] * xs;
+    if constexpr (!TR) f = f * *(const float4_t*)chan + *(const float4_t*)(chan + 256);
+    asm("" : "+v"(f));  // keeps the products out of mixed-precision multiply-adds
+    return f;
 }
 
 // OUT: an element type, or -1 for the int32 partial sums of a split
@@ -162,82 +198,124 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
         xat[j] = kI8BN * kI8BK + r * 128 + 16 * (g ^ row_key(r));
     }
 
-#pragma unroll
-    for (int t = 0; t < S - 1; ++t) fetch(t);
-    for (int t = 0; t < steps; ++t) {
-        wait_vmcnt<T::LOADS * (S - 2)>();
-        lds_barrier();
-        fetch(t + S - 1);
+    // operands of one 32-wide slice of a stage
+    struct Slice {
+        int4_t w[T::TN], x[T::TT];
+    };
+    const auto read = [&](Slice& f, int t, int s) {
         const uint8_t* const st = smem + (t % S) * STAGE;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            int4_t wf[T::TN], xf[T::TT];
+        for (int j = 0; j < T::TT; ++j) f.x[j] = lds128(st + (xat[j] ^ (32 * s)));
+        if constexpr (TR) {
+            if constexpr (T::TN == 1)
+                lds_tr8(st + wat[0] + 8192 * s, f.w);
+            else
+                lds_tr8(st + wat[0] + 8192 * s, st + wat[1] + 8192 * s, f.w);
+        } else {
 #pragma unroll
-            for (int j = 0; j < T::TT; ++j) xf[j] = lds128(st + (xat[j] ^ (32 * s)));
-            if constexpr (TR) {
-                u32x2_t lo[T::TN], hi[T::TN];
-                const uint32_t base = lds_addr(st) + s * 8192;
-                static_assert(T::TN == 1 || T::TN == 2, "blocks of the transposed reads");
-                if constexpr (T::TN == 2)
-                    asm volatile(
-                        "ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %4 offset:2048\n\t"
-                        "ds_read_b64_tr_b8 %2, %5\n\tds_read_b64_tr_b8 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
-                        : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[T::TN - 1]), "=&v"(hi[T::TN - 1])
-                        : "v"(base + wat[0]), "v"(base + wat[T::TN - 1])
-                        : "memory");
-                else
-                    asm volatile(
-                        "ds_read_b64_tr_b8 %0, %2\n\tds_read_b64_tr_b8 %1, %2 offset:2048\n\ts_waitcnt lgkmcnt(0)"
-                        : "=&v"(lo[0]), "=&v"(hi[0])
-                        : "v"(base + wat[0])
-                        : "memory");
-#pragma unroll
-                for (int i = 0; i < T::TN; ++i)
-                    wf[i] = int4_t{(int)lo[i].x, (int)lo[i].y, (int)hi[i].x, (int)hi[i].y};
-            } else {
-#pragma unroll
-                for (int i = 0; i < T::TN; ++i) wf[i] = lds128(st + (wat[i] ^ (32 * s)));
-            }
-#pragma unroll
-            for (int i = 0; i < T::TN; ++i)
-#pragma unroll
-                for (int j = 0; j < T::TT; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[i], xf[j], acc[i][j], 0, 0, 0);
+            for (int i = 0; i < T::TN; ++i) f.w[i] = lds128(st + (wat[i] ^ (32 * s)));
         }
-    }
-    wait_vmcnt<0>();
-
-    // lane: token wm + 32 j + l32, channels wn + 32 i + 8 q + 4 g + 0..3
-#pragma unroll
-    for (int j = 0; j < T::TT; ++j) {
-        const int m = m0 + wm + 32 * j + l32;
-        if (m >= a.m) continue;
-        const float xs = OUT < 0 ? 0.0f : a.xs[m];
+    };
+    const auto multiply = [&](const Slice& f) {
 #pragma unroll
         for (int i = 0; i < T::TN; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int n = n0 + wn + 32 * i + 8 * q + 4 * g;
-                const int left = a.n - n;
-                if (left <= 0) continue;
-                const int4_t v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                if constexpr (OUT < 0) {
-                    // slab rows are padded to four channels
-                    *(int4_t*)(a.partials + (int64_t)split * a.slab + (int64_t)m * a.ldp + n) = v;
-                } else {
-                    float4_t f;
+            for (int j = 0; j < T::TT; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
+    };
+
+    // the tile's channel scales and biases
+    float* const chan = (float*)(smem + S * STAGE);
+    if constexpr (!TR && OUT >= 0) {
+        const int n = n0 + (int)(threadIdx.x & 255);
+        float v = 0.0f;
+        if (n < a.n) {
+            if (threadIdx.x < 256) v = a.ws[n];
+            else if (a.bias != nullptr) v = load_any(a.bias, a.bias_dtype, n);
+        }
+        chan[threadIdx.x] = v;
+    }
+
+    Slice f0, f1;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        f[e] = (float)v[e] * xs;
-                        if (!TR && e < left) {
-                            f[e] *= a.ws[n + e];
-                            if (a.bias != nullptr) f[e] += load_any(a.bias, a.bias_dtype, n + e);
-                        }
-                    }
-                    store4<OUT < 0 ? 0 : OUT>((typename Elem<(OUT < 0 ? 0 : OUT)>::type*)a.y + (int64_t)m * a.ldy + n, f,
-                                              left);
+    for (int t = 0; t < S; ++t) fetch(t);
+    wait_vmcnt<T::LOADS * (S - 1)>();
+    lds_barrier();
+    read(f0, 0, 0);
+    for (int t = 0; t < steps; ++t) {
+        read(f1, t, 1);
+        multiply(f0);
+        read(f0, t, 2);
+        multiply(f1);
+        read(f1, t, 3);
+        multiply(f0);
+        // every wave has read the last of this stage: it is free, and the next one is whole
+        wait_vmcnt<T::LOADS * (S - 2)>();
+        lds_barrier();
+        fetch(t + S);
+        read(f0, t + 1, 0);
+        multiply(f1);
+    }
+    wait_vmcnt<0>();
+    lds_barrier();
+
+    // lane: token wm + 32 j + l32, channels wn + 32 i + 8 q + 4 g + 0..3
+    if constexpr (OUT < 0 || OUT == DK_FP32) {
+#pragma unroll
+        for (int j = 0; j < T::TT; ++j) {
+            const int m = m0 + wm + 32 * j + l32;
+            if (m >= a.m) continue;
+            const float xs = OUT < 0 ? 0.0f : a.xs[m];
+#pragma unroll
+            for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int c = wn + 32 * i + 8 * q + 4 * g, n = n0 + c;
+                    if (n >= a.n) continue;
+                    const int4_t v = quad(acc[i][j], q);
+                    if constexpr (OUT < 0)  // slab rows are padded to four channels
+                        *(int4_t*)(a.partials + (int64_t)split * a.slab + (int64_t)m * a.ldp + n) = v;
+                    else
+                        store4<DK_FP32>((float*)a.y + (int64_t)m * a.ldy + n, scaled<TR>(v, xs, chan + c), a.n - n);
+                }
+        }
+    } else {
+        // 16-bit outputs leave as whole rows: 32 tokens of the wave's channels at a time through LDS
+        typedef typename Elem<OUT>::type E;
+        constexpr int ROW = 64 * T::TN + 16;  // bytes
+        constexpr int LANES = 4 * T::TN;      // lanes a row of 16-byte pieces
+        uint8_t* const stage = smem + wave * 32 * ROW;
+#pragma unroll
+        for (int j = 0; j < T::TT; ++j) {
+            const int mrow = m0 + wm + 32 * j;
+            const float xs = mrow + l32 < a.m ? a.xs[mrow + l32] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int c = 32 * i + 8 * q + 4 * g;
+                    const float4_t v = scaled<TR>(quad(acc[i][j], q), xs, chan + wn + c);
+                    store4<OUT>((E*)(stage + l32 * ROW) + c, v, 4);
+                }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int r = 0; r < 32; r += 64 / LANES) {
+                const int row = r + lane / LANES, c = 8 * (lane % LANES), n = n0 + wn + c, m = mrow + row;
+                const typename Elem<OUT>::vec v = *(const typename Elem<OUT>::vec*)(stage + row * ROW + 2 * c);
+                if (m >= a.m || n >= a.n) continue;
+                E* const y = (E*)a.y + (int64_t)m * a.ldy + n;
+                if (n + 8 <= a.n) {
+                    *(typename Elem<OUT>::loose*)y = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (n + e < a.n) y[e] = v[e];
                 }
             }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 }
 
@@ -468,7 +546,7 @@ Int8Plan int8_plan(int64_t m, int64_t n, int64_t k, bool tr) {
 
 template <int TM, bool TR, int OUT>
 static hipError_t launch_tile(const Int8GemmArgs& a, hipStream_t s) {
-    constexpr size_t lds = (size_t)i8_stages(TM) * i8_stage_bytes(TM);
+    constexpr size_t lds = (size_t)i8_stages(TM) * i8_stage_bytes(TM) + 2048;  // channel scales and biases
     const hipError_t e = allow_dynamic_lds((const void*)int8_gemm_kernel<TM, TR, OUT>, lds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((int8_gemm_kernel<TM, TR, OUT>), dim3((unsigned)(a.m_tiles * a.n_tiles * a.splits)),
