@@ -6,6 +6,7 @@ is no fallback: every entry point raises if the library is missing or returns an
 
 import ctypes
 import os
+import struct
 import threading
 import weakref
 
@@ -62,6 +63,7 @@ class QkRope(ctypes.Structure):
                 ("n_kv_heads", c_i32), ("head_dim", c_i32), ("dtype", c_i32), ("w_dtype", c_i32), ("n_axes", c_i32),
                 ("sections", c_i32 * 4), ("interleaved", c_i32), ("positions_int64", c_i32), ("eps", c_f32),
                 ("reserved", c_i32)]
+    PACK = struct.Struct("@14P9q12if i")
 
 
 EXPORTS = {
@@ -103,17 +105,21 @@ EXPORTS = {
                         c_i32, c_vp], c_i32),
     "dk_rope_qk_bwd": ([c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i32, c_i32, c_i32, c_vp],
                        c_i32),
-    "dk_dropout_fwd": ([c_vp, c_i32, c_i64, c_vp, ctypes.POINTER(ctypes.c_double), c_i32, ctypes.POINTER(c_vp), c_i32,
-                        ctypes.POINTER(c_i64), c_i64, c_i64, c_vp], c_i32),
-    "dk_dropout_bwd": ([ctypes.POINTER(c_vp), c_i32, ctypes.POINTER(c_i64), c_vp, ctypes.POINTER(ctypes.c_double),
-                        c_i32, c_vp, c_i32, c_i64, c_i64, c_i64, c_vp], c_i32),
-    "dk_qk_rope_fwd": ([ctypes.POINTER(QkRope), c_vp], c_i32),
-    "dk_qk_rope_bwd_workspace": ([ctypes.POINTER(QkRope)], c_i64),
-    "dk_qk_rope_bwd": ([ctypes.POINTER(QkRope), c_vp, c_i64, c_vp], c_i32),
+    "dk_dropout_fwd": ([c_vp, c_i32, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_vp, c_i64, c_i64, c_vp], c_i32),
+    "dk_dropout_bwd": ([c_vp, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_i32, c_i64, c_i64, c_i64, c_vp], c_i32),
+    # dk_qk_rope descriptors are passed as packed bytes (QkRope.PACK), cheaper to make than a structure
+    "dk_qk_rope_fwd": ([c_vp, c_vp], c_i32),
+    "dk_qk_rope_bwd_workspace": ([c_vp], c_i64),
+    "dk_qk_rope_bwd": ([c_vp, c_vp, c_i64, c_vp], c_i32),
     "dk_int8_quantize": ([c_vp, c_i32, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp], c_i32),
     "dk_int8_linear_workspace": ([c_i32, c_i64, c_i64, c_i64], c_i64),
     "dk_int8_linear": ([c_i32, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_i64, c_i64, c_i64,
                         c_i64, c_vp, c_i64, c_vp], c_i32),
+    "dk_int8_linear_x_workspace": ([c_i32, c_i64, c_i64, c_i64], c_i64),
+    "dk_int8_linear_fwd": ([c_vp, c_i32, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64,
+                            c_vp, c_i64, c_vp], c_i32),
+    "dk_int8_linear_bwd": ([c_vp, c_i32, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64,
+                            c_vp], c_i32),
     "dk_swiglu_fwd": ([c_vp, c_vp, c_vp, c_i64, c_vp], c_i32),
     "dk_swiglu_bwd": ([c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp], c_i32),
     "dk_last_error": ([], ctypes.c_char_p),
@@ -161,31 +167,34 @@ def stream_of(device):
     return ctypes.c_void_p(raw_stream(device))
 
 
-class _Here:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
+_current_device = torch._C._cuda_getDevice
 
 
-_HERE = _Here()
+def call_on(device, fn, *args):
+    """check(fn(*args, current stream of `device`)), with `device` the current one during the call."""
+    idx = device.index
+    if idx == _current_device():
+        rc = fn(*args, _raw_stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, _raw_stream(idx))
+    if rc != 0:
+        raise DecikError(lib().dk_last_error().decode())
 
 
-def on_device(device):
-    """Context of a launch on `device`: the current device where it is that one already."""
-    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+def gpu_input(what, t):
+    """The device of a call's leading tensor, which must be on a GPU."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{what}: needs GPU tensors")
+    return t.device
 
 
-def gpu_tensors(what, device, **tensors):
-    """Each given tensor (None: absent) must be a GPU tensor on `device`."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise ValueError(f"{what}: {name} must be a tensor")
-        if not t.is_cuda or t.device != device:
-            raise ValueError(f"{what}: {name} must be on the GPU of the input ({device}), not on {t.device}")
+def same_gpu(what, device, *tensors):
+    """Each given tensor (None: absent) must be on the GPU `device`."""
+    for t in tensors:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.device != device):
+            raise ValueError(f"{what}: every tensor must be on the GPU of the input, {device}, not "
+                             f"{getattr(t, 'device', type(t))}")
 
 
 # element types of the entries that take more than fp16 (include/decik_nf4.h)

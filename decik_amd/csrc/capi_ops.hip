@@ -288,4 +288,70 @@ int dk_int8_linear(int transposed, const int8_t* xq, int64_t ldx, const float* x
                         "dk_int8_linear launch");
 }
 
+// workspace of a fused call: the integers (rows padded to 128 bytes), the scales, the partial sums
+int64_t dk_int8_linear_x_workspace(int backward, int64_t m, int64_t n, int64_t k) {
+    dk_clear_error();
+    const int64_t rows = m, cols = backward ? n : k, out = backward ? k : n;
+    if (!int8_sizes(rows, out, cols) || (backward && k < 1)) {
+        dk_fail("dk_int8_linear: 0 <= m, n < 2^23, 1 <= k <= 131071 (backward: 1 <= n <= 131071)");
+        return -1;
+    }
+    if (m == 0 || out == 0 || int8_fused(m, cols, backward != 0)) return 0;
+    return m * ((cols + 127) / 128 * 128) + (m + 31) / 32 * 128 + int8_plan(m, out, cols, backward != 0).partial_bytes;
+}
+
+static int int8_linear_x(bool backward, const void* x, int x_dtype, int64_t ldx, const int8_t* wq, int64_t ldw,
+                         const float* ws, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t m,
+                         int64_t out, int64_t cols, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (m == 0 || out == 0) return 0;
+    if (x == nullptr || wq == nullptr || ws == nullptr || y == nullptr) return dk_fail("dk_int8_linear: null pointer");
+    if (!is_dtype(x_dtype) || !is_dtype(y_dtype) || (bias != nullptr && !is_dtype(bias_dtype)))
+        return dk_fail("dk_int8_linear: unknown type");
+    if ((m > 1 && ldx < 0) || (m > 1 && ldy < out)) return dk_fail("dk_int8_linear: row strides");
+    if (!backward && int8_fused(m, cols, false)) {
+        if (!int8_rows_ok(wq, ldw, cols))
+            return dk_fail("dk_int8_linear: wq must be 16-byte aligned, its row stride a multiple of 16 below 2^23");
+        Int8QuantArgs q{x, nullptr, nullptr, nullptr, ldx, 0, m, (int32_t)cols};
+        Int8GemmArgs a{};
+        a.w = wq;
+        a.ws = ws;
+        a.bias = bias;
+        a.bias_dtype = bias_dtype;
+        a.y = y;
+        a.ldw = ldw;
+        a.ldy = ldy;
+        a.m = (int32_t)m;
+        a.n = (int32_t)out;
+        a.k = (int32_t)cols;
+        return check_launch(launch_int8_fused(a, q, x_dtype, y_dtype, static_cast<hipStream_t>(stream)),
+                            "dk_int8_linear launch");
+    }
+    const int64_t ldq = (cols + 127) / 128 * 128, scales = m * ldq, rest = scales + (m + 31) / 32 * 128;
+    if (workspace == nullptr || workspace_bytes < rest || !aligned_to(workspace, 16))
+        return dk_fail("dk_int8_linear: workspace too small (dk_int8_linear_x_workspace)");
+    int8_t* const q = static_cast<int8_t*>(workspace);
+    float* const xs = reinterpret_cast<float*>(q + scales);
+    if (int rc = dk_int8_quantize(x, x_dtype, ldx, backward ? ws : nullptr, q, ldq, xs, m, cols, stream)) return rc;
+    return dk_int8_linear(backward ? 1 : 0, q, ldq, xs, wq, ldw, backward ? nullptr : ws, bias, bias_dtype, y, y_dtype,
+                          ldy, m, out, cols, q + rest, workspace_bytes - rest, stream);
+}
+
+int dk_int8_linear_fwd(const void* x, int x_dtype, int64_t ldx, const int8_t* wq, int64_t ldw, const float* ws,
+                       const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t m, int64_t n,
+                       int64_t k, void* workspace, int64_t workspace_bytes, void* stream) {
+    dk_clear_error();
+    if (!int8_sizes(m, n, k)) return dk_fail("dk_int8_linear_fwd: 0 <= m, n < 2^23, 1 <= k <= 131071");
+    return int8_linear_x(false, x, x_dtype, ldx, wq, ldw, ws, bias, bias_dtype, y, y_dtype, ldy, m, n, k, workspace,
+                         workspace_bytes, stream);
+}
+
+int dk_int8_linear_bwd(const void* dy, int dy_dtype, int64_t lddy, const int8_t* wq, int64_t ldw, const float* ws,
+                       void* dx, int dx_dtype, int64_t lddx, int64_t m, int64_t n, int64_t k, void* workspace,
+                       int64_t workspace_bytes, void* stream) {
+    dk_clear_error();
+    if (!int8_sizes(m, k, n)) return dk_fail("dk_int8_linear_bwd: 0 <= m, k < 2^23, 1 <= n <= 131071");
+    return int8_linear_x(true, dy, dy_dtype, lddy, wq, ldw, ws, nullptr, 0, dx, dx_dtype, lddx, m, k, n, workspace,
+                         workspace_bytes, stream);
+}
+
 }  // extern "C"

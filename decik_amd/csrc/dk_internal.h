@@ -284,6 +284,8 @@ hipError_t launch_qk_rope(QkRopeArgs a, int dtype, bool norm, bool axes, bool ba
 
 // Products of 8-bit integers (int8_gemm.hip).
 constexpr int kInt8FewM = 32;  // forward launches of so few tokens stream the weight to registers
+// ... and of at most so many quantize x themselves, where it fits so many bytes of LDS
+constexpr int kInt8FusedM = 4, kInt8FusedLds = 32768;
 struct Int8GemmArgs {
     const int8_t* x;   // [m, k], row stride ldx, zeros from k to the next multiple of 16
     const int8_t* w;   // forward [n, k], transposed [k, n], row stride ldw
@@ -311,6 +313,8 @@ struct Int8QuantArgs {
 };
 Int8Plan int8_plan(int64_t m, int64_t n, int64_t k, bool tr);
 hipError_t launch_int8_gemm(Int8GemmArgs a, const Int8Plan& p, int out_dtype, bool tr, hipStream_t s);
+bool int8_fused(int64_t m, int64_t k, bool tr);
+hipError_t launch_int8_fused(const Int8GemmArgs& a, const Int8QuantArgs& q, int x_dtype, int out_dtype, hipStream_t s);
 hipError_t launch_int8_quantize(const Int8QuantArgs& a, int dtype, hipStream_t s);
 
 // The calling thread's error (dk_last_error); dk_fail returns 1.

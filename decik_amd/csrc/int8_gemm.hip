@@ -36,25 +36,52 @@ __device__ __forceinline__ int4_t lds128(const uint8_t* p) { return *(const int4
 // Operands from a TR stage: 16 rows of a lane's byte column, two transposed reads of 8 rows each. One asm
 // block with its own wait: the builtin counts as aliasing every load to LDS in flight and would drain the
 // ring at every read.
-__device__ __forceinline__ void lds_tr8(const uint8_t* p, int4_t (&o)[1]) {
-    int2v_t a, b;
-    asm volatile("ds_read_b64_tr_b8 %0, %2\n\tds_read_b64_tr_b8 %1, %2 offset:2048\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(a), "=&v"(b)
-                 : "v"((lds_t)p)
-                 : "memory");
-    o[0] = int4_t{a.x, a.y, b.x, b.y};
-}
-__device__ __forceinline__ void lds_tr8(const uint8_t* p, const uint8_t* q, int4_t (&o)[2]) {
+__device__ __forceinline__ void lds_tr8(const uint8_t* st, const uint32_t (&at)[2], int4_t (&o)[1][2]) {
     int2v_t a, b, c, d;
     asm volatile(
         "ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %4 offset:2048\n\t"
         "ds_read_b64_tr_b8 %2, %5\n\tds_read_b64_tr_b8 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
         : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
-        : "v"((lds_t)p), "v"((lds_t)q)
+        : "v"((lds_t)(st + at[0])), "v"((lds_t)(st + at[1]))
         : "memory");
-    o[0] = int4_t{a.x, a.y, b.x, b.y};
-    o[1] = int4_t{c.x, c.y, d.x, d.y};
+    o[0][0] = int4_t{a.x, a.y, b.x, b.y};
+    o[0][1] = int4_t{c.x, c.y, d.x, d.y};
 }
+__device__ __forceinline__ void lds_tr8(const uint8_t* st, const uint32_t (&at)[2], int4_t (&o)[2][2]) {
+    int2v_t a, b, c, d, e, f, g, h;
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %8\n\tds_read_b64_tr_b8 %1, %8 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %2, %9\n\tds_read_b64_tr_b8 %3, %9 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %4, %8 offset:8192\n\tds_read_b64_tr_b8 %5, %8 offset:10240\n\t"
+        "ds_read_b64_tr_b8 %6, %9 offset:8192\n\tds_read_b64_tr_b8 %7, %9 offset:10240\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(e), "=&v"(f), "=&v"(g), "=&v"(h)
+        : "v"((lds_t)(st + at[0])), "v"((lds_t)(st + at[1]))
+        : "memory");
+    o[0][0] = int4_t{a.x, a.y, b.x, b.y};
+    o[0][1] = int4_t{c.x, c.y, d.x, d.y};
+    o[1][0] = int4_t{e.x, e.y, f.x, f.y};
+    o[1][1] = int4_t{g.x, g.y, h.x, h.y};
+}
+__device__ __forceinline__ void lds_tr8(const uint8_t* st, const uint32_t (&at)[1], int4_t (&o)[4][1]) {
+    int2v_t a, b, c, d, e, f, g, h;
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %8\n\tds_read_b64_tr_b8 %1, %8 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %2, %8 offset:8192\n\tds_read_b64_tr_b8 %3, %8 offset:10240\n\t"
+        "ds_read_b64_tr_b8 %4, %8 offset:16384\n\tds_read_b64_tr_b8 %5, %8 offset:18432\n\t"
+        "ds_read_b64_tr_b8 %6, %8 offset:24576\n\tds_read_b64_tr_b8 %7, %8 offset:26624\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(e), "=&v"(f), "=&v"(g), "=&v"(h)
+        : "v"((lds_t)(st + at[0]))
+        : "memory");
+    o[0][0] = int4_t{a.x, a.y, b.x, b.y};
+    o[1][0] = int4_t{c.x, c.y, d.x, d.y};
+    o[2][0] = int4_t{e.x, e.y, f.x, f.y};
+    o[3][0] = int4_t{g.x, g.y, h.x, h.y};
+}
+
+template <int V>
+struct Int {
+    static constexpr int value = V;
+};
 
 template <int TM, bool TR>
 struct I8Tile {
@@ -64,6 +91,9 @@ struct I8Tile {
     static constexpr int TN = kI8BN / WN / 32, TT = TM / WM / 32;  // 32x32 blocks a wave
     static constexpr int WLOADS = kI8BN * kI8BK / 8192, XLOADS = TM * kI8BK / 8192;  // a wave and step
     static constexpr int LOADS = WLOADS + XLOADS;
+    // slices whose operands are read at once, ahead of the MFMAs: small tiles have few MFMAs a slice to hide
+    // the reads behind
+    static constexpr int U = TM == 256 ? 1 : TM == 128 ? 2 : 4;
 };
 
 template <int OUT>
@@ -198,30 +228,33 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
         xat[j] = kI8BN * kI8BK + r * 128 + 16 * (g ^ row_key(r));
     }
 
-    // operands of one 32-wide slice of a stage
-    struct Slice {
-        int4_t w[T::TN], x[T::TT];
+    // operands of U slices (32 of k each) of a stage: parts 0 .. 4 / U - 1 of step t
+    constexpr int U = T::U;
+    struct Part {
+        int4_t w[U][T::TN], x[U][T::TT];
     };
-    const auto read = [&](Slice& f, int t, int s) {
+    const auto read = [&](Part& f, int t, int part) {
         const uint8_t* const st = smem + (t % S) * STAGE;
 #pragma unroll
-        for (int j = 0; j < T::TT; ++j) f.x[j] = lds128(st + (xat[j] ^ (32 * s)));
-        if constexpr (TR) {
-            if constexpr (T::TN == 1)
-                lds_tr8(st + wat[0] + 8192 * s, f.w);
-            else
-                lds_tr8(st + wat[0] + 8192 * s, st + wat[1] + 8192 * s, f.w);
-        } else {
+        for (int u = 0; u < U; ++u) {
+            const int s = part * U + u;
 #pragma unroll
-            for (int i = 0; i < T::TN; ++i) f.w[i] = lds128(st + (wat[i] ^ (32 * s)));
+            for (int j = 0; j < T::TT; ++j) f.x[u][j] = lds128(st + (xat[j] ^ (32 * s)));
+            if constexpr (!TR) {
+#pragma unroll
+                for (int i = 0; i < T::TN; ++i) f.w[u][i] = lds128(st + (wat[i] ^ (32 * s)));
+            }
         }
+        if constexpr (TR) lds_tr8(st + part * U * 8192, wat, f.w);
     };
-    const auto multiply = [&](const Slice& f) {
+    const auto multiply = [&](const Part& f) {
 #pragma unroll
-        for (int i = 0; i < T::TN; ++i)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < T::TT; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
+            for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+                for (int j = 0; j < T::TT; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[u][i], f.x[u][j], acc[i][j], 0, 0, 0);
     };
 
     // the tile's channel scales and biases
@@ -236,25 +269,39 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
         chan[threadIdx.x] = v;
     }
 
-    Slice f0, f1;
+    Part f[2];
 #pragma unroll
     for (int t = 0; t < S; ++t) fetch(t);
     wait_vmcnt<T::LOADS * (S - 1)>();
     lds_barrier();
-    read(f0, 0, 0);
-    for (int t = 0; t < steps; ++t) {
-        read(f1, t, 1);
-        multiply(f0);
-        read(f0, t, 2);
-        multiply(f1);
-        read(f1, t, 3);
-        multiply(f0);
-        // every wave has read the last of this stage: it is free, and the next one is whole
-        wait_vmcnt<T::LOADS * (S - 2)>();
-        lds_barrier();
-        fetch(t + S);
-        read(f0, t + 1, 0);
-        multiply(f1);
+    read(f[0], 0, 0);
+    // a step whose first part is in f[P]
+    const auto step = [&](int t, auto parity) {
+        constexpr int P = decltype(parity)::value;
+#pragma unroll
+        for (int part = 0; part < 4 / U; ++part) {
+            const int now = (P + part) & 1;
+            if (part + 1 < 4 / U) {
+                read(f[now ^ 1], t, part + 1);
+            } else {
+                // every wave has read the last of this stage: it is free, and the next one is whole
+                wait_vmcnt<T::LOADS * (S - 2)>();
+                lds_barrier();
+                fetch(t + S);
+                read(f[now ^ 1], t + 1, 0);
+            }
+            multiply(f[now]);
+        }
+    };
+    if constexpr (U == 4) {
+        int t = 0;
+        for (; t + 1 < steps; t += 2) {
+            step(t, Int<0>());
+            step(t + 1, Int<1>());
+        }
+        if (t < steps) step(t, Int<0>());
+    } else {
+        for (int t = 0; t < steps; ++t) step(t, Int<0>());
     }
     wait_vmcnt<0>();
     lds_barrier();
@@ -340,6 +387,125 @@ __global__ __launch_bounds__(256) void int8_reduce_kernel(const Int8GemmArgs a) 
     store4<OUT>((typename Elem<OUT>::type*)a.y + (int64_t)m * a.ldy + n, f, left);
 }
 
+// ---- quantization of rows ------------------------------------------------------------------------
+// scale = absmax / 127, q = rint(x * (127 / absmax)) in fp32 (COL: of x times a scale per column). Rows
+// whose largest magnitude is below 2^-120 count as zeros; a row that holds an infinity or NaN gets the
+// scale NaN and zeros, so that its products are NaN. THREADS threads a row, which stays in their registers
+// between its maximum and its rounding (R groups of eight a thread), or is read again (R = 0).
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+template <int DT, bool COL>
+__device__ __forceinline__ float8_t quant_load(const Int8QuantArgs& a, int64_t row, int col) {
+    const typename Elem<DT>::type* p = (const typename Elem<DT>::type*)a.x + row * a.ldx + col;
+    float8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (col + 8 <= a.k) {
+        v = load8<DT>(p);
+        if constexpr (COL) v = v * load8<DK_FP32>(a.col_scale + col);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + e < a.k) v[e] = COL ? (float)p[e] * a.col_scale[col + e] : (float)p[e];
+    }
+    return v;
+}
+
+__device__ __forceinline__ uint32_t top8(float8_t v, uint32_t top) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[e]));
+    return top;
+}
+
+__device__ __forceinline__ u32x2_t quant8(float8_t v, float inv) {
+    u32x2_t o = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e / 4] |= ((uint32_t)(int)__builtin_rintf(v[e] * inv) & 0xFFu) << (8 * (e & 3));
+    return o;
+}
+
+// scale of a row with the largest magnitude `top` (its bits), and what its values are multiplied by (0: zeros)
+__device__ __forceinline__ void quant_scale(uint32_t top, float& inv, float& scale) {
+    const float most = __uint_as_float(top);
+    const bool bad = top >= 0x7F800000u, none = most < 7.523163845262640e-37f;  // 2^-120
+    inv = bad || none ? 0.0f : 127.0f / most;
+    scale = bad ? __builtin_nanf("") : none ? 0.0f : most / 127.0f;
+}
+
+template <int DT, bool COL, int THREADS, int R>
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void int8_quantize_kernel(const Int8QuantArgs a) {
+    constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, ROWS = BLOCK / THREADS, NW = THREADS / 64;
+    __shared__ uint32_t tops[NW];
+    const int tid = threadIdx.x % THREADS;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
+    if (THREADS == 64 && row >= a.rows) return;  // whole waves; larger groups have one row a work-group
+    const int groups = (a.k + 7) / 8, padded = (a.k + 15) / 16 * 2;
+    float8_t v[R > 0 ? R : 1];
+    uint32_t top = 0;
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int q = tid + i * THREADS;
+            if (q < groups) v[i] = quant_load<DT, COL>(a, row, 8 * q);
+            else v[i] = float8_t{0, 0, 0, 0, 0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) top = top8(v[i], top);
+    } else {
+        for (int q = tid; q < groups; q += THREADS) top = top8(quant_load<DT, COL>(a, row, 8 * q), top);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    if constexpr (NW > 1) {
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NW; ++i) top = max(top, tops[i]);
+    }
+    float inv, scale;
+    quant_scale(top, inv, scale);
+    if (tid == 0) a.scale[row] = scale;
+    int8_t* const out = a.q + row * a.ldq;
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int q = tid + i * THREADS;
+            if (q < padded) *(u32x2_t*)(out + 8 * q) = inv == 0.0f ? u32x2_t{0, 0} : quant8(v[i], inv);
+        }
+    } else {
+        for (int q = tid; q < padded; q += THREADS) {
+            const float8_t x = q < groups ? quant_load<DT, COL>(a, row, 8 * q) : float8_t{0, 0, 0, 0, 0, 0, 0, 0};
+            *(u32x2_t*)(out + 8 * q) = inv == 0.0f ? u32x2_t{0, 0} : quant8(x, inv);
+        }
+    }
+}
+
+template <int DT, bool COL>
+static void launch_quantize_typed(const Int8QuantArgs& a, hipStream_t s) {
+    const int groups = (a.k + 15) / 16 * 2;
+    const unsigned rows = (unsigned)a.rows;
+    if (groups <= 64 * 4)
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 64, 4>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
+    else if (groups <= 256 * 2)
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 256, 2>), dim3(rows), dim3(256), 0, s, a);
+    else if (groups <= 256 * 4)
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 256, 4>), dim3(rows), dim3(256), 0, s, a);
+    else if (groups <= 512 * 5)
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 512, 5>), dim3(rows), dim3(512), 0, s, a);
+    else
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 512, 0>), dim3(rows), dim3(512), 0, s, a);
+}
+
+hipError_t launch_int8_quantize(const Int8QuantArgs& a, int dtype, hipStream_t s) {
+    if (a.rows == 0) return hipSuccess;
+    const bool col = a.col_scale != nullptr;
+    if (dtype == DK_FP16)
+        col ? launch_quantize_typed<DK_FP16, true>(a, s) : launch_quantize_typed<DK_FP16, false>(a, s);
+    else if (dtype == DK_BF16)
+        col ? launch_quantize_typed<DK_BF16, true>(a, s) : launch_quantize_typed<DK_BF16, false>(a, s);
+    else
+        col ? launch_quantize_typed<DK_FP32, true>(a, s) : launch_quantize_typed<DK_FP32, false>(a, s);
+    return hipGetLastError();
+}
+
 // Few tokens: the weight streams from memory once, straight to registers. A work-group of WAVES waves
 // owns 16 channels, the waves take slices of k; 16x16x64 integer MFMAs with MT blocks of 16 tokens (rows
 // past m repeat the last one and are dropped). The exact integer sums of the waves meet in LDS.
@@ -392,134 +558,83 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Int8GemmArgs
     }
 }
 
-// ---- quantization of rows ------------------------------------------------------------------------
-// scale = absmax / 127, q = rint(x * (127 / absmax)) in fp32 (COL: of x times a scale per column). Rows
-// whose largest magnitude is below 2^-120 count as zeros; a row that holds an infinity or NaN gets the
-// scale NaN and zeros, so that its products are NaN. THREADS threads a row, which stays in their registers
-// between its maximum and its rounding (R groups of eight a thread), or is read again (R = 0).
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-
-template <int DT, bool COL>
-__device__ __forceinline__ float8_t quant_load(const Int8QuantArgs& a, int64_t row, int col) {
-    const typename Elem<DT>::type* p = (const typename Elem<DT>::type*)a.x + row * a.ldx + col;
-    float8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (col + 8 <= a.k) {
-        v = load8<DT>(p);
-        if constexpr (COL) v = v * load8<DK_FP32>(a.col_scale + col);
-    } else {
+// The same with x as it comes (fp16, bf16 or fp32): every work-group quantizes the few rows for itself
+// (they come from the L2) into LDS while its first weights are on their way, which saves the launch of the
+// quantizer and its round trip. Rows m <= 16 with m * k bytes of LDS.
+template <int DT, int WAVES, int OUT>
+__global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8GemmArgs a, const Int8QuantArgs q) {
+    constexpr int U = 8;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    __shared__ int red[WAVES][256];
+    __shared__ uint32_t tops[WAVES];
+    __shared__ float scales[16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = 16 * blockIdx.x, l16 = lane & 15, c = 16 * (lane >> 4);
+    const int cols = (a.k + 63) / 64, share = (cols + WAVES - 1) / WAVES;
+    const int begin = wave * share, end = min(cols, begin + share);
+    const int8_t* const w = a.w + (int64_t)min(n0 + l16, a.n - 1) * a.ldw + c;
+    int4_t wf[U];
+    const auto fetch = [&](int b) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (col + e < a.k) v[e] = COL ? (float)p[e] * a.col_scale[col + e] : (float)p[e];
-    }
-    return v;
-}
-
-__device__ __forceinline__ uint32_t top8(float8_t v, uint32_t top) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, abs_bits(v[e]));
-    return top;
-}
-
-__device__ __forceinline__ u32x2_t quant8(float8_t v, float inv) {
-    u32x2_t o = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e / 4] |= ((uint32_t)(int)__builtin_rintf(v[e] * inv) & 0xFFu) << (8 * (e & 3));
-    return o;
-}
-
-template <int DT, bool COL, int THREADS, int R>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void int8_quantize_kernel(const Int8QuantArgs a) {
-    constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, ROWS = BLOCK / THREADS, NW = THREADS / 64;
-    __shared__ uint32_t tops[NW];
-    const int tid = threadIdx.x % THREADS;
-    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
-    if (THREADS == 64 && row >= a.rows) return;  // whole waves; larger groups have one row a work-group
-    const int groups = (a.k + 7) / 8, padded = (a.k + 15) / 16 * 2;
-    float8_t v[R > 0 ? R : 1];
-    uint32_t top = 0;
-    if constexpr (R > 0) {
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int q = tid + i * THREADS;
-            if (q < groups) v[i] = quant_load<DT, COL>(a, row, 8 * q);
-            else v[i] = float8_t{0, 0, 0, 0, 0, 0, 0, 0};
+        for (int u = 0; u < U; ++u) {
+            const int k = 64 * (b + u);
+            wf[u] = b + u < end && k + c < a.k ? *(const int4_t*)(w + k) : int4_t{0, 0, 0, 0};
         }
+    };
+    fetch(begin);
+    const int ld = 64 * cols, groups = ld / 8;  // LDS rows, zeros past k
+    for (int m = 0; m < a.m; ++m) {
+        uint32_t top = 0;
+        for (int g = threadIdx.x; 8 * g < a.k; g += 64 * WAVES) top = top8(quant_load<DT, false>(q, m, 8 * g), top);
 #pragma unroll
-        for (int i = 0; i < R; ++i) top = top8(v[i], top);
-    } else {
-        for (int q = tid; q < groups; q += THREADS) top = top8(quant_load<DT, COL>(a, row, 8 * q), top);
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o));
-    if constexpr (NW > 1) {
-        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+        for (int o = 1; o < 64; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+        if (lane == 0) tops[wave] = top;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NW; ++i) top = max(top, tops[i]);
+        for (int i = 0; i < WAVES; ++i) top = max(top, tops[i]);
+        float inv, scale;
+        quant_scale(top, inv, scale);
+        if (threadIdx.x == 0) scales[m] = scale;
+        for (int g = threadIdx.x; g < groups; g += 64 * WAVES) {
+            float8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (8 * g < a.k) v = quant_load<DT, false>(q, m, 8 * g);
+            *(u32x2_t*)(smem + m * ld + 8 * g) = inv == 0.0f ? u32x2_t{0, 0} : quant8(v, inv);
+        }
+        __syncthreads();
     }
-    const float most = __uint_as_float(top);
-    const bool bad = top >= 0x7F800000u, none = most < 7.523163845262640e-37f;  // 2^-120
-    const float inv = bad || none ? 0.0f : 127.0f / most;
-    if (tid == 0) a.scale[row] = bad ? __builtin_nanf("") : none ? 0.0f : most / 127.0f;
-    int8_t* const out = a.q + row * a.ldq;
-    if constexpr (R > 0) {
+    const uint8_t* const x = smem + min(l16, a.m - 1) * ld + c;
+    int4_t acc = {0, 0, 0, 0};
+    for (int b = begin; b < end; b += U) {
+        if (b != begin) fetch(b);
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int q = tid + i * THREADS;
-            if (q < padded) *(u32x2_t*)(out + 8 * q) = bad ? u32x2_t{0, 0} : quant8(v[i], inv);
-        }
-    } else {
-        for (int q = tid; q < padded; q += THREADS) {
-            const float8_t x = q < groups ? quant_load<DT, COL>(a, row, 8 * q) : float8_t{0, 0, 0, 0, 0, 0, 0, 0};
-            *(u32x2_t*)(out + 8 * q) = bad ? u32x2_t{0, 0} : quant8(x, inv);
-        }
+        for (int u = 0; u < U; ++u)
+            if (b + u < end) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], lds128(x + 64 * (b + u)), acc, 0, 0, 0);
     }
-}
-
-template <int DT, bool COL>
-static void launch_quantize_typed(const Int8QuantArgs& a, hipStream_t s) {
-    const int groups = (a.k + 15) / 16 * 2;
-    const unsigned rows = (unsigned)a.rows;
-    if (groups <= 64 * 4)
-        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 64, 4>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
-    else if (groups <= 256 * 2)
-        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 256, 2>), dim3(rows), dim3(256), 0, s, a);
-    else if (groups <= 256 * 4)
-        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 256, 4>), dim3(rows), dim3(256), 0, s, a);
-    else if (groups <= 512 * 5)
-        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 512, 5>), dim3(rows), dim3(512), 0, s, a);
-    else
-        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 512, 0>), dim3(rows), dim3(512), 0, s, a);
-}
-
-hipError_t launch_int8_quantize(const Int8QuantArgs& a, int dtype, hipStream_t s) {
-    if (a.rows == 0) return hipSuccess;
-    const bool col = a.col_scale != nullptr;
-    if (dtype == DK_FP16)
-        col ? launch_quantize_typed<DK_FP16, true>(a, s) : launch_quantize_typed<DK_FP16, false>(a, s);
-    else if (dtype == DK_BF16)
-        col ? launch_quantize_typed<DK_BF16, true>(a, s) : launch_quantize_typed<DK_BF16, false>(a, s);
-    else
-        col ? launch_quantize_typed<DK_FP32, true>(a, s) : launch_quantize_typed<DK_FP32, false>(a, s);
-    return hipGetLastError();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) red[wave][l16 * 16 + 4 * (lane >> 4) + r] = acc[r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * a.m; i += 64 * WAVES) {
+        const int m = i >> 4, n = n0 + (i & 15);
+        if (n >= a.n) continue;
+        int v = 0;
+#pragma unroll
+        for (int s = 0; s < WAVES; ++s) v += red[s][i];
+        float f = (float)v * scales[m] * a.ws[n];
+        if (a.bias != nullptr) f += load_any(a.bias, a.bias_dtype, n);
+        store1<OUT>((typename Elem<OUT>::type*)a.y + (int64_t)m * a.ldy + n, f);
+    }
 }
 
 // ---- launches ------------------------------------------------------------------------------------
 
-Int8Plan int8_plan(int64_t m, int64_t n, int64_t k, bool tr) {
+static Int8Plan make_plan(int64_t m, int64_t n, int64_t k, int cus) {
     Int8Plan best{};
-    if (m <= 0 || n <= 0) return best;
-    if (!tr && m <= kInt8FewM) {
-        best.few = true;
-        best.splits = 1;
-        return best;
-    }
-    const int cus = device_cus();
     const int64_t steps = (k + kI8BK - 1) / kI8BK > 0 ? (k + kI8BK - 1) / kI8BK : 1;
     double best_us = 0;
-    // microseconds a step of a work-group, by tile height
+    // microseconds a step of a work-group, by tile height (measured: [830, 1536] x 8960 transposed at 1 to
+    // 8 splits takes within 2 us of the estimate on 128 tokens, 3 on 64)
     const int tms[3] = {256, 128, 64};
-    const double step_us[3] = {1.15, 0.65, 0.45};
+    const double step_us[3] = {1.2, 0.68, 0.43};
     for (int v = 0; v < 3; ++v) {
         const int64_t mt = (m + tms[v] - 1) / tms[v], nt = (n + kI8BN - 1) / kI8BN, tiles = mt * nt;
         for (int64_t sp = 1; sp <= steps && sp <= 32; ++sp) {
@@ -527,8 +642,8 @@ Int8Plan int8_plan(int64_t m, int64_t n, int64_t k, bool tr) {
             if ((steps + sps - 1) / sps != sp) continue;
             const int64_t rounds = (tiles * sp + cus - 1) / cus;
             const int64_t ldp = (n + 3) / 4 * 4;
-            double us = 6.0 + rounds * (sps * step_us[v] + 3.0);
-            if (sp > 1) us += 3.0 + 8.0 * sp * m * ldp / 5.0e6;  // partials written and read back
+            double us = 3.0 + rounds * (sps * step_us[v] + 1.5);
+            if (sp > 1) us += 5.0 + 8.0 * sp * m * ldp / 5.0e6;  // partials written and read back
             if (sp > 1 && sp * m * ldp * 4 > (int64_t(1) << 30)) continue;
             if (best_us == 0 || us < best_us) {
                 best_us = us;
@@ -542,6 +657,27 @@ Int8Plan int8_plan(int64_t m, int64_t n, int64_t k, bool tr) {
         }
     }
     return best;
+}
+
+Int8Plan int8_plan(int64_t m, int64_t n, int64_t k, bool tr) {
+    Int8Plan few{};
+    if (m <= 0 || n <= 0) return few;
+    if (!tr && m <= kInt8FewM) {
+        few.few = true;
+        few.splits = 1;
+        return few;
+    }
+    // a call asks twice (workspace, launch) and a model asks for the same few sizes: the last ones are kept
+    struct Kept {
+        int64_t m, n, k;
+        int cus;
+        Int8Plan p;
+    };
+    thread_local Kept kept[16] = {};
+    const int cus = device_cus();
+    Kept& e = kept[(uint64_t)(m * 31 + n * 7 + k) % 16];
+    if (e.m != m || e.n != n || e.k != k || e.cus != cus) e = Kept{m, n, k, cus, make_plan(m, n, k, cus)};
+    return e.p;
 }
 
 template <int TM, bool TR, int OUT>
@@ -575,6 +711,35 @@ static void launch_few(const Int8GemmArgs& a, int out, unsigned grid, hipStream_
         hipLaunchKernelGGL((int8_few_kernel<MT, WAVES, DK_BF16>), dim3(grid), b, 0, s, a);
     else
         hipLaunchKernelGGL((int8_few_kernel<MT, WAVES, DK_FP32>), dim3(grid), b, 0, s, a);
+}
+
+template <int DT, int WAVES>
+static void launch_few_fused(const Int8GemmArgs& a, const Int8QuantArgs& q, int out, unsigned grid, hipStream_t s) {
+    const size_t lds = (size_t)a.m * ((a.k + 63) / 64) * 64;
+    const dim3 b(64 * WAVES);
+    if (out == DK_FP16)
+        hipLaunchKernelGGL((int8_few_fused_kernel<DT, WAVES, DK_FP16>), dim3(grid), b, lds, s, a, q);
+    else if (out == DK_BF16)
+        hipLaunchKernelGGL((int8_few_fused_kernel<DT, WAVES, DK_BF16>), dim3(grid), b, lds, s, a, q);
+    else
+        hipLaunchKernelGGL((int8_few_fused_kernel<DT, WAVES, DK_FP32>), dim3(grid), b, lds, s, a, q);
+}
+
+bool int8_fused(int64_t m, int64_t k, bool tr) {
+    return !tr && m <= kInt8FusedM && m * ((k + 63) / 64) * 64 <= kInt8FusedLds;
+}
+
+hipError_t launch_int8_fused(const Int8GemmArgs& a, const Int8QuantArgs& q, int x_dtype, int out_dtype, hipStream_t s) {
+    if (a.m == 0 || a.n == 0) return hipSuccess;
+    const unsigned grid = (unsigned)((a.n + 15) / 16);
+    const bool wide = grid < 512;
+    if (x_dtype == DK_FP16)
+        wide ? launch_few_fused<DK_FP16, 16>(a, q, out_dtype, grid, s) : launch_few_fused<DK_FP16, 4>(a, q, out_dtype, grid, s);
+    else if (x_dtype == DK_BF16)
+        wide ? launch_few_fused<DK_BF16, 16>(a, q, out_dtype, grid, s) : launch_few_fused<DK_BF16, 4>(a, q, out_dtype, grid, s);
+    else
+        wide ? launch_few_fused<DK_FP32, 16>(a, q, out_dtype, grid, s) : launch_few_fused<DK_FP32, 4>(a, q, out_dtype, grid, s);
+    return hipGetLastError();
 }
 
 hipError_t launch_int8_gemm(Int8GemmArgs a, const Int8Plan& p, int out_dtype, bool tr, hipStream_t s) {

@@ -12,13 +12,17 @@ elements are +0 whatever they held. Branch b of a call at offset o is branch 0 o
 call with n branches uses up n offsets.
 """
 
-import ctypes
+import struct
 
 import torch
 
-from ._lib import DTYPES, check, gpu_tensors, lib, on_device, ptr, stream_of
+from ._lib import DTYPES, call_on, gpu_input, lib, same_gpu
 
 MAX_BRANCHES = 4
+# arrays of 1 to 4 host values, as the C entries take them
+_DOUBLES = [None] + [struct.Struct(f"{n}d").pack for n in range(1, MAX_BRANCHES + 1)]
+_POINTERS = [None] + [struct.Struct(f"{n}P").pack for n in range(1, MAX_BRANCHES + 1)]
+_LONGS = [None] + [struct.Struct(f"{n}q").pack for n in range(1, MAX_BRANCHES + 1)]
 
 
 def rng_state(seed, offset=0, device="cuda"):
@@ -35,70 +39,70 @@ def _signed(v):
 def _rows(t):
     """[rows, width] view (a copy only where the rows have no common stride)."""
     t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
-    if t2.stride(-1) == 1 or t2.shape[-1] == 1:
-        if t2.stride(0) >= 0:
-            return t2
-    return t2.contiguous()
+    if t2.stride(1) != 1 and t2.shape[1] != 1 or t2.stride(0) < 0:
+        t2 = t2.contiguous()
+    return t2
 
 
 def _common(what, t, rng, ps, dtype):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{what}: needs GPU tensors")
+    """(device, packed probabilities, type codes of t and dtype)."""
+    dev = gpu_input(what, t)
+    same_gpu(what, dev, rng)
     if t.dim() < 1:
         raise ValueError(f"{what}: needs a last axis")
-    gpu_tensors(what, t.device, rng=rng)
     if rng is None or rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous():
         raise ValueError(f"{what}: rng must hold two contiguous int64 values, seed and offset")
     if not 1 <= len(ps) <= MAX_BRANCHES:
         raise ValueError(f"{what}: 1 to {MAX_BRANCHES} branches")
-    if t.dtype not in DTYPES or dtype not in DTYPES:
+    a, b = DTYPES.get(t.dtype), DTYPES.get(dtype)
+    if a is None or b is None:
         raise ValueError(f"{what}: fp16, bf16 or fp32 only")
-    if dtype != t.dtype and torch.float32 not in (dtype, t.dtype):
+    if a != b and a != 2 and b != 2:
         raise ValueError(f"{what}: types must be equal, or one of them fp32")
-    return (ctypes.c_double * len(ps))(*(float(p) for p in ps))
+    return dev, _DOUBLES[len(ps)](*ps), a, b
 
 
 def dropout_forward(x, rng, ps, dtype=None):
     """The dropped-out x of each branch: tuple of tensors of x's shape and `dtype` (default x's),
     branch b with drop probability ps[b], from one read of x. x fp16, bf16 or fp32 [.., W]."""
-    dtype = x.dtype if dtype is None else dtype
-    p = _common("dropout_forward", x, rng, ps, dtype)
+    dtype = dtype or getattr(x, "dtype", None)
+    dev, p, a, b = _common("dropout_forward", x, rng, ps, dtype)
     x2 = _rows(x)
     rows, width = x2.shape
     n = len(ps)
-    outs = tuple(torch.empty(x.shape, dtype=dtype, device=x.device) for _ in range(n))
-    ptrs = (ctypes.c_void_p * n)(*(o.data_ptr() for o in outs))
-    lds = (ctypes.c_int64 * n)(*([width] * n))
-    with on_device(x.device):
-        check(lib().dk_dropout_fwd(ptr(x2), DTYPES[x.dtype], x2.stride(0), ptr(rng), p, n, ptrs, DTYPES[dtype], lds,
-                                   rows, width, stream_of(x.device)))
+    outs = tuple([x.new_empty(x.shape, dtype=dtype) for _ in ps])
+    call_on(dev, lib().dk_dropout_fwd, x2.data_ptr(), a, x2.stride(0), rng.data_ptr(), p, n,
+            _POINTERS[n](*[o.data_ptr() for o in outs]), b, _LONGS[n](*[width] * n), rows, width)
     return outs
 
 
 def dropout_backward(grads, rng, ps, dtype=None):
     """dx = sum of the branches' gradients through the masks of dropout_forward(x, rng, ps), summed in
     fp32 and rounded once to `dtype` (default the gradients'). A gradient may be None (zeros)."""
-    given = [g for g in grads if g is not None]
-    if len(grads) != len(ps) or not given:
-        raise ValueError("dropout_backward: one gradient a branch, at least one of them not None")
-    g0 = given[0]
-    dtype = g0.dtype if dtype is None else dtype
-    p = _common("dropout_backward", g0, rng, ps, dtype)
-    n = len(ps)
-    rows2 = []
+    what = "dropout_backward"
+    g0 = next((g for g in grads if g is not None), None)
+    if len(grads) != len(ps) or g0 is None:
+        raise ValueError(f"{what}: one gradient a branch, at least one of them not None")
+    dev, p, a, b = _common(what, g0, rng, ps, dtype or getattr(g0, "dtype", None))
+    dtype = dtype or g0.dtype
+    rows2, ptrs, lds = [], [], []
     for g in grads:
-        if g is not None:
-            gpu_tensors("dropout_backward", g0.device, grad=g)
-            if g.dtype != g0.dtype or g.shape != g0.shape:
-                raise ValueError("dropout_backward: gradients must have one shape and type")
-        rows2.append(None if g is None else _rows(g))
-    rows, width = next(g for g in rows2 if g is not None).shape
-    dx = torch.empty(g0.shape, dtype=dtype, device=g0.device)
-    ptrs = (ctypes.c_void_p * n)(*(None if g is None else g.data_ptr() for g in rows2))
-    lds = (ctypes.c_int64 * n)(*(0 if g is None else g.stride(0) for g in rows2))
-    with on_device(g0.device):
-        check(lib().dk_dropout_bwd(ptrs, DTYPES[g0.dtype], lds, ptr(rng), p, n, ptr(dx), DTYPES[dtype], width, rows,
-                                   width, stream_of(g0.device)))
+        if g is None:
+            ptrs.append(0)
+            lds.append(0)
+            continue
+        same_gpu(what, dev, g)
+        if g.dtype != g0.dtype or g.shape != g0.shape:
+            raise ValueError(f"{what}: gradients must have one shape and type")
+        g2 = _rows(g)
+        rows2.append(g2)
+        ptrs.append(g2.data_ptr())
+        lds.append(g2.stride(0))
+    rows, width = rows2[0].shape
+    n = len(ps)
+    dx = g0.new_empty(g0.shape, dtype=dtype)
+    call_on(dev, lib().dk_dropout_bwd, _POINTERS[n](*ptrs), a, _LONGS[n](*lds), rng.data_ptr(), p, n, dx.data_ptr(), b,
+            width, rows, width)
     return dx
 
 

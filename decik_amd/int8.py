@@ -13,12 +13,11 @@ Quantized rows are padded to 128 bytes; the tensors here are views of the padded
 
 import torch
 
-from ._lib import DTYPES, check, gpu_tensors, lib, on_device, ptr, stream_of
+from ._lib import DTYPES, call_on, gpu_input, lib, same_gpu
 
 
-def _padded(rows, k, device):
-    """int8 [rows, k] view of rows padded to a multiple of 128."""
-    return torch.empty((rows, (k + 127) // 128 * 128), dtype=torch.int8, device=device)[:, :k]
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _token_rows(x):
@@ -26,28 +25,35 @@ def _token_rows(x):
     return x2 if (x2.stride(1) == 1 or x2.shape[1] == 1) and x2.stride(0) >= 0 else x2.contiguous()
 
 
+def _code(what, name, dtype):
+    code = DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"{what}: {name} must be fp16, bf16 or fp32")
+    return code
+
+
 def quantize_int8(x, col_scale=None):
     """(q int8 [rows, K], scale fp32 [rows]) of x [.., K] (fp16, bf16 or fp32) row by row: scale = absmax
     / 127, q = rint(x * (127 / absmax)); col_scale fp32 [K] multiplies x first. For a weight [N, K] the rows
     are its output channels. A row with an infinity or NaN gets the scale NaN."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise ValueError("quantize_int8: needs GPU tensors")
-    if x.dim() < 1 or x.dtype not in DTYPES:
-        raise ValueError("quantize_int8: x must be fp16, bf16 or fp32 [.., K]")
-    dev = x.device
+    what = "quantize_int8"
+    dev = gpu_input(what, x)
+    same_gpu(what, dev, col_scale)
+    code = _code(what, "x", x.dtype)
+    if x.dim() < 1:
+        raise ValueError(f"{what}: x must be [.., K]")
     x2 = _token_rows(x)
     rows, k = x2.shape
     if col_scale is not None:
-        gpu_tensors("quantize_int8", dev, col_scale=col_scale)
         if tuple(col_scale.shape) != (k,) or col_scale.dtype != torch.float32:
-            raise ValueError(f"quantize_int8: col_scale must be fp32 [{k}]")
+            raise ValueError(f"{what}: col_scale must be fp32 [{k}]")
         col_scale = col_scale.contiguous()
-    q = _padded(rows, k, dev)
-    scale = torch.empty(rows, dtype=torch.float32, device=dev)
-    with on_device(dev):
-        check(lib().dk_int8_quantize(ptr(x2), DTYPES[x.dtype], x2.stride(0), ptr(col_scale), ptr(q), q.stride(0),
-                                     ptr(scale), rows, k, stream_of(dev)))
-    return q, scale
+    ld = (k + 127) // 128 * 128
+    q = x.new_empty((rows, ld), dtype=torch.int8)
+    scale = x.new_empty(rows, dtype=torch.float32)
+    call_on(dev, lib().dk_int8_quantize, x2.data_ptr(), code, x2.stride(0), _ptr(col_scale), q.data_ptr(), ld,
+            scale.data_ptr(), rows, k)
+    return q[:, :k], scale
 
 
 def dequantize_int8(q, scale, dtype=torch.float32):
@@ -56,104 +62,121 @@ def dequantize_int8(q, scale, dtype=torch.float32):
 
 
 def _int8_rows(what, name, q, zero_tail):
-    """q, or a padded copy where its rows do not start at multiples of 16 bytes or its storage ends inside
-    the last 16 (zero_tail: the padding must hold zeros, so only quantize_int8's own rows pass)."""
+    """(q, its row stride), or a padded copy where its rows do not start at multiples of 16 bytes or its
+    storage ends inside the last 16 (zero_tail: the padding must hold zeros, so only rows without any pass)."""
     if q.dim() != 2 or q.dtype != torch.int8:
         raise ValueError(f"{what}: {name} must be int8 [rows, columns]")
     rows, k = q.shape
-    ld, need = q.stride(0) if rows > 1 else (k + 15) // 16 * 16, (k + 15) // 16 * 16
-    end = q.storage_offset() + max(rows - 1, 0) * q.stride(0) + need
-    if (q.stride(1) == 1 or k == 1) and ld % 16 == 0 and need <= ld < 2 ** 23 and q.data_ptr() % 16 == 0 and \
-            end <= q.untyped_storage().nbytes() and (not zero_tail or k == need):
+    need = (k + 15) // 16 * 16
+    ld = q.stride(0) if rows > 1 else need
+    if ld % 16 == 0 and need <= ld < 2 ** 23 and (q.stride(1) == 1 or k == 1) and q.data_ptr() % 16 == 0 and \
+            q.storage_offset() + max(rows - 1, 0) * ld + need <= q.untyped_storage().nbytes() and \
+            (not zero_tail or k == need):
         return q, ld
     copy = torch.zeros((rows, need), dtype=torch.int8, device=q.device)
     copy[:, :k] = q
     return copy, need
 
 
-def _product(what, transposed, xq, ldx, xs, wq, ws, bias, dtype, m, n, k):
-    dev = xq.device
-    gpu_tensors(what, dev, x_scale=xs, wq=wq, w_scale=ws, bias=bias)
-    if dtype not in DTYPES:
-        raise ValueError(f"{what}: fp16, bf16 or fp32 outputs only")
-    wq, ldw = _int8_rows(what, "wq", wq, False)
-    if bias is not None and (tuple(bias.shape) != (n,) or bias.dtype not in DTYPES):
-        raise ValueError(f"{what}: bias must be fp16, bf16 or fp32 [{n}]")
-    if ws is not None and (tuple(ws.shape) != (n,) or ws.dtype != torch.float32):
+def _channel_args(what, ws, bias, n):
+    if ws.shape != (n,) or ws.dtype != torch.float32:
         raise ValueError(f"{what}: w_scale must be fp32 [{n}]")
-    bias = None if bias is None else bias.contiguous()
-    ws = None if ws is None else ws.contiguous()
-    y = torch.empty((m, n), dtype=dtype, device=dev)
-    with on_device(dev):
-        need = lib().dk_int8_linear_workspace(transposed, m, n, k)
-        # a tensor of its own a call: graphs and streams share none
-        work = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-        check(lib().dk_int8_linear(transposed, ptr(xq), ldx, ptr(xs), ptr(wq), ldw, ptr(ws), ptr(bias),
-                                   0 if bias is None else DTYPES[bias.dtype], ptr(y), DTYPES[dtype], n, m, n, k,
-                                   ptr(work), max(need, 0), stream_of(dev)))
-    return y
+    if bias is None:
+        return ws.contiguous(), None, 0
+    if bias.shape != (n,):
+        raise ValueError(f"{what}: bias must be [{n}]")
+    return ws.contiguous(), bias.contiguous(), _code(what, "bias", bias.dtype)
+
+
+def _workspace(x, need):
+    # a tensor of its own a call: graphs and streams share none
+    return x.new_empty(need, dtype=torch.uint8) if need > 0 else None
 
 
 def int8_matmul(xq, x_scale, wq, w_scale, bias=None, dtype=torch.float16):
     """y [M, N] = (xq . wq^T) * x_scale * w_scale (+ bias) of int8 xq [M, K] and wq [N, K] with fp32 scales
-    [M] and [N]; K <= 131071. Rows that do not start at multiples of 16 bytes are copied first."""
+    [M] and [N]; K <= 131071. Rows that do not start at multiples of 16 bytes, or of xq whose K is not one,
+    are copied first."""
     what = "int8_matmul"
-    if not isinstance(xq, torch.Tensor) or not xq.is_cuda:
-        raise ValueError(f"{what}: needs GPU tensors")
-    gpu_tensors(what, xq.device, wq=wq)
+    dev = gpu_input(what, xq)
+    same_gpu(what, dev, x_scale, wq, w_scale, bias)
     if xq.dim() != 2 or wq.dim() != 2 or xq.shape[1] != wq.shape[1]:
         raise ValueError(f"{what}: xq [M, K] and wq [N, K] must share K")
     m, k = xq.shape
-    if tuple(x_scale.shape) != (m,) or x_scale.dtype != torch.float32:
+    n = wq.shape[0]
+    if x_scale.shape != (m,) or x_scale.dtype != torch.float32:
         raise ValueError(f"{what}: x_scale must be fp32 [{m}]")
+    out = _code(what, "dtype", dtype)
     xq, ldx = _int8_rows(what, "xq", xq, True)
-    return _product(what, 0, xq, ldx, x_scale.contiguous(), wq, w_scale, bias, dtype, m, wq.shape[0], k)
+    wq, ldw = _int8_rows(what, "wq", wq, False)
+    x_scale = x_scale.contiguous()
+    ws, bias, bias_code = _channel_args(what, w_scale, bias, n)
+    y = xq.new_empty((m, n), dtype=dtype)
+    need = lib().dk_int8_linear_workspace(0, m, n, k)
+    work = _workspace(xq, need)
+    call_on(dev, lib().dk_int8_linear, 0, xq.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(),
+            _ptr(bias), bias_code, y.data_ptr(), out, n, m, n, k, _ptr(work), max(need, 0))
+    return y
 
 
 def int8_linear_forward(x, wq, w_scale, bias=None, dtype=None):
     """y [.., N] (x's type, or dtype) = x . W^T + bias for W held as wq [N, K] int8 and w_scale [N], x [.., K]
     fp16, bf16 or fp32 quantized per token."""
     what = "int8_linear_forward"
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise ValueError(f"{what}: needs GPU tensors")
-    gpu_tensors(what, x.device, wq=wq)
-    if wq.dim() != 2 or x.shape[-1] != wq.shape[1]:
+    dev = gpu_input(what, x)
+    same_gpu(what, dev, wq, w_scale, bias)
+    if wq.dim() != 2 or x.dim() < 1 or x.shape[-1] != wq.shape[1]:
         raise ValueError(f"{what}: x [.., K] and wq [N, K] must share K")
-    n, k = wq.shape
-    xq, xs = quantize_int8(x)
-    y = _product(what, 0, xq, xq.stride(0), xs, wq, w_scale, bias, x.dtype if dtype is None else dtype, xs.shape[0], n,
-                 k)
-    return y.reshape(*x.shape[:-1], n)
+    dtype = dtype or x.dtype
+    code, out = _code(what, "x", x.dtype), _code(what, "dtype", dtype)
+    wq, ldw = _int8_rows(what, "wq", wq, False)
+    n, k = wq.shape[0], x.shape[-1]
+    ws, bias, bias_code = _channel_args(what, w_scale, bias, n)
+    x2 = _token_rows(x)
+    m = x2.shape[0]
+    y = x.new_empty((*x.shape[:-1], n), dtype=dtype)
+    need = lib().dk_int8_linear_x_workspace(0, m, n, k)
+    work = _workspace(x, need)
+    call_on(dev, lib().dk_int8_linear_fwd, x2.data_ptr(), code, x2.stride(0), wq.data_ptr(), ldw, ws.data_ptr(),
+            _ptr(bias), bias_code, y.data_ptr(), out, n, m, n, k, _ptr(work), max(need, 0))
+    return y
 
 
 def int8_linear_backward(dy, wq, w_scale, k=None, dtype=None):
-    """dX [.., K] (dy's type, or dtype) = dY . W, dY * w_scale quantized per token."""
+    """dX [.., K] (dy's type, or dtype) = dY . W, dY * w_scale quantized per token. k, where given, must be
+    the weight's K."""
     what = "int8_linear_backward"
-    if not isinstance(dy, torch.Tensor) or not dy.is_cuda:
-        raise ValueError(f"{what}: needs GPU tensors")
-    gpu_tensors(what, dy.device, wq=wq, w_scale=w_scale)
-    if wq.dim() != 2 or dy.shape[-1] != wq.shape[0] or (k is not None and k != wq.shape[1]):
+    dev = gpu_input(what, dy)
+    same_gpu(what, dev, wq, w_scale)
+    if wq.dim() != 2 or dy.dim() < 1 or dy.shape[-1] != wq.shape[0] or (k is not None and k != wq.shape[1]):
         raise ValueError(f"{what}: dy [.., N] and wq [N, K] must share N")
+    dtype = dtype or dy.dtype
+    code, out = _code(what, "dy", dy.dtype), _code(what, "dtype", dtype)
     n, k = wq.shape
-    gq, gs = quantize_int8(dy, w_scale)
-    dx = _product(what, 1, gq, gq.stride(0), gs, wq, None, None, dy.dtype if dtype is None else dtype, gs.shape[0], k, n)
-    return dx.reshape(*dy.shape[:-1], k)
+    wq, ldw = _int8_rows(what, "wq", wq, False)
+    ws, _, _ = _channel_args(what, w_scale, None, n)
+    dy2 = _token_rows(dy)
+    m = dy2.shape[0]
+    dx = dy.new_empty((*dy.shape[:-1], k), dtype=dtype)
+    need = lib().dk_int8_linear_x_workspace(1, m, n, k)
+    work = _workspace(dy, need)
+    call_on(dev, lib().dk_int8_linear_bwd, dy2.data_ptr(), code, dy2.stride(0), wq.data_ptr(), ldw, ws.data_ptr(),
+            dx.data_ptr(), out, k, m, n, k, _ptr(work), max(need, 0))
+    return dx
 
 
 class Int8Linear(torch.autograd.Function):
-    """apply(x, wq, w_scale, bias) -> y: a linear with a frozen int8 weight; gradients reach x (and bias)."""
+    """apply(x, wq, w_scale, bias) -> y: a linear whose int8 weight and bias are frozen; gradients reach x."""
 
     @staticmethod
     def forward(ctx, x, wq, w_scale, bias=None):
+        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+            raise ValueError("Int8Linear: the weight's scales and the bias are frozen (detach them)")
         ctx.save_for_backward(wq, w_scale)
-        ctx.x_dtype, ctx.bias_dtype = x.dtype, None if bias is None else bias.dtype
+        ctx.x_dtype = x.dtype
         return int8_linear_forward(x, wq, w_scale, bias)
 
     @staticmethod
     def backward(ctx, grad):
         wq, w_scale = ctx.saved_tensors
-        dx = int8_linear_backward(grad, wq, w_scale, dtype=ctx.x_dtype) if ctx.needs_input_grad[0] else None
-        db = None
-        if ctx.needs_input_grad[3]:
-            db = grad.reshape(-1, grad.shape[-1]).sum(0, dtype=torch.float32).to(ctx.bias_dtype)
-        return dx, None, None, db
+        return int8_linear_backward(grad, wq, w_scale, dtype=ctx.x_dtype), None, None, None

@@ -15,12 +15,9 @@ Both take q and k token-major (strided rows of a packed projection output as the
 and give them head-major [B, H, T, D]; everything is computed in fp32 and rounded once.
 """
 
-import ctypes
-
 import torch
 
-from . import _lib
-from ._lib import DTYPES, check, gpu_tensors, lib, on_device, ptr, stream_of
+from ._lib import DTYPES, QkRope, call_on, check, gpu_input, lib, ptr, same_gpu, stream_of
 
 
 def _rows(t):
@@ -78,141 +75,132 @@ class FusedQKRope(torch.autograd.Function):
         return dq, dq.clone() if ctx.needs_input_grad[1] else None, dk, None, None, None, None
 
 
-def _token_rows(what, name, t, heads, d):
+_QK_TYPES = {torch.float16: 0, torch.bfloat16: 1}
+
+
+def _token_rows(what, t, heads, d):
     """(tensor whose [B * T] rows have one stride, that stride, B, T) of a [B, T, H * D] or [T, H * D] tensor."""
-    if t.dim() not in (2, 3) or t.shape[-1] != heads * d:
-        raise ValueError(f"{what}: {name} must be [B, T, {heads * d}] or [T, {heads * d}], not {tuple(t.shape)}")
-    b, n = (1, t.shape[0]) if t.dim() == 2 else t.shape[:2]
+    shape, width = t.shape, heads * d
+    if len(shape) not in (2, 3) or shape[-1] != width:
+        raise ValueError(f"{what}: q and k must be [B, T, H * D] or [T, H * D], here H * D = {width}, not {tuple(shape)}")
+    b, n = (1, shape[0]) if len(shape) == 2 else shape[:2]
     row = t.stride(-2)
-    if t.stride(-1) != 1 or (n > 1 and row < heads * d) or (b > 1 and t.stride(0) != n * row):
-        t = t.contiguous()
-        row = t.stride(-2)
-    elif n == 1 and b > 1:
+    if n == 1 and b > 1:
         row = t.stride(0)  # one token a sequence: the rows are the batch entries
-        if row < heads * d:
-            t = t.contiguous()
-            row = heads * d
+    elif b > 1 and t.stride(0) != n * row:
+        row = -1
+    if t.stride(-1) != 1 or (b * n > 1 and row < width):
+        t, row = t.contiguous(), width
     return t, row, b, n
 
 
-def _rotation(what, desc, device, batch, tokens, d, cos=None, sin=None, positions=None, inv_freq=None, sections=None,
-              interleaved=False):
-    """Fill the rotation fields of `desc`; returns the tensors to keep alive."""
-    if cos is not None:
-        gpu_tensors(what, device, cos=cos, sin=sin)
-        keep = []
-        for t in (cos, sin):
-            if t.shape != cos.shape or tuple(t.shape) not in ((tokens, d), (1, tokens, d), (batch, tokens, d)):
-                raise ValueError(f"{what}: cos and sin must be [T, D] or [B, T, D] of T = {tokens}, D = {d}")
-            keep.append(t.to(torch.float32).contiguous())
-        desc.cos, desc.sin = keep[0].data_ptr(), keep[1].data_ptr()
-        desc.table_batch_stride = tokens * d if cos.dim() == 3 and cos.shape[0] > 1 else 0
-        return keep
-    gpu_tensors(what, device, positions=positions, inv_freq=inv_freq)
-    sections = [int(s) for s in sections]
+def _rotation(what, dev, batch, tokens, d, tables, axes):
+    """(cos, sin, positions, inv_freq pointers, strides of tables, axes and batches, axis count, sections,
+    interleaved, int64 positions, the tensors behind the pointers) of a descriptor."""
+    if tables is not None:
+        cos, sin = tables
+        same_gpu(what, dev, cos, sin)
+        if cos.shape != sin.shape or cos.shape not in ((tokens, d), (batch, tokens, d), (1, tokens, d)):
+            raise ValueError(f"{what}: cos and sin must be [T, D] or [B, T, D] of T = {tokens}, D = {d}")
+        cos, sin = cos.to(torch.float32).contiguous(), sin.to(torch.float32).contiguous()
+        own = tokens * d if cos.dim() == 3 and cos.shape[0] > 1 else 0
+        return cos.data_ptr(), sin.data_ptr(), 0, 0, own, 0, 0, 0, (0, 0, 0, 0), 0, 0, (cos, sin)
+    positions, inv_freq, sections, interleaved = axes
+    same_gpu(what, dev, positions, inv_freq)
+    sections = tuple(int(s) for s in sections)
     n = len(sections)
     if not 1 <= n <= 4:
         raise ValueError(f"{what}: 1 to 4 axes")
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what}: positions must be int32 or int64")
-    if tuple(positions.shape) not in ((n, tokens), (n, 1, tokens), (n, batch, tokens)):
+    if positions.shape not in ((n, tokens), (n, batch, tokens), (n, 1, tokens)):
         raise ValueError(f"{what}: positions must be [{n}, T] or [{n}, B, T] of T = {tokens}, B = {batch}, not "
                          f"{tuple(positions.shape)}")
-    if inv_freq.dim() != 1 or inv_freq.numel() != d // 2:
+    if inv_freq.shape != (d // 2,):
         raise ValueError(f"{what}: inv_freq must hold {d // 2} frequencies")
     if positions.stride(-1) != 1 and tokens > 1:
         positions = positions.contiguous()
-    inv = inv_freq.to(torch.float32).contiguous()
-    desc.positions, desc.inv_freq = positions.data_ptr(), inv.data_ptr()
-    desc.positions_int64 = int(positions.dtype == torch.int64)
-    desc.pos_axis_stride = positions.stride(0)
-    desc.pos_batch_stride = positions.stride(1) if positions.dim() == 3 and positions.shape[1] > 1 else 0
-    desc.n_axes, desc.interleaved = n, int(bool(interleaved))
-    for i, s in enumerate(sections):
-        desc.sections[i] = s
-    return [positions, inv]
+    inv_freq = inv_freq.to(torch.float32).contiguous()
+    per_batch = positions.stride(1) if positions.dim() == 3 and positions.shape[1] > 1 else 0
+    return (0, 0, positions.data_ptr(), inv_freq.data_ptr(), 0, positions.stride(0), per_batch, n,
+            sections + (0,) * (4 - n), int(bool(interleaved)), int(positions.dtype == torch.int64),
+            (positions, inv_freq))
 
 
-def _norm_weights(what, desc, device, d, q_weight, k_weight):
+def _norm_weights(what, dev, d, q_weight, k_weight):
+    """(weights, their type code), contiguous; (None, None, 0) without norms."""
     if (q_weight is None) != (k_weight is None):
         raise ValueError(f"{what}: norm weights for both q and k, or for neither")
     if q_weight is None:
-        return []
-    gpu_tensors(what, device, q_weight=q_weight, k_weight=k_weight)
-    if tuple(q_weight.shape) != (d,) or tuple(k_weight.shape) != (d,):
-        raise ValueError(f"{what}: norm weights must be [{d}]")
-    if q_weight.dtype not in DTYPES or k_weight.dtype != q_weight.dtype:
-        raise ValueError(f"{what}: norm weights must share one type, fp16, bf16 or fp32")
-    keep = [q_weight.contiguous(), k_weight.contiguous()]
-    desc.q_weight, desc.k_weight, desc.w_dtype = keep[0].data_ptr(), keep[1].data_ptr(), DTYPES[q_weight.dtype]
-    return keep
+        return None, None, 0
+    same_gpu(what, dev, q_weight, k_weight)
+    code = DTYPES.get(q_weight.dtype)
+    if q_weight.shape != (d,) or k_weight.shape != (d,) or code is None or k_weight.dtype != q_weight.dtype:
+        raise ValueError(f"{what}: norm weights must both be [{d}], of one type, fp16, bf16 or fp32")
+    return q_weight.contiguous(), k_weight.contiguous(), code
 
 
-def _qk_forward(what, q, k, q_weight, k_weight, n_heads, n_kv_heads, eps, d, **rotation):
-    if not isinstance(q, torch.Tensor) or not q.is_cuda:
-        raise ValueError(f"{what}: needs GPU tensors")
-    dev = q.device
-    gpu_tensors(what, dev, k=k)
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype:
+def _descriptor(q, k, gq, gk, oq, ok, weights, dws, rot, lds, b, t, hq, hk, d, code, eps):
+    """dk_qk_rope as packed bytes, its fields in order (None: a NULL pointer)."""
+    at = [0 if v is None else v.data_ptr() for v in (q, k, gq, gk, oq, ok, weights[0], weights[1], *dws)]
+    cos, sin, pos, inv, table_batch, pos_axis, pos_batch, n_axes, sections, interleaved, pos64, _ = rot
+    return QkRope.PACK.pack(*at, cos, sin, pos, inv, *lds, table_batch, pos_axis, pos_batch, b, t, hq, hk, d, code,
+                            weights[2], n_axes, *sections, interleaved, pos64, eps, 0)
+
+
+def _qk_forward(what, q, k, q_weight, k_weight, hq, hk, eps, d, tables=None, axes=None):
+    dev = gpu_input(what, q)
+    same_gpu(what, dev, k)
+    code = _QK_TYPES.get(q.dtype)
+    if code is None or k.dtype != q.dtype:
         raise ValueError(f"{what}: q and k must both be fp16 or both bf16")
-    desc = _lib.QkRope()
-    q, desc.ld_q, b, t = _token_rows(what, "q", q, n_heads, d)
-    k, desc.ld_k, bk, tk = _token_rows(what, "k", k, n_kv_heads, d)
-    if (bk, tk) != (b, t):
+    q, ldq, b, t = _token_rows(what, q, hq, d)
+    k, ldk, bk, tk = _token_rows(what, k, hk, d)
+    if bk != b or tk != t:
         raise ValueError(f"{what}: q and k must have the same tokens")
-    keep = _norm_weights(what, desc, dev, d, q_weight, k_weight)
-    keep += _rotation(what, desc, dev, b, t, d, **rotation)
-    q_out = torch.empty((b, n_heads, t, d), dtype=q.dtype, device=dev)
-    k_out = torch.empty((b, n_kv_heads, t, d), dtype=q.dtype, device=dev)
-    desc.q, desc.k, desc.q_out, desc.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
-    desc.batch, desc.tokens, desc.n_heads, desc.n_kv_heads, desc.head_dim = b, t, n_heads, n_kv_heads, d
-    desc.dtype, desc.eps = DTYPES[q.dtype], eps
-    with on_device(dev):
-        check(lib().dk_qk_rope_fwd(ctypes.byref(desc), stream_of(dev)))
+    weights = _norm_weights(what, dev, d, q_weight, k_weight)
+    rot = _rotation(what, dev, b, t, d, tables, axes)
+    q_out, k_out = q.new_empty((b, hq, t, d)), q.new_empty((b, hk, t, d))
+    call_on(dev, lib().dk_qk_rope_fwd, _descriptor(q, k, None, None, q_out, k_out, weights, (None, None), rot,
+                                                   (ldq, ldk, 0, 0), b, t, hq, hk, d, code, eps))
     return q_out, k_out
 
 
-def _qk_backward(what, grad_q, grad_k, q, k, q_weight, k_weight, eps, weight_grads, **rotation):
-    if not isinstance(grad_q, torch.Tensor) or not grad_q.is_cuda:
-        raise ValueError(f"{what}: needs GPU tensors")
-    dev = grad_q.device
-    gpu_tensors(what, dev, grad_k=grad_k, q=q, k=k)
+def _qk_backward(what, grad_q, grad_k, q, k, q_weight, k_weight, eps, weight_grads, tables=None, axes=None):
+    dev = gpu_input(what, grad_q)
+    same_gpu(what, dev, grad_k, q, k)
     if grad_q.dim() != 4 or grad_k.dim() != 4 or grad_q.shape[0] != grad_k.shape[0] or \
             grad_q.shape[2:] != grad_k.shape[2:]:
         raise ValueError(f"{what}: gradients must be [B, H, T, D] of the same B, T and D")
-    if grad_q.dtype not in (torch.float16, torch.bfloat16) or grad_k.dtype != grad_q.dtype:
+    code = _QK_TYPES.get(grad_q.dtype)
+    if code is None or grad_k.dtype != grad_q.dtype:
         raise ValueError(f"{what}: gradients must both be fp16 or both bf16")
     b, hq, t, d = grad_q.shape
     hk = grad_k.shape[1]
-    desc = _lib.QkRope()
     gq, gk = grad_q.contiguous(), grad_k.contiguous()
-    keep = _norm_weights(what, desc, dev, d, q_weight, k_weight) + [gq, gk]
-    keep += _rotation(what, desc, dev, b, t, d, **rotation)
-    dwq = dwk = None
-    if q_weight is not None:
-        if q is None or k is None or q.dtype != grad_q.dtype or k.dtype != grad_q.dtype:
+    weights = _norm_weights(what, dev, d, q_weight, k_weight)
+    rot = _rotation(what, dev, b, t, d, tables, axes)
+    ldq = ldk = need = 0
+    dws, work = (None, None), None
+    if q_weight is None:
+        q = k = None
+    else:
+        if q is None or k is None or q.dtype != gq.dtype or k.dtype != gq.dtype:
             raise ValueError(f"{what}: norms need q and k again, of the gradients' type")
-        q, desc.ld_q, bq, tq = _token_rows(what, "q", q, hq, d)
-        k, desc.ld_k, bk, tk = _token_rows(what, "k", k, hk, d)
+        q, ldq, bq, tq = _token_rows(what, q, hq, d)
+        k, ldk, bk, tk = _token_rows(what, k, hk, d)
         if (bq, tq) != (b, t) or (bk, tk) != (b, t):
             raise ValueError(f"{what}: q, k and their gradients must have the same tokens")
-        desc.q, desc.k = q.data_ptr(), k.data_ptr()
-        keep += [q, k]
         if weight_grads:
-            dwq, dwk = torch.empty((2, d), dtype=torch.float32, device=dev).unbind()
-            desc.dw_q, desc.dw_k = dwq.data_ptr(), dwk.data_ptr()
-    dq = torch.empty((b, t, hq * d), dtype=gq.dtype, device=dev)
-    dk = torch.empty((b, t, hk * d), dtype=gq.dtype, device=dev)
-    desc.grad_q, desc.grad_k, desc.q_out, desc.k_out = gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr()
-    desc.ld_q_out, desc.ld_k_out = hq * d, hk * d
-    desc.batch, desc.tokens, desc.n_heads, desc.n_kv_heads, desc.head_dim = b, t, hq, hk, d
-    desc.dtype, desc.eps = DTYPES[gq.dtype], eps
-    with on_device(dev):
-        need = lib().dk_qk_rope_bwd_workspace(ctypes.byref(desc))
+            dws = gq.new_empty((2, d), dtype=torch.float32).unbind()
+    dq, dk = gq.new_empty((b, t, hq * d)), gq.new_empty((b, t, hk * d))
+    desc = _descriptor(q, k, gq, gk, dq, dk, weights, dws, rot, (ldq, ldk, hq * d, hk * d), b, t, hq, hk, d, code, eps)
+    if dws[0] is not None:
+        need = lib().dk_qk_rope_bwd_workspace(desc)
         # a tensor of its own a call: graphs and streams share none
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-        check(lib().dk_qk_rope_bwd(ctypes.byref(desc), ptr(ws), max(need, 0), stream_of(dev)))
-    return dq, dk, dwq, dwk
+        work = gq.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    call_on(dev, lib().dk_qk_rope_bwd, desc, None if work is None else work.data_ptr(), max(need, 0))
+    return dq, dk, *dws
 
 
 def qk_norm_rope_forward(q, k, q_weight, k_weight, cos, sin, n_heads, n_kv_heads, eps=1e-6):
@@ -220,14 +208,14 @@ def qk_norm_rope_forward(q, k, q_weight, k_weight, cos, sin, n_heads, n_kv_heads
     q [B, T, H*D] or [T, H*D], k likewise, fp16 or bf16; q_weight, k_weight [D]; cos, sin [T, D] or
     [B, T, D]."""
     return _qk_forward("qk_norm_rope_forward", q, k, q_weight, k_weight, n_heads, n_kv_heads, eps, cos.shape[-1],
-                       cos=cos, sin=sin)
+                       tables=(cos, sin))
 
 
 def qk_norm_rope_backward(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, eps=1e-6, weight_grads=True):
     """(dq [B, T, H*D], dk [B, T, HK*D], dq_weight, dk_weight fp32 [D], None without weight_grads) of
     qk_norm_rope_forward, from head-major gradients of its outputs and the same q and k."""
     return _qk_backward("qk_norm_rope_backward", grad_q, grad_k, q, k, q_weight, k_weight, eps, weight_grads,
-                        cos=cos, sin=sin)
+                        tables=(cos, sin))
 
 
 def axes_rope_forward(q, k, positions, inv_freq, sections, n_heads, n_kv_heads, interleaved=False, q_weight=None,
@@ -238,8 +226,7 @@ def axes_rope_forward(q, k, positions, inv_freq, sections, n_heads, n_kv_heads, 
     axis j % axes while that axis has some left, the others to axis 0). With q_weight and k_weight the
     heads are RMS-normalized first. The angles are exact to 2^-24 turns for positions below 2^28."""
     return _qk_forward("axes_rope_forward", q, k, q_weight, k_weight, n_heads, n_kv_heads, eps,
-                       2 * inv_freq.shape[-1], positions=positions, inv_freq=inv_freq, sections=sections,
-                       interleaved=interleaved)
+                       2 * inv_freq.shape[-1], axes=(positions, inv_freq, sections, interleaved))
 
 
 def axes_rope_backward(grad_q, grad_k, positions, inv_freq, sections, interleaved=False, q=None, k=None, q_weight=None,
@@ -247,7 +234,7 @@ def axes_rope_backward(grad_q, grad_k, positions, inv_freq, sections, interleave
     """(dq, dk, dq_weight, dk_weight) of axes_rope_forward; q and k again where it had norms (the
     weights' gradients are None where it had none, or without weight_grads)."""
     return _qk_backward("axes_rope_backward", grad_q, grad_k, q, k, q_weight, k_weight, eps, weight_grads,
-                        positions=positions, inv_freq=inv_freq, sections=sections, interleaved=interleaved)
+                        axes=(positions, inv_freq, sections, interleaved))
 
 
 def _head_major_grads(ctx, grads, b, t, d):
@@ -262,9 +249,7 @@ class _QkRotation(torch.autograd.Function):
 
     @staticmethod
     def _named(rotation, tensors):
-        if rotation[0] == "tables":
-            return dict(cos=tensors[0], sin=tensors[1])
-        return dict(positions=tensors[0], inv_freq=tensors[1], sections=rotation[1], interleaved=rotation[2])
+        return dict(tables=tensors) if rotation[0] == "tables" else dict(axes=(*tensors, *rotation[1:]))
 
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, heads, eps, rotation, *tensors):

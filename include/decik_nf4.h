@@ -378,6 +378,16 @@ int64_t dk_int8_linear_workspace(int transposed, int64_t m, int64_t n, int64_t k
 int dk_int8_linear(int transposed, const int8_t* xq, int64_t ldx, const float* xs, const int8_t* wq, int64_t ldw,
                    const float* ws, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t m,
                    int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, void* stream);
+/* Both steps in one call: forward y [m, n] = x . W^T + bias from x [m, k] of x_dtype, and the input gradient
+ * dx [m, k] = dY . W from dy [m, n], quantized in the workspace or, a few tokens, inside the product; the same
+ * results as the two calls. workspace: dk_int8_linear_x_workspace(backward, ..) bytes (0: none). */
+int64_t dk_int8_linear_x_workspace(int backward, int64_t m, int64_t n, int64_t k);
+int dk_int8_linear_fwd(const void* x, int x_dtype, int64_t ldx, const int8_t* wq, int64_t ldw, const float* ws,
+                       const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t m, int64_t n,
+                       int64_t k, void* workspace, int64_t workspace_bytes, void* stream);
+int dk_int8_linear_bwd(const void* dy, int dy_dtype, int64_t lddy, const int8_t* wq, int64_t ldw, const float* ws,
+                       void* dx, int dx_dtype, int64_t lddx, int64_t m, int64_t n, int64_t k, void* workspace,
+                       int64_t workspace_bytes, void* stream);
 
 /* out = fp16(silu(gate) * up), computed in fp32 (n elements). */
 int dk_swiglu_fwd(const uint16_t* gate, const uint16_t* up, uint16_t* out, int64_t n,

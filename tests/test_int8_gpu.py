@@ -241,7 +241,9 @@ def test_autograd(device):
 
     wq, ws = quantize_int8(make((130, 96), torch.float32, device, 1, 0.02))
     x = make((2, 33, 96), torch.float16, device, 2).requires_grad_(True)
-    bias = make((130,), torch.float16, device, 3).requires_grad_(True)
+    bias = make((130,), torch.float16, device, 3)
+    with pytest.raises(ValueError, match="frozen"):
+        Int8Linear.apply(x, wq, ws, bias.clone().requires_grad_(True))
     y = Int8Linear.apply(x, wq, ws, bias)
     dy = make(y.shape, torch.float16, device, 4)
     y.backward(dy)
@@ -253,9 +255,6 @@ def test_autograd(device):
     bound = slack * 1.001 + want.abs() * 2.0 ** -11 + slack * 2.0 ** -10 + 2.0 ** -25
     assert bool(((got - want).abs() <= bound).all())
     assert x.grad.dtype == torch.float16
-    db = dy.reshape(66, 130)
-    err = (bias.grad.double() - db.double().sum(0)).abs()
-    assert bool((err <= db.double().sum(0).abs() * 2.0 ** -11 + db.double().abs().sum(0) * 2.0 ** -17).all())
     # the forward along a direction: quantized twice, half a step a term each
     xi, xs = quantized(x.detach().reshape(66, 96))
     lin = torch.from_numpy(xi * xs.astype(np.float64)[:, None]).to(device) @ w.T + bias.double()
