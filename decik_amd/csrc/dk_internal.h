@@ -251,9 +251,10 @@ struct DropoutArgs {
     float scale[kDropoutMaxBranches];
     const int64_t* rng;  // device: seed, offset
     uint32_t width, groups, items;  // groups of eight columns a row, rows * groups
+    uint32_t div_mul, div_shift;    // set by launch_dropout
     int32_t nb;
 };
-hipError_t launch_dropout(const DropoutArgs& a, int in_dtype, int out_dtype, bool backward, hipStream_t s);
+hipError_t launch_dropout(DropoutArgs a, int in_dtype, int out_dtype, bool backward, hipStream_t s);
 
 // Norms and rotation of q and k heads (qk_rope.hip).
 constexpr int kQkMaxWaves = 4096;

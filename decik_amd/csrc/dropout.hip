@@ -30,9 +30,9 @@ __device__ __forceinline__ Philox philox10(uint32_t c0, uint32_t c1, uint32_t c2
 #pragma unroll
     for (int i = 0; i < 10; ++i) {
         const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c0 = __builtin_amdgcn_bitop3_b32((uint32_t)(b >> 32), c1, k0, 0x96);  // a ^ b ^ c
         c1 = (uint32_t)b;
-        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c2 = __builtin_amdgcn_bitop3_b32((uint32_t)(a >> 32), c3, k1, 0x96);
         c3 = (uint32_t)a;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
@@ -79,7 +79,8 @@ template <int IN, int OUT, int NB, bool BWD>
 __global__ __launch_bounds__(kDropoutThreads) void dropout_kernel(const DropoutArgs a) {
     const uint32_t i = blockIdx.x * kDropoutThreads + threadIdx.x;
     if (i >= a.items) return;
-    const uint32_t row = i / a.groups, g = i - row * a.groups;
+    // i / groups by a multiplication (exact for i < 2^31)
+    const uint32_t row = a.groups == 1 ? i : __umulhi(i, a.div_mul) >> a.div_shift, g = i - row * a.groups;
     const uint64_t seed = (uint64_t)a.rng[0], offset = (uint64_t)a.rng[1];
     const auto bits = [&](int b) {
         const uint64_t o = offset + (uint64_t)b;
@@ -150,8 +151,16 @@ static void launch_way(const DropoutArgs& a, int in, int out, unsigned grid, hip
     }
 }
 
-hipError_t launch_dropout(const DropoutArgs& a, int in_dtype, int out_dtype, bool backward, hipStream_t s) {
+hipError_t launch_dropout(DropoutArgs a, int in_dtype, int out_dtype, bool backward, hipStream_t s) {
     if (a.items == 0) return hipSuccess;
+    // i / d = (i m) >> (31 + l), l = ceil(log2 d), m = floor(2^(31 + l) / d) + 1: m d exceeds 2^(31 + l) by
+    // at most d <= 2^l, which times i < 2^31 stays below 2^(31 + l)
+    int l = 0;
+    while ((uint64_t(1) << l) < a.groups) ++l;
+    if (a.groups > 1) {
+        a.div_mul = (uint32_t)((uint64_t(1) << (31 + l)) / a.groups + 1);
+        a.div_shift = (uint32_t)(l - 1);
+    }
     const unsigned grid = (unsigned)(((uint64_t)a.items + kDropoutThreads - 1) / kDropoutThreads);
     if (backward)
         launch_way<true>(a, in_dtype, out_dtype, grid, s);

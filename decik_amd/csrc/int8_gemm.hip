@@ -394,18 +394,24 @@ __global__ __launch_bounds__(256) void int8_reduce_kernel(const Int8GemmArgs a) 
 // between its maximum and its rounding (R groups of eight a thread), or is read again (R = 0).
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-template <int DT, bool COL>
-__device__ __forceinline__ float8_t quant_load(const Int8QuantArgs& a, int64_t row, int col) {
+// eight columns of a row, zeros past the last
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::vec quant_load(const Int8QuantArgs& a, int64_t row, int col) {
     const typename Elem<DT>::type* p = (const typename Elem<DT>::type*)a.x + row * a.ldx + col;
-    float8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (col + 8 <= a.k) {
-        v = load8<DT>(p);
-        if constexpr (COL) v = v * load8<DK_FP32>(a.col_scale + col);
-    } else {
+    if (col + 8 <= a.k) return load8_raw<DT>(p);
+    typename Elem<DT>::vec v = {};
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (col + e < a.k) v[e] = COL ? (float)p[e] * a.col_scale[col + e] : (float)p[e];
-    }
+    for (int e = 0; e < 8; ++e)
+        if (col + e < a.k) v[e] = p[e];
+    return v;
+}
+
+__device__ __forceinline__ float8_t scale_load(const float* s, int col, int k) {
+    if (col + 8 <= k) return load8<DK_FP32>(s + col);
+    float8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (col + e < k) v[e] = s[col + e];
     return v;
 }
 
@@ -415,10 +421,19 @@ __device__ __forceinline__ uint32_t top8(float8_t v, uint32_t top) {
     return top;
 }
 
+// Eight values rounded to integers (to nearest even, |v inv| <= 127): in the sum with 1.5 * 2^23 the fp32 unit
+// is 1, so the addition rounds and the low byte holds the integer in two's complement.
 __device__ __forceinline__ u32x2_t quant8(float8_t v, float inv) {
-    u32x2_t o = {0, 0};
+    uint32_t b[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e / 4] |= ((uint32_t)(int)__builtin_rintf(v[e] * inv) & 0xFFu) << (8 * (e & 3));
+    for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(v[e] * inv + 12582912.0f);
+    u32x2_t o;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t lo = __builtin_amdgcn_perm(b[4 * h + 1], b[4 * h], 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(b[4 * h + 3], b[4 * h + 2], 0x04000c0cu);
+        o[h] = lo | hi;
+    }
     return o;
 }
 
@@ -430,6 +445,8 @@ __device__ __forceinline__ void quant_scale(uint32_t top, float& inv, float& sca
     scale = bad ? __builtin_nanf("") : none ? 0.0f : most / 127.0f;
 }
 
+// The row stays in registers between its maximum and its rounding (R groups of eight a thread), or is read
+// again (R = 0). THREADS threads a row.
 template <int DT, bool COL, int THREADS, int R>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void int8_quantize_kernel(const Int8QuantArgs a) {
     constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, ROWS = BLOCK / THREADS, NW = THREADS / 64;
@@ -438,19 +455,23 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void int8_quantize_k
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / THREADS;
     if (THREADS == 64 && row >= a.rows) return;  // whole waves; larger groups have one row a work-group
     const int groups = (a.k + 7) / 8, padded = (a.k + 15) / 16 * 2;
+    const auto load = [&](int q) {
+        const float8_t v = widen8<DT>(quant_load<DT>(a, row, 8 * q));
+        return COL ? v * scale_load(a.col_scale, 8 * q, a.k) : v;
+    };
     float8_t v[R > 0 ? R : 1];
     uint32_t top = 0;
     if constexpr (R > 0) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int q = tid + i * THREADS;
-            if (q < groups) v[i] = quant_load<DT, COL>(a, row, 8 * q);
+            if (q < groups) v[i] = load(q);
             else v[i] = float8_t{0, 0, 0, 0, 0, 0, 0, 0};
         }
 #pragma unroll
         for (int i = 0; i < R; ++i) top = top8(v[i], top);
     } else {
-        for (int q = tid; q < groups; q += THREADS) top = top8(quant_load<DT, COL>(a, row, 8 * q), top);
+        for (int q = tid; q < groups; q += THREADS) top = top8(load(q), top);
     }
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o));
@@ -472,7 +493,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void int8_quantize_k
         }
     } else {
         for (int q = tid; q < padded; q += THREADS) {
-            const float8_t x = q < groups ? quant_load<DT, COL>(a, row, 8 * q) : float8_t{0, 0, 0, 0, 0, 0, 0, 0};
+            const float8_t x = q < groups ? load(q) : float8_t{0, 0, 0, 0, 0, 0, 0, 0};
             *(u32x2_t*)(out + 8 * q) = inv == 0.0f ? u32x2_t{0, 0} : quant8(x, inv);
         }
     }
@@ -575,17 +596,14 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8Ge
     const int8_t* const w = a.w + (int64_t)min(n0 + l16, a.n - 1) * a.ldw + c;
     int4_t wf[U];
     const auto fetch = [&](int b) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k = 64 * (b + u);
-            wf[u] = b + u < end && k + c < a.k ? *(const int4_t*)(w + k) : int4_t{0, 0, 0, 0};
-        }
+        return b < end && 64 * b + c < a.k ? *(const int4_t*)(w + 64 * b) : int4_t{0, 0, 0, 0};
     };
-    fetch(begin);
+#pragma unroll
+    for (int u = 0; u < U; ++u) wf[u] = fetch(begin + u);
     const int ld = 64 * cols, groups = ld / 8;  // LDS rows, zeros past k
     for (int m = 0; m < a.m; ++m) {
         uint32_t top = 0;
-        for (int g = threadIdx.x; 8 * g < a.k; g += 64 * WAVES) top = top8(quant_load<DT, false>(q, m, 8 * g), top);
+        for (int g = threadIdx.x; 8 * g < a.k; g += 64 * WAVES) top = top8(widen8<DT>(quant_load<DT>(q, m, 8 * g)), top);
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o));
         if (lane == 0) tops[wave] = top;
@@ -597,7 +615,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8Ge
         if (threadIdx.x == 0) scales[m] = scale;
         for (int g = threadIdx.x; g < groups; g += 64 * WAVES) {
             float8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (8 * g < a.k) v = quant_load<DT, false>(q, m, 8 * g);
+            if (8 * g < a.k) v = widen8<DT>(quant_load<DT>(q, m, 8 * g));
             *(u32x2_t*)(smem + m * ld + 8 * g) = inv == 0.0f ? u32x2_t{0, 0} : quant8(v, inv);
         }
         __syncthreads();
@@ -605,10 +623,12 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8Ge
     const uint8_t* const x = smem + min(l16, a.m - 1) * ld + c;
     int4_t acc = {0, 0, 0, 0};
     for (int b = begin; b < end; b += U) {
-        if (b != begin) fetch(b);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (b + u < end) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], lds128(x + 64 * (b + u)), acc, 0, 0, 0);
+        for (int u = 0; u < U; ++u) {
+            if (b + u >= end) break;
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], lds128(x + 64 * (b + u)), acc, 0, 0, 0);
+            wf[u] = fetch(b + u + U);
+        }
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) red[wave][l16 * 16 + 4 * (lane >> 4) + r] = acc[r];

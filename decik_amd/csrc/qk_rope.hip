@@ -205,49 +205,52 @@ __global__ __launch_bounds__(kQkThreads) void qk_rope_kernel(const QkRopeArgs a)
 
     if constexpr (BWD && NORM) {
         if (a.slabs == nullptr) return;
-        // this work-group's sums of dw: over the heads of a wave, then over its waves
-        __shared__ float sums[kQkWaves][2][LPH * 16];
+        // this work-group's sums of dw, over the heads of its waves' passes in order
+        __shared__ float sums[kQkWaves][kWave][17];  // 17: both sides of the exchange spread over the banks
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            const bool mine = active && isq == (side == 0);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float v = mine ? (e < 8 ? da[e & 7] : db[e & 7]) : 0.0f;
-#pragma unroll
-                for (int o = LPH; o < kWave; o *= 2) v += __shfl_xor(v, o);
-                if (lane < LPH) sums[wave][side][(e < 8 ? 0 : LPH * 8) + c + (e & 7)] = v;
-            }
+        for (int e = 0; e < 8; ++e) {
+            sums[wave][lane][e] = active ? da[e] : 0.0f;
+            sums[wave][lane][8 + e] = active ? db[e] : 0.0f;
         }
         __syncthreads();
         for (int i = threadIdx.x; i < 2 * a.d; i += kQkThreads) {
-            const int side = i / a.d, d = i - side * a.d;
-            const int at = d < half ? d : LPH * 8 + d - half;
+            const int side = i >= a.d, d = side ? i - a.d : i, c0 = d < half ? d : d - half;
+            const int at = c0 / 8, e = (d < half ? 0 : 8) + c0 % 8;
             float v = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kQkWaves; ++k) v += sums[k][side][at];
+            for (int k = 0; k < kQkWaves; ++k) {
+                const int first = (blockIdx.x * kQkWaves + k) % a.passes * HPW;
+#pragma unroll
+                for (int h = 0; h < HPW; ++h)
+                    if ((first + h >= a.hq) == side) v += sums[k][h * LPH + at][e];
+            }
             a.slabs[(int64_t)blockIdx.x * 2 * a.d + i] = v;
         }
     }
 }
 
-// dw of q (columns 0 .. d - 1 of a slab) and k (d .. 2 d - 1): slabs added by 64 threads a column,
-// each in slab order, then those in thread order
+// dw of q (columns 0 .. d - 1 of a slab) and k (d .. 2 d - 1): slabs added by 64 threads a column, each in
+// slab order, then those in a fixed order
 constexpr int kSlabCols = 16, kSlabRows = 64;
 __global__ __launch_bounds__(kSlabCols* kSlabRows) void norm_weight_grad_kernel(const float* __restrict__ slabs,
                                                                                 int n, int d, float* dwq,
                                                                                 float* dwk) {
-    __shared__ float part[kSlabRows][kSlabCols + 1];
+    __shared__ float part[kSlabRows / 4][kSlabCols];
     const int cx = threadIdx.x % kSlabCols, ry = threadIdx.x / kSlabCols;
     const int col = blockIdx.x * kSlabCols + cx;
     float v = 0.0f;
-    if (col < 2 * d)
+    if (col < 2 * d) {
+#pragma unroll 4
         for (int i = ry; i < n; i += kSlabRows) v += slabs[(int64_t)i * 2 * d + col];
-    part[ry][cx] = v;
+    }
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
+    if (ry % 4 == 0) part[ry / 4][cx] = v;
     __syncthreads();
     if (ry == 0 && col < 2 * d) {
         float s = 0.0f;
-#pragma unroll 16
-        for (int i = 0; i < kSlabRows; ++i) s += part[i][cx];
+#pragma unroll
+        for (int i = 0; i < kSlabRows / 4; ++i) s += part[i][cx];
         (col < d ? dwq : dwk)[col < d ? col : col - d] = s;
     }
 }
