@@ -176,29 +176,35 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
         xoff[i] = r * (uint32_t)a.ldx + xcol[i];
     }
 
-    // loads of step t into its stage; past the last step they read nothing (and write zeros nobody reads),
-    // which keeps the number of loads in flight the same for every wait
-    const auto fetch = [&](int t) {
-        uint8_t* const st = smem + (t % S) * STAGE;
+    // where the loads of step t come from and go to; past the last step they read nothing (and write zeros
+    // nobody reads), which keeps the number of loads in flight the same for every wait
+    struct Source {
+        rsrc_t w, x;
+        uint8_t* stage;
+        int left;
+    };
+    const auto source = [&](int t) {
         const int k0 = k_begin + t * kI8BK;
         const bool live = t < steps;
-        const int left = live ? a.k - k0 : 0;
-        const rsrc_t xr = make_rsrc(xb + k0, live ? x_bytes - (uint32_t)k0 : 0u);
-        if constexpr (TR) {
-            const rsrc_t wr = make_rsrc(wb + (int64_t)k0 * a.ldw,
-                                        live ? (uint32_t)(min(kI8BK, left) - 1) * (uint32_t)a.ldw + w_bytes : 0u);
-#pragma unroll
-            for (int i = 0; i < T::WLOADS; ++i)
-                bload128_lds(wr, st + 1024 * (wave * T::WLOADS + i), woff[i]);
+        Source f;
+        f.stage = smem + (t % S) * STAGE;
+        f.left = live ? a.k - k0 : 0;
+        f.x = make_rsrc(xb + k0, live ? x_bytes - (uint32_t)k0 : 0u);
+        if constexpr (TR)
+            f.w = make_rsrc(wb + (int64_t)k0 * a.ldw,
+                            live ? (uint32_t)(min(kI8BK, f.left) - 1) * (uint32_t)a.ldw + w_bytes : 0u);
+        else
+            f.w = make_rsrc(wb + k0, live ? w_bytes - (uint32_t)k0 : 0u);
+        return f;
+    };
+    const auto fetch = [&](const Source& f, int i) {
+        if (i < T::WLOADS) {
+            bload128_lds(f.w, f.stage + 1024 * (wave * T::WLOADS + i), TR ? woff[i] : off_if(wcol[i] < f.left, woff[i]));
         } else {
-            const rsrc_t wr = make_rsrc(wb + k0, live ? w_bytes - (uint32_t)k0 : 0u);
-#pragma unroll
-            for (int i = 0; i < T::WLOADS; ++i)
-                bload128_lds(wr, st + 1024 * (wave * T::WLOADS + i), off_if(wcol[i] < left, woff[i]));
+            const int x = i - T::WLOADS;
+            bload128_lds(f.x, f.stage + kI8BN * kI8BK + 1024 * (wave * T::XLOADS + x),
+                         off_if(xcol[x] < f.left, xoff[x]));
         }
-#pragma unroll
-        for (int i = 0; i < T::XLOADS; ++i)
-            bload128_lds(xr, st + kI8BN * kI8BK + 1024 * (wave * T::XLOADS + i), off_if(xcol[i] < left, xoff[i]));
     };
 
     int16v_t acc[T::TN][T::TT];
@@ -247,14 +253,31 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
         }
         if constexpr (TR) lds_tr8(st + part * U * 8192, wat, f.w);
     };
-    const auto multiply = [&](const Part& f) {
+    // The MFMAs of a part, and between them loads `from` .. `to` - 1 of a coming step: issued at once, the loads
+    // of eight waves fill the address queue and hold up the MFMAs behind them ([830, 8960] x 1536 19.3 against
+    // 17.3 us; the 64-token tiles, whose part is a whole step, take them at once: 26.5 against 27.0 at
+    // [830, 1536] x 8960). On the largest tiles the wave that multiplies goes first (8192 tokens 562 -> 548 us;
+    // 128-token tiles are slower with it).
+    const auto multiply = [&](const Part& f, const Source& next, int from, int to) {
+        if constexpr (TM == 256) __builtin_amdgcn_s_setprio(1);
+        if constexpr (U == 4) {
+#pragma unroll
+            for (int i = from; i < to; ++i) fetch(next, i);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < T::TN; ++i)
 #pragma unroll
-                for (int j = 0; j < T::TT; ++j)
+                for (int j = 0; j < T::TT; ++j) {
                     acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[u][i], f.x[u][j], acc[i][j], 0, 0, 0);
+                    const int n = (u * T::TN + i) * T::TT + j;  // of eight
+                    if (U != 4 && n % 2 == 0 && from + n / 2 < to) {
+                        fetch(next, from + n / 2);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+        if constexpr (TM == 256) __builtin_amdgcn_s_setprio(0);
     };
 
     // the tile's channel scales and biases
@@ -269,28 +292,40 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
         chan[threadIdx.x] = v;
     }
 
+    // loads of step t + S issued in part p of steps t (after its barrier: the last part) and t + 1
+    constexpr int PARTS = 4 / U;
+    constexpr int FIRST = PARTS == 1 ? T::LOADS : PARTS == 2 ? 3 : 4;
+    static_assert(T::LOADS <= FIRST * PARTS && (PARTS == 1 || FIRST <= 4), "loads of a step");
     Part f[2];
 #pragma unroll
-    for (int t = 0; t < S; ++t) fetch(t);
-    wait_vmcnt<T::LOADS * (S - 1)>();
+    for (int t = 0; t < S - 1; ++t) {
+        const Source next = source(t);
+#pragma unroll
+        for (int i = 0; i < T::LOADS; ++i) fetch(next, i);
+    }
+    Source next = source(S - 1);
+#pragma unroll
+    for (int i = 0; i < FIRST; ++i) fetch(next, i);
+    wait_vmcnt<T::LOADS * (S - 2) + FIRST>();
     lds_barrier();
     read(f[0], 0, 0);
     // a step whose first part is in f[P]
     const auto step = [&](int t, auto parity) {
         constexpr int P = decltype(parity)::value;
 #pragma unroll
-        for (int part = 0; part < 4 / U; ++part) {
+        for (int part = 0; part < PARTS; ++part) {
             const int now = (P + part) & 1;
-            if (part + 1 < 4 / U) {
+            if (part + 1 < PARTS) {
                 read(f[now ^ 1], t, part + 1);
+                multiply(f[now], next, min(FIRST * (part + 1), T::LOADS), min(FIRST * (part + 2), T::LOADS));
             } else {
                 // every wave has read the last of this stage: it is free, and the next one is whole
                 wait_vmcnt<T::LOADS * (S - 2)>();
                 lds_barrier();
-                fetch(t + S);
+                next = source(t + S);
                 read(f[now ^ 1], t + 1, 0);
+                multiply(f[now], next, 0, FIRST);
             }
-            multiply(f[now]);
         }
     };
     if constexpr (U == 4) {
