@@ -286,7 +286,7 @@ hipError_t launch_qk_rope(QkRopeArgs a, int dtype, bool norm, bool axes, bool ba
 // Products of 8-bit integers (int8_gemm.hip).
 constexpr int kInt8FewM = 32;  // forward launches of so few tokens stream the weight to registers
 // ... and of at most so many quantize x themselves, where it fits so many bytes of LDS
-constexpr int kInt8FusedM = 4, kInt8FusedLds = 32768;
+constexpr int kInt8FusedM = 2, kInt8FusedLds = 32768;
 struct Int8GemmArgs {
     const int8_t* x;   // [m, k], row stride ldx, zeros from k to the next multiple of 16
     const int8_t* w;   // forward [n, k], transposed [k, n], row stride ldw

@@ -564,43 +564,53 @@ hipError_t launch_int8_quantize(const Int8QuantArgs& a, int dtype, hipStream_t s
 
 // Few tokens: the weight streams from memory once, straight to registers. A work-group of WAVES waves
 // owns 16 channels, the waves take slices of k; 16x16x64 integer MFMAs with MT blocks of 16 tokens (rows
-// past m repeat the last one and are dropped). The exact integer sums of the waves meet in LDS.
+// past m repeat the last one and are dropped), U 64-byte columns of the weight in flight a wave. The exact
+// integer sums of the waves meet in LDS. Bound by the weight's stream from memory and, as the tokens grow,
+// by the reads of x, which every work-group makes: [18944, 3584] with the weight from memory 18.3 us at one
+// token, 22.2 at 8, 35 at 32 with the quantizer's launch (its 68 MB take 13 us to stream). Measured and not
+// kept: 32 and 64 channels a work-group (21 - 25 us at one token; 32 at 32 tokens), columns loaded one by one
+// as they are used up (+1 us), non-temporal loads (+0 to 2 us).
 template <int MT, int WAVES, int OUT>
 __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Int8GemmArgs a) {
-    constexpr int U = 8;  // 64-byte columns of the weight in flight a wave
+    constexpr int U = 8;
     __shared__ int red[WAVES][MT][256];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n0 = 16 * blockIdx.x, l16 = lane & 15, c = 16 * (lane >> 4);
     const int cols = (a.k + 63) / 64, share = (cols + WAVES - 1) / WAVES;
     const int begin = wave * share, end = min(cols, begin + share);
-    const int8_t* const w = a.w + (int64_t)min(n0 + l16, a.n - 1) * a.ldw + c;
-    const int8_t* x[MT];
+    // buffers of this work-group's channels and of x: offsets past a row's k read zeros
+    const int kpad = (a.k + 15) & ~15;
+    const rsrc_t wr = make_rsrc(a.w + (int64_t)n0 * a.ldw, (uint32_t)((min(16, a.n - n0) - 1) * a.ldw + kpad));
+    const rsrc_t xr = make_rsrc(a.x, (uint32_t)((a.m - 1) * a.ldx + kpad));
+    const uint32_t woff = l16 * (uint32_t)a.ldw + c;
+    uint32_t xoff[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) x[t] = a.x + (int64_t)min(16 * t + l16, a.m - 1) * a.ldx + c;
+    for (int t = 0; t < MT; ++t) xoff[t] = min(16 * t + l16, a.m - 1) * (uint32_t)a.ldx + c;
     int4_t acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = int4_t{0, 0, 0, 0};
+    const int last = min(64 * end, a.k) - c;
     for (int b = begin; b < end; b += U) {
-        int4_t wf[U], xf[MT][U];
+        u32x4_t wf[U], xf[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int k = 64 * (b + u);
-            const bool ok = b + u < end && k + c < a.k;
-            wf[u] = ok ? *(const int4_t*)(w + k) : int4_t{0, 0, 0, 0};
+            const uint32_t at = off_if(64 * (b + u) < last, 64u * (b + u));
+            wf[u] = bload128(wr, woff + at);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) xf[t][u] = ok ? *(const int4_t*)(x[t] + k) : int4_t{0, 0, 0, 0};
+            for (int t = 0; t < MT; ++t) xf[u][t] = bload128(xr, xoff[t] + at);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int t = 0; t < MT; ++t)
-                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], xf[t][u], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4_t, wf[u]),
+                                                               __builtin_bit_cast(int4_t, xf[u][t]), acc[t], 0, 0, 0);
     }
     // lane: channels 4 (lane / 16) + 0..3 of token l16
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) red[wave][t][l16 * 16 + 4 * (lane >> 4) + r] = acc[t][r];
+        for (int e = 0; e < 4; ++e) red[wave][t][l16 * 16 + 4 * (lane >> 4) + e] = acc[t][e];
     __syncthreads();
     for (int i = threadIdx.x; i < 256 * MT; i += 64 * WAVES) {
         const int m = i >> 4, n = n0 + (i & 15);
@@ -616,7 +626,8 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Int8GemmArgs
 
 // The same with x as it comes (fp16, bf16 or fp32): every work-group quantizes the few rows for itself
 // (they come from the L2) into LDS while its first weights are on their way, which saves the launch of the
-// quantizer and its round trip. Rows m <= 16 with m * k bytes of LDS.
+// quantizer and its round trip: [18944, 3584] at one token 16.0 us (4.2 TB/s) against 18.3, [3584, 3584] 6.0
+// against 8.4; at two tokens equal, at four 22.0 against 19.8.
 template <int DT, int WAVES, int OUT>
 __global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8GemmArgs a, const Int8QuantArgs q) {
     constexpr int U = 8;
@@ -628,11 +639,12 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8Ge
     const int n0 = 16 * blockIdx.x, l16 = lane & 15, c = 16 * (lane >> 4);
     const int cols = (a.k + 63) / 64, share = (cols + WAVES - 1) / WAVES;
     const int begin = wave * share, end = min(cols, begin + share);
-    const int8_t* const w = a.w + (int64_t)min(n0 + l16, a.n - 1) * a.ldw + c;
-    int4_t wf[U];
-    const auto fetch = [&](int b) {
-        return b < end && 64 * b + c < a.k ? *(const int4_t*)(w + 64 * b) : int4_t{0, 0, 0, 0};
-    };
+    const int kpad = (a.k + 15) & ~15;
+    const rsrc_t wr = make_rsrc(a.w + (int64_t)n0 * a.ldw, (uint32_t)((min(16, a.n - n0) - 1) * a.ldw + kpad));
+    const uint32_t woff = l16 * (uint32_t)a.ldw + c;
+    const int last = min(64 * end, a.k) - c;
+    u32x4_t wf[U];
+    const auto fetch = [&](int b) { return bload128(wr, woff + off_if(64 * b < last, 64u * b)); };
 #pragma unroll
     for (int u = 0; u < U; ++u) wf[u] = fetch(begin + u);
     const int ld = 64 * cols, groups = ld / 8;  // LDS rows, zeros past k
@@ -661,7 +673,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8Ge
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (b + u >= end) break;
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], lds128(x + 64 * (b + u)), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4_t, wf[u]), lds128(x + 64 * (b + u)), acc, 0, 0, 0);
             wf[u] = fetch(b + u + U);
         }
     }
@@ -717,7 +729,10 @@ static Int8Plan make_plan(int64_t m, int64_t n, int64_t k, int cus) {
 Int8Plan int8_plan(int64_t m, int64_t n, int64_t k, bool tr) {
     Int8Plan few{};
     if (m <= 0 || n <= 0) return few;
-    if (!tr && m <= kInt8FewM) {
+    // Streamed weights up to 8 tokens, and up to 32 where the weight is small: at 16 / 32 tokens [3584, 3584]
+    // takes 9.4 / 11.4 us against 15.2 / 16.3 on the tiles, [8960, 1536] 10.6 / 13.6 against 14.7 / 16.2, but
+    // [18944, 3584] 26.0 / 35.1 against 22.5 / 24.0 (8 tokens: 22.2 against 22.0)
+    if (!tr && (m <= 8 || (m <= kInt8FewM && n * k <= (int64_t(1) << 24)))) {
         few.few = true;
         few.splits = 1;
         return few;
@@ -801,7 +816,9 @@ hipError_t launch_int8_gemm(Int8GemmArgs a, const Int8Plan& p, int out_dtype, bo
     if (a.m == 0 || a.n == 0) return hipSuccess;
     if (p.few) {
         const unsigned grid = (unsigned)((a.n + 15) / 16);
-        const bool wide = grid < 512;  // few work-groups: more waves of each along k
+        // few work-groups with a long k: more waves of each along it ([3584] x 18944 at 8 tokens 27.8 -> 27.0 us;
+        // [512] x 3584 is slower with them, 7.8 -> 8.3)
+        const bool wide = grid < 512 && a.k >= 8192;
         if (a.m <= 16)
             wide ? launch_few<1, 16>(a, out_dtype, grid, s) : launch_few<1, 4>(a, out_dtype, grid, s);
         else
