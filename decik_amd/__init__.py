@@ -6,6 +6,9 @@ Python API (the `solution` package name is kept as an alias, see solution/__init
 - mlp.py     Qwen2 MLP: gate+up in one fused launch, SwiGLU, down; fused backward
 - lora.py    LoRA r=16 with the A.B term fused into the GEMM epilogues; q/k/v in one launch
 - swiglu.py  SwiGLU forward/backward kernels
+- dropout.py dropout from a counter-based generator, masks never stored
+- rope.py    q/k RoPE; RMS norms of q and k heads with the rotation; positions with several axes
+- int8.py    linears in 8-bit integers with scales per token and channel
 - quant.py   bitsandbytes-layout NF4 quantizer and QuantState stand-in (no bitsandbytes needed)
 
 apply() installs the patches the reference installs for this path (solution/__init__.py:30-51):

@@ -13,13 +13,15 @@ rebuild fp16(x * (keep * scale)) in registers (dk_lora_down_dropout, dk_lora_bwd
 backward GEMM masks each branch's input gradient in its epilogue, so no dropped-out input or
 per-branch input gradient is ever stored. LoRAPair / LoRAPairFromNorm keep the reference's
 separate branch (packed keep-masks, dropped-out fp16 inputs, the input gradient through the
-masks: dk_lora_keep_pack, dk_lora_dropout_inputs, dk_lora_up, dk_lora_input_grad).
+masks: dk_lora_keep_pack, dk_lora_dropout_inputs, dk_lora_up, dk_lora_input_grad); LoRAPairSeeded is
+the same pair with masks from a counter-based generator, formed again in the backward.
 """
 
 import torch
 
 from . import nf4 as _nf4
 from . import _lib
+from .dropout import dropout_backward, dropout_forward
 from ._lib import check, lib, ptr, stream_of
 
 
@@ -232,6 +234,21 @@ class _QVDropout:
         return total
 
 
+class _QVSeeded:
+    """Dropout of the q and v LoRA branch inputs with masks formed from rng (seed, offset) when they are
+    needed: q takes the offset's, v the next one's (dk_dropout_fwd / dk_dropout_bwd, both branches from
+    one read of x and into one write of its gradient)."""
+
+    def __init__(self, rng, p):
+        self.rng, self.p = rng, p
+
+    def inputs(self, x, forward):
+        return tuple(t.reshape(-1, x.shape[-1]) for t in dropout_forward(x, self.rng, self.p, torch.float16))
+
+    def input_grad(self, gx16):
+        return dropout_backward(gx16, self.rng, self.p, torch.float32)
+
+
 def _qv_lora_forward(x, drop, adapters, scalings):
     """(out_q, out_v, u_q, u_v): out = fp16(fp16(U . B^T) * s), U = fp16(X . A^T) per branch, with
     X the branch's dropped-out fp16 input (solution/attn.py:224-228)."""
@@ -309,6 +326,31 @@ class LoRAPair:
     def apply(x, bits_q, scale_q, bits_v, scale_v, a_q, b_q, a_v, b_v, scaling_q, scaling_v, p_q, p_v):
         return LoRAPairFromNorm.apply(x, None, None, None, None, bits_q, scale_q, None, bits_v, scale_v,
                                       a_q, b_q, a_v, b_v, scaling_q, scaling_v, p_q, p_v, True)
+
+
+class LoRAPairSeeded(torch.autograd.Function):
+    """Both LoRA branches with dropout masks that are never stored: apply(x, rng, a_q, b_q, a_v, b_v,
+    scaling_q, scaling_v, p_q, p_v) -> (out_q, out_v) fp16, as LoRAPair with the masks of
+    decik_amd.dropout at rng (int64 device tensor: seed, offset; the call uses up two offsets). The
+    backward forms the same masks again; rng must not change before it. x: [.., W] fp16 or fp32;
+    gradients reach x (fp32) and the adapters."""
+
+    @staticmethod
+    def forward(ctx, x, rng, a_q, b_q, a_v, b_v, scaling_q, scaling_v, p_q, p_v):
+        if x.dtype not in (torch.float16, torch.float32):
+            raise ValueError("LoRAPairSeeded: x must be fp16 or fp32")
+        scalings, ps = (scaling_q, scaling_v), (float(p_q), float(p_v))
+        out_q, out_v, u_q, u_v = _qv_lora_forward(x, _QVSeeded(rng, ps), ((a_q, b_q), (a_v, b_v)), scalings)
+        ctx.save_for_backward(x, rng, u_q, u_v, a_q, b_q, a_v, b_v)
+        ctx.scalings, ctx.ps = scalings, ps
+        return out_q, out_v
+
+    @staticmethod
+    def backward(ctx, grad_q, grad_v):
+        x, rng, u_q, u_v, a_q, b_q, a_v, b_v = ctx.saved_tensors
+        grad_x, adapter_grads = _qv_lora_backward(x, _QVSeeded(rng, ctx.ps), ((a_q, b_q), (a_v, b_v)), ctx.scalings,
+                                                  (u_q, u_v), (grad_q, grad_v))
+        return (grad_x.to(x.dtype), None, *adapter_grads, *(None,) * 4)
 
 
 class NF4LoRALinear(torch.autograd.Function):

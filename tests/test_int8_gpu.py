@@ -110,7 +110,7 @@ def int_matrix(shape, device, seed):
 
 # tokens around the few-row kernel's blocks and the tiles, channels around 16 and 256, k around the steps
 SIZES = [(1, 1, 1), (1, 16, 64), (1, 257, 1121), (2, 40, 100), (15, 33, 128), (16, 512, 4096), (17, 48, 130),
-         (31, 300, 257), (32, 8208, 320), (33, 256, 128), (64, 255, 1536), (65, 257, 129), (127, 512, 384),
+         (20, 8208, 2100), (31, 300, 257), (32, 8208, 320), (33, 256, 128), (64, 255, 1536), (65, 257, 129), (127, 512, 384),
          (128, 100, 16), (129, 513, 2000), (255, 256, 1024), (256, 256, 256), (257, 700, 640), (300, 2057, 1121),
          (830, 256, 1536), (1000, 1000, 77), (1100, 4200, 512)]
 
