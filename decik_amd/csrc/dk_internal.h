@@ -284,7 +284,7 @@ hipError_t launch_qk_rope(QkRopeArgs a, int dtype, bool norm, bool axes, bool ba
                           hipStream_t s);
 
 // Products of 8-bit integers (int8_gemm.hip).
-constexpr int kInt8FewM = 32;  // forward launches of so few tokens stream the weight to registers
+constexpr int kInt8FewM = 32;  // forward launches of so few tokens may stream the weight to registers
 // ... and of at most so many quantize x themselves, where it fits so many bytes of LDS
 constexpr int kInt8FusedM = 2, kInt8FusedLds = 32768;
 struct Int8GemmArgs {
@@ -301,7 +301,7 @@ struct Int8GemmArgs {
 };
 struct Int8Plan {
     bool few;
-    int tm, m_tiles, n_tiles, splits, steps_per_split;
+    int tm, bn, m_tiles, n_tiles, splits, steps_per_split;
     int64_t partial_bytes;
 };
 struct Int8QuantArgs {

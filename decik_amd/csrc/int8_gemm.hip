@@ -21,12 +21,17 @@ typedef int int2v_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) const uint8_t* lds_t;
 typedef int int16v_t __attribute__((ext_vector_type(16)));
 
-constexpr int kI8Threads = 512;
-constexpr int kI8BN = 256;
 constexpr int kI8BK = 128;
 
-__host__ __device__ constexpr int i8_stage_bytes(int tm) { return (kI8BN + tm) * kI8BK; }
-__host__ __device__ constexpr int i8_stages(int tm) { return tm == 256 ? 2 : 3; }
+// tiles of TM = 256, 128 or 64 tokens by BN = 256 channels (eight waves), or 64 by 64 (four)
+__host__ __device__ constexpr int i8_waves(int bn) { return bn == 256 ? 8 : 4; }
+__host__ __device__ constexpr int i8_stage_bytes(int tm, int bn) { return (bn + tm) * kI8BK; }
+__host__ __device__ constexpr int i8_stages(int tm, int bn) {
+    return bn == 64 ? 4 : tm == 256 ? 2 : 3;
+}
+__host__ __device__ constexpr size_t i8_lds(int tm, int bn) {  // with the channels' scales and biases
+    return (size_t)i8_stages(tm, bn) * i8_stage_bytes(tm, bn) + 8 * bn;
+}
 
 // chunk permutation of a row: tokens are read 32 consecutive rows at a time
 __device__ __forceinline__ int row_key(int r) { return (r >> 1) & 7; }
@@ -36,41 +41,46 @@ __device__ __forceinline__ int4_t lds128(const uint8_t* p) { return *(const int4
 // Operands from a TR stage: 16 rows of a lane's byte column, two transposed reads of 8 rows each. One asm
 // block with its own wait: the builtin counts as aliasing every load to LDS in flight and would drain the
 // ring at every read.
+// R8: bytes of 8 rows; the next slice is 4 R8 on.
+template <int R8>
 __device__ __forceinline__ void lds_tr8(const uint8_t* st, const uint32_t (&at)[2], int4_t (&o)[1][2]) {
     int2v_t a, b, c, d;
     asm volatile(
-        "ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %4 offset:2048\n\t"
-        "ds_read_b64_tr_b8 %2, %5\n\tds_read_b64_tr_b8 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+        "ds_read_b64_tr_b8 %0, %4\n\tds_read_b64_tr_b8 %1, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b8 %2, %5\n\tds_read_b64_tr_b8 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
         : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
-        : "v"((lds_t)(st + at[0])), "v"((lds_t)(st + at[1]))
+        : "v"((lds_t)(st + at[0])), "v"((lds_t)(st + at[1])), "n"(R8)
         : "memory");
     o[0][0] = int4_t{a.x, a.y, b.x, b.y};
     o[0][1] = int4_t{c.x, c.y, d.x, d.y};
 }
+template <int R8>
 __device__ __forceinline__ void lds_tr8(const uint8_t* st, const uint32_t (&at)[2], int4_t (&o)[2][2]) {
     int2v_t a, b, c, d, e, f, g, h;
     asm volatile(
-        "ds_read_b64_tr_b8 %0, %8\n\tds_read_b64_tr_b8 %1, %8 offset:2048\n\t"
-        "ds_read_b64_tr_b8 %2, %9\n\tds_read_b64_tr_b8 %3, %9 offset:2048\n\t"
-        "ds_read_b64_tr_b8 %4, %8 offset:8192\n\tds_read_b64_tr_b8 %5, %8 offset:10240\n\t"
-        "ds_read_b64_tr_b8 %6, %9 offset:8192\n\tds_read_b64_tr_b8 %7, %9 offset:10240\n\ts_waitcnt lgkmcnt(0)"
+        "ds_read_b64_tr_b8 %0, %8\n\tds_read_b64_tr_b8 %1, %8 offset:%10\n\t"
+        "ds_read_b64_tr_b8 %2, %9\n\tds_read_b64_tr_b8 %3, %9 offset:%10\n\t"
+        "ds_read_b64_tr_b8 %4, %8 offset:%11\n\tds_read_b64_tr_b8 %5, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b8 %6, %9 offset:%11\n\tds_read_b64_tr_b8 %7, %9 offset:%12\n\ts_waitcnt lgkmcnt(0)"
         : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(e), "=&v"(f), "=&v"(g), "=&v"(h)
-        : "v"((lds_t)(st + at[0])), "v"((lds_t)(st + at[1]))
+        : "v"((lds_t)(st + at[0])), "v"((lds_t)(st + at[1])), "n"(R8), "n"(4 * R8), "n"(5 * R8)
         : "memory");
     o[0][0] = int4_t{a.x, a.y, b.x, b.y};
     o[0][1] = int4_t{c.x, c.y, d.x, d.y};
     o[1][0] = int4_t{e.x, e.y, f.x, f.y};
     o[1][1] = int4_t{g.x, g.y, h.x, h.y};
 }
+template <int R8>
 __device__ __forceinline__ void lds_tr8(const uint8_t* st, const uint32_t (&at)[1], int4_t (&o)[4][1]) {
     int2v_t a, b, c, d, e, f, g, h;
     asm volatile(
-        "ds_read_b64_tr_b8 %0, %8\n\tds_read_b64_tr_b8 %1, %8 offset:2048\n\t"
-        "ds_read_b64_tr_b8 %2, %8 offset:8192\n\tds_read_b64_tr_b8 %3, %8 offset:10240\n\t"
-        "ds_read_b64_tr_b8 %4, %8 offset:16384\n\tds_read_b64_tr_b8 %5, %8 offset:18432\n\t"
-        "ds_read_b64_tr_b8 %6, %8 offset:24576\n\tds_read_b64_tr_b8 %7, %8 offset:26624\n\ts_waitcnt lgkmcnt(0)"
+        "ds_read_b64_tr_b8 %0, %8\n\tds_read_b64_tr_b8 %1, %8 offset:%9\n\t"
+        "ds_read_b64_tr_b8 %2, %8 offset:%10\n\tds_read_b64_tr_b8 %3, %8 offset:%11\n\t"
+        "ds_read_b64_tr_b8 %4, %8 offset:%12\n\tds_read_b64_tr_b8 %5, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b8 %6, %8 offset:%14\n\tds_read_b64_tr_b8 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
         : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(e), "=&v"(f), "=&v"(g), "=&v"(h)
-        : "v"((lds_t)(st + at[0]))
+        : "v"((lds_t)(st + at[0])), "n"(R8), "n"(4 * R8), "n"(5 * R8), "n"(8 * R8), "n"(9 * R8), "n"(12 * R8),
+          "n"(13 * R8)
         : "memory");
     o[0][0] = int4_t{a.x, a.y, b.x, b.y};
     o[1][0] = int4_t{c.x, c.y, d.x, d.y};
@@ -83,13 +93,21 @@ struct Int {
     static constexpr int value = V;
 };
 
-template <int TM, bool TR>
+// chunk permutation of a TR stage's row r (along k): the eight rows of a transposed read, at one chunk or at
+// two neighbouring ones, spread over the banks
+template <int BN>
+__device__ __forceinline__ int tr_key(int r) {
+    return ((r & 7) / (256 / BN)) << 1;
+}
+
+template <int TM, int BN, bool TR>
 struct I8Tile {
+    static constexpr int NW = i8_waves(BN);
     // waves along channels and tokens
-    static constexpr int WN = TM == 256 ? (TR ? 4 : 2) : TM == 128 ? 4 : 8;
-    static constexpr int WM = 8 / WN;
-    static constexpr int TN = kI8BN / WN / 32, TT = TM / WM / 32;  // 32x32 blocks a wave
-    static constexpr int WLOADS = kI8BN * kI8BK / 8192, XLOADS = TM * kI8BK / 8192;  // a wave and step
+    static constexpr int WN = BN == 256 ? (TM == 256 ? (TR ? 4 : 2) : TM == 128 ? 4 : 8) : 2;
+    static constexpr int WM = NW / WN;
+    static constexpr int TN = BN / WN / 32, TT = TM / WM / 32;  // 32x32 blocks a wave
+    static constexpr int WLOADS = BN * kI8BK / 1024 / NW, XLOADS = TM * kI8BK / 1024 / NW;  // a wave and step
     static constexpr int LOADS = WLOADS + XLOADS;
     // slices whose operands are read at once, ahead of the MFMAs: small tiles have few MFMAs a slice to hide
     // the reads behind
@@ -114,22 +132,22 @@ __device__ __forceinline__ int4_t quad(const int16v_t& v, int q) {
     return int4_t{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
 }
 
-// four sums times the token's scale and (not TR) the channels' scales, plus their biases (256 on)
-template <bool TR>
+// four sums times the token's scale and (not TR) the channels' scales, plus their biases (BN on)
+template <bool TR, int BN>
 __device__ __forceinline__ float4_t scaled(int4_t v, float xs, const float* chan) {
     float4_t f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = (float)v[e] * xs;
-    if constexpr (!TR) f = f * *(const float4_t*)chan + *(const float4_t*)(chan + 256);
+    if constexpr (!TR) f = f * *(const float4_t*)chan + *(const float4_t*)(chan + BN);
     asm("" : "+v"(f));  // keeps the products out of mixed-precision multiply-adds
     return f;
 }
 
 // OUT: an element type, or -1 for the int32 partial sums of a split
-template <int TM, bool TR, int OUT>
-__global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8GemmArgs a) {
-    typedef I8Tile<TM, TR> T;
-    constexpr int S = i8_stages(TM), STAGE = i8_stage_bytes(TM);
+template <int TM, int BN, bool TR, int OUT>
+__global__ __launch_bounds__(64 * i8_waves(BN), 2) void int8_gemm_kernel(const Int8GemmArgs a) {
+    typedef I8Tile<TM, BN, TR> T;
+    constexpr int S = i8_stages(TM, BN), STAGE = i8_stage_bytes(TM, BN);
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, g = lane >> 5;
@@ -142,7 +160,7 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
     const int split = L / per, tile = L - split * per;
     const int band = tile / (8 * a.n_tiles), in = tile - band * 8 * a.n_tiles;
     const int rows = min(8, a.m_tiles - 8 * band);
-    const int m0 = (8 * band + in % rows) * TM, n0 = (in / rows) * kI8BN;
+    const int m0 = (8 * band + in % rows) * TM, n0 = (in / rows) * BN;
     const int k_begin = split * a.steps_per_split * kI8BK;
     const int steps = min(a.steps_per_split, (a.k + kI8BK - 1) / kI8BK - split * a.steps_per_split);
     const int kpad = (a.k + 15) & ~15, npad = (a.n + 15) & ~15;
@@ -150,8 +168,8 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
     const int8_t* const xb = a.x + (int64_t)m0 * a.ldx;
     const uint32_t x_bytes = (uint32_t)((min(TM, a.m - m0) - 1) * a.ldx + kpad);
     const int8_t* const wb = TR ? a.w + n0 : a.w + (int64_t)n0 * a.ldw;
-    const uint32_t w_bytes = TR ? (uint32_t)min(kI8BN, npad - n0)
-                                : (uint32_t)((min(kI8BN, a.n - n0) - 1) * a.ldw + kpad);
+    const uint32_t w_bytes = TR ? (uint32_t)min(BN, npad - n0)
+                                : (uint32_t)((min(BN, a.n - n0) - 1) * a.ldw + kpad);
 
     // this lane's source offsets, and its column along k, of every load of a step
     uint32_t woff[T::WLOADS], xoff[T::XLOADS];
@@ -160,9 +178,10 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
     for (int i = 0; i < T::WLOADS; ++i) {
         const int q = wave * T::WLOADS + i;
         if constexpr (TR) {
-            const int r = 4 * q + (lane >> 4);
+            constexpr int CHUNKS = BN / 16;
+            const int r = 64 / CHUNKS * q + lane / CHUNKS;
             wcol[i] = 0;
-            woff[i] = r * (uint32_t)a.ldw + 16 * ((lane & 15) ^ ((r & 7) << 1));
+            woff[i] = r * (uint32_t)a.ldw + 16 * ((lane % CHUNKS) ^ tr_key<BN>(r));
         } else {
             const int r = 8 * q + (lane >> 3);
             wcol[i] = 16 * ((lane & 7) ^ row_key(r));
@@ -202,7 +221,7 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
             bload128_lds(f.w, f.stage + 1024 * (wave * T::WLOADS + i), TR ? woff[i] : off_if(wcol[i] < f.left, woff[i]));
         } else {
             const int x = i - T::WLOADS;
-            bload128_lds(f.x, f.stage + kI8BN * kI8BK + 1024 * (wave * T::XLOADS + x),
+            bload128_lds(f.x, f.stage + BN * kI8BK + 1024 * (wave * T::XLOADS + x),
                          off_if(xcol[x] < f.left, xoff[x]));
         }
     };
@@ -222,7 +241,7 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
     for (int i = 0; i < T::TN; ++i) {
         if constexpr (TR) {
             const int r = (lane & 15) >> 1, c = (wn + 32 * i) / 16 + ((lane >> 4) & 1);
-            wat[i] = (16 * g + r) * 256 + 16 * (c ^ (r << 1)) + 8 * (lane & 1);
+            wat[i] = (16 * g + r) * BN + 16 * (c ^ tr_key<BN>(r)) + 8 * (lane & 1);
         } else {
             const int r = wn + 32 * i + l32;
             wat[i] = r * 128 + 16 * (g ^ row_key(r));
@@ -231,7 +250,7 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
 #pragma unroll
     for (int j = 0; j < T::TT; ++j) {
         const int r = wm + 32 * j + l32;
-        xat[j] = kI8BN * kI8BK + r * 128 + 16 * (g ^ row_key(r));
+        xat[j] = BN * kI8BK + r * 128 + 16 * (g ^ row_key(r));
     }
 
     // operands of U slices (32 of k each) of a stage: parts 0 .. 4 / U - 1 of step t
@@ -251,7 +270,7 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
                 for (int i = 0; i < T::TN; ++i) f.w[u][i] = lds128(st + (wat[i] ^ (32 * s)));
             }
         }
-        if constexpr (TR) lds_tr8(st + part * U * 8192, wat, f.w);
+        if constexpr (TR) lds_tr8<8 * BN>(st + part * U * 32 * BN, wat, f.w);
     };
     // The MFMAs of a part, and between them loads `from` .. `to` - 1 of a coming step: issued at once, the loads
     // of eight waves fill the address queue and hold up the MFMAs behind them ([830, 8960] x 1536 19.3 against
@@ -283,18 +302,20 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
     // the tile's channel scales and biases
     float* const chan = (float*)(smem + S * STAGE);
     if constexpr (!TR && OUT >= 0) {
-        const int n = n0 + (int)(threadIdx.x & 255);
-        float v = 0.0f;
-        if (n < a.n) {
-            if (threadIdx.x < 256) v = a.ws[n];
-            else if (a.bias != nullptr) v = load_any(a.bias, a.bias_dtype, n);
+        const int c = threadIdx.x % BN, n = n0 + c;
+        if (threadIdx.x < 2 * BN) {
+            float v = 0.0f;
+            if (n < a.n) {
+                if (threadIdx.x < BN) v = a.ws[n];
+                else if (a.bias != nullptr) v = load_any(a.bias, a.bias_dtype, n);
+            }
+            chan[threadIdx.x] = v;
         }
-        chan[threadIdx.x] = v;
     }
 
     // loads of step t + S issued in part p of steps t (after its barrier: the last part) and t + 1
     constexpr int PARTS = 4 / U;
-    constexpr int FIRST = PARTS == 1 ? T::LOADS : PARTS == 2 ? 3 : 4;
+    constexpr int FIRST = PARTS == 1 ? T::LOADS : PARTS == 2 ? (T::LOADS + 1) / 2 : 4;
     static_assert(T::LOADS <= FIRST * PARTS && (PARTS == 1 || FIRST <= 4), "loads of a step");
     Part f[2];
 #pragma unroll
@@ -358,7 +379,7 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
                     if constexpr (OUT < 0)  // slab rows are padded to four channels
                         *(int4_t*)(a.partials + (int64_t)split * a.slab + (int64_t)m * a.ldp + n) = v;
                     else
-                        store4<DK_FP32>((float*)a.y + (int64_t)m * a.ldy + n, scaled<TR>(v, xs, chan + c), a.n - n);
+                        store4<DK_FP32>((float*)a.y + (int64_t)m * a.ldy + n, scaled<TR, BN>(v, xs, chan + c), a.n - n);
                 }
         }
     } else {
@@ -376,7 +397,7 @@ __global__ __launch_bounds__(kI8Threads, 2) void int8_gemm_kernel(const Int8Gemm
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int c = 32 * i + 8 * q + 4 * g;
-                    const float4_t v = scaled<TR>(quad(acc[i][j], q), xs, chan + wn + c);
+                    const float4_t v = scaled<TR, BN>(quad(acc[i][j], q), xs, chan + wn + c);
                     store4<OUT>((E*)(stage + l32 * ROW) + c, v, 4);
                 }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -567,7 +588,7 @@ hipError_t launch_int8_quantize(const Int8QuantArgs& a, int dtype, hipStream_t s
 // past m repeat the last one and are dropped), U 64-byte columns of the weight in flight a wave. The exact
 // integer sums of the waves meet in LDS. Bound by the weight's stream from memory and, as the tokens grow,
 // by the reads of x, which every work-group makes: [18944, 3584] with the weight from memory 18.3 us at one
-// token, 22.2 at 8, 35 at 32 with the quantizer's launch (its 68 MB take 13 us to stream). Measured and not
+// token, 22.2 at 8, 35 at 32 with the quantizer's launch (its 68 MB alone take 13 us). Measured and not
 // kept: 32 and 64 channels a work-group (21 - 25 us at one token; 32 at 32 tokens), columns loaded one by one
 // as they are used up (+1 us), non-temporal loads (+0 to 2 us).
 template <int MT, int WAVES, int OUT>
@@ -694,82 +715,93 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8Ge
 
 // ---- launches ------------------------------------------------------------------------------------
 
-static Int8Plan make_plan(int64_t m, int64_t n, int64_t k, int cus) {
+static Int8Plan make_plan(int64_t m, int64_t n, int64_t k, int cus, bool tr) {
     Int8Plan best{};
     const int64_t steps = (k + kI8BK - 1) / kI8BK > 0 ? (k + kI8BK - 1) / kI8BK : 1;
     double best_us = 0;
-    // microseconds a step of a work-group, by tile height (measured: [830, 1536] x 8960 transposed at 1 to
-    // 8 splits takes within 2 us of the estimate on 128 tokens, 3 on 64)
-    const int tms[3] = {256, 128, 64};
-    const double step_us[3] = {1.2, 0.68, 0.43};
-    for (int v = 0; v < 3; ++v) {
-        const int64_t mt = (m + tms[v] - 1) / tms[v], nt = (n + kI8BN - 1) / kI8BN, tiles = mt * nt;
+    // Estimated time of a launch, fitted to 170 timed launches (17 sizes of 64 to 8192 tokens, both ways, every
+    // tile, 1 to 15 splits; root mean square of the deviation 8%; its choice within 3% of the best of each size
+    // but one, 6%): rounds of work-groups of a number of steps each, whose time grows from `light` to `full` with
+    // the share of the CUs that work, and a last part; sums of splits written and read back.
+    struct Tile {
+        int tm, bn;
+        double light, full, last;
+    };
+    const Tile tiles[4] = {{256, 256, 0.99, 1.46, 5.0}, {128, 256, 0.51, 0.91, 2.8}, {64, 256, 0.42, 0.63, 1.8},
+                           {64, 64, 0.22, 0.24, 0.2}};
+    for (const Tile& v : tiles) {
+        const int64_t mt = (m + v.tm - 1) / v.tm, nt = (n + v.bn - 1) / v.bn;
         for (int64_t sp = 1; sp <= steps && sp <= 32; ++sp) {
             const int64_t sps = (steps + sp - 1) / sp;
             if ((steps + sps - 1) / sps != sp) continue;
-            const int64_t rounds = (tiles * sp + cus - 1) / cus;
-            const int64_t ldp = (n + 3) / 4 * 4;
-            double us = 3.0 + rounds * (sps * step_us[v] + 1.5);
-            if (sp > 1) us += 5.0 + 8.0 * sp * m * ldp / 5.0e6;  // partials written and read back
-            if (sp > 1 && sp * m * ldp * 4 > (int64_t(1) << 30)) continue;
+            const int64_t wgs = mt * nt * sp, rounds = (wgs + cus - 1) / cus, sums = sp * m * ((n + 3) / 4 * 4);
+            if (sp > 1 && sums > (int64_t(1) << 28)) continue;
+            const double load = wgs < cus ? (double)wgs / cus : 1.0;
+            double us = 2.5 + rounds * (sps * (v.light + (v.full - v.light) * load) + v.last) + m * n * 0.5e-6;
+            if (sp > 1) us += 3.9 + sums * 1.5e-6;
             if (best_us == 0 || us < best_us) {
                 best_us = us;
-                best.tm = tms[v];
+                best.tm = v.tm;
+                best.bn = v.bn;
                 best.m_tiles = (int)mt;
                 best.n_tiles = (int)nt;
                 best.splits = (int)sp;
                 best.steps_per_split = (int)sps;
-                best.partial_bytes = sp > 1 ? sp * m * ldp * 4 : 0;
+                best.partial_bytes = sp > 1 ? sums * 4 : 0;
             }
         }
+    }
+    // Few tokens: the streaming kernel where its estimate is the smaller one, weights from memory on both sides
+    // (4.5 us more for the tiles). Measured, streaming / tiles, us: [3584, 3584] 9.1 / 12.0 at 8 tokens, 11.1 /
+    // 12.2 at 32; [8960, 1536] 9.4 / 9.6 and 13.5 / 10.2; [18944, 3584] 22.3 / 21.4 and 35.1 / 23.2; [3584] x
+    // 18944 27.0 / 23.3 at 8; [512] x 3584 7.9 / 10.0 and 10.3 / 10.6.
+    const double few_us = 6.5 + n * k / 5.5e6 + m * n * k * 7.9e-9 + k * 3e-4;
+    if (!tr && m <= kInt8FewM && few_us < best_us + 4.5) {
+        best = Int8Plan{};
+        best.few = true;
+        best.splits = 1;
     }
     return best;
 }
 
 Int8Plan int8_plan(int64_t m, int64_t n, int64_t k, bool tr) {
-    Int8Plan few{};
-    if (m <= 0 || n <= 0) return few;
-    // Streamed weights up to 8 tokens, and up to 32 where the weight is small: at 16 / 32 tokens [3584, 3584]
-    // takes 9.4 / 11.4 us against 15.2 / 16.3 on the tiles, [8960, 1536] 10.6 / 13.6 against 14.7 / 16.2, but
-    // [18944, 3584] 26.0 / 35.1 against 22.5 / 24.0 (8 tokens: 22.2 against 22.0)
-    if (!tr && (m <= 8 || (m <= kInt8FewM && n * k <= (int64_t(1) << 24)))) {
-        few.few = true;
-        few.splits = 1;
-        return few;
-    }
+    if (m <= 0 || n <= 0) return Int8Plan{};
     // a call asks twice (workspace, launch) and a model asks for the same few sizes: the last ones are kept
     struct Kept {
         int64_t m, n, k;
         int cus;
+        bool tr;
         Int8Plan p;
     };
     thread_local Kept kept[16] = {};
     const int cus = device_cus();
     Kept& e = kept[(uint64_t)(m * 31 + n * 7 + k) % 16];
-    if (e.m != m || e.n != n || e.k != k || e.cus != cus) e = Kept{m, n, k, cus, make_plan(m, n, k, cus)};
+    if (e.m != m || e.n != n || e.k != k || e.tr != tr || e.cus != cus)
+        e = Kept{m, n, k, cus, tr, make_plan(m, n, k, cus, tr)};
     return e.p;
 }
 
-template <int TM, bool TR, int OUT>
+template <int TM, int BN, bool TR, int OUT>
 static hipError_t launch_tile(const Int8GemmArgs& a, hipStream_t s) {
-    constexpr size_t lds = (size_t)i8_stages(TM) * i8_stage_bytes(TM) + 2048;  // channel scales and biases
-    const hipError_t e = allow_dynamic_lds((const void*)int8_gemm_kernel<TM, TR, OUT>, lds);
+    constexpr size_t lds = i8_lds(TM, BN);
+    const hipError_t e = allow_dynamic_lds((const void*)int8_gemm_kernel<TM, BN, TR, OUT>, lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((int8_gemm_kernel<TM, TR, OUT>), dim3((unsigned)(a.m_tiles * a.n_tiles * a.splits)),
-                       dim3(kI8Threads), lds, s, a);
+    hipLaunchKernelGGL((int8_gemm_kernel<TM, BN, TR, OUT>), dim3((unsigned)(a.m_tiles * a.n_tiles * a.splits)),
+                       dim3(64 * i8_waves(BN)), lds, s, a);
     return hipGetLastError();
 }
 
-template <int TM, int OUT>
-static hipError_t launch_way(const Int8GemmArgs& a, bool tr, hipStream_t s) {
-    return tr ? launch_tile<TM, true, OUT>(a, s) : launch_tile<TM, false, OUT>(a, s);
+template <bool TR, int OUT>
+static hipError_t launch_way(const Int8GemmArgs& a, int tm, int bn, hipStream_t s) {
+    if (bn == 64) return launch_tile<64, 64, TR, OUT>(a, s);
+    if (tm == 256) return launch_tile<256, 256, TR, OUT>(a, s);
+    if (tm == 128) return launch_tile<128, 256, TR, OUT>(a, s);
+    return launch_tile<64, 256, TR, OUT>(a, s);
 }
 
 template <int OUT>
-static hipError_t launch_out(const Int8GemmArgs& a, int tm, bool tr, hipStream_t s) {
-    if (tm == 256) return launch_way<256, OUT>(a, tr, s);
-    if (tm == 128) return launch_way<128, OUT>(a, tr, s);
-    return launch_way<64, OUT>(a, tr, s);
+static hipError_t launch_out(const Int8GemmArgs& a, const Int8Plan& p, bool tr, hipStream_t s) {
+    return tr ? launch_way<true, OUT>(a, p.tm, p.bn, s) : launch_way<false, OUT>(a, p.tm, p.bn, s);
 }
 
 template <int MT, int WAVES>
@@ -830,13 +862,13 @@ hipError_t launch_int8_gemm(Int8GemmArgs a, const Int8Plan& p, int out_dtype, bo
     a.splits = p.splits;
     a.steps_per_split = p.steps_per_split;
     if (p.splits == 1) {
-        if (out_dtype == DK_FP16) return launch_out<DK_FP16>(a, p.tm, tr, s);
-        if (out_dtype == DK_BF16) return launch_out<DK_BF16>(a, p.tm, tr, s);
-        return launch_out<DK_FP32>(a, p.tm, tr, s);
+        if (out_dtype == DK_FP16) return launch_out<DK_FP16>(a, p, tr, s);
+        if (out_dtype == DK_BF16) return launch_out<DK_BF16>(a, p, tr, s);
+        return launch_out<DK_FP32>(a, p, tr, s);
     }
     a.ldp = (a.n + 3) / 4 * 4;
     a.slab = (int64_t)a.m * a.ldp;
-    const hipError_t e = launch_out<-1>(a, p.tm, tr, s);
+    const hipError_t e = launch_out<-1>(a, p, tr, s);
     if (e != hipSuccess) return e;
     const unsigned grid = (unsigned)((a.slab / 4 + 255) / 256);
     if (out_dtype == DK_FP16)
