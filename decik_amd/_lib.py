@@ -115,6 +115,7 @@ EXPORTS = {
     "dk_int8_linear_workspace": ([c_i32, c_i64, c_i64, c_i64], c_i64),
     "dk_int8_linear": ([c_i32, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_i64, c_i64, c_i64,
                         c_i64, c_vp, c_i64, c_vp], c_i32),
+    "dk_int8_linear_plan": ([c_i32, c_i64, c_i64, c_i64, ctypes.POINTER(c_i32)], c_i32),
     "dk_int8_linear_x_workspace": ([c_i32, c_i64, c_i64, c_i64], c_i64),
     "dk_int8_linear_fwd": ([c_vp, c_i32, c_i64, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_i64, c_i64, c_i64, c_i64,
                             c_vp, c_i64, c_vp], c_i32),

@@ -249,6 +249,18 @@ int64_t dk_int8_linear_workspace(int transposed, int64_t m, int64_t n, int64_t k
     return int8_plan(m, n, k, transposed != 0).partial_bytes;
 }
 
+int dk_int8_linear_plan(int transposed, int64_t m, int64_t n, int64_t k, int32_t* out) {
+    dk_clear_error();
+    if (!int8_sizes(m, n, k) || out == nullptr)
+        return dk_fail("dk_int8_linear_plan: 0 <= m, n < 2^23, 1 <= k <= 131071, out set");
+    const Int8Plan p = int8_plan(m, n, k, transposed != 0);
+    out[0] = p.few ? 0 : p.tm;
+    out[1] = p.few ? 16 : p.bn;
+    out[2] = p.splits;
+    out[3] = m > 0 && int8_fused(m, k, transposed != 0) ? 1 : 0;
+    return 0;
+}
+
 int dk_int8_linear(int transposed, const int8_t* xq, int64_t ldx, const float* xs, const int8_t* wq, int64_t ldw,
                    const float* ws, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t m,
                    int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, void* stream) {

@@ -36,6 +36,11 @@ __host__ __device__ constexpr size_t i8_lds(int tm, int bn) {  // with the chann
 // chunk permutation of a row: tokens are read 32 consecutive rows at a time
 __device__ __forceinline__ int row_key(int r) { return (r >> 1) & 7; }
 
+__device__ __forceinline__ int4_t bload128i(rsrc_t r, uint32_t off) {
+    const u32x4_t v = bload128(r, off);
+    return __builtin_bit_cast(int4_t, v);
+}
+
 __device__ __forceinline__ int4_t lds128(const uint8_t* p) { return *(const int4_t*)p; }
 
 // Operands from a TR stage: 16 rows of a lane's byte column, two transposed reads of 8 rows each. One asm
@@ -612,20 +617,20 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Int8GemmArgs
     for (int t = 0; t < MT; ++t) acc[t] = int4_t{0, 0, 0, 0};
     const int last = min(64 * end, a.k) - c;
     for (int b = begin; b < end; b += U) {
-        u32x4_t wf[U], xf[U][MT];
+        int4_t wf[U], xf[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t at = off_if(64 * (b + u) < last, 64u * (b + u));
-            wf[u] = bload128(wr, woff + at);
+            wf[u] = bload128i(wr, woff + at);
 #pragma unroll
-            for (int t = 0; t < MT; ++t) xf[u][t] = bload128(xr, xoff[t] + at);
+            for (int t = 0; t < MT; ++t) xf[u][t] = bload128i(xr, xoff[t] + at);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int t = 0; t < MT; ++t)
-                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4_t, wf[u]),
-                                                               __builtin_bit_cast(int4_t, xf[u][t]), acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u],
+                                                               xf[u][t], acc[t], 0, 0, 0);
     }
     // lane: channels 4 (lane / 16) + 0..3 of token l16
 #pragma unroll
@@ -664,8 +669,8 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8Ge
     const rsrc_t wr = make_rsrc(a.w + (int64_t)n0 * a.ldw, (uint32_t)((min(16, a.n - n0) - 1) * a.ldw + kpad));
     const uint32_t woff = l16 * (uint32_t)a.ldw + c;
     const int last = min(64 * end, a.k) - c;
-    u32x4_t wf[U];
-    const auto fetch = [&](int b) { return bload128(wr, woff + off_if(64 * b < last, 64u * b)); };
+    int4_t wf[U];
+    const auto fetch = [&](int b) { return bload128i(wr, woff + off_if(64 * b < last, 64u * b)); };
 #pragma unroll
     for (int u = 0; u < U; ++u) wf[u] = fetch(begin + u);
     const int ld = 64 * cols, groups = ld / 8;  // LDS rows, zeros past k
@@ -694,7 +699,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8Ge
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (b + u >= end) break;
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(int4_t, wf[u]), lds128(x + 64 * (b + u)), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], lds128(x + 64 * (b + u)), acc, 0, 0, 0);
             wf[u] = fetch(b + u + U);
         }
     }
@@ -752,11 +757,11 @@ static Int8Plan make_plan(int64_t m, int64_t n, int64_t k, int cus, bool tr) {
         }
     }
     // Few tokens: the streaming kernel where its estimate is the smaller one, weights from memory on both sides
-    // (4.5 us more for the tiles). Measured, streaming / tiles, us: [3584, 3584] 9.1 / 12.0 at 8 tokens, 11.1 /
+    // (the tiles' estimate knows them in the caches). Measured, streaming / tiles, us: [3584, 3584] 9.1 / 12.0 at 8 tokens, 11.1 /
     // 12.2 at 32; [8960, 1536] 9.4 / 9.6 and 13.5 / 10.2; [18944, 3584] 22.3 / 21.4 and 35.1 / 23.2; [3584] x
     // 18944 27.0 / 23.3 at 8; [512] x 3584 7.9 / 10.0 and 10.3 / 10.6.
     const double few_us = 6.5 + n * k / 5.5e6 + m * n * k * 7.9e-9 + k * 3e-4;
-    if (!tr && m <= kInt8FewM && few_us < best_us + 4.5) {
+    if (!tr && m <= kInt8FewM && few_us < best_us + 3.0 + n * k / 1.4e7) {
         best = Int8Plan{};
         best.few = true;
         best.splits = 1;

@@ -11,9 +11,11 @@ own rounding at most half a step, max|dY * w_scale| / 254 of its row, a term.
 Quantized rows are padded to 128 bytes; the tensors here are views of the padded rows.
 """
 
+import ctypes
+
 import torch
 
-from ._lib import DTYPES, call_on, gpu_input, lib, same_gpu
+from ._lib import DTYPES, call_on, check, gpu_input, lib, same_gpu
 
 
 def _ptr(t):
@@ -91,6 +93,14 @@ def _channel_args(what, ws, bias, n):
 def _workspace(x, need):
     # a tensor of its own a call: graphs and streams share none
     return x.new_empty(need, dtype=torch.uint8) if need > 0 else None
+
+
+def launch_plan(transposed, m, n, k):
+    """What a product of these sizes runs as (dk_int8_linear_plan): dict of tile_tokens (0: the weight streams
+    to registers), tile_channels, splits, fused (x quantized inside)."""
+    out = (ctypes.c_int32 * 4)()
+    check(lib().dk_int8_linear_plan(int(transposed), m, n, k, out))
+    return dict(tile_tokens=out[0], tile_channels=out[1], splits=out[2], fused=bool(out[3]))
 
 
 def int8_matmul(xq, x_scale, wq, w_scale, bias=None, dtype=torch.float16):

@@ -378,6 +378,11 @@ int64_t dk_int8_linear_workspace(int transposed, int64_t m, int64_t n, int64_t k
 int dk_int8_linear(int transposed, const int8_t* xq, int64_t ldx, const float* xs, const int8_t* wq, int64_t ldw,
                    const float* ws, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t m,
                    int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, void* stream);
+/* Diagnostic, host-only: what dk_int8_linear chooses. out[0] = tokens a tile (0: the weight streams to
+ * registers), out[1] = channels a tile, out[2] = splits of k, out[3] = 1 where dk_int8_linear_fwd quantizes x
+ * inside the product. Returns 0, or nonzero on bad sizes. */
+int dk_int8_linear_plan(int transposed, int64_t m, int64_t n, int64_t k, int32_t* out);
+
 /* Both steps in one call: forward y [m, n] = x . W^T + bias from x [m, k] of x_dtype, and the input gradient
  * dx [m, k] = dY . W from dy [m, n], quantized in the workspace or, a few tokens, inside the product; the same
  * results as the two calls. workspace: dk_int8_linear_x_workspace(backward, ..) bytes (0: none). */

@@ -157,13 +157,11 @@ def test_largest_sums(device):
 
 def test_every_split(device):
     """Long k with few tiles: splits of k, both ways, the same integers as one pass."""
-    from decik_amd._lib import lib
-    from decik_amd.int8 import int8_linear_backward, int8_linear_forward, quantize_int8
+    from decik_amd.int8 import int8_linear_backward, int8_linear_forward, launch_plan, quantize_int8
 
     seen = set()
     for m, n, k in ((64, 256, 8960), (64, 8960, 256), (300, 600, 4000), (300, 4000, 600), (830, 1536, 8960)):
-        need = [lib().dk_int8_linear_workspace(0, m, n, k), lib().dk_int8_linear_workspace(1, m, k, n)]
-        seen |= {(i, v > 0) for i, v in enumerate(need)}
+        seen |= {(0, launch_plan(False, m, n, k)["splits"] > 1), (1, launch_plan(True, m, k, n)["splits"] > 1)}
         wq, ws = quantize_int8(make((n, k), torch.float32, device, 1, 0.02))
         x, dy = make((m, k), torch.float16, device, 2), make((m, n), torch.float16, device, 3, 1e-2)
         xi, xs = quantized(x)
@@ -172,6 +170,35 @@ def test_every_split(device):
         gi, gs = quantized(dy, ws)
         check(int8_linear_backward(dy, wq, ws), dot(gi, ints(wq)), gs)
     assert {(0, True), (1, True)} <= seen
+
+
+# (tokens, channels, split) of a tile and sizes that run on it, odd in every direction
+TILES = {(64, 64, False): (333, 2057, 1121), (64, 64, True): (301, 131, 9001), (64, 256, False): (2051, 1537, 257),
+         (64, 256, True): (831, 1535, 8959), (128, 256, False): (701, 9001, 131), (128, 256, True): (513, 3585, 18945),
+         (256, 256, False): (1031, 9001, 257)}
+
+
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("transposed", [False, True])
+def test_every_tile(tile, transposed, device):
+    """Each tile with ragged last tiles and steps, against exact sums (64-bit floats hold them)."""
+    from decik_amd.int8 import int8_linear_backward, int8_linear_forward, launch_plan, quantize_int8
+
+    m, n, k = TILES[tile]
+    p = launch_plan(transposed, m, n, k)
+    assert (p["tile_tokens"], p["tile_channels"], p["splits"] > 1) == tile
+    if transposed:  # sums over k: the layer's output channels
+        wq, ws = quantize_int8(make((k, n), torch.float32, device, 1, 0.02))
+        dy = make((m, k), torch.bfloat16, device, 2)
+        gq, gs = quantize_int8(dy, ws)
+        check(int8_linear_backward(dy, wq, ws), (gq.double() @ wq.double()).cpu().numpy(), gs.cpu().numpy())
+    else:
+        wq, ws = quantize_int8(make((n, k), torch.float32, device, 1, 0.02))
+        x, bias = make((m, k), torch.bfloat16, device, 2), make((n,), torch.float16, device, 3)
+        xq, xs = quantize_int8(x)
+        acc = (xq.double() @ wq.double().t().contiguous()).cpu().numpy()
+        for dtype in (torch.bfloat16, torch.float32):
+            check(int8_linear_forward(x, wq, ws, bias, dtype), acc, xs.cpu().numpy(), ws.cpu().numpy(), bias)
 
 
 def test_rows_do_not_depend_on_the_batch(device):

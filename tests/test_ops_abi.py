@@ -201,3 +201,14 @@ def test_linear_plans_cover_their_tiles():
                     need = L.dk_int8_linear_workspace(tr, m, n, k)
                     slab = 4 * m * ((n + 3) // 4 * 4)
                     assert need == 0 or (need % slab == 0 and 2 <= need // slab <= 32)
+
+
+def test_linear_plan_query():
+    from decik_amd.int8 import launch_plan
+
+    assert launch_plan(False, 1, 18944, 3584) == dict(tile_tokens=0, tile_channels=16, splits=1, fused=True)
+    assert not launch_plan(True, 1, 64, 64)["fused"] and launch_plan(True, 1, 64, 64)["tile_tokens"] == 64
+    for bad in ((-1, 1, 1), (1, 1 << 23, 1), (1, 1, 0), (1, 1, 131072)):
+        with pytest.raises(_lib.DecikError):
+            launch_plan(False, *bad)
+    assert _lib.lib().dk_int8_linear_plan(0, 1, 1, 1, None) != 0
