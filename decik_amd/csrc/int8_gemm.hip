@@ -570,6 +570,8 @@ static void launch_quantize_typed(const Int8QuantArgs& a, hipStream_t s) {
         hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 256, 2>), dim3(rows), dim3(256), 0, s, a);
     else if (groups <= 256 * 4)
         hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 256, 4>), dim3(rows), dim3(256), 0, s, a);
+    else if (groups <= 512 * 3)
+        hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 512, 3>), dim3(rows), dim3(512), 0, s, a);
     else if (groups <= 512 * 5)
         hipLaunchKernelGGL((int8_quantize_kernel<DT, COL, 512, 5>), dim3(rows), dim3(512), 0, s, a);
     else

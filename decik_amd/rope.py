@@ -94,6 +94,10 @@ def _token_rows(what, t, heads, d):
     return t, row, b, n
 
 
+def _fp32(t):
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+
+
 def _rotation(what, dev, batch, tokens, d, tables, axes):
     """(cos, sin, positions, inv_freq pointers, strides of tables, axes and batches, axis count, sections,
     interleaved, int64 positions, the tensors behind the pointers) of a descriptor."""
@@ -102,7 +106,7 @@ def _rotation(what, dev, batch, tokens, d, tables, axes):
         same_gpu(what, dev, cos, sin)
         if cos.shape != sin.shape or cos.shape not in ((tokens, d), (batch, tokens, d), (1, tokens, d)):
             raise ValueError(f"{what}: cos and sin must be [T, D] or [B, T, D] of T = {tokens}, D = {d}")
-        cos, sin = cos.to(torch.float32).contiguous(), sin.to(torch.float32).contiguous()
+        cos, sin = _fp32(cos), _fp32(sin)
         own = tokens * d if cos.dim() == 3 and cos.shape[0] > 1 else 0
         return cos.data_ptr(), sin.data_ptr(), 0, 0, own, 0, 0, 0, (0, 0, 0, 0), 0, 0, (cos, sin)
     positions, inv_freq, sections, interleaved = axes
@@ -120,7 +124,7 @@ def _rotation(what, dev, batch, tokens, d, tables, axes):
         raise ValueError(f"{what}: inv_freq must hold {d // 2} frequencies")
     if positions.stride(-1) != 1 and tokens > 1:
         positions = positions.contiguous()
-    inv_freq = inv_freq.to(torch.float32).contiguous()
+    inv_freq = _fp32(inv_freq)
     per_batch = positions.stride(1) if positions.dim() == 3 and positions.shape[1] > 1 else 0
     return (0, 0, positions.data_ptr(), inv_freq.data_ptr(), 0, positions.stride(0), per_batch, n,
             sections + (0,) * (4 - n), int(bool(interleaved)), int(positions.dtype == torch.int64),
