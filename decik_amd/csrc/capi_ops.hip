@@ -121,7 +121,9 @@ int qk_rope_common(const dk_qk_rope* d, QkRopeArgs* a) {
 constexpr int64_t kInt8MaxK = 131071, kInt8MaxLd = int64_t(1) << 23, kInt8MaxRows = int64_t(1) << 23;
 
 bool int8_sizes(int64_t m, int64_t n, int64_t k) {
-    return m >= 0 && n >= 0 && k >= 1 && k <= kInt8MaxK && m < kInt8MaxRows && n < kInt8MaxRows;
+    // (work-groups of the largest outputs fit a launch)
+    return m >= 0 && n >= 0 && k >= 1 && k <= kInt8MaxK && m < kInt8MaxRows && n < kInt8MaxRows &&
+           m * n < (int64_t(1) << 38);
 }
 
 bool int8_rows_ok(const void* p, int64_t ld, int64_t cols) {
@@ -243,7 +245,7 @@ int dk_int8_quantize(const void* x, int x_dtype, int64_t ldx, const float* col_s
 int64_t dk_int8_linear_workspace(int transposed, int64_t m, int64_t n, int64_t k) {
     dk_clear_error();
     if (!int8_sizes(m, n, k)) {
-        dk_fail("dk_int8_linear: 0 <= m, n < 2^23, 1 <= k <= 131071");
+        dk_fail("dk_int8_linear: 0 <= m, n < 2^23, m n < 2^38, 1 <= k <= 131071");
         return -1;
     }
     return int8_plan(m, n, k, transposed != 0).partial_bytes;
@@ -252,7 +254,7 @@ int64_t dk_int8_linear_workspace(int transposed, int64_t m, int64_t n, int64_t k
 int dk_int8_linear_plan(int transposed, int64_t m, int64_t n, int64_t k, int32_t* out) {
     dk_clear_error();
     if (!int8_sizes(m, n, k) || out == nullptr)
-        return dk_fail("dk_int8_linear_plan: 0 <= m, n < 2^23, 1 <= k <= 131071, out set");
+        return dk_fail("dk_int8_linear_plan: 0 <= m, n < 2^23, m n < 2^38, 1 <= k <= 131071, out set");
     const Int8Plan p = int8_plan(m, n, k, transposed != 0);
     out[0] = p.few ? 0 : p.tm;
     out[1] = p.few ? 16 : p.bn;
@@ -265,7 +267,7 @@ int dk_int8_linear(int transposed, const int8_t* xq, int64_t ldx, const float* x
                    const float* ws, const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t m,
                    int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, void* stream) {
     dk_clear_error();
-    if (!int8_sizes(m, n, k)) return dk_fail("dk_int8_linear: 0 <= m, n < 2^23, 1 <= k <= 131071");
+    if (!int8_sizes(m, n, k)) return dk_fail("dk_int8_linear: 0 <= m, n < 2^23, m n < 2^38, 1 <= k <= 131071");
     if (!is_dtype(y_dtype) || (bias != nullptr && !is_dtype(bias_dtype)))
         return dk_fail("dk_int8_linear: unknown type");
     if (transposed && (ws != nullptr || bias != nullptr))
@@ -305,7 +307,7 @@ int64_t dk_int8_linear_x_workspace(int backward, int64_t m, int64_t n, int64_t k
     dk_clear_error();
     const int64_t rows = m, cols = backward ? n : k, out = backward ? k : n;
     if (!int8_sizes(rows, out, cols) || (backward && k < 1)) {
-        dk_fail("dk_int8_linear: 0 <= m, n < 2^23, 1 <= k <= 131071 (backward: 1 <= n <= 131071)");
+        dk_fail("dk_int8_linear: 0 <= m, n < 2^23, m n < 2^38, 1 <= k <= 131071 (backward: m, k and n)");
         return -1;
     }
     if (m == 0 || out == 0 || int8_fused(m, cols, backward != 0)) return 0;
@@ -352,7 +354,7 @@ int dk_int8_linear_fwd(const void* x, int x_dtype, int64_t ldx, const int8_t* wq
                        const void* bias, int bias_dtype, void* y, int y_dtype, int64_t ldy, int64_t m, int64_t n,
                        int64_t k, void* workspace, int64_t workspace_bytes, void* stream) {
     dk_clear_error();
-    if (!int8_sizes(m, n, k)) return dk_fail("dk_int8_linear_fwd: 0 <= m, n < 2^23, 1 <= k <= 131071");
+    if (!int8_sizes(m, n, k)) return dk_fail("dk_int8_linear_fwd: 0 <= m, n < 2^23, m n < 2^38, 1 <= k <= 131071");
     return int8_linear_x(false, x, x_dtype, ldx, wq, ldw, ws, bias, bias_dtype, y, y_dtype, ldy, m, n, k, workspace,
                          workspace_bytes, stream);
 }
@@ -361,7 +363,7 @@ int dk_int8_linear_bwd(const void* dy, int dy_dtype, int64_t lddy, const int8_t*
                        void* dx, int dx_dtype, int64_t lddx, int64_t m, int64_t n, int64_t k, void* workspace,
                        int64_t workspace_bytes, void* stream) {
     dk_clear_error();
-    if (!int8_sizes(m, k, n)) return dk_fail("dk_int8_linear_bwd: 0 <= m, k < 2^23, 1 <= n <= 131071");
+    if (!int8_sizes(m, k, n)) return dk_fail("dk_int8_linear_bwd: 0 <= m, k < 2^23, m k < 2^38, 1 <= n <= 131071");
     return int8_linear_x(true, dy, dy_dtype, lddy, wq, ldw, ws, nullptr, 0, dx, dx_dtype, lddx, m, k, n, workspace,
                          workspace_bytes, stream);
 }

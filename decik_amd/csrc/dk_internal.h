@@ -298,6 +298,7 @@ struct Int8GemmArgs {
     int64_t ldx, ldw, ldy, slab;
     int32_t m, n, k, bias_dtype, ldp;
     int32_t m_tiles, n_tiles, splits, steps_per_split;
+    bool past_caches;  // y is larger than the caches
 };
 struct Int8Plan {
     bool few;

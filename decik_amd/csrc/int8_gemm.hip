@@ -5,12 +5,22 @@
 // Sums are exact in 32-bit integers (k <= 131071), so neither the order nor the split of k changes a
 // result; the scales are applied in fp32 and rounded once.
 //
-// Work-group: 8 waves, tile of TM tokens by 256 channels, steps of 128 along k. Both operands go
-// straight to LDS (16 bytes a lane) through a ring of stages, STAGES - 1 steps ahead; one wait and one
-// barrier a step. Rows of a stage are 128 bytes, their 16-byte chunks permuted by row so that the
-// operand reads (32 rows at one chunk) spread over the banks. TR stages wq as it lies (rows along k,
-// 256 bytes) and turns it through the transposed LDS read of 8-bit elements: in each 16 lanes, lanes
-// 2 r and 2 r + 1 read the 16 bytes of row r, lane i receives byte i of the 8 rows.
+// Work-group: tiles of 256, 128 or 64 tokens by 256 channels (eight waves) or 64 by 64 (four), steps of 128
+// along k. Both operands go straight to LDS (16 bytes a lane) through a ring of stages; one wait and one
+// barrier a step, before its last part, so that the next step's first operands are read behind MFMAs too.
+// Rows of a stage are 128 bytes, their 16-byte chunks permuted by row so that the operand reads (32 rows at
+// one chunk) spread over the banks. TR stages wq as it lies (rows along k, a row of the tile's channels each)
+// and turns it through the transposed LDS read of 8-bit elements: in each 16 lanes, lanes 2 r and 2 r + 1
+// read the 16 bytes of row r, lane i receives byte i of the 8 rows.
+//
+// Bound: at [8192, 18944] x 3584 the forward takes 541 us (2.06 POP/s), the input gradient 512 (2.17); torch's
+// library product of the same sizes, without scales, 616 and 571. Matrix cores are busy half of the cycles at
+// 2.0 GHz. Timing copies without the loads of the loop take 480 and 430 us, without the operand reads 550 and
+// 550, without either 440 and 380: the loads cost most, through their issue and the L2's bandwidth (64 KB a
+// step and CU), not through latency (lines touched a step or more ahead in the L2 made it 3 to 8% slower).
+// The last round of tiles is 7 to 12% idle. Also measured, not kept: tiles of 128 by 128 on four waves, two
+// work-groups a CU (equal or slower everywhere), operand reads pinned before the MFMAs (+0 to 5%), bands of
+// four token tiles (equal).
 #include "elem.h"
 #include "gemm_common.h"
 
@@ -45,8 +55,7 @@ __device__ __forceinline__ int4_t lds128(const uint8_t* p) { return *(const int4
 
 // Operands from a TR stage: 16 rows of a lane's byte column, two transposed reads of 8 rows each. One asm
 // block with its own wait: the builtin counts as aliasing every load to LDS in flight and would drain the
-// ring at every read.
-// R8: bytes of 8 rows; the next slice is 4 R8 on.
+// ring at every read. R8: bytes of 8 rows; the next slice is 4 R8 on.
 template <int R8>
 __device__ __forceinline__ void lds_tr8(const uint8_t* st, const uint32_t (&at)[2], int4_t (&o)[1][2]) {
     int2v_t a, b, c, d;
@@ -413,7 +422,9 @@ __global__ __launch_bounds__(64 * i8_waves(BN), 2) void int8_gemm_kernel(const I
                 const typename Elem<OUT>::vec v = *(const typename Elem<OUT>::vec*)(stage + row * ROW + 2 * c);
                 if (m >= a.m || n >= a.n) continue;
                 E* const y = (E*)a.y + (int64_t)m * a.ldy + n;
-                if (n + 8 <= a.n) {
+                if (n + 8 <= a.n && a.past_caches) {
+                    __builtin_nontemporal_store(v, (typename Elem<OUT>::loose*)y);
+                } else if (n + 8 <= a.n) {
                     *(typename Elem<OUT>::loose*)y = v;
                 } else {
 #pragma unroll
@@ -507,7 +518,9 @@ __device__ __forceinline__ void quant_scale(uint32_t top, float& inv, float& sca
 }
 
 // The row stays in registers between its maximum and its rounding (R groups of eight a thread), or is read
-// again (R = 0). THREADS threads a row.
+// again (R = 0). THREADS threads a row. Bound: HBM, at [8192, 18944] fp16 with column scales 107 us (4.35
+// TB/s; a large copy reaches 5.2), [8192, 3584] 18.3. Several rows a work-group, the column scales read once
+// for them, were slower (175 and 25.7 us: fewer waves).
 template <int DT, bool COL, int THREADS, int R>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void int8_quantize_kernel(const Int8QuantArgs a) {
     constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, ROWS = BLOCK / THREADS, NW = THREADS / 64;
@@ -631,8 +644,7 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Int8GemmArgs
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int t = 0; t < MT; ++t)
-                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u],
-                                                               xf[u][t], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], xf[u][t], acc[t], 0, 0, 0);
     }
     // lane: channels 4 (lane / 16) + 0..3 of token l16
 #pragma unroll
@@ -759,9 +771,9 @@ static Int8Plan make_plan(int64_t m, int64_t n, int64_t k, int cus, bool tr) {
         }
     }
     // Few tokens: the streaming kernel where its estimate is the smaller one, weights from memory on both sides
-    // (the tiles' estimate knows them in the caches). Measured, streaming / tiles, us: [3584, 3584] 9.1 / 12.0 at 8 tokens, 11.1 /
-    // 12.2 at 32; [8960, 1536] 9.4 / 9.6 and 13.5 / 10.2; [18944, 3584] 22.3 / 21.4 and 35.1 / 23.2; [3584] x
-    // 18944 27.0 / 23.3 at 8; [512] x 3584 7.9 / 10.0 and 10.3 / 10.6.
+    // (the tiles' estimate knows them in the caches). Measured, streaming / tiles, us: [3584, 3584] 9.1 / 12.0
+    // at 8 tokens, 11.1 / 12.2 at 32; [8960, 1536] 9.4 / 9.6 and 13.5 / 10.2; [18944, 3584] 22.3 / 21.4 and 35.1
+    // / 23.2; [3584] x 18944 27.0 / 23.3 at 8; [512] x 3584 7.9 / 10.0 and 10.3 / 10.6.
     const double few_us = 6.5 + n * k / 5.5e6 + m * n * k * 7.9e-9 + k * 3e-4;
     if (!tr && m <= kInt8FewM && few_us < best_us + 3.0 + n * k / 1.4e7) {
         best = Int8Plan{};
@@ -868,6 +880,9 @@ hipError_t launch_int8_gemm(Int8GemmArgs a, const Int8Plan& p, int out_dtype, bo
     a.n_tiles = p.n_tiles;
     a.splits = p.splits;
     a.steps_per_split = p.steps_per_split;
+    // an output past the size of the last cache leaves non-temporally ([8192, 18944] 556 -> 543 us); a smaller
+    // one stays for its reader, though its own launch would be faster too ([830, 8960] 18.2 against 16.7)
+    a.past_caches = a.m * (int64_t)a.n * elem_bytes(out_dtype) > (int64_t(1) << 28);
     if (p.splits == 1) {
         if (out_dtype == DK_FP16) return launch_out<DK_FP16>(a, p, tr, s);
         if (out_dtype == DK_BF16) return launch_out<DK_BF16>(a, p, tr, s);

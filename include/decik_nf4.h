@@ -370,8 +370,8 @@ int dk_qk_rope_bwd(const dk_qk_rope* a, void* workspace, int64_t workspace_bytes
  * with weight wq, xq and xs quantized from dY with col_scale = ws. The sums are exact, the result is
  * fp32(sum) * xs * ws + bias rounded once to y_dtype. xq [m, k]: zeros from k to the next multiple of 16;
  * rows of wq (and xq) are read to the next multiple of 16 of their columns, which must be allocated, with
- * whatever values. Row strides of xq and wq: multiples of 16 below 2^23, 16-byte aligned starts. bias NULL
- * or of bias_dtype. workspace: dk_int8_linear_workspace bytes (0: none). */
+ * whatever values. Row strides of xq and wq: multiples of 16 below 2^23, 16-byte aligned starts. 0 <= m, n <
+ * 2^23, m n < 2^38, 1 <= k <= 131071. bias NULL or of bias_dtype. workspace: dk_int8_linear_workspace bytes (0: none). */
 int dk_int8_quantize(const void* x, int x_dtype, int64_t ldx, const float* col_scale, int8_t* q, int64_t ldq,
                      float* scale, int64_t rows, int64_t k, void* stream);
 int64_t dk_int8_linear_workspace(int transposed, int64_t m, int64_t n, int64_t k);

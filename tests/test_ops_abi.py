@@ -148,7 +148,8 @@ def lin(tr=0, xq=P, ldx=64, xs=P, wq=P, ldw=64, ws=P, bias=None, bdt=0, y=P, ydt
 
 
 @pytest.mark.parametrize("kw,msg", [
-    (dict(m=-1), "2^23"), (dict(n=1 << 23), "2^23"), (dict(k=131072), "131071"), (dict(ydt=3), "type"), (dict(bias=P, bdt=9), "type"),
+    (dict(m=-1), "2^23"), (dict(n=1 << 23), "2^23"), (dict(m=1 << 20, n=1 << 18), "2^38"), (dict(k=131072), "131071"),
+    (dict(ydt=3), "type"), (dict(bias=P, bdt=9), "type"),
     (dict(tr=1), "transposed"), (dict(tr=1, ws=None, bias=P), "transposed"), (dict(xq=None), "null"), (dict(ws=None), "null"),
     (dict(y=None), "null"), (dict(ldx=56), "aligned"), (dict(xq=P + 4), "aligned"), (dict(ldw=60), "aligned"),
     (dict(tr=1, ws=None, ldw=16), "aligned"), (dict(ldy=31), "overlap"), (dict(m=300, k=131071, ldx=131072, ldw=131072), "workspace")])
