@@ -194,7 +194,7 @@ int64_t dk_qk_rope_bwd_workspace(const dk_qk_rope* d) {
     QkRopeArgs a{};
     if (qk_rope_common(d, &a) != 0) return -1;
     if (d->dw_q == nullptr || d->q_weight == nullptr || a.rows == 0) return 0;
-    return (int64_t)qk_rope_groups(a.rows, qk_rope_passes(a.hq, a.hk, a.d)) * 2 * a.d * (int64_t)sizeof(float);
+    return (int64_t)qk_rope_groups(a.rows, qk_rope_passes(a.hq, a.hk, a.d), true) * 2 * a.d * (int64_t)sizeof(float);
 }
 
 int dk_qk_rope_bwd(const dk_qk_rope* d, void* workspace, int64_t workspace_bytes, void* stream) {

@@ -279,7 +279,7 @@ struct QkRopeArgs {
 };
 // work-groups (slabs) of a launch
 int qk_rope_passes(int hq, int hk, int d);
-int qk_rope_groups(int64_t rows, int passes);
+int qk_rope_groups(int64_t rows, int passes, bool norm);
 hipError_t launch_qk_rope(QkRopeArgs a, int dtype, bool norm, bool axes, bool backward, float* dwq, float* dwk,
                           hipStream_t s);
 

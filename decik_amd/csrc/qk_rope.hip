@@ -13,7 +13,7 @@
 // position and frequency would be off by 2^-5.
 //
 // Bound: HBM (read and write of q and k, in the backward gradients, q and k in and dq, dk out): 8192 tokens of
-// 28 + 4 heads of 128, bf16, with norms: forward 31 us (4.6 TB/s), backward 45 (4.6 TB/s) and 4 for the sums of
+// 28 + 4 heads of 128, bf16, with norms: forward 30 us (4.8 TB/s), backward 39 (5.4 TB/s) and 4 for the sums of
 // dw; three axes without norms over 4096 tokens, fp16, 13.5 us each way (5.0 TB/s); a large copy reaches 5.2.
 // At 830 tokens 4.4 and 7.4 us, a few memory round trips.
 // Layout: a lane holds eight elements of a and their eight partners of b (two 16-byte loads, the
@@ -265,14 +265,17 @@ int qk_rope_passes(int hq, int hk, int d) {
     return (hq + hk + hpw - 1) / hpw;
 }
 
-// tokens in flight: enough waves to fill the device, each with several tokens where there are many
-int qk_rope_streams(int64_t rows, int passes) {
-    const int64_t want = kQkMaxWaves / passes;
+// Streams of tokens: as many waves as run at once (the backward with norms takes 150 registers: three a SIMD),
+// each with several tokens where there are many. At 8192 tokens the norms take 39 us backward with 3072 waves
+// against 46 with 4096 (a third of them in a second round), 39 with 2048; forward 30, 31, 35. Without norms
+// 13.7 us with 4096 over 4096 tokens, 14.1 with 3072.
+static int qk_rope_streams(int64_t rows, int passes, bool norm) {
+    const int64_t want = (norm ? 3 * kQkMaxWaves / 4 : kQkMaxWaves) / passes;
     return (int)(rows < want ? rows : (want > 0 ? want : 1));
 }
 
-int qk_rope_groups(int64_t rows, int passes) {
-    return (passes * qk_rope_streams(rows, passes) + kQkWaves - 1) / kQkWaves;
+int qk_rope_groups(int64_t rows, int passes, bool norm) {
+    return (passes * qk_rope_streams(rows, passes, norm) + kQkWaves - 1) / kQkWaves;
 }
 
 template <int DT, int LPH, bool BWD>
@@ -309,8 +312,8 @@ hipError_t launch_qk_rope(QkRopeArgs a, int dtype, bool norm, bool axes, bool ba
         return hipGetLastError();
     }
     a.passes = qk_rope_passes(a.hq, a.hk, a.d);
-    a.streams = qk_rope_streams(a.rows, a.passes);
-    const unsigned grid = (unsigned)qk_rope_groups(a.rows, a.passes);
+    a.streams = qk_rope_streams(a.rows, a.passes, norm);
+    const unsigned grid = (unsigned)qk_rope_groups(a.rows, a.passes, norm);
     if (dtype == DK_FP16) {
         if (backward)
             launch_typed<DK_FP16, true>(a, norm, axes, grid, s);
