@@ -57,7 +57,8 @@ __device__ __forceinline__ int axis_of(const QkRopeArgs& a, int j) {
 
 __device__ __forceinline__ uint64_t turn_fraction(float inv_freq) {
     const double turns = (double)inv_freq * 0.15915494309189533577;
-    return (uint64_t)((turns - floor(turns)) * 18446744073709551616.0);
+    const double part = turns - floor(turns);  // 1 for a tiny negative frequency: a whole turn, as 0
+    return part < 1.0 ? (uint64_t)(part * 18446744073709551616.0) : 0;
 }
 
 template <int DT, int LPH, bool NORM, bool AXES, bool BWD>

@@ -195,6 +195,23 @@ def test_far_positions(device):
     check(out, ref["out"], 2.0 ** -18, "q")
 
 
+@pytest.mark.parametrize("freq", [-1.0, -1e-3, -2.0 ** -40, -1e-30, 1e-30, 0.0])
+def test_signs_of_frequencies(freq, device):
+    """Negative frequencies turn the other way, tiny ones not at all."""
+    from decik_amd.rope import axes_rope_forward
+
+    d, t = 64, 5
+    q, k, _, _ = inputs(1, t, 2, 1, d, torch.float16, device)
+    pos = torch.tensor([[0, 1, 77, 2 ** 20, 2 ** 28]])
+    inv = torch.full((d // 2,), freq, dtype=torch.float32, device=device)
+    out = axes_rope_forward(q, k, pos.to(device), inv, [d // 2], 2, 1)[0]
+    angle = (pos.numpy()[0][:, None].astype(np.longdouble) * f64(inv).astype(np.longdouble))[None]
+    cos, sin = np.cos(angle).astype(np.float64), np.sin(angle).astype(np.float64)
+    ref = reference(f64(q), None, None, both(cos), both(sin), 2, 0)
+    # the fraction's error, 2^-54 turns a position at most: 2^-26 turns = 2^-23 radians at 2^28
+    check(out, ref["out"], 2.0 ** -18, "q")
+
+
 def test_strides(device):
     from decik_amd.rope import axes_rope_forward, qk_norm_rope_backward, qk_norm_rope_forward
 
