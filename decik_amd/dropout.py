@@ -15,6 +15,7 @@ call with n branches uses up n offsets.
 import struct
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import DTYPES, call_on, gpu_input, lib, same_gpu
 
@@ -120,6 +121,7 @@ class SeededDropout(torch.autograd.Function):
         return outs
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         (rng,) = ctx.saved_tensors
         if all(g is None for g in grads):

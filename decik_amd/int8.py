@@ -14,6 +14,7 @@ Quantized rows are padded to 128 bytes; the tensors here are views of the padded
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import DTYPES, call_on, check, gpu_input, lib, same_gpu
 
@@ -180,13 +181,14 @@ class Int8Linear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, wq, w_scale, bias=None):
-        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+        if any(ctx.needs_input_grad[2:]):  # (three inputs where the call names no bias)
             raise ValueError("Int8Linear: the weight's scales and the bias are frozen (detach them)")
         ctx.save_for_backward(wq, w_scale)
         ctx.x_dtype = x.dtype
         return int8_linear_forward(x, wq, w_scale, bias)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         wq, w_scale = ctx.saved_tensors
         return int8_linear_backward(grad, wq, w_scale, dtype=ctx.x_dtype), None, None, None

@@ -18,6 +18,7 @@ the same pair with masks from a counter-based generator, formed again in the bac
 """
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import nf4 as _nf4
 from . import _lib
@@ -346,6 +347,7 @@ class LoRAPairSeeded(torch.autograd.Function):
         return out_q, out_v
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_q, grad_v):
         x, rng, u_q, u_v, a_q, b_q, a_v, b_v = ctx.saved_tensors
         grad_x, adapter_grads = _qv_lora_backward(x, _QVSeeded(rng, ctx.ps), ((a_q, b_q), (a_v, b_v)), ctx.scalings,

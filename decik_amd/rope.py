@@ -16,6 +16,7 @@ and give them head-major [B, H, T, D]; everything is computed in fp32 and rounde
 """
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import DTYPES, QkRope, call_on, check, gpu_input, lib, ptr, same_gpu, stream_of
 
@@ -268,6 +269,7 @@ class _QkRotation(torch.autograd.Function):
         return outs
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         if all(g is None for g in grads):
             return (None,) * 9

@@ -9,6 +9,8 @@ import numpy as np
 import pytest
 import torch
 
+from helpers import randn16
+
 pytestmark = pytest.mark.gpu
 
 TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -149}
@@ -286,6 +288,20 @@ def test_autograd(device):
     xi, xs = quantized(x.detach().reshape(66, 96))
     lin = torch.from_numpy(xi * xs.astype(np.float64)[:, None]).to(device) @ w.T + bias.double()
     assert bool(((y.reshape(66, 130).double() - lin).abs() <= lin.abs() * 2.0 ** -11 + 2.0 ** -16).all())
+
+
+def test_without_bias(device):
+    """The bias left out of the call, or given as None: the same values and gradients."""
+    from decik_amd.int8 import Int8Linear, quantize_int8
+
+    w = quantize_int8(randn16((48, 80), 3, device))
+    results = []
+    for args in (w, (*w, None)):
+        x = randn16((5, 80), 4, device).requires_grad_(True)
+        y = Int8Linear.apply(x, *args)
+        results.append((y, torch.autograd.grad(y, x, torch.ones_like(y))[0]))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
 
 
 def test_captured_graphs(device):

@@ -161,3 +161,32 @@ def test_captured_layer_steps(device):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(results, want))
         assert not torch.equal(results[0], results[0] * 0)
+
+
+def test_second_derivatives_are_refused(device):
+    """A gradient taken with create_graph is right, and differentiating it again raises instead of leaving
+    the operators' part out."""
+    from decik_amd.dropout import rng_state, seeded_dropout
+    from decik_amd.int8 import Int8Linear, quantize_int8
+    from decik_amd.lora import LoRAPairSeeded
+    from decik_amd.rope import axes_rope
+
+    rng = rng_state(1, 0, device)
+    ab = [randn16(s, i, device, 0.05) for i, s in enumerate(((16, 64), (64, 16), (16, 64), (64, 16)))]
+    w = quantize_int8(randn16((64, 64), 8, device))
+    pos, inv = torch.arange(8, device=device)[None], torch.ones(16, device=device)
+    calls = {
+        "dropout": lambda x: seeded_dropout(x, rng, 0.25),
+        "pair": lambda x: LoRAPairSeeded.apply(x, rng, *ab, 2.0, 2.0, 0.25, 0.25)[0],
+        "rotation": lambda x: axes_rope(x, x, pos, inv, [16], 2, 2)[0],
+        "int8": lambda x: Int8Linear.apply(x, *w),
+    }
+    for name, call in calls.items():
+        x = randn16((8, 64), 9, device).requires_grad_(True)
+        y = call(x)
+        loss = (y.float() ** 2).sum()
+        once = torch.autograd.grad(loss, x, retain_graph=True)[0]
+        again = torch.autograd.grad(loss, x, create_graph=True)[0]
+        assert torch.equal(once, again.detach()), name
+        with pytest.raises(RuntimeError, match="twice"):
+            (again.float() ** 2).sum().backward()
