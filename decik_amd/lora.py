@@ -23,7 +23,7 @@ from torch.autograd.function import once_differentiable
 from . import nf4 as _nf4
 from . import _lib
 from .dropout import dropout_backward, dropout_forward
-from ._lib import check, lib, ptr, stream_of
+from ._lib import check, gpu_input, lib, ptr, same_gpu, stream_of
 
 
 def _plain(x, keep_bits):
@@ -334,14 +334,32 @@ class LoRAPairSeeded(torch.autograd.Function):
     scaling_q, scaling_v, p_q, p_v) -> (out_q, out_v) fp16, as LoRAPair with the masks of
     decik_amd.dropout at rng (int64 device tensor: seed, offset; the call uses up two offsets). The
     backward forms the same masks again; rng must not change before it. x: [.., W] fp16 or fp32;
-    gradients reach x (fp32) and the adapters."""
+    a_* [r, W], b_* [N, r] of one rank, 16 or 32; gradients reach x (in its type) and the adapters."""
+
+    @staticmethod
+    def _check(x, rng, adapters):
+        what = "LoRAPairSeeded"
+        dev = gpu_input(what, x)
+        same_gpu(what, dev, rng, *(t for pair in adapters for t in pair))
+        if x.dtype not in (torch.float16, torch.float32) or x.dim() < 1:
+            raise ValueError(f"{what}: x must be fp16 or fp32 [.., W]")
+        rank = adapters[0][0].shape[0]
+        for a, b in adapters:
+            if a.shape != (rank, x.shape[-1]) or b.dim() != 2 or b.shape[1] != rank or rank not in (16, 32):
+                raise ValueError(f"{what}: adapters must be a [r, {x.shape[-1]}] and b [N, r] of one rank, 16 or 32")
+        return dev
 
     @staticmethod
     def forward(ctx, x, rng, a_q, b_q, a_v, b_v, scaling_q, scaling_v, p_q, p_v):
-        if x.dtype not in (torch.float16, torch.float32):
-            raise ValueError("LoRAPairSeeded: x must be fp16 or fp32")
+        adapters = (a_q, b_q), (a_v, b_v)
+        dev = LoRAPairSeeded._check(x, rng, adapters)
         scalings, ps = (scaling_q, scaling_v), (float(p_q), float(p_v))
-        out_q, out_v, u_q, u_v = _qv_lora_forward(x, _QVSeeded(rng, ps), ((a_q, b_q), (a_v, b_v)), scalings)
+        if x.numel() == 0:  # no tokens: nothing to launch
+            out_q, out_v = (x.new_empty((*x.shape[:-1], b.shape[0]), dtype=torch.float16) for _, b in adapters)
+            u_q = u_v = None
+        else:
+            with torch.cuda.device(dev):
+                out_q, out_v, u_q, u_v = _qv_lora_forward(x, _QVSeeded(rng, ps), adapters, scalings)
         ctx.save_for_backward(x, rng, u_q, u_v, a_q, b_q, a_v, b_v)
         ctx.scalings, ctx.ps = scalings, ps
         return out_q, out_v
@@ -350,6 +368,8 @@ class LoRAPairSeeded(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_q, grad_v):
         x, rng, u_q, u_v, a_q, b_q, a_v, b_v = ctx.saved_tensors
+        if x.numel() == 0:
+            return (torch.zeros_like(x), None, *(torch.zeros_like(t) for t in (a_q, b_q, a_v, b_v)), *(None,) * 4)
         grad_x, adapter_grads = _qv_lora_backward(x, _QVSeeded(rng, ctx.ps), ((a_q, b_q), (a_v, b_v)), ctx.scalings,
                                                   (u_q, u_v), (grad_q, grad_v))
         return (grad_x.to(x.dtype), None, *adapter_grads, *(None,) * 4)

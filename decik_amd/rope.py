@@ -258,6 +258,8 @@ class _QkRotation(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, heads, eps, rotation, *tensors):
+        if any(ctx.needs_input_grad[7:]):
+            raise ValueError("qk rotation: tables and frequencies take no gradient (detach them)")
         d = tensors[0].shape[-1] if rotation[0] == "tables" else 2 * tensors[1].shape[-1]
         outs = _qk_forward("qk rotation", q, k, q_weight, k_weight, *heads, eps, d,
                            **_QkRotation._named(rotation, tensors))

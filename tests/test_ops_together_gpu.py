@@ -190,3 +190,32 @@ def test_second_derivatives_are_refused(device):
         assert torch.equal(once, again.detach()), name
         with pytest.raises(RuntimeError, match="twice"):
             (again.float() ** 2).sum().backward()
+
+
+def test_seeded_pair_edges(device):
+    """No tokens, one token, a middle axis, views; adapters that do not fit are refused."""
+    from decik_amd.dropout import rng_state
+    from decik_amd.lora import LoRAPairSeeded
+
+    w, r, rng = 64, 16, rng_state(1, 0, device)
+    ab = [randn16(s, i, device, 0.05).requires_grad_(True) for i, s in enumerate(((r, w), (48, r), (r, w), (32, r)))]
+    for shape in ((0, w), (2, 0, w), (1, w), (2, 3, w)):
+        x = randn16(shape, 5, device).requires_grad_(True)
+        q, v = LoRAPairSeeded.apply(x, rng, *ab, 2.0, 2.0, 0.5, 0.25)
+        assert q.shape == (*shape[:-1], 48) and v.shape == (*shape[:-1], 32)
+        grads = torch.autograd.grad(q.float().sum() + v.float().sum(), [x, *ab])
+        for g, t in zip(grads, [x, *ab]):
+            assert g.shape == t.shape and g.dtype == t.dtype and bool(g.isfinite().all())
+            assert x.numel() > 0 or not bool(g.any())
+    x = randn16((6, 2 * w), 6, device)
+    for view in (x[:, w:], x[::2, :w], x[:, ::2]):
+        outs = [LoRAPairSeeded.apply(t, rng, *ab, 2.0, 2.0, 0.5, 0.25) for t in (view, view.contiguous())]
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
+    x = x[:, :w]
+    for bad in ([ab[0][:, :32], *ab[1:]], [ab[0][:8], ab[1][:, :8], ab[2][:8], ab[3][:, :8]], [*ab[:3], ab[3][:, :8]],
+                [*ab[:2], torch.cat([ab[2]] * 2), torch.cat([ab[3]] * 2, 1)], [ab[0].cpu(), *ab[1:]]):
+        with pytest.raises(ValueError):
+            LoRAPairSeeded.apply(x, rng, *bad, 2.0, 2.0, 0.5, 0.25)
+    for args in ((x.bfloat16(), rng), (x.cpu(), rng), (x, rng.cpu())):
+        with pytest.raises(ValueError):
+            LoRAPairSeeded.apply(*args, *ab, 2.0, 2.0, 0.5, 0.25)

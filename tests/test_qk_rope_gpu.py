@@ -396,6 +396,11 @@ def test_refusals(device):
     for call in bad:
         with pytest.raises(ValueError):
             call()
+    from decik_amd.rope import axes_rope, qk_norm_rope
+    for call in (lambda: qk_norm_rope(q, k, w, w, tab.clone().requires_grad_(True), tab, h, hk),
+                 lambda: axes_rope(q, k, pos, inv.clone().requires_grad_(True), [16], h, hk)):
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
     for sections in ([15], [-1]):
         with pytest.raises(DecikError, match="sections"):
             axes_rope_forward(q, k, pos, inv, sections, h, hk)
