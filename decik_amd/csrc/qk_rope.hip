@@ -267,9 +267,9 @@ int qk_rope_passes(int hq, int hk, int d) {
 }
 
 // Streams of tokens: as many waves as run at once (the backward with norms takes 150 registers: three a SIMD),
-// each with several tokens where there are many. At 8192 tokens the norms take 39 us backward with 3072 waves
-// against 46 with 4096 (a third of them in a second round), 39 with 2048; forward 30, 31, 35. Without norms
-// 13.7 us with 4096 over 4096 tokens, 14.1 with 3072.
+// each with several tokens where there are many. At 8192 tokens the norms take 39 us backward with three waves a
+// SIMD against 46 with four (a fourth of them in a second round), 39 with two; forward 30, 31, 35. Without norms
+// 13.7 us with four over 4096 tokens, 14.1 with three.
 static int qk_rope_streams(int64_t rows, int passes, bool norm) {
     const int64_t want = (norm ? 3 * kQkMaxWaves / 4 : kQkMaxWaves) / passes;
     return (int)(rows < want ? rows : (want > 0 ? want : 1));
