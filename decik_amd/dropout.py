@@ -71,7 +71,7 @@ def dropout_forward(x, rng, ps, dtype=None):
     x2 = _rows(x)
     rows, width = x2.shape
     n = len(ps)
-    outs = tuple([x.new_empty(x.shape, dtype=dtype) for _ in ps])
+    outs = tuple([torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format) for _ in ps])
     call_on(dev, lib().dk_dropout_fwd, x2.data_ptr(), a, x2.stride(0), rng.data_ptr(), p, n,
             _POINTERS[n](*[o.data_ptr() for o in outs]), b, _LONGS[n](*[width] * n), rows, width)
     return outs
@@ -101,7 +101,7 @@ def dropout_backward(grads, rng, ps, dtype=None):
         lds.append(g2.stride(0))
     rows, width = rows2[0].shape
     n = len(ps)
-    dx = g0.new_empty(g0.shape, dtype=dtype)
+    dx = torch.empty_like(g0, dtype=dtype, memory_format=torch.contiguous_format)
     call_on(dev, lib().dk_dropout_bwd, _POINTERS[n](*ptrs), a, _LONGS[n](*lds), rng.data_ptr(), p, n, dx.data_ptr(), b,
             width, rows, width)
     return dx

@@ -52,7 +52,7 @@ def quantize_int8(x, col_scale=None):
             raise ValueError(f"{what}: col_scale must be fp32 [{k}]")
         col_scale = col_scale.contiguous()
     ld = (k + 127) // 128 * 128
-    q = x.new_empty((rows, ld), dtype=torch.int8)
+    q = x.new_empty(rows, ld, dtype=torch.int8)
     scale = x.new_empty(rows, dtype=torch.float32)
     call_on(dev, lib().dk_int8_quantize, x2.data_ptr(), code, x2.stride(0), _ptr(col_scale), q.data_ptr(), ld,
             scale.data_ptr(), rows, k)
@@ -122,7 +122,7 @@ def int8_matmul(xq, x_scale, wq, w_scale, bias=None, dtype=torch.float16):
     wq, ldw = _int8_rows(what, "wq", wq, False)
     x_scale = x_scale.contiguous()
     ws, bias, bias_code = _channel_args(what, w_scale, bias, n)
-    y = xq.new_empty((m, n), dtype=dtype)
+    y = xq.new_empty(m, n, dtype=dtype)
     need = lib().dk_int8_linear_workspace(0, m, n, k)
     work = _workspace(xq, need)
     call_on(dev, lib().dk_int8_linear, 0, xq.data_ptr(), ldx, x_scale.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(),
@@ -145,7 +145,7 @@ def int8_linear_forward(x, wq, w_scale, bias=None, dtype=None):
     ws, bias, bias_code = _channel_args(what, w_scale, bias, n)
     x2 = _token_rows(x)
     m = x2.shape[0]
-    y = x.new_empty((*x.shape[:-1], n), dtype=dtype)
+    y = x.new_empty(*x.shape[:-1], n, dtype=dtype)
     need = lib().dk_int8_linear_x_workspace(0, m, n, k)
     work = _workspace(x, need)
     call_on(dev, lib().dk_int8_linear_fwd, x2.data_ptr(), code, x2.stride(0), wq.data_ptr(), ldw, ws.data_ptr(),
@@ -168,7 +168,7 @@ def int8_linear_backward(dy, wq, w_scale, k=None, dtype=None):
     ws, _, _ = _channel_args(what, w_scale, None, n)
     dy2 = _token_rows(dy)
     m = dy2.shape[0]
-    dx = dy.new_empty((*dy.shape[:-1], k), dtype=dtype)
+    dx = dy.new_empty(*dy.shape[:-1], k, dtype=dtype)
     need = lib().dk_int8_linear_x_workspace(1, m, n, k)
     work = _workspace(dy, need)
     call_on(dev, lib().dk_int8_linear_bwd, dy2.data_ptr(), code, dy2.stride(0), wq.data_ptr(), ldw, ws.data_ptr(),

@@ -145,12 +145,13 @@ def _norm_weights(what, dev, d, q_weight, k_weight):
     return q_weight.contiguous(), k_weight.contiguous(), code
 
 
-def _descriptor(q, k, gq, gk, oq, ok, weights, dws, rot, lds, b, t, hq, hk, d, code, eps):
-    """dk_qk_rope as packed bytes, its fields in order (None: a NULL pointer)."""
-    at = [0 if v is None else v.data_ptr() for v in (q, k, gq, gk, oq, ok, weights[0], weights[1], *dws)]
+def _descriptor(at, dw_q, dw_k, weights, rot, lds, b, t, hq, hk, d, code, eps):
+    """dk_qk_rope as packed bytes, its fields in order (at: pointers of q, k, their gradients and outputs)."""
+    qw, kw, w_code = weights
     cos, sin, pos, inv, table_batch, pos_axis, pos_batch, n_axes, sections, interleaved, pos64, _ = rot
-    return QkRope.PACK.pack(*at, cos, sin, pos, inv, *lds, table_batch, pos_axis, pos_batch, b, t, hq, hk, d, code,
-                            weights[2], n_axes, *sections, interleaved, pos64, eps, 0)
+    return QkRope.PACK.pack(*at, 0 if qw is None else qw.data_ptr(), 0 if kw is None else kw.data_ptr(), dw_q, dw_k,
+                            cos, sin, pos, inv, *lds, table_batch, pos_axis, pos_batch, b, t, hq, hk, d, code, w_code,
+                            n_axes, *sections, interleaved, pos64, eps, 0)
 
 
 def _qk_forward(what, q, k, q_weight, k_weight, hq, hk, eps, d, tables=None, axes=None):
@@ -165,9 +166,10 @@ def _qk_forward(what, q, k, q_weight, k_weight, hq, hk, eps, d, tables=None, axe
         raise ValueError(f"{what}: q and k must have the same tokens")
     weights = _norm_weights(what, dev, d, q_weight, k_weight)
     rot = _rotation(what, dev, b, t, d, tables, axes)
-    q_out, k_out = q.new_empty((b, hq, t, d)), q.new_empty((b, hk, t, d))
-    call_on(dev, lib().dk_qk_rope_fwd, _descriptor(q, k, None, None, q_out, k_out, weights, (None, None), rot,
-                                                   (ldq, ldk, 0, 0), b, t, hq, hk, d, code, eps))
+    q_out, k_out = q.new_empty(b, hq, t, d), q.new_empty(b, hk, t, d)
+    at = q.data_ptr(), k.data_ptr(), 0, 0, q_out.data_ptr(), k_out.data_ptr()
+    call_on(dev, lib().dk_qk_rope_fwd,
+            _descriptor(at, 0, 0, weights, rot, (ldq, ldk, 0, 0), b, t, hq, hk, d, code, eps))
     return q_out, k_out
 
 
@@ -197,10 +199,13 @@ def _qk_backward(what, grad_q, grad_k, q, k, q_weight, k_weight, eps, weight_gra
         if (bq, tq) != (b, t) or (bk, tk) != (b, t):
             raise ValueError(f"{what}: q, k and their gradients must have the same tokens")
         if weight_grads:
-            dws = gq.new_empty((2, d), dtype=torch.float32).unbind()
-    dq, dk = gq.new_empty((b, t, hq * d)), gq.new_empty((b, t, hk * d))
-    desc = _descriptor(q, k, gq, gk, dq, dk, weights, dws, rot, (ldq, ldk, hq * d, hk * d), b, t, hq, hk, d, code, eps)
-    if dws[0] is not None:
+            dws = gq.new_empty(2, d, dtype=torch.float32).unbind()
+    dq, dk = gq.new_empty(b, t, hq * d), gq.new_empty(b, t, hk * d)
+    at = (0 if q is None else q.data_ptr(), 0 if k is None else k.data_ptr(), gq.data_ptr(), gk.data_ptr(),
+          dq.data_ptr(), dk.data_ptr())
+    dwq, dwk = (0, 0) if dws[0] is None else (dws[0].data_ptr(), dws[1].data_ptr())
+    desc = _descriptor(at, dwq, dwk, weights, rot, (ldq, ldk, hq * d, hk * d), b, t, hq, hk, d, code, eps)
+    if dwq:
         need = lib().dk_qk_rope_bwd_workspace(desc)
         # a tensor of its own a call: graphs and streams share none
         work = gq.new_empty(need, dtype=torch.uint8) if need > 0 else None
