@@ -368,3 +368,32 @@ def test_refusals(device):
             call()
     with pytest.raises(DecikError, match="131071"):
         quantize_int8(torch.zeros((1, 131072), device=device))
+
+
+# the largest tile with k split, ragged in every direction: seven splits of one narrow tile column, three uneven ones
+# of three columns
+SPLIT_TILES = {(4121, 257, 18945): 7, (6229, 725, 15023): 3}
+
+
+@pytest.mark.parametrize("size", SPLIT_TILES)
+@pytest.mark.parametrize("transposed", [False, True])
+def test_largest_tile_with_splits(size, transposed, device):
+    from decik_amd.int8 import int8_linear_backward, int8_linear_forward, launch_plan, quantize_int8
+
+    m, n, k = size
+    assert launch_plan(transposed, m, n, k) == dict(tile_tokens=256, tile_channels=256, splits=SPLIT_TILES[size],
+                                                    fused=False)
+    if transposed:  # sums over k: the layer's output channels
+        wq, ws = quantize_int8(make((k, n), torch.float32, device, 1, 0.02))
+        dy = make((m, k), torch.float16, device, 2)
+        gq, gs = quantize_int8(dy, ws)
+        acc = (gq.double() @ wq.double()).cpu().numpy()
+        for dtype in (torch.float16, torch.float32):
+            check(int8_linear_backward(dy, wq, ws, dtype=dtype), acc, gs.cpu().numpy())
+    else:
+        wq, ws = quantize_int8(make((n, k), torch.float32, device, 1, 0.02))
+        x, bias = make((m, k), torch.float16, device, 2), make((n,), torch.float32, device, 3)
+        xq, xs = quantize_int8(x)
+        acc = (xq.double() @ wq.double().t().contiguous()).cpu().numpy()
+        for dtype in (torch.float16, torch.float32):
+            check(int8_linear_forward(x, wq, ws, bias, dtype), acc, xs.cpu().numpy(), ws.cpu().numpy(), bias)

@@ -213,3 +213,25 @@ def test_linear_plan_query():
         with pytest.raises(_lib.DecikError):
             launch_plan(False, *bad)
     assert _lib.lib().dk_int8_linear_plan(0, 1, 1, 1, None) != 0
+
+
+def test_every_form_that_the_planner_chooses_is_run():
+    """Tiles with and without splits over a sweep of sizes: the GPU tests name a size for each of them, and the sizes
+    they name are planned so."""
+    from decik_amd.int8 import launch_plan
+    from test_int8_gpu import SPLIT_TILES, TILES
+
+    def form(transposed, m, n, k):
+        p = launch_plan(transposed, m, n, k)
+        return p["tile_tokens"], p["tile_channels"], p["splits"] > 1
+
+    tested = {(0, 16, False): (16, 512, 4096), **TILES, (256, 256, True): next(iter(SPLIT_TILES))}
+    for transposed in (False, True):
+        for f, size in tested.items():
+            if f[0] > 0 or not transposed:
+                assert form(transposed, *size) == f
+        seen = {form(transposed, m, n, k)
+                for m in (1, 2, 8, 16, 32, 33, 64, 100, 257, 512, 830, 2051, 6229, 8192, 65536, (1 << 23) - 1)
+                for n in (1, 16, 64, 255, 384, 724, 1536, 2057, 3584, 8960, 18944, 151936, (1 << 23) - 1)
+                for k in (1, 64, 129, 256, 512, 1121, 2048, 3584, 8960, 15022, 18944, 40000, 131071) if m * n < 1 << 38}
+        assert seen <= set(tested) and len(seen) == (8 if transposed else 9)
