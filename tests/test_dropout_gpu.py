@@ -242,3 +242,27 @@ def test_refusals(device):
                  lambda: dropout_backward([x, x[:2]], rng, (0.1, 0.2))):
         with pytest.raises(ValueError):
             call()
+
+
+@gpu
+@pytest.mark.parametrize("nb", [1, 2, 3])
+@pytest.mark.parametrize("x_dtype,dtype", [(torch.float32, torch.bfloat16), (torch.float16, torch.float32),
+                                           (torch.bfloat16, torch.float32)])
+def test_pairs_of_types(nb, x_dtype, dtype, device):
+    """The pairs with fp32 on one side that the branches above leave out, forward and backward."""
+    from decik_amd.dropout import dropout_backward, dropout_forward, rng_state
+
+    rows, width, offset, ps = 37, 1121, 12, (0.05, 0.3, 0.6)[:nb]
+    x = make((rows, width), x_dtype, device, 1)
+    rng = rng_state(SEED, offset, device)
+    outs = dropout_forward(x, rng, ps, dtype)
+    xd = x.double().cpu().numpy()
+    masks = [keep_mask(rows, width, SEED, offset + b, p) for b, p in enumerate(ps)]
+    for o, m, p in zip(outs, masks, ps):
+        assert o.dtype == dtype and o.shape == x.shape
+        check(o, np.where(m, xd * scale_of(p), 0.0))
+    grads = [make((rows, width), dtype, device, 2 + b, 1e-2) for b in range(nb)]
+    terms = [np.where(m, g.double().cpu().numpy() * scale_of(p), 0.0) for g, m, p in zip(grads, masks, ps)]
+    dx = dropout_backward(grads, rng, ps, x_dtype)
+    assert dx.dtype == x_dtype
+    check(dx, sum(terms), sum(abs(t) for t in terms))
