@@ -407,3 +407,20 @@ def test_refusals(device):
     small = torch.empty((1, t, 8), dtype=torch.float16, device=device)
     with pytest.raises(DecikError, match="head_dim"):
         axes_rope_forward(small, small, pos, inv[:4], [4], 1, 1)
+
+
+@pytest.mark.parametrize("b,t,h,hk,d", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_tables_without_norms(b, t, h, hk, d, dtype, device):
+    """No norm weights: the rotation by tables alone, which needs neither q nor k for its backward."""
+    from decik_amd.rope import qk_norm_rope, qk_norm_rope_backward, qk_norm_rope_forward
+
+    q, k, gq, gk = inputs(b, t, h, hk, d, dtype, device)
+    angle = make((b, t, d), torch.float32, device, 7, 3.0)
+    cos, sin = angle.cos(), angle.sin()
+    outs = qk_norm_rope_forward(q, k, None, None, cos, sin, h, hk)
+    grads = qk_norm_rope_backward(gq, gk, None, None, None, None, cos, sin)
+    check_all(outs, grads, q, k, gq, gk, None, None, f64(cos), f64(sin), h, hk, 0.0)
+    q, k = q.detach().requires_grad_(True), k.detach().requires_grad_(True)
+    got = torch.autograd.grad(qk_norm_rope(q, k, None, None, cos, sin, h, hk), (q, k), (gq, gk))
+    assert all(torch.equal(x, y) for x, y in zip(got, grads))
