@@ -334,7 +334,8 @@ class LoRAPairSeeded(torch.autograd.Function):
     scaling_q, scaling_v, p_q, p_v) -> (out_q, out_v) fp16, as LoRAPair with the masks of
     decik_amd.dropout at rng (int64 device tensor: seed, offset; the call uses up two offsets). The
     backward forms the same masks again; rng must not change before it. x: [.., W] fp16 or fp32;
-    a_* [r, W], b_* [N, r] of one rank, 16 or 32; gradients reach x (in its type) and the adapters."""
+    a_* [r, W], b_* [N, r] of one rank, 16 or 32, W and N multiples of 8; gradients reach x (in its type)
+    and the adapters."""
 
     @staticmethod
     def _check(x, rng, adapters):

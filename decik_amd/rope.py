@@ -234,7 +234,8 @@ def axes_rope_forward(q, k, positions, inv_freq, sections, n_heads, n_kv_heads, 
     [axes, T] or [axes, B, T]; inv_freq [D / 2] (radians a position); sections: how many of the
     frequencies each axis takes, in order of the frequencies, or interleaved (frequency j belongs to
     axis j % axes while that axis has some left, the others to axis 0). With q_weight and k_weight the
-    heads are RMS-normalized first. The angles are exact to 2^-24 turns for positions below 2^28."""
+    heads are RMS-normalized first. The angles are exact to 2^-24 turns for positions below 2^28
+    and frequencies up to 2 pi."""
     return _qk_forward("axes_rope_forward", q, k, q_weight, k_weight, n_heads, n_kv_heads, eps,
                        2 * inv_freq.shape[-1], axes=(positions, inv_freq, sections, interleaved))
 
