@@ -15,7 +15,7 @@
 //
 // Bound: HBM and, nearly as much, the vector units: the generator takes 20 wide 32-bit products a group and
 // branch. Sixteen bits an element instead of 32 halve its share. Two branches of [8192, 3584] fp16: forward
-// 30 us (5.8 TB/s), backward 36 (4.9 TB/s); a large copy reaches 5.2 TB/s. Three-input exclusive ors and the
+// 30 to 32 us (5.8 to 5.5 TB/s), backward 36 to 37 (4.9); a large copy reaches 5.2 TB/s. Three-input exclusive ors and the
 // row by a multiplication instead of a division took 2 to 3 us off each. One thread a group keeps every load
 // of a wave contiguous and the device full.
 #include "elem.h"

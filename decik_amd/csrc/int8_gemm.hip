@@ -13,11 +13,12 @@
 // and turns it through the transposed LDS read of 8-bit elements: in each 16 lanes, lanes 2 r and 2 r + 1
 // read the 16 bytes of row r, lane i receives byte i of the 8 rows.
 //
-// Bound: at [8192, 18944] x 3584 the forward takes 541 us (2.06 POP/s), the input gradient 512 (2.17); torch's
-// library product of the same sizes, without scales, 616 and 571. Matrix cores are busy half of the cycles at
-// 2.0 GHz. Timing copies without the loads of the loop take 480 and 430 us, without the operand reads 550 and
-// 550, without either 440 and 380: the loads cost most, through their issue and the L2's bandwidth (64 KB a
-// step and CU), not through latency (lines touched a step or more ahead in the L2 made it 3 to 8% slower).
+// Bound: at [8192, 18944] x 3584 the forward takes 504 to 541 us from GPU to GPU (2.06 to 2.21 POP/s), the input
+// gradient 474 to 512 (2.17 to 2.35); torch's library product of the same sizes, without scales, 514 to 616 and
+// 569 to 571. Matrix cores are busy 59 and 62% of the cycles, at 1.7 GHz under this load. On the GPU of 541 and
+// 512 us, timing copies without the loads of the loop took 480 and 430, without the operand reads 550 and 550,
+// without either 440 and 380: the loads cost most, through their issue and the L2's bandwidth (64 KB a step and
+// CU), not through latency (lines touched a step or more ahead in the L2 made it 3 to 8% slower).
 // The last round of tiles is 7 to 12% idle. Also measured, not kept: tiles of 128 by 128 on four waves, two
 // work-groups a CU (equal or slower everywhere), operand reads pinned before the MFMAs (+0 to 5%), bands of
 // four token tiles (equal).
@@ -518,9 +519,9 @@ __device__ __forceinline__ void quant_scale(uint32_t top, float& inv, float& sca
 }
 
 // The row stays in registers between its maximum and its rounding (R groups of eight a thread), or is read
-// again (R = 0). THREADS threads a row. Bound: HBM, at [8192, 18944] fp16 with column scales 107 us (4.35
-// TB/s; a large copy reaches 5.2), [8192, 3584] 18.3. Several rows a work-group, the column scales read once
-// for them, were slower (175 and 25.7 us: fewer waves).
+// again (R = 0). THREADS threads a row. Bound: HBM, at [8192, 18944] fp16 with column scales 97 to 107 us (4.8 to
+// 4.35 TB/s; a large copy reaches 5.2), [8192, 3584] 18.1. Several rows a work-group, the column scales read once
+// for them, were slower (175 and 25.7 us beside 107 and 18.3: fewer waves).
 template <int DT, bool COL, int THREADS, int R>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void int8_quantize_kernel(const Int8QuantArgs a) {
     constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, ROWS = BLOCK / THREADS, NW = THREADS / 64;
@@ -666,8 +667,9 @@ __global__ __launch_bounds__(64 * WAVES) void int8_few_kernel(const Int8GemmArgs
 
 // The same with x as it comes (fp16, bf16 or fp32): every work-group quantizes the few rows for itself
 // (they come from the L2) into LDS while its first weights are on their way, which saves the launch of the
-// quantizer and its round trip: [18944, 3584] at one token 16.0 us (4.2 TB/s) against 18.3, [3584, 3584] 6.0
-// against 8.4; at two tokens equal, at four 22.0 against 19.8.
+// quantizer and its round trip. Weights from memory: [18944, 3584] at one token 16.0 us (4.2 TB/s) against 18.3,
+// [3584, 3584] 6.0 against 8.4; at two tokens equal, at four 22.0 against 19.8. A repeated [18944, 3584] (68 MB) is
+// read from the last cache: 14.4.
 template <int DT, int WAVES, int OUT>
 __global__ __launch_bounds__(64 * WAVES) void int8_few_fused_kernel(const Int8GemmArgs a, const Int8QuantArgs q) {
     constexpr int U = 8;
@@ -738,9 +740,10 @@ static Int8Plan make_plan(int64_t m, int64_t n, int64_t k, int cus, bool tr) {
     Int8Plan best{};
     const int64_t steps = (k + kI8BK - 1) / kI8BK > 0 ? (k + kI8BK - 1) / kI8BK : 1;
     double best_us = 0;
-    // Estimated time of a launch, fitted to 170 timed launches (17 sizes of 64 to 8192 tokens, both ways, every
-    // tile, 1 to 15 splits; root mean square of the deviation 8%; its choice within 3% of the best of each size
-    // but one, 6%): rounds of work-groups of a number of steps each, whose time grows from `light` to `full` with
+    // Estimated time of a launch, fitted to 170 timed launches (17 sizes of 64 to 8192 tokens and summed axes of
+    // 1121 to 18944, both ways, every tile, 1 to 15 splits; root mean square of the deviation 8%; its choice within
+    // 3% of the best of each size but one, 6%; on shorter sums it extrapolates: [8192, 8960] x 384 86 us, measured
+    // 63, [8192, 3584] x 512 39 and 29): rounds of work-groups of a number of steps each, whose time grows from `light` to `full` with
     // the share of the CUs that work, and a last part; sums of splits written and read back.
     struct Tile {
         int tm, bn;

@@ -13,9 +13,10 @@
 // position and frequency would be off by 2^-5.
 //
 // Bound: HBM (read and write of q and k, in the backward gradients, q and k in and dq, dk out): 8192 tokens of
-// 28 + 4 heads of 128, bf16, with norms: forward 30 us (4.8 TB/s), backward 39 (5.4 TB/s) and 4 for the sums of
-// dw; three axes without norms over 4096 tokens, fp16, 13.5 us each way (5.0 TB/s); a large copy reaches 5.2.
-// At 830 tokens 4.4 and 7.4 us, a few memory round trips.
+// 28 + 4 heads of 128, bf16, with norms: forward 30 to 32 us with q and k from memory (4.8 to 4.5 TB/s), 25 with them in
+// the last cache, backward 39 to 41 (5.4 to 5.1 TB/s) and 4 for the sums of dw; three axes without norms over 4096 tokens,
+// fp16, 16.2 and 16.8 us from memory (4.2 and 4.0 TB/s), 12.4 and 12.5 from that cache; a large copy reaches 5.2.
+// At 830 tokens 4.5 and 7.2 us, a few memory round trips.
 // Layout: a lane holds eight elements of a and their eight partners of b (two 16-byte loads, the
 // rotation and most of the norm's sum need no other lane), LPH lanes a head, 64 / LPH heads a pass. A
 // wave serves one pass -- so each lane has one head, its weights stay in registers and the
