@@ -740,11 +740,11 @@ static Int8Plan make_plan(int64_t m, int64_t n, int64_t k, int cus, bool tr) {
     Int8Plan best{};
     const int64_t steps = (k + kI8BK - 1) / kI8BK > 0 ? (k + kI8BK - 1) / kI8BK : 1;
     double best_us = 0;
-    // Estimated time of a launch, fitted to 170 timed launches (17 sizes of 64 to 8192 tokens and summed axes of
-    // 1121 to 18944, both ways, every tile, 1 to 15 splits; root mean square of the deviation 8%; its choice within
-    // 3% of the best of each size but one, 6%; on shorter sums it extrapolates: [8192, 8960] x 384 86 us, measured
-    // 63, [8192, 3584] x 512 39 and 29): rounds of work-groups of a number of steps each, whose time grows from `light` to `full` with
-    // the share of the CUs that work, and a last part; sums of splits written and read back.
+    // Estimated time of a launch, fitted to 170 timed launches (17 sizes of 64 to 8192 tokens and summed axes of 1121
+    // to 18944, both ways, every tile, 1 to 15 splits; root mean square of the deviation 8%; its choice within 3% of
+    // the best of each size but one, 6%; on shorter sums it extrapolates: [8192, 8960] x 384 86 us, measured 63,
+    // [8192, 3584] x 512 39 and 29): rounds of work-groups of a number of steps each, whose time grows from `light`
+    // to `full` with the share of the CUs that work, and a last part; sums of splits written and read back.
     struct Tile {
         int tm, bn;
         double light, full, last;
