@@ -66,6 +66,19 @@ class QkRope(ctypes.Structure):
     PACK = struct.Struct("@14P9q12if i")
 
 
+class ResidualNorm(ctypes.Structure):
+    """dk_residual_norm: a call of the residual stream (dk_residual_norm_fwd, dk_residual_norm_bwd)."""
+
+    _fields_ = [("x", c_vp), ("residual", c_vp), ("grad_h", c_vp), ("grad_y", c_vp), ("h", c_vp), ("y", c_vp),
+                ("dx", c_vp), ("dresidual", c_vp), ("dgate", c_vp), ("weight", c_vp), ("post_weight", c_vp),
+                ("gate", c_vp), ("dweight", c_vp), ("dpost_weight", c_vp), ("ld_x", c_i64), ("ld_residual", c_i64),
+                ("ld_grad_h", c_i64), ("ld_grad_y", c_i64), ("ld_gate", c_i64), ("rows", c_i64), ("width", c_i64),
+                ("x_dtype", c_i32), ("stream_dtype", c_i32), ("y_dtype", c_i32), ("weight_dtype", c_i32),
+                ("post_dtype", c_i32), ("gate_dtype", c_i32), ("gate_kind", c_i32), ("residual_scale", c_f32),
+                ("eps", c_f32), ("reserved", c_i32)]
+    PACK = struct.Struct("@14P7q7i2fi")
+
+
 EXPORTS = {
     "dk_nf4_dequant": ([ctypes.POINTER(NF4Weight), c_vp, c_vp], c_i32),
     "dk_nf4_dequant_batched": ([ctypes.POINTER(NF4Weight), ctypes.POINTER(c_vp), c_i32, c_vp], c_i32),
@@ -111,6 +124,10 @@ EXPORTS = {
     "dk_qk_rope_fwd": ([c_vp, c_vp], c_i32),
     "dk_qk_rope_bwd_workspace": ([c_vp], c_i64),
     "dk_qk_rope_bwd": ([c_vp, c_vp, c_i64, c_vp], c_i32),
+    # packed bytes as well (ResidualNorm.PACK)
+    "dk_residual_norm_fwd": ([c_vp, c_vp], c_i32),
+    "dk_residual_norm_bwd_workspace": ([c_vp], c_i64),
+    "dk_residual_norm_bwd": ([c_vp, c_vp, c_i64, c_vp], c_i32),
     "dk_int8_quantize": ([c_vp, c_i32, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp], c_i32),
     "dk_int8_linear_workspace": ([c_i32, c_i64, c_i64, c_i64], c_i64),
     "dk_int8_linear": ([c_i32, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i32, c_vp, c_i32, c_i64, c_i64, c_i64,

@@ -132,6 +132,65 @@ bool int8_rows_ok(const void* p, int64_t ld, int64_t cols) {
 
 bool rows_fit(int64_t ld, int heads, int d) { return ld >= (int64_t)heads * d; }
 
+// everything of a residual-stream call but its outputs and gradients
+int residual_norm_common(const dk_residual_norm* d, ResidualNormArgs* a) {
+    if (d == nullptr) return dk_fail("dk_residual_norm: null descriptor");
+    const int x = d->x_dtype;
+    if (!is_dtype(x) || (d->stream_dtype != x && d->stream_dtype != DK_FP32) ||
+        (d->y_dtype != x && d->y_dtype != DK_FP32))
+        return dk_fail("dk_residual_norm: x must be fp16, bf16 or fp32, the stream and y of x's type or fp32");
+    if (d->width < 1 || d->width > kNormMaxWidth) return dk_fail("dk_residual_norm: width must be 1 to 16384");
+    if (d->rows < 0 || d->rows >= (int64_t)INT32_MAX - 65535)
+        return dk_fail("dk_residual_norm: rows must be non-negative and below 2^31 - 65536");
+    if ((d->weight != nullptr && !is_dtype(d->weight_dtype)) || (d->post_weight != nullptr && !is_dtype(d->post_dtype)))
+        return dk_fail("dk_residual_norm: unknown weight type");
+    if (d->gate_kind < DK_GATE_NONE || d->gate_kind > DK_GATE_ELEMENT)
+        return dk_fail("dk_residual_norm: unknown kind of gate");
+    if (d->gate_kind != DK_GATE_NONE && !is_dtype(d->gate_dtype)) return dk_fail("dk_residual_norm: unknown gate type");
+    const bool empty = d->rows == 0;
+    if (!empty && d->x == nullptr) return dk_fail("dk_residual_norm: null pointer");
+    if (d->gate_kind != DK_GATE_NONE && !empty && d->gate == nullptr) return dk_fail("dk_residual_norm: null gate");
+    if (d->rows > 1 && (d->ld_x < 0 || d->ld_residual < 0 || d->ld_grad_h < 0 || d->ld_grad_y < 0 || d->ld_gate < 0))
+        return dk_fail("dk_residual_norm: negative row stride");
+    a->x = d->x;
+    a->res = d->residual;
+    a->w = d->weight;
+    a->pw = d->post_weight;
+    a->gate = d->gate;
+    a->ldx = d->ld_x;
+    a->ldr = d->ld_residual;
+    a->ldgate = d->ld_gate;
+    a->rows = (int32_t)d->rows;
+    a->width = (int32_t)d->width;
+    a->w_dtype = d->weight_dtype;
+    a->pw_dtype = d->post_dtype;
+    a->gate_dtype = d->gate_dtype;
+    a->gate_kind = d->gate_kind;
+    a->scale = d->residual_scale;
+    a->eps = d->eps;
+    a->inv_width = 1.0f / (float)d->width;
+    return 0;
+}
+
+// which gradients of a backward are sums over the rows
+int residual_norm_sums(const dk_residual_norm* d, ResidualNormArgs* a) {
+    if (d->dweight != nullptr && d->weight == nullptr)
+        return dk_fail("dk_residual_norm_bwd: no weight to take a gradient of");
+    if (d->dpost_weight != nullptr && d->post_weight == nullptr)
+        return dk_fail("dk_residual_norm_bwd: no post weight to take a gradient of");
+    if (d->dgate != nullptr && d->gate_kind == DK_GATE_NONE)
+        return dk_fail("dk_residual_norm_bwd: no gate to take a gradient of");
+    a->slab_w = d->dweight != nullptr;
+    a->slab_pw = d->dpost_weight != nullptr;
+    a->slab_gate = d->dgate != nullptr && d->gate_kind == DK_GATE_CHANNEL;
+    a->nslabs = (int)a->slab_w + (int)a->slab_pw + (int)a->slab_gate;
+    return 0;
+}
+
+int64_t residual_norm_bytes(const ResidualNormArgs& a) {
+    return (int64_t)residual_norm_groups(a.rows, a.width, true) * a.nslabs * a.width * (int64_t)sizeof(float);
+}
+
 }  // namespace
 
 extern "C" {
@@ -366,6 +425,57 @@ int dk_int8_linear_bwd(const void* dy, int dy_dtype, int64_t lddy, const int8_t*
     if (!int8_sizes(m, k, n)) return dk_fail("dk_int8_linear_bwd: 0 <= m, k < 2^23, m k < 2^38, 1 <= n <= 131071");
     return int8_linear_x(true, dy, dy_dtype, lddy, wq, ldw, ws, nullptr, 0, dx, dx_dtype, lddx, m, k, n, workspace,
                          workspace_bytes, stream);
+}
+
+int dk_residual_norm_fwd(const dk_residual_norm* d, void* stream) {
+    dk_clear_error();
+    ResidualNormArgs a{};
+    if (int rc = residual_norm_common(d, &a)) return rc;
+    if (a.rows == 0) return 0;
+    if ((d->weight != nullptr && d->y == nullptr) || (d->weight == nullptr && d->h == nullptr))
+        return dk_fail("dk_residual_norm_fwd: y with a weight, h without one");
+    a.h = d->h;
+    a.y = d->y;
+    return check_launch(launch_residual_norm(a, d->x_dtype, d->stream_dtype, d->y_dtype, false, nullptr, nullptr,
+                                             nullptr, static_cast<hipStream_t>(stream)),
+                        "dk_residual_norm_fwd launch");
+}
+
+int64_t dk_residual_norm_bwd_workspace(const dk_residual_norm* d) {
+    dk_clear_error();
+    ResidualNormArgs a{};
+    if (residual_norm_common(d, &a) != 0 || residual_norm_sums(d, &a) != 0) return -1;
+    return residual_norm_bytes(a);
+}
+
+int dk_residual_norm_bwd(const dk_residual_norm* d, void* workspace, int64_t workspace_bytes, void* stream) {
+    dk_clear_error();
+    ResidualNormArgs a{};
+    if (int rc = residual_norm_common(d, &a)) return rc;
+    if (int rc = residual_norm_sums(d, &a)) return rc;
+    if (a.rows == 0 && a.nslabs == 0) return 0;
+    if (a.rows > 0) {
+        if (d->dx == nullptr) return dk_fail("dk_residual_norm_bwd: null pointer");
+        if ((d->weight != nullptr) != (d->grad_y != nullptr))
+            return dk_fail("dk_residual_norm_bwd: grad_y where there is a weight, and only there");
+        if (d->dresidual != nullptr && d->residual == nullptr)
+            return dk_fail("dk_residual_norm_bwd: no residual to take a gradient of");
+        const int64_t need = residual_norm_bytes(a);
+        if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16)))
+            return dk_fail("dk_residual_norm_bwd: workspace too small (dk_residual_norm_bwd_workspace)");
+    }
+    a.gh = d->grad_h;
+    a.gy = d->grad_y;
+    a.ldgh = d->ld_grad_h;
+    a.ldgy = d->ld_grad_y;
+    a.dx = d->dx;
+    a.dres = d->dresidual;
+    a.dgate = d->gate_kind == DK_GATE_CHANNEL ? nullptr : d->dgate;
+    a.slabs = a.nslabs > 0 ? static_cast<float*>(workspace) : nullptr;
+    return check_launch(launch_residual_norm(a, d->x_dtype, d->stream_dtype, d->y_dtype, true, d->dweight,
+                                             d->dpost_weight, a.slab_gate ? static_cast<float*>(d->dgate) : nullptr,
+                                             static_cast<hipStream_t>(stream)),
+                        "dk_residual_norm_bwd launch");
 }
 
 }  // extern "C"

@@ -319,6 +319,25 @@ bool int8_fused(int64_t m, int64_t k, bool tr);
 hipError_t launch_int8_fused(const Int8GemmArgs& a, const Int8QuantArgs& q, int x_dtype, int out_dtype, hipStream_t s);
 hipError_t launch_int8_quantize(const Int8QuantArgs& a, int dtype, hipStream_t s);
 
+// The residual stream with its norms and gate (residual_norm.hip).
+constexpr int kNormMaxWidth = 16384;
+struct ResidualNormArgs {
+    const void *x, *res, *gh, *gy, *w, *pw, *gate;
+    void *h, *y, *dx, *dres;
+    void* dgate;  // a gate a token or an element
+    float* slabs; // backward: sums of the shared gradients a work-group: weight, post weight, channel gate
+    int64_t ldx, ldr, ldgh, ldgy, ldgate;
+    int32_t rows, width;
+    int32_t w_dtype, pw_dtype, gate_dtype, gate_kind;
+    int32_t nslabs;
+    bool slab_w, slab_pw, slab_gate;
+    float scale, eps, inv_width;
+};
+// work-groups (slabs) of a launch
+int residual_norm_groups(int64_t rows, int width, bool backward);
+hipError_t launch_residual_norm(ResidualNormArgs a, int x_dtype, int stream_dtype, int y_dtype, bool backward,
+                                float* dw, float* dpw, float* dgate_channel, hipStream_t s);
+
 // The calling thread's error (dk_last_error); dk_fail returns 1.
 int dk_fail(const char* msg);
 void dk_clear_error();

@@ -394,6 +394,50 @@ int dk_int8_linear_bwd(const void* dy, int dy_dtype, int64_t lddy, const int8_t*
                        void* dx, int dx_dtype, int64_t lddx, int64_t m, int64_t n, int64_t k, void* workspace,
                        int64_t workspace_bytes, void* stream);
 
+/* ---- the residual stream between two blocks, no counterpart in the reference --------------- */
+
+/* h = residual_scale * residual + gate * N(x) * post_weight and y = N(h) * weight over rows of `width`
+ * elements, N(v) = v / sqrt(mean(v^2) + eps), in fp32 with y formed from h before h is rounded. residual NULL:
+ * no stream; post_weight NULL: x without its norm; weight NULL: no y. The gate (any of the three types) has a
+ * value a channel [width], a token (row r at r * ld_gate) or an element (rows ld_gate apart), or there is none.
+ * Forward writes h (NULL: not wanted, only with a weight) and y. Backward takes grad_h (NULL: zeros) and grad_y (iff there is a
+ * weight), the forward's inputs, and writes dx, dresidual (NULL: not wanted), dgate (NULL: not wanted; a channel:
+ * fp32 [width], else of gate_dtype with packed rows), dweight and dpost_weight (fp32 [width], NULL: not wanted).
+ * x and dx are of x_dtype; residual, h and their gradients of stream_dtype, y and grad_y of y_dtype: each x's type
+ * or DK_FP32. Outputs have packed rows; input rows may have any non-negative stride (elements) and start at any
+ * element. 1 <= width <= 16384, rows < 2^31 - 65536. The gradients of the weights and of a channel's gate are
+ * added in a fixed order: the same bits every run. */
+#define DK_GATE_NONE 0
+#define DK_GATE_CHANNEL 1
+#define DK_GATE_TOKEN 2
+#define DK_GATE_ELEMENT 3
+typedef struct {
+    const void* x;
+    const void* residual;
+    const void* grad_h;
+    const void* grad_y;
+    void* h;
+    void* y;
+    void* dx;
+    void* dresidual;
+    void* dgate;
+    const void* weight;
+    const void* post_weight;
+    const void* gate;
+    float* dweight;
+    float* dpost_weight;
+    int64_t ld_x, ld_residual, ld_grad_h, ld_grad_y, ld_gate;
+    int64_t rows, width;
+    int32_t x_dtype, stream_dtype, y_dtype;
+    int32_t weight_dtype, post_dtype, gate_dtype, gate_kind;
+    float residual_scale, eps;
+    int32_t reserved;
+} dk_residual_norm;
+int dk_residual_norm_fwd(const dk_residual_norm* d, void* stream);
+/* workspace of the backward: bytes (0: none), -1 on a bad descriptor */
+int64_t dk_residual_norm_bwd_workspace(const dk_residual_norm* d);
+int dk_residual_norm_bwd(const dk_residual_norm* d, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* out = fp16(silu(gate) * up), computed in fp32 (n elements). */
 int dk_swiglu_fwd(const uint16_t* gate, const uint16_t* up, uint16_t* out, int64_t n,
                   void* stream);
