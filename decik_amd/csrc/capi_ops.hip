@@ -181,9 +181,8 @@ int residual_norm_sums(const dk_residual_norm* d, ResidualNormArgs* a) {
     if (d->dgate != nullptr && d->gate_kind == DK_GATE_NONE)
         return dk_fail("dk_residual_norm_bwd: no gate to take a gradient of");
     a->slab_w = d->dweight != nullptr;
-    a->slab_pw = d->dpost_weight != nullptr;
-    a->slab_gate = d->dgate != nullptr && d->gate_kind == DK_GATE_CHANNEL;
-    a->nslabs = (int)a->slab_w + (int)a->slab_pw + (int)a->slab_gate;
+    a->slab_q = d->dpost_weight != nullptr || (d->dgate != nullptr && d->gate_kind == DK_GATE_CHANNEL);
+    a->nslabs = (int)a->slab_w + (int)a->slab_q;
     return 0;
 }
 
@@ -473,7 +472,7 @@ int dk_residual_norm_bwd(const dk_residual_norm* d, void* workspace, int64_t wor
     a.dgate = d->gate_kind == DK_GATE_CHANNEL ? nullptr : d->dgate;
     a.slabs = a.nslabs > 0 ? static_cast<float*>(workspace) : nullptr;
     return check_launch(launch_residual_norm(a, d->x_dtype, d->stream_dtype, d->y_dtype, true, d->dweight,
-                                             d->dpost_weight, a.slab_gate ? static_cast<float*>(d->dgate) : nullptr,
+                                             d->dpost_weight, d->gate_kind == DK_GATE_CHANNEL ? static_cast<float*>(d->dgate) : nullptr,
                                              static_cast<hipStream_t>(stream)),
                         "dk_residual_norm_bwd launch");
 }

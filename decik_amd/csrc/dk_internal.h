@@ -325,12 +325,12 @@ struct ResidualNormArgs {
     const void *x, *res, *gh, *gy, *w, *pw, *gate;
     void *h, *y, *dx, *dres;
     void* dgate;  // a gate a token or an element
-    float* slabs; // backward: sums of the shared gradients a work-group: weight, post weight, channel gate
+    float* slabs; // backward, sums a work-group: the weight's gradient, dh ux (post weight, channel gate)
     int64_t ldx, ldr, ldgh, ldgy, ldgate;
     int32_t rows, width;
     int32_t w_dtype, pw_dtype, gate_dtype, gate_kind;
     int32_t nslabs;
-    bool slab_w, slab_pw, slab_gate;
+    bool slab_w, slab_q;
     float scale, eps, inv_width;
 };
 // work-groups (slabs) of a launch

@@ -20,11 +20,18 @@
 
 namespace dk {
 
-constexpr int kNormMaxThreads = 512;
+constexpr int kNormMaxThreads = 512;  // eight waves: group_sum
 
-template <int DT>
+// How a row's columns fall to the threads. EVEN: a multiple of eight. TAIL: the last thread takes the last eight columns.
+// In both, columns that another thread has as well -- the threads past the row's end repeat its last eight -- are
+// computed and written alike (the same values) and left out of the sums: no load or store depends on the thread, so
+// that a row's loads are waited for by count, past the stores behind them. SHORT: fewer than eight columns, one thread
+// reads them one by one.
+enum { EVEN, TAIL, SHORT };
+
+template <int DT, int MODE>
 __device__ __forceinline__ typename Elem<DT>::vec fetch8(const typename Elem<DT>::type* p, int n) {
-    if (n >= 8) return load8_raw<DT>(p);
+    if constexpr (MODE != SHORT) return load8_raw<DT>(p);
     typename Elem<DT>::vec v = {};
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -32,16 +39,17 @@ __device__ __forceinline__ typename Elem<DT>::vec fetch8(const typename Elem<DT>
     return v;
 }
 
-// eight values of a type known at run time; n of them exist
+// eight values of a type known at run time
+template <int MODE>
 __device__ __forceinline__ float8_t fetch8_any(const void* p, int dtype, int64_t at, int n) {
-    if (dtype == DK_FP32) return fetch8<DK_FP32>((const float*)p + at, n);
-    if (dtype == DK_BF16) return widen8<DK_BF16>(fetch8<DK_BF16>((const __bf16*)p + at, n));
-    return widen8<DK_FP16>(fetch8<DK_FP16>((const _Float16*)p + at, n));
+    if (dtype == DK_FP32) return fetch8<DK_FP32, MODE>((const float*)p + at, n);
+    if (dtype == DK_BF16) return widen8<DK_BF16>(fetch8<DK_BF16, MODE>((const __bf16*)p + at, n));
+    return widen8<DK_FP16>(fetch8<DK_FP16, MODE>((const _Float16*)p + at, n));
 }
 
-template <int DT>
+template <int DT, int MODE>
 __device__ __forceinline__ void put8(typename Elem<DT>::type* p, float8_t v, int n) {
-    if (n >= 8) {
+    if constexpr (MODE != SHORT) {
         store8<DT>(p, v);
     } else {
 #pragma unroll
@@ -50,41 +58,62 @@ __device__ __forceinline__ void put8(typename Elem<DT>::type* p, float8_t v, int
     }
 }
 
+template <int MODE>
 __device__ __forceinline__ void put8_any(void* p, int dtype, int64_t at, float8_t v, int n) {
     if (dtype == DK_FP32)
-        put8<DK_FP32>((float*)p + at, v, n);
+        put8<DK_FP32, MODE>((float*)p + at, v, n);
     else if (dtype == DK_BF16)
-        put8<DK_BF16>((__bf16*)p + at, v, n);
+        put8<DK_BF16, MODE>((__bf16*)p + at, v, n);
     else
-        put8<DK_FP16>((_Float16*)p + at, v, n);
+        put8<DK_FP16, MODE>((_Float16*)p + at, v, n);
 }
 
 __device__ __forceinline__ float sum8(float8_t v) {
     return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
 }
 
+// v of the lane that a data-parallel primitive names
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+
+// sum over each eight lanes (all get it)
+__device__ __forceinline__ float sum_of8(float v) {
+    v += dpp<0xB1>(v);          // lanes 1 0 3 2
+    v += dpp<0x4E>(v);          // lanes 2 3 0 1
+    return v + dpp<0x141>(v);   // mirrored eight
+}
+
+// sum over the 64 lanes (all get it) without a round through LDS
+__device__ __forceinline__ float wave_sum(float v) {
+    v = sum_of8(v);
+    v += dpp<0x140>(v);  // mirrored sixteen
+    const int u = __builtin_bit_cast(int, v);
+    const auto row = [&](int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(u, lane)); };
+    return (row(0) + row(16)) + (row(32) + row(48));
+}
+
 // sums of two values over the work-group (all get them)
 __device__ __forceinline__ float2_t group_sum(float a, float b, float2_t* slot) {
-#pragma unroll
-    for (int o = 1; o < kWave; o *= 2) {
-        a += __shfl_xor(a, o);
-        b += __shfl_xor(b, o);
-    }
+    a = wave_sum(a);
+    b = wave_sum(b);
     const int waves = blockDim.x / kWave;
     if (waves == 1) return float2_t{a, b};
     if (threadIdx.x % kWave == 0) slot[threadIdx.x / kWave] = float2_t{a, b};
     __syncthreads();
-    float2_t s = slot[0];
-    for (int w = 1; w < waves; ++w) {
-        const float2_t o = slot[w];
-        s.x += o.x;
-        s.y += o.y;
-    }
-    return s;
+    // the waves' sums, one a lane of each eight, added across the eight
+    const int w = threadIdx.x % 8;
+    float2_t s = slot[w];
+    s = w < waves ? s : float2_t{0.0f, 0.0f};
+    return float2_t{sum_of8(s.x), sum_of8(s.y)};
 }
 
-template <int XT, int ST, int YT, int V, bool BWD>
-__global__ __launch_bounds__(kNormMaxThreads) void residual_norm_kernel(const ResidualNormArgs a) {
+// FULL: stream, weight, h (backward: its gradient, and the residual's) are all there, and no row's gate
+template <int XT, int ST, int YT, int V, int MODE, bool FULL, bool BWD>
+__global__ __launch_bounds__(kNormMaxThreads, V > 1 ? 2 : ST == YT && ST == DK_FP32 ? 3 : 4) void residual_norm_kernel(
+    const ResidualNormArgs a) {
+#pragma clang fp contract(fast)
     typedef typename Elem<XT>::type x_t;
     typedef typename Elem<ST>::type s_t;
     typedef typename Elem<YT>::type y_t;
@@ -95,35 +124,56 @@ __global__ __launch_bounds__(kNormMaxThreads) void residual_norm_kernel(const Re
         return group_sum(p, q, slots[turn]);
     };
     const int width = a.width;
-    int col[V], n[V];
+    // this thread's columns of pass v: col[v] .. col[v] + 7, the first skip[v] of them another thread's too
+    int col[V], skip[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        col[v] = 8 * (int)(threadIdx.x + v * blockDim.x);
-        n[v] = min(max(width - col[v], 0), 8);
-        if (n[v] == 0) col[v] = 0;
+        const int c = 8 * (int)(threadIdx.x + v * blockDim.x);
+        col[v] = MODE == SHORT ? 0 : min(c, width - 8);
+        skip[v] = MODE == SHORT ? c : min(c - col[v], 8);
     }
-    const bool norm = a.w != nullptr, post = a.pw != nullptr, stream = a.res != nullptr;
-    const bool grad_h = BWD && a.gh != nullptr;
-
-    // weights and gate stay in registers (HOLD), or, four passes, come from the caches at each use
-    constexpr bool HOLD = V < 4;
-    float8_t held_w[V], held_pw[V], held_gate[V], dw[V], dpw[V], dgate[V];
-    const auto gate_at = [&](int64_t row, int v) -> float8_t {
-        if (a.gate_kind == DK_GATE_CHANNEL) return fetch8_any(a.gate, a.gate_dtype, col[v], n[v]);
-        if (a.gate_kind == DK_GATE_ELEMENT) return fetch8_any(a.gate, a.gate_dtype, row * a.ldgate + col[v], n[v]);
-        if (a.gate_kind == DK_GATE_TOKEN) return float8_t{} + load_any(a.gate, a.gate_dtype, row * a.ldgate);
-        return float8_t{} + 1.0f;
+    const bool lead = MODE != SHORT || threadIdx.x == 0;
+    const int n = MODE == SHORT ? width : 8;
+    // the sum over a pass's columns
+    const auto sum = [&](float8_t f, int v) {
+        if constexpr (MODE == TAIL) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = e < skip[v] ? 0.0f : f[e];
+            return sum8(f);
+        }
+        return skip[v] > 0 ? 0.0f : sum8(f);
     };
-    const auto weight = [&](int v) { return HOLD ? held_w[v] : fetch8_any(a.w, a.w_dtype, col[v], n[v]); };
-    const auto post_weight = [&](int v) { return HOLD ? held_pw[v] : fetch8_any(a.pw, a.pw_dtype, col[v], n[v]); };
-    const auto gate = [&](int64_t row, int v) { return HOLD ? held_gate[v] : gate_at(row, v); };
+    const bool norm = FULL || a.w != nullptr, post = a.pw != nullptr, stream = FULL || a.res != nullptr;
+    const bool grad_h = BWD && (FULL || a.gh != nullptr);
+
+    // The weights stay in registers (HOLD), or, four passes, come from the caches at each use. A channel's gate is held as
+    // its product with post_weight, and one sum, of dh ux, gives both their gradients in the second launch.
+    constexpr bool HOLD = V < 4;
+    const bool by_row = !FULL && a.gate_kind > DK_GATE_CHANNEL;
+    float8_t held_w[V], held_pw[V], gate_row[V], dw[V], dq[V];
+    const auto weight_at = [&](int v) {
+        return norm ? fetch8_any<MODE>(a.w, a.w_dtype, col[v], n) : float8_t{};
+    };
+    const auto branch_weight_at = [&](int v) {
+        float8_t q = float8_t{} + 1.0f;
+        if (post) q = fetch8_any<MODE>(a.pw, a.pw_dtype, col[v], n);
+        if (a.gate_kind == DK_GATE_CHANNEL) q = q * fetch8_any<MODE>(a.gate, a.gate_dtype, col[v], n);
+        return q;
+    };
+    const auto gate_at = [&](int64_t row, int v) -> float8_t {
+        if (a.gate_kind == DK_GATE_ELEMENT)
+            return fetch8_any<MODE>(a.gate, a.gate_dtype, row * a.ldgate + col[v], n);
+        return float8_t{} + load_any(a.gate, a.gate_dtype, row * a.ldgate);
+    };
+    const auto weight = [&](int v) { return HOLD ? held_w[v] : weight_at(v); };
+    const auto branch_weight = [&](int v) { return HOLD ? held_pw[v] : branch_weight_at(v); };
+    const auto gate = [&](int64_t row, int v) { return HOLD ? gate_row[v] : gate_at(row, v); };
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        dw[v] = dpw[v] = dgate[v] = float8_t{};
+        dw[v] = dq[v] = float8_t{};
         if constexpr (HOLD) {
-            held_w[v] = norm ? fetch8_any(a.w, a.w_dtype, col[v], n[v]) : float8_t{};
-            held_pw[v] = post ? fetch8_any(a.pw, a.pw_dtype, col[v], n[v]) : float8_t{};
-            if (a.gate_kind <= DK_GATE_CHANNEL) held_gate[v] = gate_at(0, v);
+            held_w[v] = weight_at(v);
+            held_pw[v] = branch_weight_at(v);
         }
     }
 
@@ -133,17 +183,20 @@ __global__ __launch_bounds__(kNormMaxThreads) void residual_norm_kernel(const Re
     const auto fetch = [&](int64_t row) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            rx8[v] = fetch8<XT>((const x_t*)a.x + row * a.ldx + col[v], n[v]);
-            if (stream) rr8[v] = fetch8<ST>((const s_t*)a.res + row * a.ldr + col[v], n[v]);
+            rx8[v] = fetch8<XT, MODE>((const x_t*)a.x + row * a.ldx + col[v], n);
+            rr8[v] = {};
+            if (stream) rr8[v] = fetch8<ST, MODE>((const s_t*)a.res + row * a.ldr + col[v], n);
             if constexpr (BWD) {
-                if (grad_h) rg8[v] = fetch8<ST>((const s_t*)a.gh + row * a.ldgh + col[v], n[v]);
-                if (norm) ry8[v] = fetch8<YT>((const y_t*)a.gy + row * a.ldgy + col[v], n[v]);
+                rg8[v] = {};
+                ry8[v] = {};
+                if (grad_h) rg8[v] = fetch8<ST, MODE>((const s_t*)a.gh + row * a.ldgh + col[v], n);
+                if (norm) ry8[v] = fetch8<YT, MODE>((const y_t*)a.gy + row * a.ldgy + col[v], n);
             }
         }
     };
 
     int row = blockIdx.x;
-    if (HOLD && row < a.rows) fetch(row);
+    if (HOLD) fetch(min(row, a.rows - 1));
     for (; row < a.rows; row += gridDim.x) {
         float8_t x[V], h[V], gh[V], gy[V];
         const int64_t at = (int64_t)row * width;
@@ -151,44 +204,55 @@ __global__ __launch_bounds__(kNormMaxThreads) void residual_norm_kernel(const Re
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             x[v] = widen8<XT>(rx8[v]);
-            h[v] = stream ? widen8<ST>(rr8[v]) * a.scale : float8_t{};
-            gh[v] = gy[v] = float8_t{};
+            h[v] = widen8<ST>(rr8[v]) * a.scale;  // zeros without a stream
+            if (!FULL && !stream) h[v] = float8_t{};
             if constexpr (BWD) {
-                if (grad_h) gh[v] = widen8<ST>(rg8[v]);
-                if (norm) gy[v] = widen8<YT>(ry8[v]);
+                gh[v] = widen8<ST>(rg8[v]);
+                gy[v] = widen8<YT>(ry8[v]);
             }
-            if (HOLD && a.gate_kind > DK_GATE_CHANNEL) held_gate[v] = gate_at(row, v);
+            if (HOLD && by_row) gate_row[v] = gate_at(row, v);
         }
-        if (HOLD && row + (int)gridDim.x < a.rows) fetch(row + gridDim.x);
+        if constexpr (HOLD) {
+            // the loaded registers are free for the next row: without this they live on, and copies of the next row's
+            // wait for its loads at the end of this one
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                asm volatile("" : "+v"(x[v]), "+v"(h[v]));
+                if constexpr (BWD) asm volatile("" : "+v"(gh[v]), "+v"(gy[v]));
+            }
+            fetch(min(row + (int)gridDim.x, a.rows - 1));
+        }
 
         float rx = 1.0f;
         if (post) {
             float s = 0.0f;
 #pragma unroll
-            for (int v = 0; v < V; ++v) s += sum8(x[v] * x[v]);
+            for (int v = 0; v < V; ++v) s += sum(x[v] * x[v], v);
             rx = rsqrtf(reduce(s, 0.0f).x * a.inv_width + a.eps);
         }
-        // x becomes the normalized row, branch() what the gate takes
-        const auto branch = [&](int v) { return post ? x[v] * post_weight(v) : x[v]; };
+        // x becomes the normalized row
         float sh = 0.0f, su = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             x[v] = x[v] * rx;
-            h[v] = h[v] + gate(row, v) * branch(v);
-            sh += sum8(h[v] * h[v]);
+            const float8_t p = x[v] * branch_weight(v);
+            h[v] = h[v] + (by_row ? gate(row, v) * p : p);
+            sh += sum(h[v] * h[v], v);
             if constexpr (BWD) {
-                if (norm) su += sum8(gy[v] * weight(v) * h[v]);
+                if (norm) su += sum(gy[v] * weight(v) * h[v], v);
             }
         }
         if constexpr (!BWD) {
-            if (a.h != nullptr) {
+            if (FULL || a.h != nullptr) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) put8<ST>((s_t*)a.h + at + col[v], h[v], n[v]);
+                for (int v = 0; v < V; ++v)
+                    if (lead) put8<ST, MODE>((s_t*)a.h + at + col[v], h[v], n);
             }
             if (norm) {
                 const float rh = rsqrtf(reduce(sh, 0.0f).x * a.inv_width + a.eps);
 #pragma unroll
-                for (int v = 0; v < V; ++v) put8<YT>((y_t*)a.y + at + col[v], h[v] * rh * weight(v), n[v]);
+                for (int v = 0; v < V; ++v)
+                    if (lead) put8<YT, MODE>((y_t*)a.y + at + col[v], h[v] * rh * weight(v), n);
             }
         } else {
             if (norm) {
@@ -206,23 +270,22 @@ __global__ __launch_bounds__(kNormMaxThreads) void residual_norm_kernel(const Re
             float sv = 0.0f, sg = 0.0f;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                if (a.dres != nullptr) put8<ST>((s_t*)a.dres + at + col[v], gh[v] * a.scale, n[v]);
-                const float8_t dg = gh[v] * branch(v);
-                if (a.gate_kind == DK_GATE_CHANNEL)
-                    dgate[v] = dgate[v] + dg;
-                else if (a.gate_kind == DK_GATE_ELEMENT && a.dgate != nullptr)
-                    put8_any(a.dgate, a.gate_dtype, at + col[v], dg, n[v]);
-                sg += sum8(dg);
-                gh[v] = gh[v] * gate(row, v);
-                if (post) {
-                    dpw[v] = dpw[v] + gh[v] * x[v];
-                    gh[v] = gh[v] * post_weight(v);
-                    sv += sum8(gh[v] * x[v]);
+                if ((FULL || a.dres != nullptr) && lead) put8<ST, MODE>((s_t*)a.dres + at + col[v], gh[v] * a.scale, n);
+                if (by_row) {
+                    const float8_t dg = gh[v] * (x[v] * branch_weight(v));
+                    if (a.gate_kind == DK_GATE_TOKEN)
+                        sg += sum(dg, v);
+                    else if (a.dgate != nullptr && lead)
+                        put8_any<MODE>(a.dgate, a.gate_dtype, at + col[v], dg, n);
+                    gh[v] = gh[v] * gate(row, v);
                 }
+                dq[v] = dq[v] + gh[v] * x[v];
+                gh[v] = gh[v] * branch_weight(v);
+                if (post) sv += sum(gh[v] * x[v], v);
             }
-            if (post || a.gate_kind == DK_GATE_TOKEN) {
+            if (post || (!FULL && a.gate_kind == DK_GATE_TOKEN)) {
                 const float2_t s = reduce(sv, sg);
-                if (a.gate_kind == DK_GATE_TOKEN && a.dgate != nullptr && threadIdx.x == 0) {
+                if (!FULL && a.gate_kind == DK_GATE_TOKEN && a.dgate != nullptr && threadIdx.x == 0) {
                     if (a.gate_dtype == DK_FP32)
                         store1<DK_FP32>((float*)a.dgate + row, s.y);
                     else if (a.gate_dtype == DK_BF16)
@@ -237,7 +300,8 @@ __global__ __launch_bounds__(kNormMaxThreads) void residual_norm_kernel(const Re
                 }
             }
 #pragma unroll
-            for (int v = 0; v < V; ++v) put8<XT>((x_t*)a.dx + at + col[v], gh[v], n[v]);
+            for (int v = 0; v < V; ++v)
+                if (lead) put8<XT, MODE>((x_t*)a.dx + at + col[v], gh[v], n);
         }
     }
     if constexpr (BWD) {
@@ -245,26 +309,27 @@ __global__ __launch_bounds__(kNormMaxThreads) void residual_norm_kernel(const Re
         float* slab = a.slabs + (int64_t)blockIdx.x * a.nslabs * width;
         const auto leave = [&](const float8_t* sums) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) put8<DK_FP32>(slab + col[v], sums[v], n[v]);
+            for (int v = 0; v < V; ++v)
+                if (lead) put8<DK_FP32, MODE>(slab + col[v], sums[v], n);
             slab += width;
         };
         if (a.slab_w) leave(dw);
-        if (a.slab_pw) leave(dpw);
-        if (a.slab_gate) leave(dgate);
+        if (a.slab_q) leave(dq);
     }
 }
 
-// columns of all slabs, `cols` a slab: each added by 16 threads in slab order, then those in a fixed order
+// Columns of all slabs (dweight's sums, then those of dh ux), each added by 16 threads in slab order, then those in a
+// fixed order.
 constexpr int kSumCols = 64, kSumRows = 16;
-__global__ __launch_bounds__(kSumCols* kSumRows) void slab_sum_kernel(const float* __restrict__ slabs, int n, int cols,
-                                                                      int width, float* o0, float* o1, float* o2) {
+__global__ __launch_bounds__(kSumCols* kSumRows) void residual_norm_sum_kernel(const ResidualNormArgs a, int n, float* dw,
+                                                                               float* dpw, float* dgate) {
     __shared__ float part[kSumRows][kSumCols];
     const int cx = threadIdx.x % kSumCols, ry = threadIdx.x / kSumCols;
-    const int col = blockIdx.x * kSumCols + cx;
+    const int cols = a.nslabs * a.width, col = blockIdx.x * kSumCols + cx;
     float v = 0.0f;
     if (col < cols) {
 #pragma unroll 8
-        for (int i = ry; i < n; i += kSumRows) v += slabs[(int64_t)i * cols + col];
+        for (int i = ry; i < n; i += kSumRows) v += a.slabs[(int64_t)i * cols + col];
     }
     part[ry][cx] = v;
     __syncthreads();
@@ -272,8 +337,13 @@ __global__ __launch_bounds__(kSumCols* kSumRows) void slab_sum_kernel(const floa
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < kSumRows; ++i) s += part[i][cx];
-        const int which = col / width;
-        (which == 0 ? o0 : which == 1 ? o1 : o2)[col - which * width] = s;
+        if (a.slab_w && col < a.width) {
+            dw[col] = s;
+        } else {
+            const int c = a.slab_w ? col - a.width : col;
+            if (dpw != nullptr) dpw[c] = a.gate_kind == DK_GATE_CHANNEL ? s * load_any(a.gate, a.gate_dtype, c) : s;
+            if (dgate != nullptr) dgate[c] = a.pw != nullptr ? s * load_any(a.pw, a.pw_dtype, c) : s;
+        }
     }
 }
 
@@ -287,19 +357,35 @@ static int norm_threads(int width) {
 // Work-groups: as many as the CUs hold at once, each with several rows where there are many.
 int residual_norm_groups(int64_t rows, int width, bool backward) {
     const int waves = norm_threads(width) / kWave;
-    const int64_t per_cu = backward ? (12 + waves - 1) / waves : (24 + waves - 1) / waves;
+    const int64_t per_cu = backward ? (waves > 8 ? 1 : 16 / waves) : (24 + waves - 1) / waves;
     const int64_t want = per_cu * 256;
     return (int)(rows < want ? rows : want);
 }
 
+template <int XT, int ST, int YT, int V, int MODE, bool BWD>
+static void launch_full(const ResidualNormArgs& a, unsigned grid, hipStream_t s) {
+    const dim3 g(grid), t(norm_threads(a.width));
+    const bool ends = BWD ? a.gh != nullptr && a.dres != nullptr : a.h != nullptr;
+    if (V < 4 && ends && a.res != nullptr && a.w != nullptr && a.gate_kind <= DK_GATE_CHANNEL)
+        hipLaunchKernelGGL((residual_norm_kernel<XT, ST, YT, V, MODE, (V < 4), BWD>), g, t, 0, s, a);
+    else
+        hipLaunchKernelGGL((residual_norm_kernel<XT, ST, YT, V, MODE, false, BWD>), g, t, 0, s, a);
+}
+
 template <int XT, int ST, int YT, bool BWD>
 static void launch_sized(const ResidualNormArgs& a, unsigned grid, hipStream_t s) {
-    const dim3 threads(norm_threads(a.width));
-    switch (norm_passes(a.width)) {
-        case 1: hipLaunchKernelGGL((residual_norm_kernel<XT, ST, YT, 1, BWD>), dim3(grid), threads, 0, s, a); break;
-        case 2: hipLaunchKernelGGL((residual_norm_kernel<XT, ST, YT, 2, BWD>), dim3(grid), threads, 0, s, a); break;
-        default: hipLaunchKernelGGL((residual_norm_kernel<XT, ST, YT, 4, BWD>), dim3(grid), threads, 0, s, a); break;
-    }
+    const int passes = norm_passes(a.width);
+    if (a.width < 8)
+        hipLaunchKernelGGL((residual_norm_kernel<XT, ST, YT, 1, SHORT, false, BWD>), dim3(grid),
+                           dim3(norm_threads(a.width)), 0, s, a);
+    else if (a.width % 8 == 0)
+        passes == 1   ? launch_full<XT, ST, YT, 1, EVEN, BWD>(a, grid, s)
+        : passes == 2 ? launch_full<XT, ST, YT, 2, EVEN, BWD>(a, grid, s)
+                      : launch_full<XT, ST, YT, 4, EVEN, BWD>(a, grid, s);
+    else
+        passes == 1   ? launch_full<XT, ST, YT, 1, TAIL, BWD>(a, grid, s)
+        : passes == 2 ? launch_full<XT, ST, YT, 2, TAIL, BWD>(a, grid, s)
+                      : launch_full<XT, ST, YT, 4, TAIL, BWD>(a, grid, s);
 }
 
 template <bool BWD>
@@ -328,16 +414,9 @@ hipError_t launch_residual_norm(ResidualNormArgs a, int x_dtype, int stream_dtyp
         else
             launch_typed<false>(a, x_dtype, stream_dtype, y_dtype, grid, s);
     }
-    if (a.nslabs > 0) {
-        float* out[3] = {nullptr, nullptr, nullptr};
-        int i = 0;
-        if (a.slab_w) out[i++] = dw;
-        if (a.slab_pw) out[i++] = dpw;
-        if (a.slab_gate) out[i++] = dgate_channel;
-        const int cols = a.nslabs * a.width;
-        hipLaunchKernelGGL(slab_sum_kernel, dim3((cols + kSumCols - 1) / kSumCols), dim3(kSumCols * kSumRows), 0, s,
-                           a.slabs, (int)grid, cols, a.width, out[0], out[1], out[2]);
-    }
+    if (a.nslabs > 0)
+        hipLaunchKernelGGL(residual_norm_sum_kernel, dim3((a.nslabs * a.width + kSumCols - 1) / kSumCols),
+                           dim3(kSumCols * kSumRows), 0, s, a, (int)grid, dw, dpw, dgate_channel);
     return hipGetLastError();
 }
 
