@@ -66,6 +66,17 @@ class QkRope(ctypes.Structure):
     PACK = struct.Struct("@14P9q12if i")
 
 
+class ScaledRope(ctypes.Structure):
+    """dk_scaled_rope: a rotation of part of each head (dk_scaled_rope_fwd, dk_scaled_rope_bwd)."""
+
+    _fields_ = [("q", c_vp), ("k", c_vp), ("q_out", c_vp), ("k_out", c_vp), ("positions", c_vp), ("inv_freq", c_vp),
+                ("q_stride", c_i64 * 3), ("k_stride", c_i64 * 3), ("pos_batch_stride", c_i64), ("batch", c_i64),
+                ("tokens", c_i64), ("n_heads", c_i32), ("n_kv_heads", c_i32), ("head_dim", c_i32),
+                ("rotary_dim", c_i32), ("dtype", c_i32), ("pairs", c_i32), ("positions_int64", c_i32),
+                ("factor", c_f32)]
+    PACK = struct.Struct("@6P9q7if")
+
+
 class ResidualNorm(ctypes.Structure):
     """dk_residual_norm: a call of the residual stream (dk_residual_norm_fwd, dk_residual_norm_bwd)."""
 
@@ -124,7 +135,9 @@ EXPORTS = {
     "dk_qk_rope_fwd": ([c_vp, c_vp], c_i32),
     "dk_qk_rope_bwd_workspace": ([c_vp], c_i64),
     "dk_qk_rope_bwd": ([c_vp, c_vp, c_i64, c_vp], c_i32),
-    # packed bytes as well (ResidualNorm.PACK)
+    # packed bytes as well (ScaledRope.PACK, ResidualNorm.PACK)
+    "dk_scaled_rope_fwd": ([c_vp, c_vp], c_i32),
+    "dk_scaled_rope_bwd": ([c_vp, c_vp], c_i32),
     "dk_residual_norm_fwd": ([c_vp, c_vp], c_i32),
     "dk_residual_norm_bwd_workspace": ([c_vp], c_i64),
     "dk_residual_norm_bwd": ([c_vp, c_vp, c_i64, c_vp], c_i32),

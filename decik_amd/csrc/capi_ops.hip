@@ -477,4 +477,61 @@ int dk_residual_norm_bwd(const dk_residual_norm* d, void* workspace, int64_t wor
                         "dk_residual_norm_bwd launch");
 }
 
+static int scaled_rope(const dk_scaled_rope* d, bool backward, void* stream) {
+    dk_clear_error();
+    if (d == nullptr) return dk_fail("dk_scaled_rope: null descriptor");
+    if (d->dtype != DK_FP16 && d->dtype != DK_BF16) return dk_fail("dk_scaled_rope: q and k must be fp16 or bf16");
+    if (d->head_dim < 1 || d->head_dim > 1024) return dk_fail("dk_scaled_rope: head_dim must be 1 to 1024");
+    if (d->rotary_dim < 0 || d->rotary_dim > d->head_dim || d->rotary_dim % 2 != 0)
+        return dk_fail("dk_scaled_rope: rotary_dim must be even and from 0 to head_dim");
+    if (d->n_heads < 1 || d->n_kv_heads < 1 || d->n_heads > 65536 || d->n_kv_heads > 65536)
+        return dk_fail("dk_scaled_rope: 1 to 65536 heads each");
+    if (d->batch < 0 || d->tokens < 0 || d->tokens >= INT32_MAX || d->batch >= INT32_MAX ||
+        d->batch * d->tokens >= (int64_t(1) << 24))  // (threads of a launch are below 2^32)
+        return dk_fail("dk_scaled_rope: batch * tokens must be non-negative and below 2^24");
+    if (d->batch * d->tokens == 0) return 0;
+    if (d->q == nullptr || d->k == nullptr || d->q_out == nullptr || d->k_out == nullptr)
+        return dk_fail("dk_scaled_rope: null pointer");
+    if (d->rotary_dim > 0 && (d->positions == nullptr || d->inv_freq == nullptr))
+        return dk_fail("dk_scaled_rope: positions and inv_freq must be set");
+    for (int i = 0; i < 3; ++i)
+        if (d->q_stride[i] < 0 || d->k_stride[i] < 0) return dk_fail("dk_scaled_rope: negative stride");
+    ScaledRopeArgs a{};
+    a.q = d->q;
+    a.k = d->k;
+    a.oq = d->q_out;
+    a.ok = d->k_out;
+    a.pos = d->positions;
+    a.inv_freq = d->inv_freq;
+    const int64_t t = d->tokens, hd = d->head_dim;
+    for (int i = 0; i < 3; ++i) {
+        a.q_in[i] = d->q_stride[i];
+        a.k_in[i] = d->k_stride[i];
+    }
+    for (int side = 0; side < 2; ++side) {
+        const int64_t h = side ? d->n_kv_heads : d->n_heads;
+        int64_t* const st = side ? a.k_st : a.q_st;
+        st[0] = t * h * hd;
+        st[1] = backward ? h * hd : hd;
+        st[2] = backward ? hd : t * hd;
+    }
+    a.pos_batch = d->pos_batch_stride;
+    a.tokens = (uint32_t)t;
+    a.rows = (uint32_t)(d->batch * t);
+    a.hq = d->n_heads;
+    a.hk = d->n_kv_heads;
+    a.d = d->head_dim;
+    a.r = d->rotary_dim;
+    a.pairs = d->pairs;
+    a.pos64 = d->positions_int64;
+    a.factor = d->factor;
+    a.sin_factor = backward ? -d->factor : d->factor;
+    return check_launch(launch_scaled_rope(a, d->dtype, static_cast<hipStream_t>(stream)),
+                        backward ? "dk_scaled_rope_bwd launch" : "dk_scaled_rope_fwd launch");
+}
+
+int dk_scaled_rope_fwd(const dk_scaled_rope* d, void* stream) { return scaled_rope(d, false, stream); }
+
+int dk_scaled_rope_bwd(const dk_scaled_rope* d, void* stream) { return scaled_rope(d, true, stream); }
+
 }  // extern "C"

@@ -338,6 +338,20 @@ int residual_norm_groups(int64_t rows, int width, bool backward);
 hipError_t launch_residual_norm(ResidualNormArgs a, int x_dtype, int stream_dtype, int y_dtype, bool backward,
                                 float* dw, float* dpw, float* dgate_channel, hipStream_t s);
 
+// Rotary positions of part of each head (scaled_rope.hip).
+struct ScaledRopeArgs {
+    const void *q, *k;
+    void *oq, *ok;
+    const void* pos;
+    const float* inv_freq;
+    int64_t q_in[3], k_in[3], q_st[3], k_st[3];  // strides of batch, token and head, elements
+    int64_t pos_batch;
+    uint32_t tokens, rows;  // tokens a batch entry, batch * tokens
+    int32_t hq, hk, d, r, pairs, pos64, tpw;
+    float factor, sin_factor;  // sin_factor: -factor backward
+};
+hipError_t launch_scaled_rope(ScaledRopeArgs a, int dtype, hipStream_t s);
+
 // The calling thread's error (dk_last_error); dk_fail returns 1.
 int dk_fail(const char* msg);
 void dk_clear_error();

@@ -73,4 +73,12 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
     return (float)((const _Float16*)p)[i];
 }
 
+// inv_freq (radians a position) in turns, as a fraction of 2^64: a product with an integer position wraps where whole
+// turns drop out.
+__device__ __forceinline__ uint64_t turn_fraction(float inv_freq) {
+    const double turns = (double)inv_freq * 0.15915494309189533577;
+    const double part = turns - floor(turns);  // 1 for a tiny negative frequency: a whole turn, as 0
+    return part < 1.0 ? (uint64_t)(part * 18446744073709551616.0) : 0;
+}
+
 }  // namespace dk

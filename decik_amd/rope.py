@@ -11,14 +11,18 @@ Next to it, without a counterpart in the reference (dk_qk_rope_fwd / dk_qk_rope_
   qk_norm_rope_*  RMS norms of every query and key head (weights [D]) with the rotation in one pass
   axes_rope_*     rotary positions with several axes (time, height, width), the angles formed from
                   integer positions and frequencies, with or without the norms
-Both take q and k token-major (strided rows of a packed projection output as they are), fp16 or bf16,
+  scaled_rope_*   rotary positions of the first part of each head, in halves or in pairs, from positions and
+                  frequencies (scaled_frequencies: stretched for long contexts), any strides (dk_scaled_rope_*)
+All take q and k token-major (strided rows of a packed projection output as they are), fp16 or bf16,
 and give them head-major [B, H, T, D]; everything is computed in fp32 and rounded once.
 """
+
+import math
 
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import DTYPES, QkRope, call_on, check, gpu_input, lib, ptr, same_gpu, stream_of
+from ._lib import DTYPES, QkRope, ScaledRope, call_on, check, gpu_input, lib, ptr, same_gpu, stream_of
 
 
 def _rows(t):
@@ -304,3 +308,177 @@ def axes_rope(q, k, positions, inv_freq, sections, n_heads, n_kv_heads, interlea
     """axes_rope_forward, differentiable in q, k and the norm weights."""
     return _QkRotation.apply(q, k, q_weight, k_weight, (n_heads, n_kv_heads), eps,
                              ("axes", tuple(int(s) for s in sections), bool(interleaved)), positions, inv_freq)
+
+
+LAYOUTS = ("half", "pairs")
+
+
+def scaled_frequencies(rotary_dim, base=10000.0, scaling=None, length=None, device=None):
+    """(inv_freq fp32 [rotary_dim / 2] in radians a position, the factor of cos and sin) of a rotation of rotary_dim
+    elements, for a context stretched as a model's configuration says. scaling: None or a dict with "rope_type" (or
+    "type") and
+      default  nothing more
+      linear   factor: every frequency over factor
+      ntk      factor: base times factor^(R / (R - 2)), which stretches the slowest frequency by factor
+      dynamic  factor, original_max_position_embeddings: as ntk for the `length` of the call, where that is longer
+      yarn     factor, original_max_position_embeddings; beta_fast 32, beta_slow 1, attention_factor 0.1 ln factor + 1:
+               frequencies of more than beta_fast turns in the original length are kept, those of fewer than beta_slow are
+               divided by factor, a ramp over their index between
+      llama3   factor, low_freq_factor, high_freq_factor, original_max_position_embeddings: the same with a ramp over
+               the number of turns
+      longrope short_factor, long_factor (a divisor a frequency; the second where `length` is longer than the original),
+               original_max_position_embeddings, and factor or attention_factor (sqrt(1 + ln factor / ln original))
+    Computed in 64 bits and rounded once."""
+    what = "scaled_frequencies"
+    r = int(rotary_dim)
+    if r < 2 or r % 2:
+        raise ValueError(f"{what}: rotary_dim must be even and positive")
+    s = dict(scaling or {})
+    kind = s.get("rope_type", s.get("type", "default"))
+
+    def given(name):
+        if s.get(name) is None:
+            raise ValueError(f"{what}: {kind} needs {name}")
+        return s[name]
+
+    i = torch.arange(r // 2, dtype=torch.float64)
+    stretch = lambda by: base if r == 2 else base * by ** (r / (r - 2))  # noqa: E731
+    inv, attention = float(base) ** (-2.0 * i / r), 1.0
+    if kind == "linear":
+        inv = inv / given("factor")
+    elif kind == "ntk":
+        inv = stretch(given("factor")) ** (-2.0 * i / r)
+    elif kind == "dynamic":
+        factor, original = given("factor"), given("original_max_position_embeddings")
+        if length is not None and length > original:
+            inv = stretch(factor * length / original - (factor - 1)) ** (-2.0 * i / r)
+    elif kind == "yarn":
+        factor, original = given("factor"), given("original_max_position_embeddings")
+        fast, slow = s.get("beta_fast") or 32.0, s.get("beta_slow") or 1.0
+        # the index whose frequency makes n turns in the original length
+        index = lambda n: r * math.log(original / (n * 2.0 * math.pi)) / (2.0 * math.log(base))  # noqa: E731
+        low, high = max(math.floor(index(fast)), 0), min(math.ceil(index(slow)), r - 1)
+        slowed = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        inv = inv * (1.0 - slowed) + inv / factor * slowed
+        attention = s.get("attention_factor")
+        if attention is None:
+            attention = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    elif kind == "llama3":
+        factor, low, high = given("factor"), given("low_freq_factor"), given("high_freq_factor")
+        turns = given("original_max_position_embeddings") * inv / (2.0 * math.pi)
+        kept = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        inv = inv * kept + inv / factor * (1.0 - kept)
+    elif kind == "longrope":
+        original = given("original_max_position_embeddings")
+        by = given("long_factor" if length is not None and length > original else "short_factor")
+        if len(by) != r // 2:
+            raise ValueError(f"{what}: longrope needs {r // 2} divisors")
+        inv = inv / torch.tensor(by, dtype=torch.float64)
+        attention = s.get("attention_factor")
+        if attention is None:
+            factor = given("factor")
+            attention = math.sqrt(1.0 + math.log(factor) / math.log(original)) if factor > 1.0 else 1.0
+    elif kind != "default":
+        raise ValueError(f"{what}: unknown kind of scaling {kind!r}")
+    return inv.to(torch.float32).to(device), float(attention)
+
+
+def _scaled_rope(what, entry, q, k, batch, tokens, heads, d, q_strides, k_strides, positions, inv_freq, layout, factor,
+                 shapes):
+    dev = q.device
+    same_gpu(what, dev, k, positions, inv_freq)
+    code = _QK_TYPES.get(q.dtype)
+    if code is None or k.dtype != q.dtype:
+        raise ValueError(f"{what}: q and k must both be fp16 or both bf16")
+    if layout not in LAYOUTS:
+        raise ValueError(f"{what}: layout must be one of {LAYOUTS}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: positions must be int32 or int64")
+    if positions.shape not in ((tokens,), (batch, tokens), (1, tokens)):
+        raise ValueError(f"{what}: positions must be [T] or [B, T] of T = {tokens}, B = {batch}, not {tuple(positions.shape)}")
+    if inv_freq.dim() != 1 or 2 * inv_freq.shape[0] > d:
+        raise ValueError(f"{what}: inv_freq must hold at most D / 2 = {d // 2} frequencies")
+    if tokens > 1 and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    inv_freq = _fp32(inv_freq)
+    pos_batch = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+    outs = q.new_empty(shapes[0]), q.new_empty(shapes[1])
+    call_on(dev, entry, ScaledRope.PACK.pack(q.data_ptr(), k.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(),
+                                             positions.data_ptr(), inv_freq.data_ptr(), *q_strides, *k_strides, pos_batch,
+                                             batch, tokens, *heads, d, 2 * inv_freq.shape[0], code, layout == "pairs",
+                                             positions.dtype == torch.int64, factor))
+    return outs
+
+
+def _token_major(what, t, heads):
+    """(t, B, T, D, strides of batch, token and head) of a [B, T, H * D] or [T, H * D] tensor."""
+    if t.dim() not in (2, 3) or heads < 1 or t.shape[-1] % heads or t.shape[-1] == 0:
+        raise ValueError(f"{what}: q and k must be [B, T, H * D] or [T, H * D], here H = {heads}, not {tuple(t.shape)}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1 or min(t.stride()) < 0:
+        t = t.contiguous()
+    b, n = (1, t.shape[0]) if t.dim() == 2 else t.shape[:2]
+    d = t.shape[-1] // heads
+    return t, b, n, d, (t.stride(0) if t.dim() == 3 else 0, t.stride(-2), d)
+
+
+def scaled_rope_forward(q, k, positions, inv_freq, n_heads, n_kv_heads, layout="half", factor=1.0):
+    """(q_out [B, H, T, D], k_out [B, HK, T, D]): the first 2 len(inv_freq) elements of every head turned by positions
+    ([T] or [B, T], int32 or int64) times inv_freq (radians a position), cos and sin times factor; the others as they
+    are. layout "half": element j turns with j + len(inv_freq), "pairs": 2 j with 2 j + 1. q [B, T, H*D] or [T, H*D]
+    (any strides of the first axes), k likewise, fp16 or bf16. The angles are exact to 2^-24 turns for positions below
+    2^28 and frequencies up to 2 pi."""
+    what = "scaled_rope_forward"
+    gpu_input(what, q)
+    same_gpu(what, q.device, k)
+    q, b, t, d, q_strides = _token_major(what, q, n_heads)
+    k, bk, tk, dk, k_strides = _token_major(what, k, n_kv_heads)
+    if (bk, tk, dk) != (b, t, d):
+        raise ValueError(f"{what}: q and k must have the same tokens and head size")
+    return _scaled_rope(what, lib().dk_scaled_rope_fwd, q, k, b, t, (n_heads, n_kv_heads), d, q_strides, k_strides,
+                        positions, inv_freq, layout, factor, ((b, n_heads, t, d), (b, n_kv_heads, t, d)))
+
+
+def scaled_rope_backward(grad_q, grad_k, positions, inv_freq, layout="half", factor=1.0):
+    """(dq [B, T, H*D], dk [B, T, HK*D]) of scaled_rope_forward from gradients [B, H, T, D] of its outputs."""
+    what = "scaled_rope_backward"
+    gpu_input(what, grad_q)
+    same_gpu(what, grad_q.device, grad_k)
+    if grad_q.dim() != 4 or grad_k.dim() != 4 or grad_q.shape[0] != grad_k.shape[0] or \
+            grad_q.shape[2:] != grad_k.shape[2:]:
+        raise ValueError(f"{what}: gradients must be [B, H, T, D] of the same B, T and D")
+    b, hq, t, d = grad_q.shape
+    hk = grad_k.shape[1]
+    grads = [g if d <= 1 or g.stride(3) == 1 else g.contiguous() for g in (grad_q, grad_k)]
+    strides = [(g.stride(0), g.stride(2), g.stride(1)) for g in grads]
+    return _scaled_rope(what, lib().dk_scaled_rope_bwd, *grads, b, t, (hq, hk), d, *strides, positions, inv_freq, layout,
+                        factor, ((b, t, hq * d), (b, t, hk * d)))
+
+
+class _ScaledRope(torch.autograd.Function):
+    """apply(q, k, positions, inv_freq, heads, layout, factor) -> (q_out, k_out)."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, heads, layout, factor):
+        if ctx.needs_input_grad[3]:
+            raise ValueError("scaled_rope: frequencies take no gradient (detach them)")
+        outs = scaled_rope_forward(q, k, positions, inv_freq, *heads, layout, factor)
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.heads, ctx.layout, ctx.factor, ctx.shapes, ctx.outs = heads, layout, factor, (q.shape, k.shape), outs[0].shape
+        ctx.qk_dtype, ctx.device = q.dtype, q.device
+        ctx.set_materialize_grads(False)
+        return outs
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        if all(g is None for g in grads):
+            return (None,) * 7
+        b, _, t, d = ctx.outs
+        gq, gk = _head_major_grads(ctx, grads, b, t, d)
+        dq, dk = scaled_rope_backward(gq, gk, *ctx.saved_tensors, ctx.layout, ctx.factor)
+        return dq.reshape(ctx.shapes[0]), dk.reshape(ctx.shapes[1]), None, None, None, None, None
+
+
+def scaled_rope(q, k, positions, inv_freq, n_heads, n_kv_heads, layout="half", factor=1.0):
+    """scaled_rope_forward, differentiable in q and k."""
+    return _ScaledRope.apply(q, k, positions, inv_freq, (n_heads, n_kv_heads), layout, factor)

@@ -394,6 +394,32 @@ int dk_int8_linear_bwd(const void* dy, int dy_dtype, int64_t lddy, const int8_t*
                        void* dx, int dx_dtype, int64_t lddx, int64_t m, int64_t n, int64_t k, void* workspace,
                        int64_t workspace_bytes, void* stream);
 
+/* Rotary positions of the first rotary_dim elements of every q and k head, no counterpart in the reference: pair j
+ * (elements j and j + rotary_dim / 2, or with `pairs` 2 j and 2 j + 1) turns by positions[b, t] * inv_freq[j], its
+ * cosine and sine times `factor`, in fp32 and rounded once; the other elements are copied. Forward reads heads at
+ * q + b q_stride[0] + t q_stride[1] + head q_stride[2] (elements, k alike; any start) and writes packed
+ * [batch, heads, tokens, head_dim]; backward turns the other way, reads gradients with the same kind of strides and
+ * writes packed [batch, tokens, heads * head_dim]. positions: int32 or int64, [tokens] for each batch entry,
+ * pos_batch_stride apart (0: shared); angles are exact to 2^-24 turns for positions below 2^28 and frequencies up to
+ * 2 pi. dtype fp16 or bf16; 1 <= head_dim <= 1024, rotary_dim even and from 0 to head_dim, 1 to 65536 heads each,
+ * batch * tokens below 2^24. */
+typedef struct {
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    const void* positions;
+    const float* inv_freq;
+    int64_t q_stride[3], k_stride[3];
+    int64_t pos_batch_stride;
+    int64_t batch, tokens;
+    int32_t n_heads, n_kv_heads, head_dim, rotary_dim;
+    int32_t dtype, pairs, positions_int64;
+    float factor;
+} dk_scaled_rope;
+int dk_scaled_rope_fwd(const dk_scaled_rope* d, void* stream);
+int dk_scaled_rope_bwd(const dk_scaled_rope* d, void* stream);
+
 /* ---- the residual stream between two blocks, no counterpart in the reference --------------- */
 
 /* h = residual_scale * residual + gate * N(x) * post_weight and y = N(h) * weight over rows of `width`
