@@ -130,6 +130,14 @@ bool int8_rows_ok(const void* p, int64_t ld, int64_t cols) {
     return aligned_to(p, 16) && ld % 16 == 0 && ld >= (cols + 15) / 16 * 16 && ld < kInt8MaxLd;
 }
 
+bool int4_sizes(int64_t m, int64_t n, int64_t k) {
+    // (work-groups of the largest outputs fit a launch)
+    const int64_t most = int64_t(1) << 23, area = int64_t(1) << 37;
+    return m >= 0 && n >= 0 && m < most && n < most && k >= 1 && k <= (int64_t(1) << 20) && m * n < area && m * k < area;
+}
+
+const char* const kInt4Sizes = "dk_int4_linear: 0 <= m, n < 2^23, m n < 2^37, m k < 2^37, 1 <= k <= 2^20";
+
 bool rows_fit(int64_t ld, int heads, int d) { return ld >= (int64_t)heads * d; }
 
 // everything of a residual-stream call but its outputs and gradients
@@ -533,5 +541,79 @@ static int scaled_rope(const dk_scaled_rope* d, bool backward, void* stream) {
 int dk_scaled_rope_fwd(const dk_scaled_rope* d, void* stream) { return scaled_rope(d, false, stream); }
 
 int dk_scaled_rope_bwd(const dk_scaled_rope* d, void* stream) { return scaled_rope(d, true, stream); }
+
+int64_t dk_int4_linear_workspace(int backward, int copy, int64_t m, int64_t n, int64_t k) {
+    dk_clear_error();
+    if (!int4_sizes(m, n, k)) {
+        dk_fail(kInt4Sizes);
+        return -1;
+    }
+    if (m == 0 || n == 0) return 0;
+    const int64_t sum = backward ? n : k;
+    return (int4_plan(m, n, k, backward != 0).partial_bytes + 15) / 16 * 16 + (copy ? m * ((sum + 7) / 8 * 16) : 0);
+}
+
+int dk_int4_linear_plan(int backward, int64_t m, int64_t n, int64_t k, int32_t* out) {
+    dk_clear_error();
+    if (!int4_sizes(m, n, k) || m == 0 || n == 0 || out == nullptr) return dk_fail(kInt4Sizes);
+    const Int4Plan p = int4_plan(m, n, k, backward != 0);
+    out[0] = p.tokens;
+    out[1] = p.few ? p.waves : 0;
+    out[2] = p.splits;
+    return 0;
+}
+
+int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, int64_t ldw,
+                   const uint32_t* meta, int64_t group, int scale_dtype, const void* bias, int bias_dtype, void* y,
+                   int y_dtype, int64_t ldy, int64_t m, int64_t n, int64_t k, int copy, void* workspace,
+                   int64_t workspace_bytes, void* stream) {
+    dk_clear_error();
+    if (!int4_sizes(m, n, k)) return dk_fail(kInt4Sizes);
+    if ((x_dtype != DK_FP16 && x_dtype != DK_BF16) || (y_dtype != x_dtype && y_dtype != DK_FP32))
+        return dk_fail("dk_int4_linear: x must be fp16 or bf16, y of x's type or fp32");
+    if (scale_dtype != DK_FP16 && scale_dtype != DK_BF16) return dk_fail("dk_int4_linear: scales must be fp16 or bf16");
+    if (bias != nullptr && (backward || !is_dtype(bias_dtype)))
+        return dk_fail("dk_int4_linear: a bias of a known type, and only forward");
+    if (group < 32 || group % 32 != 0 || group > (int64_t(1) << 20))
+        return dk_fail("dk_int4_linear: group must be a multiple of 32 up to 2^20");
+    if (m == 0 || (backward ? k : n) == 0) return 0;
+    const int64_t cols = backward ? k : n, sum = backward ? n : k;
+    if (y == nullptr) return dk_fail("dk_int4_linear: null pointer");
+    if (m > 1 && ldy < cols) return dk_fail("dk_int4_linear: output rows overlap");
+    if (n == 0) return dk_fail("dk_int4_linear: the sum has no terms");
+    if (x == nullptr || packed == nullptr || meta == nullptr) return dk_fail("dk_int4_linear: null pointer");
+    if (!aligned_to(packed, 16) || ldw % 64 != 0 || ldw < (k + 127) / 128 * 64 || ldw > (int64_t(1) << 20) ||
+        !aligned_to(meta, 4))
+        return dk_fail("dk_int4_linear: packed must be 16-byte aligned, its row stride a multiple of 64 that holds k");
+    if (m > 1 && (ldx < 0 || ldx >= (int64_t(1) << 23)))
+        return dk_fail("dk_int4_linear: x's row stride must be non-negative and below 2^23");
+    if (!copy && (sum % 8 != 0 || !aligned_to(x, 16) || (m > 1 && ldx % 8 != 0)))
+        return dk_fail("dk_int4_linear: without copy x needs 16-byte aligned rows of a multiple of 8 columns");
+    const Int4Plan p = int4_plan(m, n, k, backward != 0);
+    const int64_t partial = (p.partial_bytes + 15) / 16 * 16, need = partial + (copy ? m * ((sum + 7) / 8 * 16) : 0);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16)))
+        return dk_fail("dk_int4_linear: workspace too small (dk_int4_linear_workspace)");
+    Int4Args a{};
+    a.x = x;
+    a.w = packed;
+    a.meta = meta;
+    a.bias = bias;
+    a.y = y;
+    a.partials = static_cast<float*>(workspace);
+    a.padded = copy ? reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + partial) : nullptr;
+    a.ldx = m > 1 ? ldx : 0;
+    a.ldw = ldw;
+    a.ldy = ldy;
+    a.m = (int32_t)m;
+    a.n = (int32_t)n;
+    a.k = (int32_t)k;
+    a.groups = (int32_t)((k + group - 1) / group);
+    a.group_units = (int32_t)(group / 32);
+    a.scale_dtype = scale_dtype;
+    a.bias_dtype = bias_dtype;
+    a.y_dtype = y_dtype;
+    return check_launch(launch_int4(a, p, x_dtype, backward != 0, static_cast<hipStream_t>(stream)),
+                        "dk_int4_linear launch");
+}
 
 }  // extern "C"

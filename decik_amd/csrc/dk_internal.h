@@ -352,6 +352,29 @@ struct ScaledRopeArgs {
 };
 hipError_t launch_scaled_rope(ScaledRopeArgs a, int dtype, hipStream_t s);
 
+// Products with weights of 4-bit integers (int4_linear.hip).
+constexpr int kInt4FewM = 64;  // forward launches of so few tokens stream the weight to registers
+struct Int4Args {
+    const void* x;       // [m, k], backward dy [m, n]: 16-byte aligned rows, or `padded` set
+    const uint8_t* w;    // [n, ldw], blocks of 128 columns
+    const uint32_t* meta;  // [n, groups]: scale, zero point
+    const void* bias;
+    void* y;
+    float* partials;     // splits > 1
+    uint16_t* padded;    // room for x with aligned rows, or null
+    int64_t ldx, ldw, ldy, slab;
+    int32_t m, n, k, kpad, x_cols, groups, group_units, scale_dtype, bias_dtype, y_dtype;
+    uint32_t group_mul;
+    int32_t blocks, blocks_per_split, splits, m_tiles, n_tiles;
+};
+struct Int4Plan {
+    bool few;
+    int tokens, waves, m_tiles, n_tiles, splits, steps_per_split;
+    int64_t partial_bytes;
+};
+Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward);
+hipError_t launch_int4(Int4Args a, const Int4Plan& p, int dtype, bool backward, hipStream_t s);
+
 // The calling thread's error (dk_last_error); dk_fail returns 1.
 int dk_fail(const char* msg);
 void dk_clear_error();

@@ -1,0 +1,305 @@
+"""Linear layers in 4-bit integers (decik_amd.int4) against the formulas in 64 bits: every form (few tokens by 16, 32 and
+64 and by 4, 8 and 16 waves; tiles whole and split), groups, zero points, types, odd sizes, strides, and the
+packing, on the CPU.
+
+Tolerances, with S = sum over k of |x| scale |code - zero|. Forward: operands are exact, a chain of fp32 sums has at most 32 +
+K / 32 terms (32 in an MFMA, then MFMAs, groups, waves or splits), so the sum is within (64 + K / 32) 2^-24 of S, in bf16 of
+S + 48 sum |x| scale, since there code + 16 is summed and taken off again (at most 31 + 32 and the zero point); then
+one rounding, half a step. Backward: a weight is rounded once, half a step of its type (fp16: at least 2^-25), in bf16
+from an fp32 multiply-add within 2^-18 of the scale; the sums as before with N."""
+
+import pytest
+import torch
+
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+TINY = {F16: 2.0 ** -25, BF16: 2.0 ** -134, F32: 2.0 ** -149}
+
+
+def make(shape, dtype, device, seed, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * std).to(dtype).to(device)
+
+
+def random_parts(n, k, group, dtype, seed, zeros=True):
+    g = torch.Generator().manual_seed(seed)
+    groups = -(-k // group)
+    codes = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8)
+    scales = (torch.rand((n, groups), generator=g) * 0.02 + 1e-3).to(dtype)
+    zs = torch.randint(0, 17, (n, groups), generator=g, dtype=torch.uint8) if zeros else None
+    return codes, scales, zs
+
+
+def values(codes, scales, zeros, group):
+    """(W, scale of every element) in float64."""
+    k = codes.shape[1]
+    s = scales.double().repeat_interleave(group, 1)[:, :k]
+    z = 8.0 if zeros is None else zeros.double().repeat_interleave(group, 1)[:, :k]
+    return (codes.double() - z) * s, s
+
+
+def check(got, value, mag, what):
+    assert got.shape == value.shape, what
+    err = (got.double() - value).abs()
+    bound = value.abs() * (torch.finfo(got.dtype).eps / 2) + mag + TINY[got.dtype]
+    assert bool((err <= bound).all()), f"{what}: worst excess {(err - bound).max().item():.3e}"
+
+
+def check_forward(y, x, w, s, bias, what="y"):
+    k = x.shape[1]
+    xd, w, s = x.double(), w.to(x.device), s.to(x.device)
+    value = xd @ w.t().contiguous()
+    mag = xd.abs() @ w.abs().t().contiguous()
+    if x.dtype == BF16:
+        mag = mag + 48 * (xd.abs() @ s.t().contiguous())
+    mag = mag * (64 + k / 32) * 2.0 ** -24
+    if bias is not None:
+        value = value + bias.double()
+        mag = mag + (value.abs() + bias.double().abs()) * 2.0 ** -24
+    check(y, value, mag, what)
+
+
+def check_backward(dx, dy, w, s, what="dx"):
+    n = dy.shape[1]
+    dd, w, s = dy.double(), w.to(dy.device), s.to(dy.device)
+    off = w.abs() * (torch.finfo(dy.dtype).eps / 2 * 1.01 + (64 + n / 32) * 2.0 ** -24)
+    off = off + (2.0 ** -25 if dy.dtype == F16 else s * 2.0 ** -18)
+    check(dx, dd @ w, dd.abs() @ off, what)
+
+
+# ---- packing, on the CPU -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n,k,group", [(1, 1, 32), (3, 127, 32), (5, 128, 128), (7, 129, 64), (2, 300, 96), (4, 1000, 4096), (0, 8, 32)])
+def test_packing_round_trip(n, k, group):
+    from decik_amd.int4 import dequantize_int4, int4_weight
+
+    codes, scales, zeros = random_parts(n, k, group, BF16, 1)
+    w = int4_weight(codes, scales, zeros, group)
+    assert w.packed.shape == (n, -(-k // 128) * 64) and w.shape == (n, k)
+    assert torch.equal(w.codes(), codes) and torch.equal(w.scales, scales) and torch.equal(w.zeros, zeros)
+    assert torch.equal(dequantize_int4(w).double(), values(codes, scales, zeros, group)[0].float().double())
+    assert torch.equal(int4_weight(codes, scales, None, group).zeros, torch.full_like(zeros, 8))
+
+
+def test_packed_layout():
+    """Word 4 q + j of a block: columns 32 j + 8 q + e, column e in bits 4 (e // 2) + 16 (e % 2)."""
+    from decik_amd.int4 import int4_weight
+
+    codes, scales, _ = random_parts(2, 256, 128, F16, 3)
+    words = int4_weight(codes, scales, None, 128).packed.view(torch.int32).long() & 0xFFFFFFFF
+    for n, b, q, j, e in ((0, 0, 0, 0, 0), (1, 1, 3, 2, 7), (0, 1, 2, 3, 4), (1, 0, 1, 0, 1)):
+        word = int(words[n, 16 * b + 4 * q + j])
+        assert word >> (4 * (e // 2) + 16 * (e % 2)) & 15 == int(codes[n, 128 * b + 32 * j + 8 * q + e])
+
+
+def test_quantize():
+    """Values off by at most half a scale and the scale's own rounding; extremes, zeros and numbers that are none."""
+    from decik_amd.int4 import dequantize_int4, quantize_int4
+
+    w = make((9, 300), F32, "cpu", 1, 0.02)
+    w[0, :32] = 0.0
+    w[1, :32] = w[1, :32].abs() + 0.01
+    w[2, 5] = float("inf")
+    w[3, 5] = float("nan")
+    for symmetric in (False, True):
+        for dtype in (F16, BF16):
+            q = quantize_int4(w, 32, symmetric, dtype)
+            d = dequantize_int4(q)
+            assert q.scale_dtype == dtype and not d[0, :32].any() and not d[2, :32].any() and not d[3, :32].any()
+            s = q.scales.float().repeat_interleave(32, 1)[:, :300]
+            keep = torch.ones_like(w, dtype=torch.bool)
+            keep[2:4, :32] = False
+            # (a scale rounded down leaves the extremes up to 15 half steps of the scale outside)
+            assert bool(((d - w).abs() <= s * (0.5 + 16 * torch.finfo(dtype).eps))[keep].all())
+
+
+def test_refusals_of_weights():
+    from decik_amd.int4 import int4_weight, quantize_int4
+
+    codes, scales, zeros = random_parts(4, 64, 32, F16, 1)
+    for args, msg in (((codes.int(), scales, zeros, 32), "uint8"), ((codes[0], scales, zeros, 32), "uint8"), ((codes, scales, zeros, 48), "32"),
+                      ((codes, scales, zeros, 64), "scales"), ((codes, scales.float(), zeros, 32), "scales"), ((codes, scales, zeros[:2], 32), "zeros"),
+                      ((codes + 1, scales, zeros, 32), "0 to 15"), ((codes, scales, zeros + 17, 32), "0 to 16"), ((codes[:, :0], scales[:, :0], None, 32), "K")):
+        with pytest.raises(ValueError, match=msg):
+            int4_weight(*args)
+    for args, msg in (((codes,), "fp16"), ((scales, 40), "32"), ((scales, 32, False, F32), "scale_dtype"), ((scales[0],), "N, K")):
+        with pytest.raises(ValueError, match=msg):
+            quantize_int4(*args)
+
+
+# ---- products ------------------------------------------------------------------------------------
+
+# tokens, rows, columns: each form and what lies around its edges
+FORWARD = [(1, 1, 1), (1, 17, 128), (2, 100, 129), (15, 333, 1121), (16, 48, 4096), (16, 48, 8961), (1, 8200, 2100), (3, 16500, 640), (17, 40, 640),
+           (31, 257, 5000), (32, 9000, 2049), (33, 70, 512), (64, 300, 4100), (64, 17000, 256), (65, 256, 128), (65, 3, 130), (128, 255, 1000),
+           (129, 257, 4096), (300, 700, 1121), (830, 1536, 1536), (257, 1000, 31)]
+BACKWARD = [(1, 1, 1), (1, 128, 17), (2, 129, 300), (16, 1121, 333), (32, 640, 256), (33, 1000, 257), (64, 4096, 128), (65, 31, 600), (128, 2057, 1121),
+            (129, 300, 513), (300, 1121, 700), (830, 1536, 1536), (37, 2057, 1121), (50, 200, 600)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", FORWARD)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_forward(m, n, k, dtype, device):
+    from decik_amd.int4 import int4_linear_forward, int4_weight
+
+    x, bias = make((m, k), dtype, device, 2), make((n,), dtype, device, 3)
+    for group, zeros, scale_dtype in ((32, True, dtype), (64, False, F16), (128, True, BF16), (96, True, dtype), (2 ** 20, True, dtype)):
+        parts = random_parts(n, k, group, scale_dtype, group, zeros)
+        weight = int4_weight(*(None if p is None else p.to(device) for p in parts), group)
+        w, s = values(*parts, group)
+        check_forward(int4_linear_forward(x, weight, bias), x, w, s, bias, f"group {group}")
+        check_forward(int4_linear_forward(x, weight, None, F32), x, w, s, None, f"group {group} fp32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", BACKWARD)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_backward(m, n, k, dtype, device):
+    from decik_amd.int4 import int4_linear_backward, int4_weight
+
+    dy = make((m, n), dtype, device, 2)
+    for group, zeros, scale_dtype in ((32, True, dtype), (64, False, F16), (128, True, BF16), (96, True, dtype), (2 ** 20, True, dtype)):
+        parts = random_parts(n, k, group, scale_dtype, group, zeros)
+        weight = int4_weight(*(None if p is None else p.to(device) for p in parts), group)
+        w, s = values(*parts, group)
+        check_backward(int4_linear_backward(dy, weight), dy, w, s, f"group {group}")
+        check_backward(int4_linear_backward(dy, weight, F32), dy, w, s, f"group {group} fp32")
+
+
+@pytest.mark.gpu
+def test_every_form_is_tested(device):
+    """The sizes above reach every token tile, wave count and both split and whole sums."""
+    from decik_amd.int4 import launch_plan
+
+    plans = [launch_plan(False, *s) for s in FORWARD]
+    assert {(p["tile_tokens"], p["waves"]) for p in plans} == {(16, 4), (16, 8), (16, 16), (32, 4), (32, 8), (32, 16), (64, 4), (64, 8), (128, 0)}
+    assert {p["splits"] > 1 for p in plans if p["waves"] == 0} == {True, False}
+    plans = [launch_plan(True, *s) for s in BACKWARD]
+    assert {p["tile_tokens"] for p in plans} == {32, 64, 128}
+    assert {(p["tile_tokens"], p["splits"] > 1) for p in plans} == {(t, s) for t in (32, 64, 128) for s in (True, False)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 5, 40, 200])
+def test_strides_and_batches(m, device):
+    """Rows that start anywhere, shared rows, transposed activations, three axes: the values of contiguous copies."""
+    from decik_amd.int4 import int4_linear_backward, int4_linear_forward, int4_weight
+
+    n, k = 72, 264
+    weight = int4_weight(*(p.to(device) for p in random_parts(n, k, 64, F16, 1)), 64)
+    for fn, cols, out in ((int4_linear_forward, k, n), (int4_linear_backward, n, k)):
+        wide = make((m, 3 * cols + 8), F16, device, 2)
+        for x in (wide[:, 8:8 + cols], wide[:, 3:3 + cols], make((cols, m), F16, device, 3).t(), wide[:1, :cols].expand(m, cols),
+                  make((m, 2 * cols), F16, device, 4)[:, ::2]):
+            y = fn(x, weight)
+            assert y.shape == (m, out) and torch.equal(y, fn(x.contiguous(), weight))
+        x3 = make((2, m, cols), F16, device, 5)
+        assert torch.equal(fn(x3, weight), fn(x3.reshape(-1, cols), weight).view(2, m, out))
+        assert torch.equal(fn(x3[0, 0], weight), fn(x3[0, :1], weight)[0])
+        assert fn(x3[:, :0], weight).shape == (2, 0, out)
+
+
+@pytest.mark.gpu
+def test_no_rows_in_the_weight(device):
+    from decik_amd.int4 import int4_linear_backward, int4_linear_forward, int4_weight
+
+    weight = int4_weight(*(p.to(device) for p in random_parts(0, 64, 32, F16, 1)), 32)
+    assert int4_linear_forward(make((3, 64), F16, device, 1), weight).shape == (3, 0)
+    assert torch.equal(int4_linear_backward(make((3, 0), F16, device, 1), weight), torch.zeros((3, 64), dtype=F16, device=device))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 20, 200])
+def test_rows_without_numbers_stay_alone(m, device):
+    """An infinity or NaN of a token shows in that token alone; what lies behind a row is not read into it."""
+    from decik_amd.int4 import int4_linear_backward, int4_linear_forward, int4_weight
+
+    n, k = 200, 328
+    weight = int4_weight(*(p.to(device) for p in random_parts(n, k, 32, BF16, 1)), 32)
+    for fn, cols in ((int4_linear_forward, k), (int4_linear_backward, n)):
+        for dtype in (F16, BF16):
+            wide = torch.full((m, cols + 8), float("nan"), dtype=dtype, device=device)
+            wide[:, :cols] = make((m, cols), dtype, device, 2)
+            x = wide[:, :cols]
+            clean = fn(x.contiguous(), weight)
+            assert torch.equal(fn(x, weight), clean) and bool(clean.isfinite().all())
+            x = x.contiguous()
+            x[1, cols - 1], x[2, 0] = float("inf"), float("nan")
+            got = fn(x, weight)
+            keep = [i for i in range(m) if i not in (1, 2)]
+            assert torch.equal(got[keep], clean[keep]) and not bool(got[2].isfinite().any())
+
+
+@pytest.mark.gpu
+def test_outputs_take_any_row_length(device):
+    """Rows behind the last token and columns behind the last row are left as they were (allocations of the outputs' sizes
+    inside larger buffers are written by the C entry)."""
+    from decik_amd import _lib
+    from decik_amd.int4 import int4_linear_forward, int4_linear_backward, int4_weight
+
+    for m, n, k in ((3, 45, 96), (200, 300, 136), (70, 31, 264)):
+        weight = int4_weight(*(p.to(device) for p in random_parts(n, k, 32, F16, 1)), 32)
+        for back, cols, total in ((0, n, k), (1, k, n)):
+            x = make((m, total), F16, device, 2)
+            want = (int4_linear_backward if back else int4_linear_forward)(x, weight)
+            out = torch.full((m + 2, cols + 3), 7.0, dtype=F16, device=device)
+            copy = int(total % 8 != 0)
+            need = _lib.lib().dk_int4_linear_workspace(back, copy, m, n, k)
+            work = torch.empty(max(need, 1), dtype=torch.uint8, device=device)
+            _lib.call_on(device, _lib.lib().dk_int4_linear, back, x.data_ptr(), 0, total, weight.packed.data_ptr(),
+                         weight.packed.stride(0), weight.meta.data_ptr(), 32, 0, None, 0, out.data_ptr(), 0, cols + 3, m, n, k, copy,
+                         work.data_ptr(), need)
+            assert torch.equal(out[:m, :cols], want)
+            assert bool((out[m:] == 7).all()) and bool((out[:, cols:] == 7).all())
+
+
+@pytest.mark.gpu
+def test_autograd_and_differences(device):
+    """Gradients through autograd equal the backward's; along a direction they equal the 64-bit form's, which is linear
+    in x, so that a difference of step 1 is exact."""
+    from decik_amd.int4 import Int4Linear, int4_linear_backward, int4_weight
+
+    m, n, k, group = 37, 100, 200, 32
+    parts = random_parts(n, k, group, F16, 1)
+    weight = int4_weight(*(p.to(device) for p in parts), group)
+    w, s = values(*parts, group)
+    x, bias, dy = make((m, k), F16, device, 2).requires_grad_(), make((n,), F16, device, 3), make((m, n), F16, device, 4)
+    Int4Linear.apply(x, weight, bias).backward(dy)
+    assert torch.equal(x.grad, int4_linear_backward(dy, weight))
+    step = make((m, k), F16, "cpu", 5).double()
+    slope = ((step @ w.t()) * dy.double().cpu()).sum()
+    room = ((x.grad.double().cpu().abs() * 2.0 ** -11 + dy.double().cpu().abs() @ (w.abs() * 2.0 ** -10 + 2.0 ** -25)) * step.abs()).sum()
+    assert abs(float((x.grad.double().cpu() * step).sum() - slope)) <= float(room)
+    x.grad = None
+    Int4Linear.apply(x, weight).backward(dy)
+    assert torch.equal(x.grad, int4_linear_backward(dy, weight))
+    with pytest.raises(ValueError, match="frozen"):
+        Int4Linear.apply(x, weight, bias.clone().requires_grad_())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 17, 1121), (40, 513, 4100), (200, 300, 4096)])
+def test_same_bits_every_run(m, n, k, device):
+    from decik_amd.int4 import int4_linear_backward, int4_linear_forward, int4_weight
+
+    weight = int4_weight(*(p.to(device) for p in random_parts(n, k, 32, F16, 1)), 32)
+    x, dy = make((m, k), F16, device, 2), make((m, n), F16, device, 3)
+    y, dx = int4_linear_forward(x, weight), int4_linear_backward(dy, weight)
+    for _ in range(3):
+        assert torch.equal(y, int4_linear_forward(x, weight)) and torch.equal(dx, int4_linear_backward(dy, weight))
+
+
+@pytest.mark.gpu
+def test_refusals(device):
+    from decik_amd.int4 import int4_linear_backward, int4_linear_forward, int4_weight
+
+    weight = int4_weight(*(p.to(device) for p in random_parts(8, 64, 32, F16, 1)), 32)
+    x, dy = make((4, 64), F16, device, 1), make((4, 8), F16, device, 2)
+    for args, kw, msg in (((x[:, :32], weight), {}, "64"), ((x.float(), weight), {}, "fp16"), ((x, weight), dict(dtype=BF16), "dtype"),
+                          ((x.cpu(), weight), {}, "GPU"), ((x, weight.to("cpu")), {}, "GPU"), ((x, weight, dy[0, :4]), {}, "bias"),
+                          ((x, weight, dy[0].double()), {}, "bias"), ((x, weight.packed), {}, "Int4Weight"), ((x, weight, dy[0].cpu()), {}, "GPU")):
+        with pytest.raises(ValueError, match=msg):
+            int4_linear_forward(*args, **kw)
+    for args, msg in (((x, weight), "8"), ((dy.float(), weight), "fp16"), ((dy, x), "Int4Weight")):
+        with pytest.raises(ValueError, match=msg):
+            int4_linear_backward(*args)
