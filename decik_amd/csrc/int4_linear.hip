@@ -14,6 +14,9 @@
 // From pairs to operands, fp16: 0x6400 | q is 1024 + q, 0x6400 | 16 q is 1024 + 16 q, and one packed subtraction or
 // multiply-add leaves q - zero, exactly. bf16: 0x4180 | 8 q is 16 + q; there is no packed bf16 arithmetic, so 16 + zero
 // times the sum of x, from one more MFMA, is taken off the group's sum.
+#include <cstdio>
+#include <cstdlib>
+
 #include "elem.h"
 #include "gemm_common.h"
 
@@ -209,13 +212,22 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
     }
 }
 
-// ---- forward, many tokens ------------------------------------------------------------------------
-// Tiles of 128 tokens by 256 rows of the weight, eight waves of 64 by 64. The tokens' block of 128 columns goes to LDS
-// (two stages, 16-byte chunks permuted by row against bank conflicts), the weight to registers, a block ahead.
-constexpr int kI4TileM = 128, kI4TileN = 256, kI4Waves = 8;
-constexpr int kI4StageBytes = kI4TileM * kI4Block * 2;
+// ---- tiles ---------------------------------------------------------------------------------------
+// Tiles of 32 C tokens by 256 rows of the weight (forward) or 256 columns (backward), eight waves of 16 C by 64. The sum
+// goes in steps of 64 terms through a ring of three stages of LDS, filled by loads that go there directly: one wait and
+// one barrier a step, loads two steps ahead. The weight stays in 4 bits up to each wave's registers.
+// W is rounded to the activations' type here. fp16: (code - zero) exact, one packed product. bf16: the pair
+// 1024 + code, as fp16, times scale - (1024 + zero) scale by mixed multiply-adds in fp32 (its constant is within 2^-13 of
+// a scale), then one rounding.
+constexpr int kI4Waves = 8, kI4TileN = 256, kI4Step = 64, kI4Ring = 3;
 
-// consecutive tiles on one XCD, token tiles fastest within bands of eight (the same order as the 8-bit products)
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+// 16-byte chunk of a row of 128 bytes: neighbouring rows share the banks' two halves, pairs of rows are permuted
+__device__ __forceinline__ int chunk_key(int row) { return (row >> 1) & 7; }
+
+// Consecutive tiles on one XCD, token tiles fastest within bands of eight, so that the tiles of an XCD at one time share
+// rows of both operands.
 __device__ __forceinline__ void tile_of(const Int4Args& a, int& m_tile, int& n_tile, int& split) {
     const int per = a.m_tiles * a.n_tiles, nwg = per * a.splits;
     const int xcd = blockIdx.x & 7, r8 = nwg & 7;
@@ -228,67 +240,141 @@ __device__ __forceinline__ void tile_of(const Int4Args& a, int& m_tile, int& n_t
     n_tile = in / rows;
 }
 
-// 16 rows of `cols` outputs a wave holds through LDS leave as 16-byte pieces
+// The activations' part of a stage: rows of 64 terms (128 bytes), at least 64 rows; a wave's loads of a step.
+template <int C>
+struct I4Tokens {
+    static constexpr int TM = 32 * C, BYTES = (TM < 64 ? 64 : TM) * 128, LOADS = BYTES / 1024 / kI4Waves;
+    rsrc_t src;
+    uint32_t at[LOADS];
+    int col[LOADS];
+    int wave;
+    __device__ __forceinline__ void set(const Int4Args& a, int m0, int w, int lane) {
+        const int toks = min(TM, a.m - m0);
+        wave = w;
+        src = make_rsrc((const uint16_t*)a.x + (int64_t)m0 * a.ldx, (uint32_t)(((toks - 1) * a.ldx + a.x_cols) * 2));
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int row = 8 * (wave * LOADS + i) + (lane >> 3);
+            col[i] = 8 * ((lane & 7) ^ chunk_key(row));
+            at[i] = off_if(row < toks, (row * (uint32_t)a.ldx + col[i]) * 2);
+        }
+    }
+    // columns c0 .. c0 + 63 (live: the step exists)
+    __device__ __forceinline__ void fetch(uint8_t* stage, const Int4Args& a, int c0, bool live) const {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            bload128_lds(src, stage + 1024 * (wave * LOADS + i),
+                         off_if(live && c0 + col[i] < a.x_cols, at[i] + 2 * (uint32_t)c0));
+    }
+};
+
+// scale and zero point as the tiles multiply with them
 template <int DT>
-__device__ __forceinline__ void put_row8(const Int4Args& a, const uint16_t* from, int64_t at, int left) {
+struct I4Group;
+template <>
+struct I4Group<DK_FP16> {
+    ZeroF16 zero;
+    half2_t scale;
+    __device__ __forceinline__ void set(uint32_t meta, int scale_dtype) {
+        zero.set(meta);
+        const _Float16 s = scale_dtype == DK_FP16 ? __builtin_bit_cast(_Float16, (uint16_t)meta) : (_Float16)I4<DK_BF16>::scale(meta);
+        scale = half2_t{s, s};
+    }
+    // weights of a word's columns 0 .. 7
+    __device__ __forceinline__ half8_t weights(uint32_t d) const {
+        u32x4_t v = __builtin_bit_cast(u32x4_t, unpack8<DK_FP16>(d, zero));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t pair = v[i];  // (a bit_cast of the element itself would take element 0)
+            v[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, pair) * scale);
+        }
+        return __builtin_bit_cast(half8_t, v);
+    }
+};
+template <>
+struct I4Group<DK_BF16> {
+    float whole, whole_zero, part, part_zero;  // of 1024 + code, and of 1024 + 16 code
+    __device__ __forceinline__ void set(uint32_t meta, int scale_dtype) {
+        whole = scale_of(meta, scale_dtype);
+        const float z = zero_of(meta);
+        whole_zero = (-1024.0f - z) * whole;
+        part = whole * 0.0625f;
+        part_zero = (-64.0f - z) * whole;
+    }
+    static __device__ __forceinline__ uint32_t pair(uint32_t v, float by, float plus) {
+        const half2_t h = __builtin_bit_cast(half2_t, v);
+        const float2_t f = float2_t{__builtin_fmaf((float)h[0], by, plus), __builtin_fmaf((float)h[1], by, plus)};
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
+    }
+    __device__ __forceinline__ bf16x8_t weights(uint32_t d) const {
+        const uint32_t h = d >> 8;
+        return __builtin_bit_cast(bf16x8_t, u32x4_t{pair(and_or(d, 0x000F000Fu, 0x64006400u), whole, whole_zero),
+                                                    pair(and_or(d, 0x00F000F0u, 0x64006400u), part, part_zero),
+                                                    pair(and_or(h, 0x000F000Fu, 0x64006400u), whole, whole_zero),
+                                                    pair(and_or(h, 0x00F000F0u, 0x64006400u), part, part_zero)});
+    }
+};
+
+template <int DT>
+__device__ __forceinline__ void put4(const Int4Args& a, int64_t at, float4_t v, int left) {
     typedef typename Elem<DT>::type E;
-    if (left >= 8) {
-        *(typename Elem<DT>::loose*)((E*)a.y + at) = *(const typename Elem<DT>::vec*)from;
+    typedef E vec4 __attribute__((ext_vector_type(4)));
+    typedef vec4 loose4 __attribute__((aligned(sizeof(E))));
+    asm("" : "+v"(v));
+    if (left >= 4) {
+        *(loose4*)((E*)a.y + at) = __builtin_convertvector(v, vec4);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < left) ((E*)a.y)[at + e] = ((const E*)from)[e];
+        for (int e = 0; e < 4; ++e)
+            if (e < left) ((E*)a.y)[at + e] = (E)v[e];
     }
 }
 
-template <int DT, int GJ>
+// ---- forward, many tokens: two steps a block of 128 columns; the weight's block and its groups' words every other step
+constexpr int kI4WBytes = kI4TileN * 64;
+template <int C, int GJ>
+constexpr size_t int4_tile_lds() {
+    constexpr size_t ring = kI4Ring * I4Tokens<C>::BYTES + 2 * (kI4WBytes + 4 / GJ * kI4TileN * 4);
+    constexpr size_t out = kI4Waves * (C < 4 ? 16 * C : 64) * 72 * 2;
+    return ring > out ? ring : out;
+}
+
+template <int DT, int C, int GJ>
 __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4Args a) {
     typedef typename I4<DT>::vec vec;
-    constexpr int UNITS = 4 / GJ, R = 4, C = 4, XLOADS = kI4StageBytes / 1024 / kI4Waves;
+    constexpr int UNITS = 4 / GJ, R = 4, XB = I4Tokens<C>::BYTES, WB = kI4WBytes + UNITS * kI4TileN * 4;
+    constexpr int METAS = UNITS == 4 ? 2 : 1, WLOADS = 2 + METAS;  // a wave's loads of a block
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
     int mt, nt, split;
     tile_of(a, mt, nt, split);
-    const int m0 = mt * kI4TileM, n0 = nt * kI4TileN;
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    const int b0 = split * a.blocks_per_split, steps = min(a.blocks_per_split, a.blocks - b0);
+    const int m0 = mt * 32 * C, n0 = nt * kI4TileN;
+    const int wm = (wave & 1) * 16 * C, wn = (wave >> 1) * 64;
+    const int b0 = split * a.blocks_per_split, blocks = min(a.blocks_per_split, a.blocks - b0);
 
-    const int rows = min(64, a.n - n0 - wn), toks = min(kI4TileM, a.m - m0);
-    const rsrc_t wr = make_rsrc(a.w + (int64_t)(n0 + wn) * a.ldw, rows > 0 ? (uint32_t)(rows * a.ldw) : 0u);
-    const rsrc_t mr = make_rsrc(a.meta + (int64_t)(n0 + wn) * a.groups, rows > 0 ? (uint32_t)(rows * a.groups * 4) : 0u);
-    const rsrc_t xr = make_rsrc((const uint16_t*)a.x + (int64_t)m0 * a.ldx, (uint32_t)(((toks - 1) * a.ldx + a.x_cols) * 2));
-    uint32_t x_at[XLOADS];
-    int x_col[XLOADS];
+    I4Tokens<C> x;
+    x.set(a, m0, wave, lane);
+    const int rows = min(kI4TileN, a.n - n0);
+    const rsrc_t wr = make_rsrc(a.w + (int64_t)n0 * a.ldw, (uint32_t)(rows * a.ldw));
+    const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(rows * a.groups * 4));
+    uint8_t* const weights = smem + kI4Ring * XB;
+    const auto fetch_x = [&](int h) { x.fetch(smem + (h % kI4Ring) * XB, a, b0 * kI4Block + kI4Step * h, h < 2 * blocks); };
+    const auto fetch_w = [&](int b) {
+        uint8_t* const stage = weights + (b & 1) * WB;
+        const bool live = b < blocks;
 #pragma unroll
-    for (int i = 0; i < XLOADS; ++i) {
-        const int row = 4 * (wave * XLOADS + i) + (lane >> 4);
-        x_col[i] = 8 * ((lane & 15) ^ (row & 15));
-        x_at[i] = off_if(row < toks, (row * (uint32_t)a.ldx + x_col[i]) * 2);
-    }
-    const auto fetch_x = [&](int t) {
-        const int k0 = (b0 + t) * kI4Block;
+        for (int i = 0; i < 2; ++i) {  // 16 rows of 64 bytes a load
+            const uint32_t row = 16 * (2 * wave + i) + (lane >> 2);
+            bload128_lds(wr, stage + 1024 * (2 * wave + i),
+                         off_if(live, row * (uint32_t)a.ldw + 64 * (uint32_t)(b0 + b) + 16 * (lane & 3)));
+        }
 #pragma unroll
-        for (int i = 0; i < XLOADS; ++i)
-            bload128_lds(xr, smem + (t & 1) * kI4StageBytes + 1024 * (wave * XLOADS + i),
-                         off_if(t < steps && k0 + x_col[i] < a.x_cols, x_at[i] + 2 * (uint32_t)k0));
-    };
-    struct Weights {
-        u32x4_t w[R];
-        uint32_t meta[R][UNITS];
-    };
-    const auto fetch_w = [&](Weights& f, int t) {
-        const uint32_t b = b0 + t;
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const uint32_t row = 16 * i + r;
-            f.w[i] = bload128(wr, off_if(t < steps, row * (uint32_t)a.ldw + 16 * q + 64 * b));
-#pragma unroll
-            for (int u = 0; u < UNITS; ++u) {
-                const uint32_t g = min(group_at(a, 4 * b + GJ * u), (uint32_t)a.groups - 1);
-                f.meta[i][u] = __builtin_amdgcn_raw_buffer_load_b32(
-                    mr, (int)off_if(t < steps, (row * (uint32_t)a.groups + g) * 4), 0, 0);
-            }
+        for (int i = 0; i < METAS; ++i) {  // 64 rows of one unit a load; with one unit waves 4 to 7 repeat 0 to 3's
+            const int load = UNITS == 1 ? wave & 3 : METAS * wave + i, u = load >> 2;
+            const uint32_t row = 64 * (load & 3) + lane;
+            const uint32_t g = min(group_at(a, 4 * (b0 + b) + GJ * u), (uint32_t)a.groups - 1);
+            bload32_lds(mr, stage + kI4WBytes + 256 * load, off_if(live, (row * (uint32_t)a.groups + g) * 4));
         }
     };
 
@@ -297,65 +383,48 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
     for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[i][c] = float4_t{};
-    const vec ones = __builtin_bit_cast(vec, u32x4_t{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u});  // bf16
 
-    Weights f;
-    fetch_w(f, 0);
-    fetch_x(0);
-    for (int t = 0; t < steps; ++t) {
-        wait_vmcnt<0>();
-        lds_barrier();  // the stage is whole, and every wave has read the one before it
-        const Weights now = f;
-        fetch_w(f, t + 1);
-        fetch_x(t + 1);
-        const uint8_t* const stage = smem + (t & 1) * kI4StageBytes;
+    const auto multiply = [&](int h, int j0, const u32x4_t (&w)[R], const I4Group<DT> (&g)[R][UNITS]) {
+        const uint8_t* const stage = smem + (h % kI4Ring) * XB;
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            float4_t s[R][C], xs[C];
+        for (int j = 0; j < 2; ++j) {
+            vec xv[C];
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                xs[c] = float4_t{};
-#pragma unroll
-                for (int i = 0; i < R; ++i) s[i][c] = float4_t{};
-            }
-            ZeroF16 z[R];
-            if constexpr (DT == DK_FP16) {
-#pragma unroll
-                for (int i = 0; i < R; ++i) z[i].set(now.meta[i][u]);
-            }
-#pragma unroll
-            for (int j = GJ * u; j < GJ * (u + 1); ++j) {
-                vec x[C];
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const int row = wm + 16 * c + r;
-                    x[c] = *(const vec*)(stage + row * 256 + 16 * ((4 * j + q) ^ r));
-                }
-#pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const vec w = unpack8<DT>(now.w[i][j], z[i]);
-#pragma unroll
-                    for (int c = 0; c < C; ++c) s[i][c] = I4<DT>::mfma(x[c], w, s[i][c]);
-                }
-                if constexpr (DT == DK_BF16) {
-#pragma unroll
-                    for (int c = 0; c < C; ++c) xs[c] = I4<DT>::mfma(x[c], ones, xs[c]);
-                }
+                const int row = wm + 16 * c + r;
+                xv[c] = *(const vec*)(stage + row * 128 + 16 * ((4 * j + q) ^ chunk_key(r)));
             }
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const float scale = scale_of(now.meta[i][u], a.scale_dtype);
-                const float taken = -16.0f - zero_of(now.meta[i][u]);
+                const vec wv = g[i][(j0 + j) / GJ].weights(w[i][j0 + j]);
 #pragma unroll
-                for (int c = 0; c < C; ++c)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float v = s[i][c][e];
-                        if constexpr (DT == DK_BF16) v = __builtin_fmaf(taken, xs[c][e], v);
-                        acc[i][c][e] = __builtin_fmaf(v, scale, acc[i][c][e]);
-                    }
+                for (int c = 0; c < C; ++c) acc[i][c] = I4<DT>::mfma(xv[c], wv, acc[i][c]);
             }
         }
+    };
+    fetch_x(0);
+    fetch_w(0);
+    fetch_x(1);
+    for (int b = 0; b < blocks; ++b) {
+        wait_vmcnt<I4Tokens<C>::LOADS>();  // all but the next step's
+        lds_barrier();                     // the stages are whole, and every wave has read those before them
+        fetch_x(2 * b + 2);
+        fetch_w(b + 1);
+        u32x4_t w[R];
+        I4Group<DT> g[R][UNITS];
+        const uint8_t* const stage = weights + (b & 1) * WB;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            w[i] = *(const u32x4_t*)(stage + (wn + 16 * i + r) * 64 + 16 * q);
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u)
+                g[i][u].set(*(const uint32_t*)(stage + kI4WBytes + 4 * (kI4TileN * u + wn + 16 * i + r)), a.scale_dtype);
+        }
+        multiply(2 * b, 0, w, g);
+        wait_vmcnt<I4Tokens<C>::LOADS + WLOADS>();
+        lds_barrier();
+        fetch_x(2 * b + 3);
+        multiply(2 * b + 1, 2, w, g);
     }
     wait_vmcnt<0>();
     lds_barrier();
@@ -381,200 +450,199 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
         }
         return;
     }
-    uint16_t* const mine = (uint16_t*)smem + wave * 64 * 72;  // rows of 64 outputs, padded
+    // 16-bit outputs leave as pieces of 16 bytes: up to 64 tokens of the wave's 64 rows at a time through LDS
+    constexpr int PART = C < 4 ? C : 4;
+    typedef typename Elem<DT>::type E;
+    E* const mine = (E*)smem + wave * 16 * PART * 72;
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int n = n0 + wn + 16 * i + r;
-        const float bias = a.bias != nullptr && n < a.n ? load_any(a.bias, a.bias_dtype, n) : 0.0f;
+    for (int part = 0; part < C / PART; ++part) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int i = 0; i < R; ++i) {
+            const int n = n0 + wn + 16 * i + r;
+            const float bias = a.bias != nullptr && n < a.n ? load_any(a.bias, a.bias_dtype, n) : 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) store1<DT>(mine + (16 * c + 4 * q + e) * 72 + 16 * i + r, acc[i][c][e] + bias);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+            for (int c = 0; c < PART; ++c)
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        const int row = 8 * s + (lane >> 3), m = m0 + wm + row, n = n0 + wn + 8 * (lane & 7);
-        if (m < a.m && n < a.n) put_row8<DT>(a, mine + row * 72 + 8 * (lane & 7), (int64_t)m * a.ldy + n, a.n - n);
+                for (int e = 0; e < 4; ++e)
+                    store1<DT>(mine + (16 * c + 4 * q + e) * 72 + 16 * i + r, acc[i][part * PART + c][e] + bias);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int s = 0; s < 2 * PART; ++s) {
+            const int row = 8 * s + (lane >> 3), m = m0 + wm + 16 * PART * part + row, n = n0 + wn + 8 * (lane & 7);
+            if (m >= a.m || n >= a.n) continue;
+            const E* const from = mine + row * 72 + 8 * (lane & 7);
+            E* const to = (E*)a.y + (int64_t)m * a.ldy + n;
+            if (n + 8 <= a.n) {
+                *(typename Elem<DT>::loose*)to = *(const typename Elem<DT>::vec*)from;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (n + e < a.n) to[e] = from[e];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
 // ---- backward ------------------------------------------------------------------------------------
-// Tiles of 32 C tokens by 256 columns, four waves of 16 C by 128. A lane holds one dword of eight columns of each of
-// eight rows; halves of two rows' dwords joined in one register unpack to pairs along the rows, MFMA j's operand
-// for column j of every lane's dword, so that the weight needs no other layout than the forward's. Its sums come out eight
-// columns a lane. Rows' scales and zero points go through LDS, a block of 128 rows ahead, as do dy's columns.
-constexpr int kI4BackN = 128, kI4BackCols = 256, kI4BackUnits = kI4BackCols / 32;
+// The weight's layout is the forward's. Lanes r and r + 8 of an MFMA operand hold columns j and j + 4 of the
+// same word (j = 0 .. 3: four MFMAs), each of its eight rows' words; halves of two rows' words joined in one register
+// unpack to pairs along the rows. Rows' scales and zero points go through tables of 64 rows by the tile's eight units
+// of 32 columns: their words come a step before the step's other loads, and the threads (an entry each) make the tables
+// of the next step.
+constexpr int kI4BackUnits = 8, kI4Table = kI4BackUnits * kI4Step;
 
 template <int DT>
-struct BackMeta;  // of the eight rows of a lane and step
+struct BackRows;  // of the eight rows of a lane
 template <>
-struct BackMeta<DK_FP16> {
-    half8_t scale, zero;  // scale, -(1024 + zero)
+struct BackRows<DK_FP16> {
     typedef _Float16 elem;
-    static constexpr int bytes = 2;
+    half8_t scale, zero;  // -(1024 + zero)
+    static __device__ __forceinline__ void keep(elem* table, int e, uint32_t meta, int scale_dtype) {
+        table[e] = (elem)scale_of(meta, scale_dtype);
+        table[kI4Table + e] = (elem)(-1024.0f - zero_of(meta));
+    }
+    // weights of rows 2 p and 2 p + 1: 1024 + code
+    __device__ __forceinline__ uint32_t pair(uint32_t v, int p) const {
+        const half2_t w = __builtin_bit_cast(half2_t, v) + half2_t{zero[2 * p], zero[2 * p + 1]};
+        return __builtin_bit_cast(uint32_t, w * half2_t{scale[2 * p], scale[2 * p + 1]});
+    }
 };
 template <>
-struct BackMeta<DK_BF16> {
-    float8_t scale, zero;  // scale, -(16 + zero) scale
+struct BackRows<DK_BF16> {
     typedef float elem;
-    static constexpr int bytes = 4;
+    float8_t scale, zero;  // -(1024 + zero) scale
+    static __device__ __forceinline__ void keep(elem* table, int e, uint32_t meta, int scale_dtype) {
+        const float s = scale_of(meta, scale_dtype);
+        table[e] = s;
+        table[kI4Table + e] = (-1024.0f - zero_of(meta)) * s;
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t v, int p) const {
+        const half2_t h = __builtin_bit_cast(half2_t, v);
+        const float2_t f = float2_t{__builtin_fmaf((float)h[0], scale[2 * p], zero[2 * p]),
+                                    __builtin_fmaf((float)h[1], scale[2 * p + 1], zero[2 * p + 1])};
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
+    }
 };
 
-// MFMA operands of one pair of rows for the eight columns of their dwords: two weights a register
-template <int DT>
-__device__ __forceinline__ void weights_of_pair(uint32_t d0, uint32_t d1, const BackMeta<DT>& m, int pair, uint32_t (&o)[8]) {
-    const uint32_t even = perm_lo(d0, d1), odd = perm_hi(d0, d1);  // columns 0 2 4 6, columns 1 3 5 7
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t v = h ? odd : even;
-            if constexpr (DT == DK_FP16) {
-                half2_t w = __builtin_bit_cast(half2_t, and_or(v >> (4 * i), 0x000F000Fu, 0x64006400u));
-                w = w + half2_t{m.zero[2 * pair], m.zero[2 * pair + 1]};
-                w = w * half2_t{m.scale[2 * pair], m.scale[2 * pair + 1]};
-                o[2 * i + h] = __builtin_bit_cast(uint32_t, w);
-            } else {
-                const uint32_t w = and_or(i == 0 ? v << 3 : v >> (4 * i - 3), 0x00780078u, 0x41804180u);
-                typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-                const float2_t f = float2_t{__builtin_fmaf(__builtin_bit_cast(float, w << 16), m.scale[2 * pair], m.zero[2 * pair]),
-                                            __builtin_fmaf(__builtin_bit_cast(float, w & 0xFFFF0000u), m.scale[2 * pair + 1],
-                                                           m.zero[2 * pair + 1])};
-                o[2 * i + h] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
-            }
-        }
-    }
+constexpr int kI4BackWBytes = kI4Step * 128;  // 64 rows of 256 columns
+template <int DT, int C>
+constexpr int int4_back_stage() {
+    return I4Tokens<C>::BYTES + kI4BackWBytes + 2 * kI4Table * (int)sizeof(typename BackRows<DT>::elem);
 }
 
 template <int DT, int C>
-constexpr size_t int4_back_lds() {
-    return 2 * (32 * C * kI4BackN * 2 + 2 * kI4BackUnits * kI4BackN * BackMeta<DT>::bytes);
-}
-
-template <int DT, int C>
-__global__ __launch_bounds__(256, 2) void int4_back_kernel(const Int4Args a) {
+__global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4Args a) {
     typedef typename I4<DT>::vec vec;
-    typedef typename BackMeta<DT>::elem meta_t;
-    constexpr int TM = 32 * C, XBYTES = TM * kI4BackN * 2, XLOADS = XBYTES / 4096, TABLE = kI4BackUnits * kI4BackN;
-    constexpr int STAGE = XBYTES + 2 * TABLE * (int)sizeof(meta_t), METAS = TABLE / 256;
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    typedef typename BackRows<DT>::elem meta_t;
+    constexpr int XB = I4Tokens<C>::BYTES, STAGE = int4_back_stage<DT, C>();
+    extern __shared__ __attribute__((aligned(32))) uint8_t smem[];
+    uint32_t* const raw = (uint32_t*)(smem + kI4Ring * STAGE);  // two steps' words of the groups
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
     int mt, kt, split;
     tile_of(a, mt, kt, split);
-    const int m0 = mt * TM, k0 = kt * kI4BackCols;
-    const int wm = (wave & 1) * 16 * C, wk = (wave >> 1) * 128;
-    const int b0 = split * a.blocks_per_split, steps = min(a.blocks_per_split, a.blocks - b0);  // of 128 rows
+    const int m0 = mt * 32 * C, k0 = kt * 256;
+    const int wm = (wave & 1) * 16 * C, wk = wave >> 1;  // the wave's 64 columns: half wk & 1 of block wk >> 1
+    const int n_begin = split * a.blocks_per_split * kI4Block;
+    const int n_end = min(a.n, n_begin + a.blocks_per_split * kI4Block), steps = (n_end - n_begin + kI4Step - 1) / kI4Step;
 
-    const int toks = min(TM, a.m - m0);
-    const rsrc_t xr = make_rsrc((const uint16_t*)a.x + (int64_t)m0 * a.ldx, (uint32_t)(((toks - 1) * a.ldx + a.x_cols) * 2));
-    uint32_t x_at[XLOADS];
-    int x_col[XLOADS];
-#pragma unroll
-    for (int i = 0; i < XLOADS; ++i) {
-        const int row = 4 * (wave * XLOADS + i) + (lane >> 4);
-        x_col[i] = 8 * ((lane & 15) ^ (row & 15));
-        x_at[i] = off_if(row < toks, (row * (uint32_t)a.ldx + x_col[i]) * 2);
-    }
-    const auto fetch_x = [&](int t) {
-        const int n0 = (b0 + t) * kI4BackN;
-#pragma unroll
-        for (int i = 0; i < XLOADS; ++i)
-            bload128_lds(xr, smem + (t & 1) * STAGE + 1024 * (wave * XLOADS + i),
-                         off_if(t < steps && n0 + x_col[i] < a.x_cols, x_at[i] + 2 * (uint32_t)n0));
-    };
-    // scales and zero points of 128 rows and the tile's eight units of 32 columns: thread's entries 256 i + threadIdx.x,
-    // entry = unit * 128 + row
-    uint32_t metas[METAS];
-    const auto fetch_meta = [&](int t) {
-        const int n0 = (b0 + t) * kI4BackN, rows = t < steps ? min(kI4BackN, a.n - n0) : 0;
-        const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(rows * a.groups * 4));
-#pragma unroll
-        for (int i = 0; i < METAS; ++i) {
-            const int e = 256 * i + threadIdx.x, row = e & 127, unit = e >> 7;
-            const uint32_t g = min(group_at(a, k0 / 32 + unit), (uint32_t)a.groups - 1);
-            metas[i] = __builtin_amdgcn_raw_buffer_load_b32(mr, (int)off_if(row < rows, (row * (uint32_t)a.groups + g) * 4), 0, 0);
-        }
-    };
-    const auto keep_meta = [&](int t) {
-        meta_t* const table = (meta_t*)(smem + (t & 1) * STAGE + XBYTES);
-#pragma unroll
-        for (int i = 0; i < METAS; ++i) {
-            const int e = 256 * i + threadIdx.x;
-            const float s = scale_of(metas[i], a.scale_dtype), z = zero_of(metas[i]);
-            table[e] = (meta_t)s;
-            table[TABLE + e] = (meta_t)(DT == DK_FP16 ? -1024.0f - z : (-16.0f - z) * s);
-        }
-    };
-    // dwords of the eight rows of a lane in step s (32 rows) of block t
-    struct Rows {
-        uint32_t d[8];
-    };
-    const bool cols = k0 + wk < a.kpad;
-    const uint32_t w_at = (uint32_t)((k0 + wk) / 2) + 4 * r;
-    const auto fetch_w = [&](Rows& f, int t, int s) {
-        const int n0 = (b0 + t) * kI4BackN, rows = t < steps && cols ? min(kI4BackN, a.n - n0) : 0;
+    I4Tokens<C> x;
+    x.set(a, m0, wave, lane);
+    // Words of a stage: row 8 q + i of a step's half lies so that the four rows that a read takes (q = 0 .. 3) use different
+    // banks: chunks swap halves of the row by bit 3 of the row, rows swap places in their pair by bit 4.
+    const int w_slot = 8 * wave + (lane >> 3), w_row = w_slot ^ ((w_slot >> 4) & 1);
+    const int w_chunk = (lane & 7) ^ (((w_row >> 3) & 1) << 2);
+    const uint32_t w_col = (uint32_t)k0 / 2 + 16 * w_chunk;
+    const bool w_live = w_col < (uint32_t)a.ldw;
+    const int e_row = threadIdx.x & 63;
+    const uint32_t e_group = min(group_at(a, k0 / 32 + (threadIdx.x >> 6)), (uint32_t)a.groups - 1);
+    const auto fetch = [&](int h) {
+        const int n0 = n_begin + kI4Step * h;
+        const bool live = h < steps;
+        uint8_t* const stage = smem + (h % kI4Ring) * STAGE;
+        x.fetch(stage, a, n0, live);
+        const int rows = live ? min(kI4Step, n_end - n0) : 0;
         const rsrc_t wr = make_rsrc(a.w + (int64_t)n0 * a.ldw, (uint32_t)(rows * a.ldw));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int row = 32 * s + 8 * q + i;
-            f.d[i] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)off_if(row < rows, row * (uint32_t)a.ldw + w_at), 0, 0);
-        }
+        bload128_lds(wr, stage + XB + 1024 * wave, off_if(w_live && w_row < rows, w_row * (uint32_t)a.ldw + w_col));
     };
+    const auto fetch_meta = [&](int h) {
+        const int n0 = n_begin + kI4Step * h, rows = h < steps ? min(kI4Step, n_end - n0) : 0;
+        const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(rows * a.groups * 4));
+        bload32_lds(mr, raw + (h & 1) * kI4Table + 64 * wave, off_if(e_row < rows, (e_row * (uint32_t)a.groups + e_group) * 4));
+    };
+    const auto table = [&](int h) { return (meta_t*)(smem + (h % kI4Ring) * STAGE + XB + kI4BackWBytes); };
 
-    float4_t acc[C][8];
+    float4_t acc[C][4];
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[c][j] = float4_t{};
+        for (int j = 0; j < 4; ++j) acc[c][j] = float4_t{};
 
-    const auto step = [&](const Rows& f, int t, int s) {
-        const uint8_t* const stage = smem + (t & 1) * STAGE;
-        const meta_t* const table = (const meta_t*)(stage + XBYTES) + ((wk / 32) + (r & 3)) * kI4BackN + 32 * s + 8 * q;
-        BackMeta<DT> m;
-        m.scale = *(const decltype(m.scale)*)table;
-        m.zero = *(const decltype(m.zero)*)(table + TABLE);
-        vec x[C];
+    // this lane's word of a row: word 4 q' + j' of its block with j' = 2 (wk & 1) + (r & 1), q' = (r >> 1) & 3
+    const int unit = 4 * (wk >> 1) + 2 * (wk & 1) + (r & 1), chunk = 4 * (wk >> 1) + ((r >> 1) & 3);
+    const int word = 2 * (wk & 1) + (r & 1), shift = 8 * (r >> 3);
+    const auto multiply = [&](int h) {
+        const uint8_t* const stage = smem + (h % kI4Ring) * STAGE;
+        const meta_t* const t = table(h) + unit * kI4Step;
 #pragma unroll
-        for (int c = 0; c < C; ++c) x[c] = *(const vec*)(stage + (wm + 16 * c + r) * 256 + 16 * ((4 * s + q) ^ r));
-        uint32_t w[4][8];
+        for (int s = 0; s < 2; ++s) {
+            vec xv[C];
 #pragma unroll
-        for (int p = 0; p < 4; ++p) weights_of_pair<DT>(f.d[2 * p], f.d[2 * p + 1], m, p, w[p]);
+            for (int c = 0; c < C; ++c) {
+                const int row = wm + 16 * c + r;
+                xv[c] = *(const vec*)(stage + row * 128 + 16 * ((4 * s + q) ^ chunk_key(r)));
+            }
+            uint32_t d[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const vec b = __builtin_bit_cast(vec, u32x4_t{w[0][j], w[1][j], w[2][j], w[3][j]});
+            for (int i = 0; i < 8; ++i) {
+                const int row = 32 * s + 8 * q + i, slot = row ^ ((row >> 4) & 1);
+                d[i] = *(const uint32_t*)(stage + XB + slot * 128 + 16 * (chunk ^ (((row >> 3) & 1) << 2)) + 4 * word);
+            }
+            BackRows<DT> m;
+            m.scale = *(const decltype(m.scale)*)(t + 32 * s + 8 * q);
+            m.zero = *(const decltype(m.zero)*)(t + kI4Table + 32 * s + 8 * q);
+            uint32_t w[4][4];
 #pragma unroll
-            for (int c = 0; c < C; ++c) acc[c][j] = I4<DT>::mfma(x[c], b, acc[c][j]);
+            for (int p = 0; p < 4; ++p) {
+                const uint32_t even = perm_lo(d[2 * p], d[2 * p + 1]) >> shift, odd = perm_hi(d[2 * p], d[2 * p + 1]) >> shift;
+                w[0][p] = m.pair(and_or(even, 0x000F000Fu, 0x64006400u), p);
+                w[1][p] = m.pair(and_or(odd, 0x000F000Fu, 0x64006400u), p);
+                w[2][p] = m.pair(and_or(even >> 4, 0x000F000Fu, 0x64006400u), p);
+                w[3][p] = m.pair(and_or(odd >> 4, 0x000F000Fu, 0x64006400u), p);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const vec wv = __builtin_bit_cast(vec, u32x4_t{w[j][0], w[j][1], w[j][2], w[j][3]});
+#pragma unroll
+                for (int c = 0; c < C; ++c) acc[c][j] = I4<DT>::mfma(xv[c], wv, acc[c][j]);
+            }
         }
     };
-
-    Rows f[2];
+    const auto keep = [&](int h) {
+        BackRows<DT>::keep(table(h), threadIdx.x, raw[(h & 1) * kI4Table + threadIdx.x], a.scale_dtype);
+    };
     fetch_meta(0);
-    fetch_w(f[0], 0, 0);
-    fetch_x(0);
-    keep_meta(0);
     fetch_meta(1);
-    for (int t = 0; t < steps; ++t) {
-        wait_vmcnt<0>();
-        lds_barrier();  // stage t is whole, and every wave has read the one before it
-        keep_meta(t + 1);
-        fetch_w(f[1], t, 1);
-        fetch_x(t + 1);
-        fetch_meta(t + 2);
-        step(f[0], t, 0);
-        fetch_w(f[0], t, 2);
-        step(f[1], t, 1);
-        fetch_w(f[1], t, 3);
-        step(f[0], t, 2);
-        fetch_w(f[0], t + 1, 0);
-        step(f[1], t, 3);
+    fetch(0);
+    fetch(1);
+    wait_vmcnt<2 * I4Tokens<C>::LOADS + 2>();
+    keep(0);  // (a wave's own words)
+    for (int h = 0; h < steps; ++h) {
+        wait_vmcnt<I4Tokens<C>::LOADS + 1>();  // all but the next step's
+        lds_barrier();  // the stage is whole, and every wave has read the one before it
+        keep(h + 1);
+        fetch_meta(h + 2);
+        fetch(h + 2);
+        multiply(h);
     }
     wait_vmcnt<0>();
 
-    // lane: tokens wm + 16 c + 4 q + e, columns 32 (r & 3) + 8 (r >> 2) + 0 .. 7 of the wave's 128
-    const int k = k0 + wk + 32 * (r & 3) + 8 * (r >> 2), left = a.k - k;
+    // lane: tokens wm + 16 c + 4 q + e, four columns
+    const int k = k0 + 128 * (wk >> 1) + 32 * word + 8 * ((r >> 1) & 3) + 4 * (r >> 3), left = a.k - k;
     if (left <= 0) return;
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -582,24 +650,15 @@ __global__ __launch_bounds__(256, 2) void int4_back_kernel(const Int4Args a) {
         for (int e = 0; e < 4; ++e) {
             const int m = m0 + wm + 16 * c + 4 * q + e;
             if (m >= a.m) continue;
-            float8_t v;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = acc[c][j][e];
-            const int dt = a.splits > 1 ? DK_FP32 : a.y_dtype;
-            const int64_t at = a.splits > 1 ? split * a.slab + (int64_t)m * a.k + k : (int64_t)m * a.ldy + k;
-            void* const out = a.splits > 1 ? (void*)a.partials : a.y;
-            if (dt == DK_FP32) {
-                if (left >= 8) store8<DK_FP32>((float*)out + at, v);
-                else
-                    for (int j = 0; j < 8; ++j)
-                        if (j < left) ((float*)out)[at + j] = v[j];
+            const float4_t v = float4_t{acc[c][0][e], acc[c][1][e], acc[c][2][e], acc[c][3][e]};
+            if (a.splits > 1) {
+                Int4Args p = a;
+                p.y = a.partials;
+                put4<DK_FP32>(p, split * a.slab + (int64_t)m * a.k + k, v, left);
+            } else if (a.y_dtype == DK_FP32) {
+                put4<DK_FP32>(a, (int64_t)m * a.ldy + k, v, left);
             } else {
-                typedef typename Elem<DT>::type E;
-                if (left >= 8) store8<DT>((E*)out + at, v);
-                else
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (j < left) store1<DT>((E*)out + at + j, v[j]);
+                put4<DT>(a, (int64_t)m * a.ldy + k, v, left);
             }
         }
 }
@@ -666,18 +725,40 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
         p.n_tiles = (int)groups;
         return p;
     }
-    const int64_t steps = backward ? (n + kI4BackN - 1) / kI4BackN : blocks;
-    p.tokens = backward ? (m <= 32 ? 32 : m <= 64 ? 64 : 128) : kI4TileM;
-    p.m_tiles = (int)((m + p.tokens - 1) / p.tokens);
-    const int64_t cols = backward ? k : n;
-    p.n_tiles = (int)((cols + 255) / 256);
-    // splits of the sum until the tiles fill the CUs (the backward's work-groups run two a CU), at least four steps each
-    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles, fill = backward ? 512 : 256;
-    int64_t want = tiles >= fill * 3 / 4 ? 1 : fill / tiles;
-    if (want > steps / 4) want = steps / 4;
-    if (want < 1) want = 1;
-    p.steps_per_split = (int)((steps + want - 1) / want);
-    p.splits = (int)((steps + p.steps_per_split - 1) / p.steps_per_split);
+    // (Tuning hook, read on every call: DECIK_INT4_PLAN = "tokens,splits" forces a tile and the splits of the sum.)
+    // Tokens a tile: the largest of 256, 128, 64 (backward also 32) whose tiles take the fewest rounds of the CUs, a
+    // round's time taken as its tokens and the weight's unpacking.
+    const int64_t cols = backward ? k : n, steps = backward ? (n + kI4Block - 1) / kI4Block : blocks;
+    p.n_tiles = (int)((cols + kI4TileN - 1) / kI4TileN);
+    double best = 0.0;
+    int forced_tokens = 0, forced_splits = 0;
+    if (const char* v = std::getenv("DECIK_INT4_PLAN"))
+        if (std::sscanf(v, "%d,%d", &forced_tokens, &forced_splits) != 2 || forced_splits < 1 || forced_splits > steps)
+            forced_tokens = 0;
+    if (forced_tokens != 256 && forced_tokens != 128 && forced_tokens != 64 && !(backward && forced_tokens == 32))
+        forced_tokens = 0;
+    for (int tokens = 256; tokens >= (backward ? 32 : 64); tokens /= 2) {
+        if (forced_tokens != 0 && tokens != forced_tokens) continue;
+        const int64_t m_tiles = (m + tokens - 1) / tokens, tiles = m_tiles * p.n_tiles;
+        if (forced_tokens == 0 && tokens > 64 && m <= tokens / 2) continue;
+        // splits of the sum until the tiles fill the CUs, at least four blocks each
+        int64_t splits = tiles >= 192 ? 1 : 256 / tiles;
+        if (splits > steps / 4) splits = steps / 4;
+        if (splits < 1) splits = 1;
+        if (forced_tokens != 0) splits = forced_splits;
+        const int64_t per = (steps + splits - 1) / splits;
+        splits = (steps + per - 1) / per;
+        const int64_t rounds = (tiles * splits + 255) / 256;
+        const double cost = (double)rounds * per * (tokens + 64) * 256 +
+                            (splits > 1 ? (double)splits * m * cols / 16 : 0.0);
+        if (best == 0.0 || cost < best) {
+            best = cost;
+            p.tokens = tokens;
+            p.m_tiles = (int)m_tiles;
+            p.splits = (int)splits;
+            p.steps_per_split = (int)per;
+        }
+    }
     p.partial_bytes = p.splits > 1 ? (int64_t)p.splits * m * cols * 4 : 0;
     return p;
 }
@@ -695,6 +776,14 @@ static hipError_t launch_few(const Int4Args& a, const Int4Plan& p, hipStream_t s
     return hipGetLastError();
 }
 
+template <int DT, int C, int GJ>
+static hipError_t launch_tile(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
+    constexpr size_t lds = int4_tile_lds<C, GJ>();
+    if (hipError_t e = allow_dynamic_lds((const void*)int4_tile_kernel<DT, C, GJ>, lds)) return e;
+    hipLaunchKernelGGL((int4_tile_kernel<DT, C, GJ>), dim3(p.m_tiles * p.n_tiles * p.splits), dim3(64 * kI4Waves), lds, s, a);
+    return hipGetLastError();
+}
+
 template <int DT, int GJ>
 static hipError_t launch_forward(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
     if (p.few) {
@@ -702,17 +791,16 @@ static hipError_t launch_forward(const Int4Args& a, const Int4Plan& p, hipStream
         if (p.tokens == 32) return launch_few<DT, 2, GJ, 2>(a, p, s);
         return launch_few<DT, 4, GJ, 2>(a, p, s);
     }
-    constexpr size_t lds = kI4Waves * 64 * 72 * 2 > 2 * kI4StageBytes ? kI4Waves * 64 * 72 * 2 : 2 * kI4StageBytes;
-    if (hipError_t e = allow_dynamic_lds((const void*)int4_tile_kernel<DT, GJ>, lds)) return e;
-    hipLaunchKernelGGL((int4_tile_kernel<DT, GJ>), dim3(p.m_tiles * p.n_tiles * p.splits), dim3(64 * kI4Waves), lds, s, a);
-    return hipGetLastError();
+    if (p.tokens == 256) return launch_tile<DT, 8, GJ>(a, p, s);
+    if (p.tokens == 128) return launch_tile<DT, 4, GJ>(a, p, s);
+    return launch_tile<DT, 2, GJ>(a, p, s);
 }
 
 template <int DT, int C>
 static hipError_t launch_back(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
-    constexpr size_t lds = int4_back_lds<DT, C>();
+    constexpr size_t lds = kI4Ring * int4_back_stage<DT, C>() + 2 * kI4Table * sizeof(uint32_t);
     if (hipError_t e = allow_dynamic_lds((const void*)int4_back_kernel<DT, C>, lds)) return e;
-    hipLaunchKernelGGL((int4_back_kernel<DT, C>), dim3(p.m_tiles * p.n_tiles * p.splits), dim3(256), lds, s, a);
+    hipLaunchKernelGGL((int4_back_kernel<DT, C>), dim3(p.m_tiles * p.n_tiles * p.splits), dim3(64 * kI4Waves), lds, s, a);
     return hipGetLastError();
 }
 
@@ -721,7 +809,8 @@ static hipError_t launch_typed(const Int4Args& a, const Int4Plan& p, bool backwa
     if (backward) {
         if (p.tokens == 32) return launch_back<DT, 1>(a, p, s);
         if (p.tokens == 64) return launch_back<DT, 2>(a, p, s);
-        return launch_back<DT, 4>(a, p, s);
+        if (p.tokens == 128) return launch_back<DT, 4>(a, p, s);
+        return launch_back<DT, 8>(a, p, s);
     }
     if (a.group_units % 4 == 0) return launch_forward<DT, 4>(a, p, s);
     if (a.group_units % 2 == 0) return launch_forward<DT, 2>(a, p, s);
