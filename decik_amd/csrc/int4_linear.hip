@@ -45,7 +45,13 @@ struct I4<DK_BF16> {
     static __device__ __forceinline__ float scale(uint32_t meta) { return __builtin_bit_cast(float, meta << 16); }
 };
 
-__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) { return (v & mask) | bits; }
+// (v & mask) | bits in one instruction: it takes no literals and one scalar register, so the mask is held in one of those
+// and the bits in a vector register
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) {
+    asm("" : "+s"(mask));
+    asm("" : "+v"(bits));
+    return (v & mask) | bits;
+}
 
 __device__ __forceinline__ float zero_of(uint32_t meta) { return (float)((meta >> 16) & 0xFF); }
 
@@ -493,7 +499,9 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
 // unpack to pairs along the rows. Rows' scales and zero points go through tables of 64 rows by the tile's eight units
 // of 32 columns: their words come a step before the step's other loads, and the threads (an entry each) make the tables
 // of the next step.
-constexpr int kI4BackUnits = 8, kI4Table = kI4BackUnits * kI4Step;
+constexpr int kI4BackUnits = 8, kI4Entries = kI4BackUnits * kI4Step;
+// a unit's rows in a table: padded, so that the two units that a wave reads use different banks
+constexpr int kI4Unit = kI4Step + 32, kI4Table = kI4BackUnits * kI4Unit;
 
 template <int DT>
 struct BackRows;  // of the eight rows of a lane
@@ -572,7 +580,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     const auto fetch_meta = [&](int h) {
         const int n0 = n_begin + kI4Step * h, rows = h < steps ? min(kI4Step, n_end - n0) : 0;
         const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(rows * a.groups * 4));
-        bload32_lds(mr, raw + (h & 1) * kI4Table + 64 * wave, off_if(e_row < rows, (e_row * (uint32_t)a.groups + e_group) * 4));
+        bload32_lds(mr, raw + (h & 1) * kI4Entries + 64 * wave, off_if(e_row < rows, (e_row * (uint32_t)a.groups + e_group) * 4));
     };
     const auto table = [&](int h) { return (meta_t*)(smem + (h % kI4Ring) * STAGE + XB + kI4BackWBytes); };
 
@@ -587,7 +595,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     const int word = 2 * (wk & 1) + (r & 1), shift = 8 * (r >> 3);
     const auto multiply = [&](int h) {
         const uint8_t* const stage = smem + (h % kI4Ring) * STAGE;
-        const meta_t* const t = table(h) + unit * kI4Step;
+        const meta_t* const t = table(h) + unit * kI4Unit;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             vec xv[C];
@@ -623,7 +631,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
         }
     };
     const auto keep = [&](int h) {
-        BackRows<DT>::keep(table(h), threadIdx.x, raw[(h & 1) * kI4Table + threadIdx.x], a.scale_dtype);
+        BackRows<DT>::keep(table(h), kI4Unit * wave + lane, raw[(h & 1) * kI4Entries + threadIdx.x], a.scale_dtype);
     };
     fetch_meta(0);
     fetch_meta(1);
@@ -798,7 +806,7 @@ static hipError_t launch_forward(const Int4Args& a, const Int4Plan& p, hipStream
 
 template <int DT, int C>
 static hipError_t launch_back(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
-    constexpr size_t lds = kI4Ring * int4_back_stage<DT, C>() + 2 * kI4Table * sizeof(uint32_t);
+    constexpr size_t lds = kI4Ring * int4_back_stage<DT, C>() + 2 * kI4Entries * sizeof(uint32_t);
     if (hipError_t e = allow_dynamic_lds((const void*)int4_back_kernel<DT, C>, lds)) return e;
     hipLaunchKernelGGL((int4_back_kernel<DT, C>), dim3(p.m_tiles * p.n_tiles * p.splits), dim3(64 * kI4Waves), lds, s, a);
     return hipGetLastError();
