@@ -229,6 +229,12 @@ constexpr int kI4Waves = 8, kI4TileN = 256, kI4Step = 64, kI4Ring = 3;
 
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
+// An offset in a stage that every step adds its stage's to: held as it is, or each read's would be formed again.
+__device__ __forceinline__ uint32_t held(uint32_t v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 // 16-byte chunk of a row of 128 bytes: neighbouring rows share the banks' two halves, pairs of rows are permuted
 __device__ __forceinline__ int chunk_key(int row) { return (row >> 1) & 7; }
 
@@ -340,7 +346,7 @@ __device__ __forceinline__ void put4(const Int4Args& a, int64_t at, float4_t v, 
 constexpr int kI4WBytes = kI4TileN * 64;
 template <int C, int GJ>
 constexpr size_t int4_tile_lds() {
-    constexpr size_t ring = kI4Ring * I4Tokens<C>::BYTES + 2 * (kI4WBytes + 4 / GJ * kI4TileN * 4);
+    constexpr size_t ring = kI4Ring * (I4Tokens<C>::BYTES + kI4WBytes + 4 / GJ * kI4TileN * 4);
     constexpr size_t out = kI4Waves * (C < 4 ? 16 * C : 64) * 72 * 2;
     return ring > out ? ring : out;
 }
@@ -367,7 +373,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
     uint8_t* const weights = smem + kI4Ring * XB;
     const auto fetch_x = [&](int h) { x.fetch(smem + (h % kI4Ring) * XB, a, b0 * kI4Block + kI4Step * h, h < 2 * blocks); };
     const auto fetch_w = [&](int b) {
-        uint8_t* const stage = weights + (b & 1) * WB;
+        uint8_t* const stage = weights + (b % kI4Ring) * WB;
         const bool live = b < blocks;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {  // 16 rows of 64 bytes a load
@@ -390,47 +396,77 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[i][c] = float4_t{};
 
-    const auto multiply = [&](int h, int j0, const u32x4_t (&w)[R], const I4Group<DT> (&g)[R][UNITS]) {
-        const uint8_t* const stage = smem + (h % kI4Ring) * XB;
+    // A step is four parts: each 32 terms by half of the tokens. Operands of a part are read in the one before, across
+    // the steps too: the wait and the barrier of a step come before its last part, when all of it has been read.
+    constexpr int H = C / 2;
+    vec xv[2][H], wv[2][R];
+    u32x4_t raw[R];
+    I4Group<DT> group[R];
+    const uint32_t x_off[2] = {held((wm + r) * 128 + 16 * (q ^ chunk_key(r))), held((wm + r) * 128 + 16 * ((4 + q) ^ chunk_key(r)))};
+    const uint32_t w_off = held(kI4Ring * XB + (wn + r) * 64 + 16 * q);
+    const uint32_t g_off = held(kI4Ring * XB + kI4WBytes + 4 * (wn + r));
+    // xs, ws: where the step's tokens and the block's weights are
+    const auto read_x = [&](uint32_t xs, int part) {
+        const uint8_t* const at = smem + (x_off[part >> 1] + xs);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            vec xv[C];
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int row = wm + 16 * c + r;
-                xv[c] = *(const vec*)(stage + row * 128 + 16 * ((4 * j + q) ^ chunk_key(r)));
-            }
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const vec wv = g[i][(j0 + j) / GJ].weights(w[i][j0 + j]);
-#pragma unroll
-                for (int c = 0; c < C; ++c) acc[i][c] = I4<DT>::mfma(xv[c], wv, acc[i][c]);
-            }
-        }
+        for (int c = 0; c < H; ++c) xv[part & 1][c] = *(const vec*)(at + (H * (part & 1) + c) * 2048);
     };
-    fetch_x(0);
-    fetch_w(0);
-    fetch_x(1);
-    for (int b = 0; b < blocks; ++b) {
-        wait_vmcnt<I4Tokens<C>::LOADS>();  // all but the next step's
-        lds_barrier();                     // the stages are whole, and every wave has read those before them
-        fetch_x(2 * b + 2);
-        fetch_w(b + 1);
-        u32x4_t w[R];
-        I4Group<DT> g[R][UNITS];
-        const uint8_t* const stage = weights + (b & 1) * WB;
+    const auto read_raw = [&](uint32_t ws) {
+        const uint8_t* const at = smem + (w_off + ws);
+#pragma unroll
+        for (int i = 0; i < R; ++i) raw[i] = *(const u32x4_t*)(at + 1024 * i);
+    };
+    // operands of slice j (32 columns) of a block
+    const auto unpack = [&](uint32_t ws, int j) {
+        const uint8_t* const at = smem + (g_off + ws);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            w[i] = *(const u32x4_t*)(stage + (wn + 16 * i + r) * 64 + 16 * q);
-#pragma unroll
-            for (int u = 0; u < UNITS; ++u)
-                g[i][u].set(*(const uint32_t*)(stage + kI4WBytes + 4 * (kI4TileN * u + wn + 16 * i + r)), a.scale_dtype);
+            if (j % GJ == 0) group[i].set(*(const uint32_t*)(at + 4 * (kI4TileN * (j / GJ) + 16 * i)), a.scale_dtype);
+            wv[j & 1][i] = group[i].weights(raw[i][j]);
         }
-        multiply(2 * b, 0, w, g);
-        wait_vmcnt<I4Tokens<C>::LOADS + WLOADS>();
-        lds_barrier();
-        fetch_x(2 * b + 3);
-        multiply(2 * b + 1, 2, w, g);
+    };
+    const auto multiply = [&](int v) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int c = 0; c < H; ++c) {
+                float4_t& s = acc[i][H * (v & 1) + c];
+                s = I4<DT>::mfma(xv[v & 1][c], wv[(v >> 1) & 1][i], s);
+            }
+    };
+    constexpr int GROUP = I4Tokens<C>::LOADS + WLOADS;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        fetch_x(i);
+        fetch_w(i);
+    }
+    wait_vmcnt<2 * GROUP>();
+    lds_barrier();
+    uint32_t xs = 0, ws = 0, next_ws = 0;
+    read_raw(0);
+    read_x(0, 0);
+    unpack(0, 0);
+    for (int b = 0; b < blocks; ++b) {
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {  // parts of two steps
+            if ((v & 3) == 3) {
+                wait_vmcnt<GROUP>();  // all but the newest step's and the newest block's
+                lds_barrier();
+                fetch_x(2 * b + (v >> 2) + 3);
+                if (v == 7) fetch_w(b + 3);
+                xs = xs == 2 * XB ? 0 : xs + XB;
+                read_x(xs, 0);
+            } else {
+                read_x(xs, (v & 3) + 1);
+            }
+            multiply(v);
+            if (v == 7) ws = next_ws;
+            if (v & 1) unpack(ws, ((v >> 1) + 1) & 3);
+            if (v == 5) {  // (the next block is there since the step before)
+                next_ws = ws == 2 * WB ? 0 : ws + WB;
+                read_raw(next_ws);
+            }
+        }
     }
     wait_vmcnt<0>();
     lds_barrier();
@@ -495,8 +531,8 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
 
 // ---- backward ------------------------------------------------------------------------------------
 // The weight's layout is the forward's. Lanes r and r + 8 of an MFMA operand hold columns j and j + 4 of the
-// same word (j = 0 .. 3: four MFMAs), each of its eight rows' words; halves of two rows' words joined in one register
-// unpack to pairs along the rows. Rows' scales and zero points go through tables of 64 rows by the tile's eight units
+// same word (j = 0 .. 3: four MFMAs), each of its eight rows' words; the bytes with those columns of two rows' words, joined in
+// one register, unpack to pairs along the rows. Rows' scales and zero points go through tables of 64 rows by the tile's eight units
 // of 32 columns: their words come a step before the step's other loads, and the threads (an entry each) make the tables
 // of the next step.
 constexpr int kI4BackUnits = 8, kI4Entries = kI4BackUnits * kI4Step;
@@ -548,7 +584,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     typedef typename BackRows<DT>::elem meta_t;
     constexpr int XB = I4Tokens<C>::BYTES, STAGE = int4_back_stage<DT, C>();
     extern __shared__ __attribute__((aligned(32))) uint8_t smem[];
-    uint32_t* const raw = (uint32_t*)(smem + kI4Ring * STAGE);  // two steps' words of the groups
+    uint32_t* const raw = (uint32_t*)(smem + kI4Ring * STAGE);  // four steps' words of the groups
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
     int mt, kt, split;
@@ -580,7 +616,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     const auto fetch_meta = [&](int h) {
         const int n0 = n_begin + kI4Step * h, rows = h < steps ? min(kI4Step, n_end - n0) : 0;
         const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(rows * a.groups * 4));
-        bload32_lds(mr, raw + (h & 1) * kI4Entries + 64 * wave, off_if(e_row < rows, (e_row * (uint32_t)a.groups + e_group) * 4));
+        bload32_lds(mr, raw + (h & 3) * kI4Entries + 64 * wave, off_if(e_row < rows, (e_row * (uint32_t)a.groups + e_group) * 4));
     };
     const auto table = [&](int h) { return (meta_t*)(smem + (h % kI4Ring) * STAGE + XB + kI4BackWBytes); };
 
@@ -592,60 +628,96 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
 
     // this lane's word of a row: word 4 q' + j' of its block with j' = 2 (wk & 1) + (r & 1), q' = (r >> 1) & 3
     const int unit = 4 * (wk >> 1) + 2 * (wk & 1) + (r & 1), chunk = 4 * (wk >> 1) + ((r >> 1) & 3);
-    const int word = 2 * (wk & 1) + (r & 1), shift = 8 * (r >> 3);
-    const auto multiply = [&](int h) {
-        const uint8_t* const stage = smem + (h % kI4Ring) * STAGE;
-        const meta_t* const t = table(h) + unit * kI4Unit;
+    const int word = 2 * (wk & 1) + (r & 1);
+    // its bytes: of each half of two rows' words, the one that holds its four columns
+    const uint32_t pick = r < 8 ? 0x06040200u : 0x07050301u;
+    // the parts of a step as in the forward
+    constexpr int H = C < 2 ? 1 : C / 2, PARTS = C < 2 ? 2 : 4;  // 32 tokens: a part is 32 terms of all tokens
+    vec xv[2][H], wv[2][4];
+    uint32_t d[8];
+    BackRows<DT> rows;
+    const uint32_t x_off[2] = {held((wm + r) * 128 + 16 * (q ^ chunk_key(r))), held((wm + r) * 128 + 16 * ((4 + q) ^ chunk_key(r)))};
+    // (row 8 q + i lies at 8 q + i ^ bit 4 of it, which is bit 1 of q)
+    const uint32_t w_off = XB + 8 * q * 128 + 16 * (chunk ^ ((q & 1) << 2)) + 4 * word, swap = 128 * ((q >> 1) & 1);
+    const uint32_t w_even = held(w_off + swap), w_odd = held(w_off - swap);
+    const uint32_t t_off = held(XB + kI4BackWBytes + (unit * kI4Unit + 8 * q) * (uint32_t)sizeof(meta_t));
+    // at: where the step's stage is
+    const auto read_x = [&](uint32_t at, int part) {
+        const int s = part / (PARTS / 2), half = PARTS == 4 ? part & 1 : 0;
+        const uint8_t* const p = smem + (x_off[s] + at);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            vec xv[C];
+        for (int c = 0; c < H; ++c) xv[part & 1][c] = *(const vec*)(p + (H * half + c) * 2048);
+    };
+    const auto read_w = [&](uint32_t at, int s) {
+        const uint8_t *const even = smem + (w_even + at) + 4096 * s, *const odd = smem + (w_odd + at) + 4096 * s;
+        const uint8_t* const t = smem + (t_off + at) + 32 * s * sizeof(meta_t);
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int row = wm + 16 * c + r;
-                xv[c] = *(const vec*)(stage + row * 128 + 16 * ((4 * s + q) ^ chunk_key(r)));
-            }
-            uint32_t d[8];
+        for (int i = 0; i < 8; ++i) d[i] = *(const uint32_t*)((i & 1 ? odd : even) + 128 * i);
+        rows.scale = *(const decltype(rows.scale)*)t;
+        rows.zero = *(const decltype(rows.zero)*)(t + kI4Table * sizeof(meta_t));
+    };
+    const auto unpack = [&](int s) {
+        uint32_t w[4][4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = 32 * s + 8 * q + i, slot = row ^ ((row >> 4) & 1);
-                d[i] = *(const uint32_t*)(stage + XB + slot * 128 + 16 * (chunk ^ (((row >> 3) & 1) << 2)) + 4 * word);
-            }
-            BackRows<DT> m;
-            m.scale = *(const decltype(m.scale)*)(t + 32 * s + 8 * q);
-            m.zero = *(const decltype(m.zero)*)(t + kI4Table + 32 * s + 8 * q);
-            uint32_t w[4][4];
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const uint32_t even = perm_lo(d[2 * p], d[2 * p + 1]) >> shift, odd = perm_hi(d[2 * p], d[2 * p + 1]) >> shift;
-                w[0][p] = m.pair(and_or(even, 0x000F000Fu, 0x64006400u), p);
-                w[1][p] = m.pair(and_or(odd, 0x000F000Fu, 0x64006400u), p);
-                w[2][p] = m.pair(and_or(even >> 4, 0x000F000Fu, 0x64006400u), p);
-                w[3][p] = m.pair(and_or(odd >> 4, 0x000F000Fu, 0x64006400u), p);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const vec wv = __builtin_bit_cast(vec, u32x4_t{w[j][0], w[j][1], w[j][2], w[j][3]});
-#pragma unroll
-                for (int c = 0; c < C; ++c) acc[c][j] = I4<DT>::mfma(xv[c], wv, acc[c][j]);
-            }
+        for (int p = 0; p < 4; ++p) {
+            // nibbles of row 2 p: columns 0 2 1 3, then of row 2 p + 1
+            const uint32_t v = __builtin_amdgcn_perm(d[2 * p + 1], d[2 * p], pick);
+            w[0][p] = rows.pair(and_or(v, 0x000F000Fu, 0x64006400u), p);
+            w[1][p] = rows.pair(and_or(v >> 8, 0x000F000Fu, 0x64006400u), p);
+            w[2][p] = rows.pair(and_or(v >> 4, 0x000F000Fu, 0x64006400u), p);
+            w[3][p] = rows.pair(and_or(v >> 12, 0x000F000Fu, 0x64006400u), p);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wv[s][j] = __builtin_bit_cast(vec, u32x4_t{w[j][0], w[j][1], w[j][2], w[j][3]});
     };
-    const auto keep = [&](int h) {
-        BackRows<DT>::keep(table(h), kI4Unit * wave + lane, raw[(h & 1) * kI4Entries + threadIdx.x], a.scale_dtype);
+    const auto multiply = [&](int part) {
+        const int s = part / (PARTS / 2), half = PARTS == 4 ? part & 1 : 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < H; ++c) {
+                float4_t& t = acc[H * half + c][j];
+                t = I4<DT>::mfma(xv[part & 1][c], wv[s][j], t);
+            }
     };
+    const auto keep = [&](int h) {  // (a wave's own words)
+        BackRows<DT>::keep(table(h), kI4Unit * wave + lane, raw[(h & 3) * kI4Entries + threadIdx.x], a.scale_dtype);
+    };
+    constexpr int GROUP = I4Tokens<C>::LOADS + 2;
     fetch_meta(0);
     fetch_meta(1);
-    fetch(0);
-    fetch(1);
-    wait_vmcnt<2 * I4Tokens<C>::LOADS + 2>();
-    keep(0);  // (a wave's own words)
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        fetch_meta(i + 2 < 4 ? i + 2 : 3);
+        fetch(i);
+    }
+    wait_vmcnt<2 * GROUP>();
+    keep(0);
+    keep(1);
+    lds_barrier();
+    uint32_t at = 0;
+    read_x(0, 0);
+    read_w(0, 0);
+    unpack(0);
     for (int h = 0; h < steps; ++h) {
-        wait_vmcnt<I4Tokens<C>::LOADS + 1>();  // all but the next step's
-        lds_barrier();  // the stage is whole, and every wave has read the one before it
-        keep(h + 1);
-        fetch_meta(h + 2);
-        fetch(h + 2);
-        multiply(h);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+            const bool last = part == PARTS - 1, turns = part % (PARTS / 2) == PARTS / 2 - 1;  // the slice's last part
+            if (last) {
+                wait_vmcnt<GROUP>();  // all but the newest step's
+                lds_barrier();
+                keep(h + 2);
+                fetch_meta(h + 4);
+                fetch(h + 3);
+                at = at == 2 * STAGE ? 0 : at + STAGE;
+                read_x(at, 0);
+            } else {
+                read_x(at, part + 1);
+            }
+            if (turns) read_w(at, last ? 0 : 1);
+            multiply(part);
+            if (turns) unpack(last ? 0 : 1);
+        }
     }
     wait_vmcnt<0>();
 
@@ -806,7 +878,7 @@ static hipError_t launch_forward(const Int4Args& a, const Int4Plan& p, hipStream
 
 template <int DT, int C>
 static hipError_t launch_back(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
-    constexpr size_t lds = kI4Ring * int4_back_stage<DT, C>() + 2 * kI4Entries * sizeof(uint32_t);
+    constexpr size_t lds = kI4Ring * int4_back_stage<DT, C>() + 4 * kI4Entries * sizeof(uint32_t);
     if (hipError_t e = allow_dynamic_lds((const void*)int4_back_kernel<DT, C>, lds)) return e;
     hipLaunchKernelGGL((int4_back_kernel<DT, C>), dim3(p.m_tiles * p.n_tiles * p.splits), dim3(64 * kI4Waves), lds, s, a);
     return hipGetLastError();
