@@ -136,7 +136,7 @@ EXPORTS = {
     "dk_qk_rope_bwd_workspace": ([c_vp], c_i64),
     "dk_qk_rope_bwd": ([c_vp, c_vp, c_i64, c_vp], c_i32),
     "dk_int4_linear_workspace": ([c_i32, c_i32, c_i64, c_i64, c_i64], c_i64),
-    "dk_int4_linear": ([c_i32, c_vp, c_i32, c_i64, c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_i32, c_vp, c_i32, c_i64, c_i64,
+    "dk_int4_linear": ([c_i32, c_vp, c_i32, c_i64, c_vp, c_vp, c_i64, c_i32, c_vp, c_i32, c_vp, c_i32, c_i64, c_i64,
                         c_i64, c_i64, c_i32, c_vp, c_i64, c_vp], c_i32),
     "dk_int4_linear_plan": ([c_i32, c_i64, c_i64, c_i64, ctypes.POINTER(c_i32)], c_i32),
     # packed bytes as well (ScaledRope.PACK, ResidualNorm.PACK)

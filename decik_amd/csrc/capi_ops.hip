@@ -563,8 +563,8 @@ int dk_int4_linear_plan(int backward, int64_t m, int64_t n, int64_t k, int32_t* 
     return 0;
 }
 
-int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, int64_t ldw,
-                   const uint32_t* meta, int64_t group, int scale_dtype, const void* bias, int bias_dtype, void* y,
+int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, const uint32_t* meta,
+                   int64_t group, int scale_dtype, const void* bias, int bias_dtype, void* y,
                    int y_dtype, int64_t ldy, int64_t m, int64_t n, int64_t k, int copy, void* workspace,
                    int64_t workspace_bytes, void* stream) {
     dk_clear_error();
@@ -582,9 +582,8 @@ int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const 
     if (m > 1 && ldy < cols) return dk_fail("dk_int4_linear: output rows overlap");
     if (n == 0) return dk_fail("dk_int4_linear: the sum has no terms");
     if (x == nullptr || packed == nullptr || meta == nullptr) return dk_fail("dk_int4_linear: null pointer");
-    if (!aligned_to(packed, 16) || ldw % 64 != 0 || ldw < (k + 127) / 128 * 64 || ldw > (int64_t(1) << 20) ||
-        !aligned_to(meta, 4))
-        return dk_fail("dk_int4_linear: packed must be 16-byte aligned, its row stride a multiple of 64 that holds k");
+    if (!aligned_to(packed, 16) || !aligned_to(meta, 4))
+        return dk_fail("dk_int4_linear: packed must be 16-byte aligned, meta 4-byte aligned");
     if (m > 1 && (ldx < 0 || ldx >= (int64_t(1) << 23)))
         return dk_fail("dk_int4_linear: x's row stride must be non-negative and below 2^23");
     if (!copy && (sum % 8 != 0 || !aligned_to(x, 16) || (m > 1 && ldx % 8 != 0)))
@@ -602,7 +601,6 @@ int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const 
     a.partials = static_cast<float*>(workspace);
     a.padded = copy ? reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + partial) : nullptr;
     a.ldx = m > 1 ? ldx : 0;
-    a.ldw = ldw;
     a.ldy = ldy;
     a.m = (int32_t)m;
     a.n = (int32_t)n;

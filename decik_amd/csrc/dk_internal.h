@@ -356,14 +356,14 @@ hipError_t launch_scaled_rope(ScaledRopeArgs a, int dtype, hipStream_t s);
 constexpr int kInt4FewM = 64;  // forward launches of so few tokens stream the weight to registers
 struct Int4Args {
     const void* x;       // [m, k], backward dy [m, n]: 16-byte aligned rows, or `padded` set
-    const uint8_t* w;    // [n, ldw], blocks of 128 columns
-    const uint32_t* meta;  // [n, groups]: scale, zero point
+    const uint8_t* w;      // tiles of 16 rows by 128 columns [ceil(n / 16), kblocks, 1024]
+    const uint32_t* meta;  // scale, zero point [ceil(n / 16), groups, 16]
     const void* bias;
     void* y;
     float* partials;     // splits > 1
     uint16_t* padded;    // room for x with aligned rows, or null
-    int64_t ldx, ldw, ldy, slab;
-    int32_t m, n, k, kpad, x_cols, groups, group_units, scale_dtype, bias_dtype, y_dtype;
+    int64_t ldx, ldy, slab;
+    int32_t m, n, k, kblocks, x_cols, groups, group_units, scale_dtype, bias_dtype, y_dtype;
     uint32_t group_mul;
     int32_t blocks, blocks_per_split, splits, m_tiles, n_tiles;
 };

@@ -7,10 +7,12 @@
 // backward sums over rows, each with its own scale, so there W is rounded once to 16 bits, as the matrix cores take it (at
 // most half a step of the type a weight, of alternating sign along a sum).
 //
-// Layout of a row: blocks of 128 columns in 64 bytes, so that a lane's 16 bytes are its operands of four MFMAs as they lie:
-// dword 4 q + j of a block holds columns 32 j + 8 q + 0 .. 7, column 2 i of those in bits 4 i, column 2 i + 1 in bits
-// 16 + 4 i (a shift and a mask leave a pair in the halves of a register). In each MFMA lane l = 16 q + r holds k
-// = 8 q + 0 .. 7 of row r of its operand. `meta` holds a group's scale (low 16 bits) and zero point (next byte).
+// Layout: tiles of 16 rows by 128 columns in 1024 bytes, a row of tiles after the other, so that a wave's load is one
+// piece of memory and a lane's 16 bytes are its operands of four MFMAs as they lie: the 16 bytes 16 q + r hold row r,
+// their dword j columns 32 j + 8 q + 0 .. 7, column 2 i of those in bits 4 i, column 2 i + 1 in bits 16 + 4 i (a
+// shift and a mask leave a pair in the halves of a register). In each MFMA lane l = 16 q + r holds k = 8 q + 0 .. 7 of
+// row r of its operand. `meta` holds groups' words, a scale (low 16 bits) and a zero point (next byte), by tile rows, groups
+// and the tile's 16 rows.
 // From pairs to operands, fp16: 0x6400 | q is 1024 + q, 0x6400 | 16 q is 1024 + 16 q, and one packed subtraction or
 // multiply-add leaves q - zero, exactly. bf16: 0x4180 | 8 q is 16 + q; there is no packed bf16 arithmetic, so 16 + zero
 // times the sum of x, from one more MFMA, is taken off the group's sum.
@@ -22,7 +24,7 @@
 
 namespace dk {
 
-constexpr int kI4Block = 128;  // columns of a block
+constexpr int kI4Block = 128, kI4Tile = 1024;  // columns of a tile, its bytes
 
 template <int DT>
 struct I4;
@@ -120,13 +122,13 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
     const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * C;
-    const int rows = min(16, a.n - n0), toks = min(16 * C, a.m - m0);
+    const int toks = min(16 * C, a.m - m0);
     const int per = (a.blocks + NW - 1) / NW, b0 = wave * per, b1 = min(a.blocks, b0 + per);
 
-    const rsrc_t wr = make_rsrc(a.w + (int64_t)n0 * a.ldw, (uint32_t)(rows * a.ldw));
-    const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(rows * a.groups * 4));
+    const rsrc_t wr = make_rsrc(a.w + (int64_t)blockIdx.x * a.kblocks * kI4Tile, (uint32_t)(a.kblocks * kI4Tile));
+    const rsrc_t mr = make_rsrc(a.meta + (int64_t)blockIdx.x * a.groups * 16, (uint32_t)(a.groups * 64));
     const rsrc_t xr = make_rsrc((const uint16_t*)a.x + (int64_t)m0 * a.ldx, (uint32_t)(((toks - 1) * a.ldx + a.x_cols) * 2));
-    const uint32_t w_at = r * (uint32_t)a.ldw + 16 * q, m_at = r * (uint32_t)a.groups * 4;
+    const uint32_t w_at = 16 * lane, m_at = 4 * r;
     uint32_t x_at[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) x_at[c] = off_if(16 * c + r < toks, (16 * c + r) * (uint32_t)a.ldx * 2 + 16 * q);
@@ -139,13 +141,13 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
     Stage st[P];
     const auto fetch = [&](Stage& s, int b) {
         const bool live = b < b1;
-        s.w = bload128(wr, off_if(live, w_at + 64 * (uint32_t)b));
+        s.w = bload128(wr, off_if(live, w_at + kI4Tile * (uint32_t)b));
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             const uint32_t unit = 4 * b + GJ * u;
             // (a last block's units past k have no group: they read the last one's, for x of zeros)
             const uint32_t g = min(group_at(a, unit), (uint32_t)a.groups - 1);
-            s.meta[u] = __builtin_amdgcn_raw_buffer_load_b32(mr, (int)off_if(live, m_at + 4 * g), 0, 0);
+            s.meta[u] = __builtin_amdgcn_raw_buffer_load_b32(mr, (int)off_if(live, m_at + 64 * g), 0, 0);
         }
 #pragma unroll
         for (int c = 0; c < C; ++c)
@@ -252,10 +254,10 @@ __device__ __forceinline__ void tile_of(const Int4Args& a, int& m_tile, int& n_t
     n_tile = in / rows;
 }
 
-// The activations' part of a stage: rows of 64 terms (128 bytes), at least 64 rows; a wave's loads of a step.
+// The activations' part of a stage: rows of 64 terms (128 bytes), and a wave's loads of a step.
 template <int C>
 struct I4Tokens {
-    static constexpr int TM = 32 * C, BYTES = (TM < 64 ? 64 : TM) * 128, LOADS = BYTES / 1024 / kI4Waves;
+    static constexpr int TM = 32 * C, BYTES = TM * 128, LOADS = BYTES / 1024 / kI4Waves;
     rsrc_t src;
     uint32_t at[LOADS];
     int col[LOADS];
@@ -367,26 +369,24 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
 
     I4Tokens<C> x;
     x.set(a, m0, wave, lane);
-    const int rows = min(kI4TileN, a.n - n0);
-    const rsrc_t wr = make_rsrc(a.w + (int64_t)n0 * a.ldw, (uint32_t)(rows * a.ldw));
-    const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(rows * a.groups * 4));
+    const int tiles = (min(kI4TileN, a.n - n0) + 15) / 16;
+    const rsrc_t wr = make_rsrc(a.w + (int64_t)(n0 / 16) * a.kblocks * kI4Tile, (uint32_t)(tiles * a.kblocks * kI4Tile));
+    const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(tiles * a.groups * 64));
     uint8_t* const weights = smem + kI4Ring * XB;
     const auto fetch_x = [&](int h) { x.fetch(smem + (h % kI4Ring) * XB, a, b0 * kI4Block + kI4Step * h, h < 2 * blocks); };
     const auto fetch_w = [&](int b) {
         uint8_t* const stage = weights + (b % kI4Ring) * WB;
         const bool live = b < blocks;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {  // 16 rows of 64 bytes a load
-            const uint32_t row = 16 * (2 * wave + i) + (lane >> 2);
-            bload128_lds(wr, stage + 1024 * (2 * wave + i),
-                         off_if(live, row * (uint32_t)a.ldw + 64 * (uint32_t)(b0 + b) + 16 * (lane & 3)));
-        }
+        for (int i = 0; i < 2; ++i)  // a tile a load
+            bload128_lds(wr, stage + kI4Tile * (2 * wave + i),
+                         off_if(live, kI4Tile * ((2 * wave + i) * (uint32_t)a.kblocks + (uint32_t)(b0 + b)) + 16 * lane));
 #pragma unroll
         for (int i = 0; i < METAS; ++i) {  // 64 rows of one unit a load; with one unit waves 4 to 7 repeat 0 to 3's
             const int load = UNITS == 1 ? wave & 3 : METAS * wave + i, u = load >> 2;
-            const uint32_t row = 64 * (load & 3) + lane;
+            const uint32_t tile = 4 * (load & 3) + q;
             const uint32_t g = min(group_at(a, 4 * (b0 + b) + GJ * u), (uint32_t)a.groups - 1);
-            bload32_lds(mr, stage + kI4WBytes + 256 * load, off_if(live, (row * (uint32_t)a.groups + g) * 4));
+            bload32_lds(mr, stage + kI4WBytes + 256 * load, off_if(live, 64 * (tile * (uint32_t)a.groups + g) + 4 * r));
         }
     };
 
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
     u32x4_t raw[R];
     I4Group<DT> group[R];
     const uint32_t x_off[2] = {held((wm + r) * 128 + 16 * (q ^ chunk_key(r))), held((wm + r) * 128 + 16 * ((4 + q) ^ chunk_key(r)))};
-    const uint32_t w_off = held(kI4Ring * XB + (wn + r) * 64 + 16 * q);
+    const uint32_t w_off = held(kI4Ring * XB + wn * 64 + 16 * lane);
     const uint32_t g_off = held(kI4Ring * XB + kI4WBytes + 4 * (wn + r));
     // xs, ws: where the step's tokens and the block's weights are
     const auto read_x = [&](uint32_t xs, int part) {
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
     const auto read_raw = [&](uint32_t ws) {
         const uint8_t* const at = smem + (w_off + ws);
 #pragma unroll
-        for (int i = 0; i < R; ++i) raw[i] = *(const u32x4_t*)(at + 1024 * i);
+        for (int i = 0; i < R; ++i) raw[i] = *(const u32x4_t*)(at + kI4Tile * i);
     };
     // operands of slice j (32 columns) of a block
     const auto unpack = [&](uint32_t ws, int j) {
@@ -600,23 +600,23 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     // banks: chunks swap halves of the row by bit 3 of the row, rows swap places in their pair by bit 4.
     const int w_slot = 8 * wave + (lane >> 3), w_row = w_slot ^ ((w_slot >> 4) & 1);
     const int w_chunk = (lane & 7) ^ (((w_row >> 3) & 1) << 2);
-    const uint32_t w_col = (uint32_t)k0 / 2 + 16 * w_chunk;
-    const bool w_live = w_col < (uint32_t)a.ldw;
-    const int e_row = threadIdx.x & 63;
+    const uint32_t w_block = k0 / kI4Block + (w_chunk >> 2);
+    const bool w_live = w_block < (uint32_t)a.kblocks;
+    const uint32_t w_at = kI4Tile * ((w_row >> 4) * (uint32_t)a.kblocks + w_block) + 16 * (16 * (w_chunk & 3) + (w_row & 15));
     const uint32_t e_group = min(group_at(a, k0 / 32 + (threadIdx.x >> 6)), (uint32_t)a.groups - 1);
     const auto fetch = [&](int h) {
         const int n0 = n_begin + kI4Step * h;
         const bool live = h < steps;
         uint8_t* const stage = smem + (h % kI4Ring) * STAGE;
         x.fetch(stage, a, n0, live);
-        const int rows = live ? min(kI4Step, n_end - n0) : 0;
-        const rsrc_t wr = make_rsrc(a.w + (int64_t)n0 * a.ldw, (uint32_t)(rows * a.ldw));
-        bload128_lds(wr, stage + XB + 1024 * wave, off_if(w_live && w_row < rows, w_row * (uint32_t)a.ldw + w_col));
+        const int tiles = live ? (min(kI4Step, n_end - n0) + 15) / 16 : 0;
+        const rsrc_t wr = make_rsrc(a.w + (int64_t)(n0 / 16) * a.kblocks * kI4Tile, (uint32_t)(tiles * a.kblocks * kI4Tile));
+        bload128_lds(wr, stage + XB + 1024 * wave, off_if(w_live, w_at));
     };
     const auto fetch_meta = [&](int h) {
-        const int n0 = n_begin + kI4Step * h, rows = h < steps ? min(kI4Step, n_end - n0) : 0;
-        const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(rows * a.groups * 4));
-        bload32_lds(mr, raw + (h & 3) * kI4Entries + 64 * wave, off_if(e_row < rows, (e_row * (uint32_t)a.groups + e_group) * 4));
+        const int n0 = n_begin + kI4Step * h, tiles = h < steps ? (min(kI4Step, n_end - n0) + 15) / 16 : 0;
+        const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(tiles * a.groups * 64));
+        bload32_lds(mr, raw + (h & 3) * kI4Entries + 64 * wave, 64 * (q * (uint32_t)a.groups + e_group) + 4 * r);
     };
     const auto table = [&](int h) { return (meta_t*)(smem + (h % kI4Ring) * STAGE + XB + kI4BackWBytes); };
 
@@ -632,7 +632,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     // its bytes: of each half of two rows' words, the one that holds its four columns
     const uint32_t pick = r < 8 ? 0x06040200u : 0x07050301u;
     // the parts of a step as in the forward
-    constexpr int H = C < 2 ? 1 : C / 2, PARTS = C < 2 ? 2 : 4;  // 32 tokens: a part is 32 terms of all tokens
+    constexpr int H = C / 2;
     vec xv[2][H], wv[2][4];
     uint32_t d[8];
     BackRows<DT> rows;
@@ -643,10 +643,9 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     const uint32_t t_off = held(XB + kI4BackWBytes + (unit * kI4Unit + 8 * q) * (uint32_t)sizeof(meta_t));
     // at: where the step's stage is
     const auto read_x = [&](uint32_t at, int part) {
-        const int s = part / (PARTS / 2), half = PARTS == 4 ? part & 1 : 0;
-        const uint8_t* const p = smem + (x_off[s] + at);
+        const uint8_t* const p = smem + (x_off[part >> 1] + at);
 #pragma unroll
-        for (int c = 0; c < H; ++c) xv[part & 1][c] = *(const vec*)(p + (H * half + c) * 2048);
+        for (int c = 0; c < H; ++c) xv[part & 1][c] = *(const vec*)(p + (H * (part & 1) + c) * 2048);
     };
     const auto read_w = [&](uint32_t at, int s) {
         const uint8_t *const even = smem + (w_even + at) + 4096 * s, *const odd = smem + (w_odd + at) + 4096 * s;
@@ -671,13 +670,12 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
         for (int j = 0; j < 4; ++j) wv[s][j] = __builtin_bit_cast(vec, u32x4_t{w[j][0], w[j][1], w[j][2], w[j][3]});
     };
     const auto multiply = [&](int part) {
-        const int s = part / (PARTS / 2), half = PARTS == 4 ? part & 1 : 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int c = 0; c < H; ++c) {
-                float4_t& t = acc[H * half + c][j];
-                t = I4<DT>::mfma(xv[part & 1][c], wv[s][j], t);
+                float4_t& t = acc[H * (part & 1) + c][j];
+                t = I4<DT>::mfma(xv[part & 1][c], wv[part >> 1][j], t);
             }
     };
     const auto keep = [&](int h) {  // (a wave's own words)
@@ -701,8 +699,8 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     unpack(0);
     for (int h = 0; h < steps; ++h) {
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-            const bool last = part == PARTS - 1, turns = part % (PARTS / 2) == PARTS / 2 - 1;  // the slice's last part
+        for (int part = 0; part < 4; ++part) {
+            const bool last = part == 3, turns = part & 1;  // turns: the 32 terms' last part
             if (last) {
                 wait_vmcnt<GROUP>();  // all but the newest step's
                 lds_barrier();
@@ -745,25 +743,46 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
 
 // ---- joins and copies ----------------------------------------------------------------------------
 
-// y = sum of the splits' partial sums (in their order) + bias
+// y = sum of the splits' partial sums (in their order) + bias; four columns a thread
 __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a, int cols) {
-    const int64_t total = (int64_t)a.m * cols, step = (int64_t)gridDim.x * 256 * 4;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < total; i += step) {
-        typedef float4_t loose4 __attribute__((aligned(4)));
-        const int count = (int)min((int64_t)4, total - i);
+    typedef float4_t loose4 __attribute__((aligned(4)));
+    const int n = 4 * (blockIdx.x * 256 + threadIdx.x), left = cols - n;
+    if (left <= 0) return;
+    float4_t bias = {};
+    if (a.bias != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < left) bias[e] = load_any(a.bias, a.bias_dtype, n + e);
+    }
+    for (int64_t m = blockIdx.y; m < a.m; m += gridDim.y) {
+        const float* p = a.partials + m * cols + n;
         float4_t v = {};
-        for (int s = 0; s < a.splits; ++s) {
-            const float* const p = a.partials + s * a.slab + i;
-            if (count == 4) {
-                v = v + *(const loose4*)p;
-            } else {
-                for (int e = 0; e < count; ++e) v[e] += p[e];
+        if (left >= 4) {
+            int s = 0;
+            for (; s + 4 <= a.splits; s += 4) {
+                float4_t t[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[e] = *(const loose4*)(p + e * a.slab);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v = v + t[e];
+                p += 4 * a.slab;
+            }
+            for (; s < a.splits; ++s, p += a.slab) v = v + *(const loose4*)p;
+        } else {
+            for (int s = 0; s < a.splits; ++s, p += a.slab) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < left) v[e] += p[e];
             }
         }
-        for (int e = 0; e < count; ++e) {
-            const int64_t m = (i + e) / cols, n = i + e - m * cols;
-            store_out(a, m * a.ldy + n, a.bias != nullptr ? v[e] + load_any(a.bias, a.bias_dtype, n) : v[e]);
-        }
+        v = v + bias;
+        const int64_t at = m * a.ldy + n;
+        if (a.y_dtype == DK_FP32)
+            put4<DK_FP32>(a, at, v, left);
+        else if (a.y_dtype == DK_BF16)
+            put4<DK_BF16>(a, at, v, left);
+        else
+            put4<DK_FP16>(a, at, v, left);
     }
 }
 
@@ -805,38 +824,44 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
         p.n_tiles = (int)groups;
         return p;
     }
-    // (Tuning hook, read on every call: DECIK_INT4_PLAN = "tokens,splits" forces a tile and the splits of the sum.)
-    // Tokens a tile: the largest of 256, 128, 64 (backward also 32) whose tiles take the fewest rounds of the CUs, a
-    // round's time taken as its tokens and the weight's unpacking.
+    // Tokens a tile (256, 128 or 64) and splits of the sum: the least estimate of the time. A round of the
+    // CUs takes the times below a block of 128 terms (measured at 4096 and 830 tokens, fp16; tiles of 64 tokens run two
+    // work-groups a CU), a split's partial sums go to memory and back at about 5 TB/s, their join takes a launch.
+    // Measured against the choice: [830, 8960] x 1536 forward 36 us (256 tokens 46, 64 tokens 45), backward 49 in six
+    // splits of 128 tokens (8 of 256: 53, 3 of 64: 71); [512, 4096] x 4096 forward 41 in four splits of 128 (two of 64: 45,
+    // eight of 256: 47).
+    // (Tuning hook, read on every call: DECIK_INT4_PLAN = "tokens,splits" forces a plan.)
     const int64_t cols = backward ? k : n, steps = backward ? (n + kI4Block - 1) / kI4Block : blocks;
     p.n_tiles = (int)((cols + kI4TileN - 1) / kI4TileN);
-    double best = 0.0;
     int forced_tokens = 0, forced_splits = 0;
     if (const char* v = std::getenv("DECIK_INT4_PLAN"))
-        if (std::sscanf(v, "%d,%d", &forced_tokens, &forced_splits) != 2 || forced_splits < 1 || forced_splits > steps)
+        if (std::sscanf(v, "%d,%d", &forced_tokens, &forced_splits) != 2 || forced_splits < 1 || forced_splits > steps ||
+            (forced_tokens != 256 && forced_tokens != 128 && forced_tokens != 64))
             forced_tokens = 0;
-    if (forced_tokens != 256 && forced_tokens != 128 && forced_tokens != 64 && !(backward && forced_tokens == 32))
-        forced_tokens = 0;
-    for (int tokens = 256; tokens >= (backward ? 32 : 64); tokens /= 2) {
+    double best = 0.0;
+    for (int tokens = 256; tokens >= 64; tokens /= 2) {
         if (forced_tokens != 0 && tokens != forced_tokens) continue;
         const int64_t m_tiles = (m + tokens - 1) / tokens, tiles = m_tiles * p.n_tiles;
-        if (forced_tokens == 0 && tokens > 64 && m <= tokens / 2) continue;
-        // splits of the sum until the tiles fill the CUs, at least four blocks each
-        int64_t splits = tiles >= 192 ? 1 : 256 / tiles;
-        if (splits > steps / 4) splits = steps / 4;
-        if (splits < 1) splits = 1;
-        if (forced_tokens != 0) splits = forced_splits;
-        const int64_t per = (steps + splits - 1) / splits;
-        splits = (steps + per - 1) / per;
-        const int64_t rounds = (tiles * splits + 255) / 256;
-        const double cost = (double)rounds * per * (tokens + 64) * 256 +
-                            (splits > 1 ? (double)splits * m * cols / 16 : 0.0);
-        if (best == 0.0 || cost < best) {
-            best = cost;
-            p.tokens = tokens;
-            p.m_tiles = (int)m_tiles;
-            p.splits = (int)splits;
-            p.steps_per_split = (int)per;
+        for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+            if (forced_tokens != 0) want = forced_splits;
+            if (want > 1 && (want > steps / 2 || tiles * want > 1024) && forced_tokens == 0) break;
+            const int64_t per = (steps + want - 1) / want, splits = (steps + per - 1) / per, groups = tiles * splits;
+            double block = 0.0;  // us of a block of 128 terms, over all rounds
+            if (tokens > 64) {
+                block = (double)((groups + 255) / 256) * (tokens == 256 ? 3.7 : 2.7);
+            } else {
+                const int64_t rest = groups % 512;
+                block = (double)(groups / 512) * 3.3 + (rest == 0 ? 0.0 : rest <= 256 ? 2.2 : 3.3);
+            }
+            const double cost = block * (double)per + (splits > 1 ? 4.0 + (double)(splits * m * cols) * 8 / 5e6 : 0.0);
+            if (best == 0.0 || cost < best) {
+                best = cost;
+                p.tokens = tokens;
+                p.m_tiles = (int)m_tiles;
+                p.splits = (int)splits;
+                p.steps_per_split = (int)per;
+            }
+            if (forced_tokens != 0) break;
         }
     }
     p.partial_bytes = p.splits > 1 ? (int64_t)p.splits * m * cols * 4 : 0;
@@ -887,7 +912,6 @@ static hipError_t launch_back(const Int4Args& a, const Int4Plan& p, hipStream_t 
 template <int DT>
 static hipError_t launch_typed(const Int4Args& a, const Int4Plan& p, bool backward, hipStream_t s) {
     if (backward) {
-        if (p.tokens == 32) return launch_back<DT, 1>(a, p, s);
         if (p.tokens == 64) return launch_back<DT, 2>(a, p, s);
         if (p.tokens == 128) return launch_back<DT, 4>(a, p, s);
         return launch_back<DT, 8>(a, p, s);
@@ -900,7 +924,7 @@ static hipError_t launch_typed(const Int4Args& a, const Int4Plan& p, bool backwa
 hipError_t launch_int4(Int4Args a, const Int4Plan& p, int dtype, bool backward, hipStream_t s) {
     const int cols = backward ? a.k : a.n, sum = backward ? a.n : a.k;
     a.group_mul = (uint32_t)((0x100000000ull + a.group_units - 1) / (uint64_t)a.group_units);
-    a.kpad = (a.k + kI4Block - 1) / kI4Block * kI4Block;
+    a.kblocks = (a.k + kI4Block - 1) / kI4Block;
     a.blocks = (sum + 127) / 128;
     a.x_cols = (sum + 7) / 8 * 8;
     a.blocks_per_split = p.steps_per_split;
@@ -919,8 +943,7 @@ hipError_t launch_int4(Int4Args a, const Int4Plan& p, int dtype, bool backward, 
     }
     hipError_t e = dtype == DK_FP16 ? launch_typed<DK_FP16>(a, p, backward, s) : launch_typed<DK_BF16>(a, p, backward, s);
     if (e != hipSuccess || p.splits == 1) return e;
-    const int64_t grid = ((int64_t)a.m * cols + 1023) / 1024;
-    hipLaunchKernelGGL(int4_join_kernel, dim3((unsigned)(grid < 8192 ? grid : 8192)), dim3(256), 0, s, a, cols);
+    hipLaunchKernelGGL(int4_join_kernel, dim3((cols + 1023) / 1024, a.m < 4096 ? a.m : 4096), dim3(256), 0, s, a, cols);
     return hipGetLastError();
 }
 

@@ -17,13 +17,14 @@ from torch.autograd.function import once_differentiable
 
 from ._lib import DTYPES, call_on, check, gpu_input, lib, same_gpu
 
-BLOCK = 128  # columns of a block in the packed rows
+ROWS, BLOCK = 16, 128  # rows and columns of a tile of packed codes
 _TYPES = {torch.float16: 0, torch.bfloat16: 1}
 
 
 class Int4Weight:
-    """A weight [n, k] in groups of `group` columns: packed uint8 [n, ceil(k / 128) * 64] (the layout of
-    dk_int4_linear), meta int32 [n, ceil(k / group)] (scale and zero point), scale_dtype. Not changed in place by any call."""
+    """A weight [n, k] in groups of `group` columns, as dk_int4_linear takes it: packed uint8 [ceil(n / 16), ceil(k / 128),
+    1024] (tiles of 16 rows by 128 columns), meta int32 [ceil(n / 16), ceil(k / group), 16] (scale and zero point),
+    scale_dtype. No call changes it."""
 
     __slots__ = ("packed", "meta", "n", "k", "group", "scale_dtype")
 
@@ -44,18 +45,24 @@ class Int4Weight:
     @property
     def scales(self):
         """[n, groups], of scale_dtype."""
-        return (self.meta & 0xFFFF).to(torch.int16).view(self.scale_dtype)
+        return (self._by_row() & 0xFFFF).to(torch.int16).view(self.scale_dtype)
 
     @property
     def zeros(self):
         """uint8 [n, groups]."""
-        return (self.meta >> 16).to(torch.uint8)
+        return (self._by_row() >> 16).to(torch.uint8)
+
+    def _by_row(self):
+        tiles, groups, _ = self.meta.shape
+        return self.meta.transpose(1, 2).reshape(tiles * ROWS, groups)[:self.n]
 
     def codes(self):
         """uint8 [n, k], unpacked."""
-        words = self.packed.view(torch.int32).view(self.n, -(-self.k // BLOCK), 4, 4)  # [n, block, q, j]
+        tiles, blocks, _ = self.packed.shape
+        words = self.packed.view(torch.int32).view(tiles, blocks, 4, ROWS, 4)  # [.., q, row, j]
         cols = torch.stack([(words >> s) & 15 for s in _SHIFTS], -1).to(torch.uint8)
-        return cols.transpose(2, 3).reshape(self.n, -(-self.k // BLOCK) * BLOCK)[:, :self.k].contiguous()
+        # [tile, row, block, j, q, column]
+        return cols.permute(0, 3, 1, 4, 2, 5).reshape(tiles * ROWS, blocks * BLOCK)[:self.n, :self.k].contiguous()
 
 
 # bits of columns 0 .. 7 of a word
@@ -82,16 +89,18 @@ def int4_weight(codes, scales, zeros=None, group=128):
             raise ValueError(f"{what}: codes, scales and zeros must be on one device")
     if n and (int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 16)):
         raise ValueError(f"{what}: codes must be 0 to 15, zeros 0 to 16")
-    blocks = -(-k // BLOCK)
-    cols = torch.zeros((n, blocks * BLOCK), dtype=torch.uint8, device=codes.device)
-    cols[:, :k] = codes
-    cols = cols.view(n, blocks, 4, 4, 8).transpose(2, 3)  # [n, block, q, j, column]
-    words = torch.zeros((n, blocks, 4, 4), dtype=torch.int32, device=codes.device)
+    tiles, blocks = -(-n // ROWS), -(-k // BLOCK)
+    cols = torch.zeros((tiles * ROWS, blocks * BLOCK), dtype=torch.uint8, device=codes.device)
+    cols[:n, :k] = codes
+    cols = cols.view(tiles, ROWS, blocks, 4, 4, 8).permute(0, 2, 4, 1, 3, 5)  # [tile, block, q, row, j, column]
+    words = torch.zeros((tiles, blocks, 4, ROWS, 4), dtype=torch.int32, device=codes.device)
     for e, shift in enumerate(_SHIFTS):
         words |= cols[..., e].to(torch.int32) << shift
-    meta = scales.contiguous().view(torch.int16).to(torch.int32) & 0xFFFF
-    meta |= 8 << 16 if zeros is None else zeros.to(torch.int32) << 16
-    return Int4Weight(words.view(n, blocks * 16).view(torch.uint8), meta, n, k, group, scales.dtype)
+    meta = torch.zeros((tiles * ROWS, shape[1]), dtype=torch.int32, device=codes.device)
+    meta[:n] = scales.contiguous().view(torch.int16).to(torch.int32) & 0xFFFF
+    meta[:n] |= 8 << 16 if zeros is None else zeros.to(torch.int32) << 16
+    return Int4Weight(words.view(tiles, blocks, 256).view(torch.uint8), meta.view(tiles, ROWS, shape[1]).transpose(1, 2).contiguous(),
+                      n, k, group, scales.dtype)
 
 
 def quantize_int4(w, group=128, symmetric=False, scale_dtype=None):
@@ -175,8 +184,8 @@ def _product(what, backward, x, weight, bias, dtype):
     need = lib().dk_int4_linear_workspace(backward, copy, m, n, k)
     # a tensor of its own a call: graphs and streams share none
     work = x.new_empty(need, dtype=torch.uint8) if need > 0 else None
-    call_on(dev, lib().dk_int4_linear, backward, x2.data_ptr(), code, ldx, weight.packed.data_ptr(), weight.packed.stride(0),
-            weight.meta.data_ptr(), weight.group, _TYPES[weight.scale_dtype], None if bias is None else bias.data_ptr(),
+    call_on(dev, lib().dk_int4_linear, backward, x2.data_ptr(), code, ldx, weight.packed.data_ptr(), weight.meta.data_ptr(),
+            weight.group, _TYPES[weight.scale_dtype], None if bias is None else bias.data_ptr(),
             bias_code, y.data_ptr(), out, cols, m, n, k, copy, None if work is None else work.data_ptr(), max(need, 0))
     return y
 

@@ -423,18 +423,18 @@ int dk_scaled_rope_bwd(const dk_scaled_rope* d, void* stream);
 /* Linear layers whose frozen weight [n, k] holds 4-bit integers, no counterpart in the reference:
  *   W[r, c] = (code - zero) * scale, scale and zero point of row r's group c / group (group a multiple of 32)
  *   forward   y [m, n] = x [m, k] . W^T + bias,   backward  dx [m, k] = dy [m, n] . W
- * packed: rows of ldw bytes (a multiple of 64 that holds k), 16-byte aligned, blocks of 128 columns in 64 bytes: 32-bit
- * word 4 q + j of a block holds its columns 32 j + 8 q + 0 .. 7, column 2 i of these in bits 4 i, 2 i + 1 in bits
- * 16 + 4 i; columns from k on any code. meta [n, ceil(k / group)] (packed rows): the scale's 16 bits (scale_dtype
- * fp16 or bf16) and, from bit 16, the zero point, 0 to 16. x of x_dtype fp16 or bf16, y of it or fp32; the bias NULL or
+ * packed: tiles of 16 rows by 128 columns in 1024 bytes [ceil(n / 16), ceil(k / 128)], 16-byte aligned. Of a tile the 16
+ * bytes at 16 (16 q + r) hold row r, their 32-bit word j columns 32 j + 8 q + 0 .. 7, column 2 i of these in bits 4 i,
+ * 2 i + 1 in bits 16 + 4 i. meta [ceil(n / 16), ceil(k / group), 16]: a row's and group's scale (16 bits, scale_dtype
+ * fp16 or bf16) and, from bit 16, the zero point, 0 to 16. Rows from n on: zeros in both; columns from k on: any code. x of x_dtype fp16 or bf16, y of it or fp32; the bias NULL or
  * of bias_dtype. Forward: exact integers times x, group sums in fp32 times the scale, one rounding. Backward: W
  * rounded once to x_dtype, sums in fp32. Sums go in an order that depends on the sizes alone. `copy` = 1: x has rows
  * that do not start at multiples of 16 bytes or a number of columns that is no multiple of 8; it is then copied to
  * the workspace first. workspace: dk_int4_linear_workspace(..) bytes (0: none). 0 <= m, n < 2^23, m n < 2^37,
  * m k < 2^37, 1 <= k <= 2^20. */
 int64_t dk_int4_linear_workspace(int backward, int copy, int64_t m, int64_t n, int64_t k);
-int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, int64_t ldw,
-                   const uint32_t* meta, int64_t group, int scale_dtype, const void* bias, int bias_dtype, void* y,
+int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, const uint32_t* meta,
+                   int64_t group, int scale_dtype, const void* bias, int bias_dtype, void* y,
                    int y_dtype, int64_t ldy, int64_t m, int64_t n, int64_t k, int copy, void* workspace,
                    int64_t workspace_bytes, void* stream);
 /* Diagnostic, host-only: out[0] = tokens a tile, out[1] = waves that share a row's columns (0: tiles of 256 rows or

@@ -81,21 +81,25 @@ def test_packing_round_trip(n, k, group):
 
     codes, scales, zeros = random_parts(n, k, group, BF16, 1)
     w = int4_weight(codes, scales, zeros, group)
-    assert w.packed.shape == (n, -(-k // 128) * 64) and w.shape == (n, k)
+    assert w.packed.shape == (-(-n // 16), -(-k // 128), 1024) and w.shape == (n, k)
     assert torch.equal(w.codes(), codes) and torch.equal(w.scales, scales) and torch.equal(w.zeros, zeros)
     assert torch.equal(dequantize_int4(w).double(), values(codes, scales, zeros, group)[0].float().double())
     assert torch.equal(int4_weight(codes, scales, None, group).zeros, torch.full_like(zeros, 8))
 
 
 def test_packed_layout():
-    """Word 4 q + j of a block: columns 32 j + 8 q + e, column e in bits 4 (e // 2) + 16 (e % 2)."""
+    """Bytes 16 (16 q + r) of a tile hold row r; their word j columns 32 j + 8 q + e, column e in bits 4 (e // 2) + 16 (e % 2)."""
     from decik_amd.int4 import int4_weight
 
-    codes, scales, _ = random_parts(2, 256, 128, F16, 3)
-    words = int4_weight(codes, scales, None, 128).packed.view(torch.int32).long() & 0xFFFFFFFF
-    for n, b, q, j, e in ((0, 0, 0, 0, 0), (1, 1, 3, 2, 7), (0, 1, 2, 3, 4), (1, 0, 1, 0, 1)):
-        word = int(words[n, 16 * b + 4 * q + j])
+    codes, scales, zeros = random_parts(35, 256, 128, F16, 3)
+    weight = int4_weight(codes, scales, zeros, 128)
+    words = weight.packed.view(torch.int32).long() & 0xFFFFFFFF
+    for n, b, q, j, e in ((0, 0, 0, 0, 0), (17, 1, 3, 2, 7), (34, 1, 2, 3, 4), (15, 0, 1, 0, 1)):
+        word = int(words[n // 16, b, 4 * (16 * q + n % 16) + j])
         assert word >> (4 * (e // 2) + 16 * (e % 2)) & 15 == int(codes[n, 128 * b + 32 * j + 8 * q + e])
+        meta = int(weight.meta[n // 16, b, n % 16])
+        assert meta & 0xFFFF == int(scales[n, b].view(torch.int16)) and meta >> 16 == int(zeros[n, b])
+    assert not weight.meta[2, :, 3:].any() and not words[2, :].view(2, 4, 16, 4)[:, :, 3:].any()
 
 
 def test_quantize():
@@ -252,8 +256,7 @@ def test_outputs_take_any_row_length(device):
             copy = int(total % 8 != 0)
             need = _lib.lib().dk_int4_linear_workspace(back, copy, m, n, k)
             work = torch.empty(max(need, 1), dtype=torch.uint8, device=device)
-            _lib.call_on(device, _lib.lib().dk_int4_linear, back, x.data_ptr(), 0, total, weight.packed.data_ptr(),
-                         weight.packed.stride(0), weight.meta.data_ptr(), 32, 0, None, 0, out.data_ptr(), 0, cols + 3, m, n, k, copy,
+            _lib.call_on(device, _lib.lib().dk_int4_linear, back, x.data_ptr(), 0, total, weight.packed.data_ptr(), weight.meta.data_ptr(), 32, 0, None, 0, out.data_ptr(), 0, cols + 3, m, n, k, copy,
                          work.data_ptr(), need)
             assert torch.equal(out[:m, :cols], want)
             assert bool((out[m:] == 7).all()) and bool((out[:, cols:] == 7).all())
