@@ -354,6 +354,7 @@ hipError_t launch_scaled_rope(ScaledRopeArgs a, int dtype, hipStream_t s);
 
 // Products with weights of 4-bit integers (int4_linear.hip).
 constexpr int kInt4FewM = 64;  // forward launches of so few tokens stream the weight to registers
+constexpr int kInt4FewLds = 65536;  // ... and of at most 16 keep them in LDS where they take so many bytes
 struct Int4Args {
     const void* x;       // [m, k], backward dy [m, n]: 16-byte aligned rows, or `padded` set
     const uint8_t* w;      // tiles of 16 rows by 128 columns [ceil(n / 16), kblocks, 1024]
@@ -365,11 +366,11 @@ struct Int4Args {
     int64_t ldx, ldy, slab;
     int32_t m, n, k, kblocks, x_cols, groups, group_units, scale_dtype, bias_dtype, y_dtype;
     uint32_t group_mul;
-    int32_t blocks, blocks_per_split, splits, m_tiles, n_tiles;
+    int32_t blocks, blocks_per_split, splits, m_tiles, n_tiles, shares;
 };
 struct Int4Plan {
-    bool few;
-    int tokens, waves, m_tiles, n_tiles, splits, steps_per_split;
+    bool few, in_lds;
+    int tokens, waves, shares, m_tiles, n_tiles, splits, steps_per_split;
     int64_t partial_bytes;
 };
 Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward);

@@ -111,22 +111,30 @@ __device__ __forceinline__ void store_out(const Int4Args& a, int64_t at, float v
 }
 
 // ---- forward, few tokens -------------------------------------------------------------------------
-// A work-group takes 16 rows of the weight and 16 C tokens; its NW waves share the columns, each streaming its blocks
-// to registers (P blocks in flight), and join their sums through LDS. GJ: the 32-column units a scale is
-// constant over (4, 2 or 1).
-template <int DT, int C, int GJ, int NW, int P>
+// A wave takes 16 rows of the weight and 16 C tokens, and streams its share of the columns to registers, P blocks ahead.
+// The NW waves of a work-group are NW / a.shares row tiles by a.shares shares of the columns, whose sums meet in
+// LDS. The tokens come from the caches with each block, or (XL) from LDS, where the work-group keeps all of them: every load
+// costs the address unit as much as one of the weight, whatever it hits. GJ: the 32-column units a scale is constant
+// over (4, 2 or 1).
+constexpr int kI4RowPad = 64;  // bytes behind a token's row in LDS: neighbouring rows start in other banks
+constexpr int few_ahead(int c, bool xl) { return xl ? 4 : c == 4 ? 1 : 2; }
+
+__host__ __device__ constexpr int few_x_bytes(int m, int kblocks) { return m * (kblocks * 256 + kI4RowPad); }
+
+template <int DT, int C, int GJ, int NW, bool XL>
 __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
     typedef typename I4<DT>::vec vec;
-    constexpr int UNITS = 4 / GJ;
-    __shared__ float sums[NW][C * 4][64];
+    constexpr int UNITS = 4 / GJ, P = few_ahead(C, XL), XC = XL ? 1 : C, XJ = XL ? 1 : 4;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * C;
-    const int toks = min(16 * C, a.m - m0);
-    const int per = (a.blocks + NW - 1) / NW, b0 = wave * per, b1 = min(a.blocks, b0 + per);
+    const int share = wave % a.shares, tile = blockIdx.x * (NW / a.shares) + wave / a.shares;
+    const int m0 = blockIdx.y * 16 * C, toks = min(16 * C, a.m - m0);
+    const int per = (a.blocks + a.shares - 1) / a.shares, b0 = share * per;
+    const int b1 = tile < a.n_tiles ? min(a.blocks, b0 + per) : 0;
 
-    const rsrc_t wr = make_rsrc(a.w + (int64_t)blockIdx.x * a.kblocks * kI4Tile, (uint32_t)(a.kblocks * kI4Tile));
-    const rsrc_t mr = make_rsrc(a.meta + (int64_t)blockIdx.x * a.groups * 16, (uint32_t)(a.groups * 64));
+    const rsrc_t wr = make_rsrc(a.w + (int64_t)tile * a.kblocks * kI4Tile, (uint32_t)(a.kblocks * kI4Tile));
+    const rsrc_t mr = make_rsrc(a.meta + (int64_t)tile * a.groups * 16, (uint32_t)(a.groups * 64));
     const rsrc_t xr = make_rsrc((const uint16_t*)a.x + (int64_t)m0 * a.ldx, (uint32_t)(((toks - 1) * a.ldx + a.x_cols) * 2));
     const uint32_t w_at = 16 * lane, m_at = 4 * r;
     uint32_t x_at[C];
@@ -136,7 +144,7 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
     struct Stage {
         u32x4_t w;
         uint32_t meta[UNITS];
-        u32x4_t x[C][4];
+        u32x4_t x[XC][XJ];
     };
     Stage st[P];
     const auto fetch = [&](Stage& s, int b) {
@@ -144,23 +152,39 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
         s.w = bload128(wr, off_if(live, w_at + kI4Tile * (uint32_t)b));
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            const uint32_t unit = 4 * b + GJ * u;
             // (a last block's units past k have no group: they read the last one's, for x of zeros)
-            const uint32_t g = min(group_at(a, unit), (uint32_t)a.groups - 1);
+            const uint32_t g = min(group_at(a, 4 * b + GJ * u), (uint32_t)a.groups - 1);
             s.meta[u] = __builtin_amdgcn_raw_buffer_load_b32(mr, (int)off_if(live, m_at + 64 * g), 0, 0);
         }
+        if constexpr (!XL) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+            for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int col = kI4Block * b + 32 * j + 8 * q;
-                s.x[c][j] = bload128(xr, off_if(live && col < a.x_cols, x_at[c] + 256 * (uint32_t)b + 64 * j));
-            }
+                for (int j = 0; j < 4; ++j) {
+                    const int col = kI4Block * b + 32 * j + 8 * q;
+                    s.x[c][j] = bload128(xr, off_if(live && col < a.x_cols, x_at[c] + 256 * (uint32_t)b + 64 * j));
+                }
+        }
     };
+#pragma unroll
+    for (int p = 0; p < P; ++p) fetch(st[p], b0 + p);
+
+    const int pitch = a.kblocks * 256 + kI4RowPad;
+    const uint8_t* const x_row = smem + (r < toks ? r : 0) * pitch + 16 * q;  // (other rows' results are not stored)
+    if constexpr (XL) {
+        // the tokens' rows, zeros behind their columns
+        const int chunks = pitch / 16, total = toks * chunks;
+        for (int i = threadIdx.x; i < total; i += 64 * NW) {
+            const int row = i / chunks, c = i - row * chunks;
+            *(u32x4_t*)(smem + 16 * i) = bload128(xr, off_if(8 * c < a.x_cols, (uint32_t)(row * a.ldx + 8 * c) * 2));
+        }
+        __syncthreads();
+    }
+
     float4_t acc[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = float4_t{};
-    const auto compute = [&](const Stage& s) {
+    const auto compute = [&](const Stage& s, int b) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             const uint32_t meta = s.meta[u];
@@ -180,7 +204,11 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
                 const vec w = unpack8<DT>(s.w[j], z);
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    const vec x = __builtin_bit_cast(vec, s.x[c][j]);
+                    vec x;
+                    if constexpr (XL)
+                        x = *(const vec*)(x_row + 256 * b + 64 * j);
+                    else
+                        x = __builtin_bit_cast(vec, s.x[c][j]);
                     t[c] = I4<DT>::mfma(x, w, t[c]);
                     if constexpr (DT == DK_BF16) t[c] = I4<DT>::mfma(x, taken, t[c]);
                 }
@@ -192,29 +220,31 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
                 for (int i = 0; i < 4; ++i) acc[c][i] = __builtin_fmaf(t[c][i], scale, acc[c][i]);
         }
     };
-#pragma unroll
-    for (int p = 0; p < P; ++p) fetch(st[p], b0 + p);
     for (int b = b0; b < b1; b += P) {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            compute(st[p]);
+            // (past the share's end: weights and scales of zeros; the tokens' columns stay within LDS)
+            compute(st[p], XL ? min(b + p, a.kblocks - 1) : b + p);
             fetch(st[p], b + p + P);
         }
     }
 
-    // lane: row n0 + r, tokens m0 + 16 c + 4 q + i
+    // lane: row 16 tile + r, tokens m0 + 16 c + 4 q + i
+    if constexpr (XL) __syncthreads();
+    float(*const sums)[C * 4][64] = (float(*)[C * 4][64])smem;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[wave][4 * c + i][lane] = acc[c][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < C * 4 * 64; e += 64 * NW) {
-        const int slot = e >> 6, l = e & 63;
-        const int m = m0 + 16 * (slot >> 2) + 4 * (l >> 4) + (slot & 3), n = n0 + (l & 15);
+    const int slots = C * 4 * 64;
+    for (int e = threadIdx.x; e < NW / a.shares * slots; e += 64 * NW) {
+        const int t = e / slots, slot = e / 64 % (C * 4), l = e & 63;
+        const int m = m0 + 16 * (slot >> 2) + 4 * (l >> 4) + (slot & 3);
+        const int n = 16 * (blockIdx.x * (NW / a.shares) + t) + (l & 15);
         if (m >= a.m || n >= a.n) continue;
         float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) v += sums[w][slot][l];
+        for (int w = 0; w < a.shares; ++w) v += sums[t * a.shares + w][slot][l];
         if (a.bias != nullptr) v += load_any(a.bias, a.bias_dtype, n);
         store_out(a, (int64_t)m * a.ldy + n, v);
     }
@@ -816,12 +846,20 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
     if (!backward && m <= kInt4FewM) {
         p.few = true;
         p.tokens = m <= 16 ? 16 : m <= 32 ? 32 : 64;
-        const int64_t groups = (n + 15) / 16;
-        p.waves = groups < 512 && blocks >= 32 ? 16 : groups < 1024 && blocks >= 16 ? 8 : 4;
-        if (p.tokens == 64 && p.waves == 16) p.waves = 8;
         p.splits = 1;
         p.m_tiles = 1;
-        p.n_tiles = (int)groups;
+        p.n_tiles = (int)((n + 15) / 16);
+        p.in_lds = m <= 16 && few_x_bytes((int)m, (int)blocks) <= kInt4FewLds;
+        p.waves = 4;
+        p.shares = 4;
+        if (const char* v = std::getenv("DECIK_INT4_FEW")) {
+            int w = 0, sh = 0, l = 0;
+            if (std::sscanf(v, "%d,%d,%d", &w, &sh, &l) == 3) {
+                p.waves = w;
+                p.shares = sh;
+                p.in_lds = p.in_lds && l;
+            }
+        }
         return p;
     }
     // Tokens a tile (256, 128 or 64) and splits of the sum: the least estimate of the time. A round of the
@@ -868,17 +906,24 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
     return p;
 }
 
-template <int DT, int C, int GJ, int P>
-static hipError_t launch_few(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
-    const dim3 grid(p.n_tiles, (a.m + 16 * C - 1) / (16 * C));
-    switch (p.waves) {
-        case 16:
-            if constexpr (C < 4) hipLaunchKernelGGL((int4_few_kernel<DT, C, GJ, 16, P>), grid, dim3(1024), 0, s, a);
-            break;
-        case 8: hipLaunchKernelGGL((int4_few_kernel<DT, C, GJ, 8, P>), grid, dim3(512), 0, s, a); break;
-        default: hipLaunchKernelGGL((int4_few_kernel<DT, C, GJ, 4, P>), grid, dim3(256), 0, s, a);
-    }
+template <int DT, int C, int GJ, int NW, bool XL>
+static hipError_t launch_waves(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
+    const int tiles = NW / p.shares;
+    const size_t sums = (size_t)NW * C * 4 * 64 * sizeof(float), x = XL ? (size_t)few_x_bytes(a.m, a.kblocks) : 0;
+    const size_t lds = sums > x ? sums : x;
+    if (lds > 65536)
+        if (hipError_t e = allow_dynamic_lds((const void*)int4_few_kernel<DT, C, GJ, NW, XL>, lds)) return e;
+    hipLaunchKernelGGL((int4_few_kernel<DT, C, GJ, NW, XL>), dim3((a.n_tiles + tiles - 1) / tiles, (a.m + 16 * C - 1) / (16 * C)),
+                       dim3(64 * NW), lds, s, a);
     return hipGetLastError();
+}
+
+template <int DT, int C, int GJ, bool XL>
+static hipError_t launch_few(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
+    if constexpr (C < 4)
+        if (p.waves == 16) return launch_waves<DT, C, GJ, 16, XL>(a, p, s);
+    if (p.waves >= 8) return launch_waves<DT, C, GJ, 8, XL>(a, p, s);
+    return launch_waves<DT, C, GJ, 4, XL>(a, p, s);
 }
 
 template <int DT, int C, int GJ>
@@ -892,9 +937,9 @@ static hipError_t launch_tile(const Int4Args& a, const Int4Plan& p, hipStream_t 
 template <int DT, int GJ>
 static hipError_t launch_forward(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
     if (p.few) {
-        if (p.tokens == 16) return launch_few<DT, 1, GJ, 4>(a, p, s);
-        if (p.tokens == 32) return launch_few<DT, 2, GJ, 2>(a, p, s);
-        return launch_few<DT, 4, GJ, 2>(a, p, s);
+        if (p.tokens == 32) return launch_few<DT, 2, GJ, false>(a, p, s);
+        if (p.tokens == 64) return launch_few<DT, 4, GJ, false>(a, p, s);
+        return p.in_lds ? launch_few<DT, 1, GJ, true>(a, p, s) : launch_few<DT, 1, GJ, false>(a, p, s);
     }
     if (p.tokens == 256) return launch_tile<DT, 8, GJ>(a, p, s);
     if (p.tokens == 128) return launch_tile<DT, 4, GJ>(a, p, s);
@@ -931,6 +976,7 @@ hipError_t launch_int4(Int4Args a, const Int4Plan& p, int dtype, bool backward, 
     a.splits = p.splits;
     a.m_tiles = p.m_tiles;
     a.n_tiles = p.n_tiles;
+    a.shares = p.shares;
     a.slab = (int64_t)a.m * cols;
     if (a.padded != nullptr) {
         const int ld = a.x_cols;
