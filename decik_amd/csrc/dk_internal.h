@@ -353,8 +353,8 @@ struct ScaledRopeArgs {
 hipError_t launch_scaled_rope(ScaledRopeArgs a, int dtype, hipStream_t s);
 
 // Products with weights of 4-bit integers (int4_linear.hip).
-constexpr int kInt4FewM = 64;  // forward launches of so few tokens stream the weight to registers
-constexpr int kInt4FewLds = 65536;  // ... and of at most 16 keep them in LDS where they take so many bytes
+constexpr int kInt4FewM = 16;  // forward launches of so few tokens stream the weight to registers
+constexpr int kInt4FewLds = 155648;  // and keep at most so many bytes of the tokens in LDS
 struct Int4Args {
     const void* x;       // [m, k], backward dy [m, n]: 16-byte aligned rows, or `padded` set
     const uint8_t* w;      // tiles of 16 rows by 128 columns [ceil(n / 16), kblocks, 1024]
@@ -369,7 +369,7 @@ struct Int4Args {
     int32_t blocks, blocks_per_split, splits, m_tiles, n_tiles, shares;
 };
 struct Int4Plan {
-    bool few, in_lds;
+    bool few;
     int tokens, waves, shares, m_tiles, n_tiles, splits, steps_per_split;
     int64_t partial_bytes;
 };

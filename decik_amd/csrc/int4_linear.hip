@@ -111,79 +111,62 @@ __device__ __forceinline__ void store_out(const Int4Args& a, int64_t at, float v
 }
 
 // ---- forward, few tokens -------------------------------------------------------------------------
-// A wave takes 16 rows of the weight and 16 C tokens, and streams its share of the columns to registers, P blocks ahead.
-// The NW waves of a work-group are NW / a.shares row tiles by a.shares shares of the columns, whose sums meet in
-// LDS. The tokens come from the caches with each block, or (XL) from LDS, where the work-group keeps all of them: every load
-// costs the address unit as much as one of the weight, whatever it hits. GJ: the 32-column units a scale is constant
-// over (4, 2 or 1).
+// Up to 16 tokens. The NW waves of a work-group are NW / a.shares tiles of 16 rows by a.shares shares of the split's
+// columns, whose sums meet in LDS; each streams its share of the weight to registers, four blocks ahead. The tokens' columns
+// of the split are kept in LDS: from the caches with each block they cost the address unit four loads for the
+// weight's one, and the L2 as much traffic as the weight from four tokens on ([3584, 18944] at 16 tokens: 22 us that
+// way). GJ: the 32-column units a scale is constant over (4, 2 or 1).
 constexpr int kI4RowPad = 64;  // bytes behind a token's row in LDS: neighbouring rows start in other banks
-constexpr int few_ahead(int c, bool xl) { return xl ? 4 : c == 4 ? 1 : 2; }
+constexpr int kI4Ahead = 4;
 
-__host__ __device__ constexpr int few_x_bytes(int m, int kblocks) { return m * (kblocks * 256 + kI4RowPad); }
+__host__ __device__ constexpr int few_x_bytes(int m, int blocks) { return m * (blocks * 256 + kI4RowPad); }
 
-template <int DT, int C, int GJ, int NW, bool XL>
+template <int DT, int GJ, int NW>
 __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
     typedef typename I4<DT>::vec vec;
-    constexpr int UNITS = 4 / GJ, P = few_ahead(C, XL), XC = XL ? 1 : C, XJ = XL ? 1 : 4;
+    constexpr int UNITS = 4 / GJ, P = kI4Ahead;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
-    const int share = wave % a.shares, tile = blockIdx.x * (NW / a.shares) + wave / a.shares;
-    const int m0 = blockIdx.y * 16 * C, toks = min(16 * C, a.m - m0);
-    const int per = (a.blocks + a.shares - 1) / a.shares, b0 = share * per;
-    const int b1 = tile < a.n_tiles ? min(a.blocks, b0 + per) : 0;
+    const int tiles = NW / a.shares, share = wave % a.shares, tile = blockIdx.x * tiles + wave / a.shares;
+    const int first = blockIdx.y * a.blocks_per_split, blocks = min(a.blocks_per_split, a.blocks - first);
+    const int per = (blocks + a.shares - 1) / a.shares, b0 = share * per;  // blocks of the split
+    const int b1 = wave / a.shares < tiles && tile < a.n_tiles ? min(blocks, b0 + per) : 0;
 
-    const rsrc_t wr = make_rsrc(a.w + (int64_t)tile * a.kblocks * kI4Tile, (uint32_t)(a.kblocks * kI4Tile));
+    const rsrc_t wr = make_rsrc(a.w + ((int64_t)tile * a.kblocks + first) * kI4Tile, (uint32_t)(blocks * kI4Tile));
     const rsrc_t mr = make_rsrc(a.meta + (int64_t)tile * a.groups * 16, (uint32_t)(a.groups * 64));
-    const rsrc_t xr = make_rsrc((const uint16_t*)a.x + (int64_t)m0 * a.ldx, (uint32_t)(((toks - 1) * a.ldx + a.x_cols) * 2));
-    const uint32_t w_at = 16 * lane, m_at = 4 * r;
-    uint32_t x_at[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) x_at[c] = off_if(16 * c + r < toks, (16 * c + r) * (uint32_t)a.ldx * 2 + 16 * q);
-
     struct Stage {
         u32x4_t w;
         uint32_t meta[UNITS];
-        u32x4_t x[XC][XJ];
     };
     Stage st[P];
     const auto fetch = [&](Stage& s, int b) {
         const bool live = b < b1;
-        s.w = bload128(wr, off_if(live, w_at + kI4Tile * (uint32_t)b));
+        s.w = bload128(wr, off_if(live, kI4Tile * (uint32_t)b + 16 * lane));
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             // (a last block's units past k have no group: they read the last one's, for x of zeros)
-            const uint32_t g = min(group_at(a, 4 * b + GJ * u), (uint32_t)a.groups - 1);
-            s.meta[u] = __builtin_amdgcn_raw_buffer_load_b32(mr, (int)off_if(live, m_at + 64 * g), 0, 0);
-        }
-        if constexpr (!XL) {
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int col = kI4Block * b + 32 * j + 8 * q;
-                    s.x[c][j] = bload128(xr, off_if(live && col < a.x_cols, x_at[c] + 256 * (uint32_t)b + 64 * j));
-                }
+            const uint32_t g = min(group_at(a, 4 * (first + b) + GJ * u), (uint32_t)a.groups - 1);
+            s.meta[u] = __builtin_amdgcn_raw_buffer_load_b32(mr, (int)off_if(live, 64 * g + 4 * r), 0, 0);
         }
     };
 #pragma unroll
     for (int p = 0; p < P; ++p) fetch(st[p], b0 + p);
 
-    const int pitch = a.kblocks * 256 + kI4RowPad;
-    const uint8_t* const x_row = smem + (r < toks ? r : 0) * pitch + 16 * q;  // (other rows' results are not stored)
-    if constexpr (XL) {
-        // the tokens' rows, zeros behind their columns
-        const int chunks = pitch / 16, total = toks * chunks;
+    // the tokens' rows, zeros behind their columns
+    const int pitch = blocks * 256 + kI4RowPad;
+    {
+        const rsrc_t xr = make_rsrc((const uint16_t*)a.x, (uint32_t)(((a.m - 1) * a.ldx + a.x_cols) * 2));
+        const int chunks = pitch / 16, total = a.m * chunks, cols = a.x_cols - first * kI4Block;
         for (int i = threadIdx.x; i < total; i += 64 * NW) {
-            const int row = i / chunks, c = i - row * chunks;
-            *(u32x4_t*)(smem + 16 * i) = bload128(xr, off_if(8 * c < a.x_cols, (uint32_t)(row * a.ldx + 8 * c) * 2));
+            const int row = i / chunks, c = 8 * (i - row * chunks);
+            *(u32x4_t*)(smem + 16 * i) = bload128(xr, off_if(c < cols, (uint32_t)(row * a.ldx + first * kI4Block + c) * 2));
         }
-        __syncthreads();
     }
+    __syncthreads();
+    const uint8_t* const x_row = smem + (r < a.m ? r : 0) * pitch + 16 * q;  // (other rows' results are not stored)
 
-    float4_t acc[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = float4_t{};
+    float4_t acc = {};
     const auto compute = [&](const Stage& s, int b) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
@@ -196,57 +179,43 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
                 const __bf16 t = (__bf16)(-16.0f - zero_of(meta));
                 taken = vec{t, t, t, t, t, t, t, t};
             }
-            float4_t t[C];
-#pragma unroll
-            for (int c = 0; c < C; ++c) t[c] = float4_t{};
+            float4_t t = {};
 #pragma unroll
             for (int j = GJ * u; j < GJ * (u + 1); ++j) {
-                const vec w = unpack8<DT>(s.w[j], z);
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    vec x;
-                    if constexpr (XL)
-                        x = *(const vec*)(x_row + 256 * b + 64 * j);
-                    else
-                        x = __builtin_bit_cast(vec, s.x[c][j]);
-                    t[c] = I4<DT>::mfma(x, w, t[c]);
-                    if constexpr (DT == DK_BF16) t[c] = I4<DT>::mfma(x, taken, t[c]);
-                }
+                const vec w = unpack8<DT>(s.w[j], z), x = *(const vec*)(x_row + 256 * b + 64 * j);
+                t = I4<DT>::mfma(x, w, t);
+                if constexpr (DT == DK_BF16) t = I4<DT>::mfma(x, taken, t);
             }
             const float scale = scale_of(meta, a.scale_dtype);
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[c][i] = __builtin_fmaf(t[c][i], scale, acc[c][i]);
+            for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(t[i], scale, acc[i]);
         }
     };
     for (int b = b0; b < b1; b += P) {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            // (past the share's end: weights and scales of zeros; the tokens' columns stay within LDS)
-            compute(st[p], XL ? min(b + p, a.kblocks - 1) : b + p);
+            compute(st[p], min(b + p, blocks - 1));  // (past the share's end: weights and scales of zeros)
             fetch(st[p], b + p + P);
         }
     }
 
-    // lane: row 16 tile + r, tokens m0 + 16 c + 4 q + i
-    if constexpr (XL) __syncthreads();
-    float(*const sums)[C * 4][64] = (float(*)[C * 4][64])smem;
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sums[wave][4 * c + i][lane] = acc[c][i];
+    // lane: row 16 tile + r, tokens 4 q + i
     __syncthreads();
-    const int slots = C * 4 * 64;
-    for (int e = threadIdx.x; e < NW / a.shares * slots; e += 64 * NW) {
-        const int t = e / slots, slot = e / 64 % (C * 4), l = e & 63;
-        const int m = m0 + 16 * (slot >> 2) + 4 * (l >> 4) + (slot & 3);
-        const int n = 16 * (blockIdx.x * (NW / a.shares) + t) + (l & 15);
+    float(*const sums)[4][64] = (float(*)[4][64])smem;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < tiles * 256; e += 64 * NW) {
+        const int t = e >> 8, l = e & 63, m = 4 * (l >> 4) + ((e >> 6) & 3), n = 16 * (blockIdx.x * tiles + t) + (l & 15);
         if (m >= a.m || n >= a.n) continue;
         float v = 0.0f;
-        for (int w = 0; w < a.shares; ++w) v += sums[t * a.shares + w][slot][l];
-        if (a.bias != nullptr) v += load_any(a.bias, a.bias_dtype, n);
-        store_out(a, (int64_t)m * a.ldy + n, v);
+        for (int w = 0; w < a.shares; ++w) v += sums[t * a.shares + w][(e >> 6) & 3][l];
+        if (a.splits > 1) {
+            a.partials[blockIdx.y * a.slab + (int64_t)m * a.n + n] = v;
+        } else {
+            if (a.bias != nullptr) v += load_any(a.bias, a.bias_dtype, n);
+            store_out(a, (int64_t)m * a.ldy + n, v);
+        }
     }
 }
 
@@ -845,21 +814,17 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
     const int64_t blocks = (k + kI4Block - 1) / kI4Block;
     if (!backward && m <= kInt4FewM) {
         p.few = true;
-        p.tokens = m <= 16 ? 16 : m <= 32 ? 32 : 64;
-        p.splits = 1;
+        p.tokens = 16;
         p.m_tiles = 1;
         p.n_tiles = (int)((n + 15) / 16);
-        p.in_lds = m <= 16 && few_x_bytes((int)m, (int)blocks) <= kInt4FewLds;
         p.waves = 4;
         p.shares = 4;
-        if (const char* v = std::getenv("DECIK_INT4_FEW")) {
-            int w = 0, sh = 0, l = 0;
-            if (std::sscanf(v, "%d,%d,%d", &w, &sh, &l) == 3) {
-                p.waves = w;
-                p.shares = sh;
-                p.in_lds = p.in_lds && l;
-            }
-        }
+        p.splits = 1;
+        if (const char* v = std::getenv("DECIK_INT4_FEW")) std::sscanf(v, "%d,%d,%d", &p.waves, &p.shares, &p.splits);
+        while (few_x_bytes((int)m, (int)((blocks + p.splits - 1) / p.splits)) > kInt4FewLds) ++p.splits;
+        p.steps_per_split = (int)((blocks + p.splits - 1) / p.splits);
+        p.splits = (int)((blocks + p.steps_per_split - 1) / p.steps_per_split);
+        p.partial_bytes = p.splits > 1 ? (int64_t)p.splits * m * n * 4 : 0;
         return p;
     }
     // Tokens a tile (256, 128 or 64) and splits of the sum: the least estimate of the time. A round of the
@@ -906,24 +871,14 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
     return p;
 }
 
-template <int DT, int C, int GJ, int NW, bool XL>
-static hipError_t launch_waves(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
-    const int tiles = NW / p.shares;
-    const size_t sums = (size_t)NW * C * 4 * 64 * sizeof(float), x = XL ? (size_t)few_x_bytes(a.m, a.kblocks) : 0;
-    const size_t lds = sums > x ? sums : x;
-    if (lds > 65536)
-        if (hipError_t e = allow_dynamic_lds((const void*)int4_few_kernel<DT, C, GJ, NW, XL>, lds)) return e;
-    hipLaunchKernelGGL((int4_few_kernel<DT, C, GJ, NW, XL>), dim3((a.n_tiles + tiles - 1) / tiles, (a.m + 16 * C - 1) / (16 * C)),
-                       dim3(64 * NW), lds, s, a);
-    return hipGetLastError();
-}
-
-template <int DT, int C, int GJ, bool XL>
+template <int DT, int GJ, int NW>
 static hipError_t launch_few(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
-    if constexpr (C < 4)
-        if (p.waves == 16) return launch_waves<DT, C, GJ, 16, XL>(a, p, s);
-    if (p.waves >= 8) return launch_waves<DT, C, GJ, 8, XL>(a, p, s);
-    return launch_waves<DT, C, GJ, 4, XL>(a, p, s);
+    const int tiles = NW / p.shares;
+    const size_t sums = NW * 4 * 64 * sizeof(float), x = few_x_bytes(a.m, p.steps_per_split), lds = sums > x ? sums : x;
+    if (lds > 65536)
+        if (hipError_t e = allow_dynamic_lds((const void*)int4_few_kernel<DT, GJ, NW>, kInt4FewLds)) return e;
+    hipLaunchKernelGGL((int4_few_kernel<DT, GJ, NW>), dim3((a.n_tiles + tiles - 1) / tiles, a.splits), dim3(64 * NW), lds, s, a);
+    return hipGetLastError();
 }
 
 template <int DT, int C, int GJ>
@@ -937,9 +892,9 @@ static hipError_t launch_tile(const Int4Args& a, const Int4Plan& p, hipStream_t 
 template <int DT, int GJ>
 static hipError_t launch_forward(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
     if (p.few) {
-        if (p.tokens == 32) return launch_few<DT, 2, GJ, false>(a, p, s);
-        if (p.tokens == 64) return launch_few<DT, 4, GJ, false>(a, p, s);
-        return p.in_lds ? launch_few<DT, 1, GJ, true>(a, p, s) : launch_few<DT, 1, GJ, false>(a, p, s);
+        if (p.waves == 16) return launch_few<DT, GJ, 16>(a, p, s);
+        if (p.waves == 8) return launch_few<DT, GJ, 8>(a, p, s);
+        return launch_few<DT, GJ, 4>(a, p, s);
     }
     if (p.tokens == 256) return launch_tile<DT, 8, GJ>(a, p, s);
     if (p.tokens == 128) return launch_tile<DT, 4, GJ>(a, p, s);
