@@ -559,7 +559,8 @@ int dk_int4_linear_plan(int backward, int64_t m, int64_t n, int64_t k, int32_t* 
     const Int4Plan p = int4_plan(m, n, k, backward != 0);
     out[0] = p.tokens;
     out[1] = p.few ? p.waves : 0;
-    out[2] = p.splits;
+    out[2] = p.few ? p.shares : 0;
+    out[3] = p.splits;
     return 0;
 }
 

@@ -112,19 +112,19 @@ __device__ __forceinline__ void store_out(const Int4Args& a, int64_t at, float v
 
 // ---- forward, few tokens -------------------------------------------------------------------------
 // Up to 16 tokens. The NW waves of a work-group are NW / a.shares tiles of 16 rows by a.shares shares of the split's
-// columns, whose sums meet in LDS; each streams its share of the weight to registers, four blocks ahead. The tokens' columns
+// columns, whose sums meet in LDS; each streams its share of the weight to registers, P blocks ahead. The tokens' columns
 // of the split are kept in LDS: from the caches with each block they cost the address unit four loads for the
 // weight's one, and the L2 as much traffic as the weight from four tokens on ([3584, 18944] at 16 tokens: 22 us that
 // way). GJ: the 32-column units a scale is constant over (4, 2 or 1).
 constexpr int kI4RowPad = 64;  // bytes behind a token's row in LDS: neighbouring rows start in other banks
-constexpr int kI4Ahead = 4;
 
-__host__ __device__ constexpr int few_x_bytes(int m, int blocks) { return m * (blocks * 256 + kI4RowPad); }
+// (whole loads of a wave)
+__host__ __device__ constexpr int few_x_bytes(int m, int blocks) { return (m * (blocks * 256 + kI4RowPad) + 1023) / 1024 * 1024; }
 
-template <int DT, int GJ, int NW>
+template <int DT, int GJ, int NW, int P>
 __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
     typedef typename I4<DT>::vec vec;
-    constexpr int UNITS = 4 / GJ, P = kI4Ahead;
+    constexpr int UNITS = 4 / GJ;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, q = lane >> 4;
@@ -150,20 +150,21 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
             s.meta[u] = __builtin_amdgcn_raw_buffer_load_b32(mr, (int)off_if(live, 64 * g + 4 * r), 0, 0);
         }
     };
-#pragma unroll
-    for (int p = 0; p < P; ++p) fetch(st[p], b0 + p);
-
     // the tokens' rows, zeros behind their columns
     const int pitch = blocks * 256 + kI4RowPad;
     {
         const rsrc_t xr = make_rsrc((const uint16_t*)a.x, (uint32_t)(((a.m - 1) * a.ldx + a.x_cols) * 2));
         const int chunks = pitch / 16, total = a.m * chunks, cols = a.x_cols - first * kI4Block;
-        for (int i = threadIdx.x; i < total; i += 64 * NW) {
-            const int row = i / chunks, c = 8 * (i - row * chunks);
-            *(u32x4_t*)(smem + 16 * i) = bload128(xr, off_if(c < cols, (uint32_t)(row * a.ldx + first * kI4Block + c) * 2));
+        for (int i = 64 * wave; i < total; i += 64 * NW) {
+            const int row = (i + lane) / chunks, c = 8 * (i + lane - row * chunks);
+            bload128_lds(xr, smem + 16 * i,
+                         off_if(row < a.m && c < cols, (uint32_t)(row * a.ldx + first * kI4Block + c) * 2));
         }
     }
-    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < P; ++p) fetch(st[p], b0 + p);
+    wait_vmcnt<P>();  // the tokens, and of the weight (and its scales) some
+    lds_barrier();
     const uint8_t* const x_row = smem + (r < a.m ? r : 0) * pitch + 16 * q;  // (other rows' results are not stored)
 
     float4_t acc = {};
@@ -191,13 +192,17 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
             for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(t[i], scale, acc[i]);
         }
     };
-    for (int b = b0; b < b1; b += P) {
+    int b = b0;
+    for (; b + P < b1; b += P) {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            compute(st[p], min(b + p, blocks - 1));  // (past the share's end: weights and scales of zeros)
+            compute(st[p], b + p);
             fetch(st[p], b + p + P);
         }
     }
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+        if (b + p < b1) compute(st[p], b + p);
 
     // lane: row 16 tile + r, tokens 4 q + i
     __syncthreads();
@@ -817,11 +822,22 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
         p.tokens = 16;
         p.m_tiles = 1;
         p.n_tiles = (int)((n + 15) / 16);
-        p.waves = 4;
-        p.shares = 4;
+        // Splits where the tokens' columns do not fit the LDS. Where they take much of it and there are more row tiles than CUs,
+        // work-groups of 16 waves with as many tiles as one round of the CUs needs; else one tile a work-group, four or eight
+        // waves sharing its columns. us, in turn with four waves, eight, sixteen sharing and the choice: [18944] x 3584 at
+        // 1 token 11.1, 11.0, 13.6, 11.0; at 16 30.4, 24.7, 26.4, 14.1; [8960] x 1536 at 1 token 4.8, 5.2, 6.9, 4.8; at 16 6.3,
+        // 6.7, 8.3, 5.6; [4096] x 4096 at 4 tokens 5.9, 5.3, 5.3, 5.3.
         p.splits = 1;
-        if (const char* v = std::getenv("DECIK_INT4_FEW")) std::sscanf(v, "%d,%d,%d", &p.waves, &p.shares, &p.splits);
         while (few_x_bytes((int)m, (int)((blocks + p.splits - 1) / p.splits)) > kInt4FewLds) ++p.splits;
+        const int x_bytes = few_x_bytes((int)m, (int)((blocks + p.splits - 1) / p.splits));
+        const int64_t groups = (int64_t)p.n_tiles * p.splits;
+        if (x_bytes > 32768 && groups > 256) {
+            const int64_t tiles = (groups + 255) / 256;
+            p.waves = 16;
+            p.shares = tiles < 16 ? 16 / (int)tiles : 1;
+        } else {
+            p.waves = p.shares = p.n_tiles >= 512 && blocks <= 16 ? 4 : 8;
+        }
         p.steps_per_split = (int)((blocks + p.splits - 1) / p.splits);
         p.splits = (int)((blocks + p.steps_per_split - 1) / p.steps_per_split);
         p.partial_bytes = p.splits > 1 ? (int64_t)p.splits * m * n * 4 : 0;
@@ -871,14 +887,21 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
     return p;
 }
 
-template <int DT, int GJ, int NW>
-static hipError_t launch_few(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
+template <int DT, int GJ, int NW, int P>
+static hipError_t launch_ahead(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
     const int tiles = NW / p.shares;
     const size_t sums = NW * 4 * 64 * sizeof(float), x = few_x_bytes(a.m, p.steps_per_split), lds = sums > x ? sums : x;
     if (lds > 65536)
-        if (hipError_t e = allow_dynamic_lds((const void*)int4_few_kernel<DT, GJ, NW>, kInt4FewLds)) return e;
-    hipLaunchKernelGGL((int4_few_kernel<DT, GJ, NW>), dim3((a.n_tiles + tiles - 1) / tiles, a.splits), dim3(64 * NW), lds, s, a);
+        if (hipError_t e = allow_dynamic_lds((const void*)int4_few_kernel<DT, GJ, NW, P>, kInt4FewLds)) return e;
+    hipLaunchKernelGGL((int4_few_kernel<DT, GJ, NW, P>), dim3((a.n_tiles + tiles - 1) / tiles, a.splits), dim3(64 * NW), lds, s, a);
     return hipGetLastError();
+}
+
+template <int DT, int GJ, int NW>
+static hipError_t launch_few(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
+    // (groups of 32 columns: eight blocks ahead would not fit the registers of 16 waves)
+    if (GJ > 1 && p.steps_per_split > 4 * p.shares) return launch_ahead<DT, GJ, NW, GJ == 1 ? 4 : 8>(a, p, s);
+    return launch_ahead<DT, GJ, NW, 4>(a, p, s);
 }
 
 template <int DT, int C, int GJ>

@@ -119,9 +119,10 @@ def quantize_int4(w, group=128, symmetric=False, scale_dtype=None):
         raise ValueError(f"{what}: scale_dtype must be fp16 or bf16")
     n, k = w.shape
     groups = -(-k // group)
-    v = torch.zeros((n, groups * group), device=w.device)
+    width = min(group, k)  # (one group where it is longer than a row)
+    v = torch.zeros((n, groups * width), device=w.device)
     v[:, :k] = w
-    v = v.view(n, groups, group)
+    v = v.view(n, groups, width)
     if symmetric:
         scales, lo = v.abs().amax(-1) / 7.0, None
     else:
@@ -133,22 +134,23 @@ def quantize_int4(w, group=128, symmetric=False, scale_dtype=None):
     by = torch.where(ok, scales.float(), torch.ones_like(scales, dtype=torch.float32))
     zeros = torch.full_like(by, 8.0) if symmetric else torch.where(ok, torch.round(-lo / by), 8.0).clamp(0, 15)
     codes = torch.round(v / by[..., None]).add_(zeros[..., None]).clamp_(0, 15)
-    codes = torch.where(ok[..., None], codes, zeros[..., None]).to(torch.uint8).view(n, groups * group)[:, :k]
+    codes = torch.where(ok[..., None], codes, zeros[..., None]).to(torch.uint8).view(n, groups * width)[:, :k]
     return int4_weight(codes.contiguous(), scales, None if symmetric else zeros.to(torch.uint8), group)
 
 
 def dequantize_int4(weight, dtype=torch.float32):
     """The values the weight stands for, [N, K] of `dtype`."""
-    values = weight.codes().float() - weight.zeros.float().repeat_interleave(weight.group, 1)[:, :weight.k]
-    return (values * weight.scales.float().repeat_interleave(weight.group, 1)[:, :weight.k]).to(dtype)
+    times = min(weight.group, weight.k)  # (one group where it is longer than a row)
+    zeros, scales = (t.float().repeat_interleave(times, 1)[:, :weight.k] for t in (weight.zeros, weight.scales))
+    return ((weight.codes().float() - zeros) * scales).to(dtype)
 
 
 def launch_plan(backward, m, n, k):
-    """What a product of these sizes runs as (dk_int4_linear_plan): dict of tile_tokens, waves (that share a row's
-    columns; 0: tiles of 256 rows or columns) and splits of the sum."""
-    out = (ctypes.c_int32 * 3)()
+    """What a product of these sizes runs as (dk_int4_linear_plan): dict of tile_tokens, waves (of a work-group that streams
+    the weight; 0: tiles of 256 rows or columns), shares (waves that share a row's columns) and splits of the sum."""
+    out = (ctypes.c_int32 * 4)()
     check(lib().dk_int4_linear_plan(int(backward), m, n, k, out))
-    return dict(tile_tokens=out[0], waves=out[1], splits=out[2])
+    return dict(tile_tokens=out[0], waves=out[1], shares=out[2], splits=out[3])
 
 
 def _product(what, backward, x, weight, bias, dtype):

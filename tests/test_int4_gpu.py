@@ -1,5 +1,5 @@
-"""Linear layers in 4-bit integers (decik_amd.int4) against the formulas in 64 bits: every form (few tokens by 16, 32 and
-64 and by 4, 8 and 16 waves; tiles whole and split), groups, zero points, types, odd sizes, strides, and the
+"""Linear layers in 4-bit integers (decik_amd.int4) against the formulas in 64 bits: every form (few tokens by 4, 8
+and 16 waves; tiles whole and split), groups, zero points, types, odd sizes, strides, and the
 packing, on the CPU.
 
 Tolerances, with S = sum over k of |x| scale |code - zero|. Few tokens: operands are exact, a chain of fp32 sums has at most
@@ -33,8 +33,9 @@ def random_parts(n, k, group, dtype, seed, zeros=True):
 def values(codes, scales, zeros, group):
     """(W, scale of every element) in float64."""
     k = codes.shape[1]
-    s = scales.double().repeat_interleave(group, 1)[:, :k]
-    z = 8.0 if zeros is None else zeros.double().repeat_interleave(group, 1)[:, :k]
+    times = min(group, k)  # (one group where it is longer than a row)
+    s = scales.double().repeat_interleave(times, 1)[:, :k]
+    z = 8.0 if zeros is None else zeros.double().repeat_interleave(times, 1)[:, :k]
     return (codes.double() - z) * s, s
 
 
@@ -85,6 +86,16 @@ def test_packing_round_trip(n, k, group):
     assert torch.equal(w.codes(), codes) and torch.equal(w.scales, scales) and torch.equal(w.zeros, zeros)
     assert torch.equal(dequantize_int4(w).double(), values(codes, scales, zeros, group)[0].float().double())
     assert torch.equal(int4_weight(codes, scales, None, group).zeros, torch.full_like(zeros, 8))
+
+
+def test_one_group_a_row():
+    """Groups far longer than a row cost no memory of their length."""
+    from decik_amd.int4 import dequantize_int4, quantize_int4
+
+    w = make((5, 70), F32, "cpu", 1, 0.02)
+    for symmetric in (False, True):
+        one, exact = (quantize_int4(w, g, symmetric) for g in (2 ** 20, 96))
+        assert one.meta.shape == (1, 1, 16) and torch.equal(dequantize_int4(one), dequantize_int4(exact))
 
 
 def test_packed_layout():
@@ -140,9 +151,10 @@ def test_refusals_of_weights():
 # ---- products ------------------------------------------------------------------------------------
 
 # tokens, rows, columns: each form and what lies around its edges
-FORWARD = [(1, 1, 1), (1, 17, 128), (2, 100, 129), (15, 333, 1121), (16, 48, 4096), (16, 48, 8961), (1, 8200, 2100), (3, 16500, 640), (17, 40, 640),
-           (31, 257, 5000), (32, 9000, 2049), (33, 70, 512), (64, 300, 4100), (64, 17000, 256), (65, 256, 128), (65, 3, 130), (128, 255, 1000),
-           (129, 257, 4096), (300, 700, 1121), (830, 1536, 1536), (257, 1000, 31)]
+FORWARD = [(1, 1, 1), (1, 17, 128), (2, 100, 129), (15, 333, 1121), (16, 48, 4096), (16, 48, 8961), (1, 8200, 2100), (3, 16500, 640), (1, 8200, 30),
+           (16, 4200, 1100), (9, 8209, 2100), (16, 18944, 1121), (16, 70000, 1030), (16, 40, 18944), (13, 3600, 9728), (7, 257, 70000),
+           (17, 40, 640), (31, 257, 5000), (32, 3000, 2049), (33, 70, 512), (64, 300, 4100), (65, 256, 128), (65, 3, 130), (128, 255, 1000),
+           (129, 257, 4096), (300, 700, 1121), (830, 1536, 1536), (257, 1000, 31), (2000, 3000, 1121), (600, 20000, 300)]
 BACKWARD = [(1, 1, 1), (1, 128, 17), (2, 129, 300), (16, 1121, 333), (32, 640, 256), (33, 1000, 257), (64, 4096, 128), (65, 31, 600), (128, 2057, 1121),
             (129, 300, 513), (300, 1121, 700), (830, 1536, 1536), (37, 2057, 1121), (50, 200, 600)]
 
@@ -177,16 +189,38 @@ def test_backward(m, n, k, dtype, device):
         check_backward(int4_linear_backward(dy, weight, F32), dy, w, s, f"group {group} fp32")
 
 
-@pytest.mark.gpu
-def test_every_form_is_tested(device):
-    """The sizes above reach every token tile, wave count and both split and whole sums."""
+def test_every_form_for_few_tokens_is_tested():
+    """The sizes above reach every number of waves, one tile of rows a work-group and several, one split of the columns and several; the
+    tiles for more tokens are tested one by one below."""
     from decik_amd.int4 import launch_plan
 
     plans = [launch_plan(False, *s) for s in FORWARD]
-    assert {(p["tile_tokens"], p["waves"]) for p in plans} == {(16, 4), (16, 8), (16, 16), (32, 4), (32, 8), (32, 16), (64, 4), (64, 8), (64, 0), (128, 0), (256, 0)}
-    assert {p["splits"] > 1 for p in plans if p["waves"] == 0} == {True, False}
-    plans = [launch_plan(True, *s) for s in BACKWARD]
-    assert {(p["tile_tokens"], p["splits"] > 1) for p in plans} == {(t, s) for t in (32, 64, 128, 256) for s in (True, False)}
+    few = {(p["waves"], p["shares"]) for p in plans if p["waves"]}
+    assert few >= {(4, 4), (8, 8), (16, 8), (16, 5), (16, 3), (16, 1)}
+    assert {p["splits"] > 1 for p in plans if p["waves"] == 8} == {p["splits"] > 1 for p in plans if p["waves"] == 16} == {True, False}
+    assert {p["tile_tokens"] for p in plans if not p["waves"]} == {64, 128, 256}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [64, 128, 256])
+@pytest.mark.parametrize("splits", [1, 2, 5])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_every_tile(tokens, splits, dtype, device, monkeypatch):
+    """Each tile, whole and split, both ways, at sizes with edges in every direction and at whole ones."""
+    from decik_amd.int4 import int4_linear_backward, int4_linear_forward, int4_weight, launch_plan
+
+    monkeypatch.setenv("DECIK_INT4_PLAN", f"{tokens},{splits}")
+    for m, n, k in ((300, 700, 1121), (tokens, 768, 768), (70, 1300, 650)):
+        assert launch_plan(False, m, n, k)["tile_tokens"] == launch_plan(True, m, n, k)["tile_tokens"] == tokens
+        assert (launch_plan(False, m, n, k)["splits"] > 1) == (launch_plan(True, m, n, k)["splits"] > 1) == (splits > 1)
+        x, dy, bias = make((m, k), dtype, device, 2), make((m, n), dtype, device, 3), make((n,), F32, device, 4)
+        for group in (32, 64, 128):
+            parts = [p.to(device) for p in random_parts(n, k, group, dtype, group)]
+            weight = int4_weight(*parts, group)
+            w, s = values(*parts, group)
+            for out in (None, F32):
+                check_forward(int4_linear_forward(x, weight, bias, out), x, w, s, bias, f"forward {m} {group}")
+                check_backward(int4_linear_backward(dy, weight, out), dy, w, s, f"backward {m} {group}")
 
 
 @pytest.mark.gpu
