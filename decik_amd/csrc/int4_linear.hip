@@ -13,9 +13,10 @@
 // shift and a mask leave a pair in the halves of a register). In each MFMA lane l = 16 q + r holds k = 8 q + 0 .. 7 of
 // row r of its operand. `meta` holds groups' words, a scale (low 16 bits) and a zero point (next byte), by tile rows, groups
 // and the tile's 16 rows.
-// From pairs to operands, fp16: 0x6400 | q is 1024 + q, 0x6400 | 16 q is 1024 + 16 q, and one packed subtraction or
-// multiply-add leaves q - zero, exactly. bf16: 0x4180 | 8 q is 16 + q; there is no packed bf16 arithmetic, so 16 + zero
-// times the sum of x, from one more MFMA, is taken off the group's sum.
+// From pairs to operands: 0x6400 | q is 1024 + q as fp16, 0x6400 | 16 q is 1024 + 16 q. fp16: one packed subtraction or
+// multiply-add leaves q - zero, exactly, one packed product the weight. bf16: mixed multiply-adds give (1024 + q) scale -
+// (1024 + zero) scale in fp32, and one conversion a pair rounds: a scale has 11 bits at most, so both products are
+// exact and the difference is scale (q - zero) without any error (with 1 for the scale, q - zero).
 #include <cstdio>
 #include <cstdlib>
 
@@ -62,38 +63,70 @@ __device__ __forceinline__ float scale_of(uint32_t meta, int scale_dtype) {
     return scale_dtype == DK_BF16 ? I4<DK_BF16>::scale(meta) : I4<DK_FP16>::scale(meta);
 }
 
-// pairs of zero-point constants of a row for the forward: fp16 -(1024 + zero) and -(64 + zero); bf16 unused
-struct ZeroF16 {
-    half2_t whole, part;
-    __device__ __forceinline__ void set(uint32_t meta) {
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+// Constants of a row's group, and operands of a word's columns 0 .. 7: the integers code - zero, or the weights.
+template <int DT>
+struct I4Group;
+template <>
+struct I4Group<DK_FP16> {
+    half2_t whole, part, scale;  // -(1024 + zero), -(64 + zero)
+    __device__ __forceinline__ void set_zero(uint32_t meta) {
         const _Float16 z = (_Float16)zero_of(meta);
         const _Float16 a = (_Float16)-1024.0f - z, b = (_Float16)-64.0f - z;
         whole = half2_t{a, a};
         part = half2_t{b, b};
     }
-};
-
-// eight operands of a dword: fp16 code - zero, bf16 16 + code
-template <int DT>
-__device__ __forceinline__ typename I4<DT>::vec unpack8(uint32_t d, const ZeroF16& z) {
-    u32x4_t o;
-    if constexpr (DT == DK_FP16) {
-        const uint32_t h = d >> 8;
-        const half2_t sixteenth = half2_t{(_Float16)0.0625f, (_Float16)0.0625f};
-        const auto even = [&](uint32_t v) {
-            return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, and_or(v, 0x000F000Fu, 0x64006400u)) + z.whole);
-        };
-        const auto odd = [&](uint32_t v) {
-            return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2_t, and_or(v, 0x00F000F0u, 0x64006400u)),
-                                                                          sixteenth, z.part));
-        };
-        o = u32x4_t{even(d), odd(d), even(h), odd(h)};
-    } else {
-        o = u32x4_t{and_or(d << 3, 0x00780078u, 0x41804180u), and_or(d >> 1, 0x00780078u, 0x41804180u),
-                    and_or(d >> 5, 0x00780078u, 0x41804180u), and_or(d >> 9, 0x00780078u, 0x41804180u)};
+    __device__ __forceinline__ void set(uint32_t meta, int scale_dtype) {
+        set_zero(meta);
+        const _Float16 s = scale_dtype == DK_FP16 ? __builtin_bit_cast(_Float16, (uint16_t)meta) : (_Float16)I4<DK_BF16>::scale(meta);
+        scale = half2_t{s, s};
     }
-    return __builtin_bit_cast(typename I4<DT>::vec, o);
-}
+    __device__ __forceinline__ half2_t even(uint32_t v) const {
+        return __builtin_bit_cast(half2_t, and_or(v, 0x000F000Fu, 0x64006400u)) + whole;
+    }
+    __device__ __forceinline__ half2_t odd(uint32_t v) const {
+        const half2_t sixteenth = half2_t{(_Float16)0.0625f, (_Float16)0.0625f};
+        return __builtin_elementwise_fma(__builtin_bit_cast(half2_t, and_or(v, 0x00F000F0u, 0x64006400u)), sixteenth, part);
+    }
+    static __device__ __forceinline__ half8_t join(half2_t a, half2_t b, half2_t c, half2_t d) {
+        return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+    __device__ __forceinline__ half8_t integers(uint32_t d) const { return join(even(d), odd(d), even(d >> 8), odd(d >> 8)); }
+    __device__ __forceinline__ half8_t weights(uint32_t d) const {
+        return join(even(d) * scale, odd(d) * scale, even(d >> 8) * scale, odd(d >> 8) * scale);
+    }
+};
+template <>
+struct I4Group<DK_BF16> {
+    float whole, whole_zero, part, part_zero;  // of 1024 + code, and of 1024 + 16 code
+    __device__ __forceinline__ void set_scale(uint32_t meta, float s) {
+        const float z = zero_of(meta);
+        whole = s;
+        whole_zero = (-1024.0f - z) * s;
+        part = s * 0.0625f;
+        part_zero = (-64.0f - z) * s;
+    }
+    __device__ __forceinline__ void set_zero(uint32_t meta) {
+        float one = 1.0f;
+        asm("" : "+v"(one));  // a factor: a product by 1 is made a conversion and a sum
+        set_scale(meta, one);
+    }
+    __device__ __forceinline__ void set(uint32_t meta, int scale_dtype) { set_scale(meta, scale_of(meta, scale_dtype)); }
+    static __device__ __forceinline__ uint32_t pair(uint32_t v, float by, float plus) {
+        const half2_t h = __builtin_bit_cast(half2_t, v);
+        const float2_t f = float2_t{__builtin_fmaf((float)h[0], by, plus), __builtin_fmaf((float)h[1], by, plus)};
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
+    }
+    __device__ __forceinline__ bf16x8_t weights(uint32_t d) const {
+        const uint32_t h = d >> 8;
+        return __builtin_bit_cast(bf16x8_t, u32x4_t{pair(and_or(d, 0x000F000Fu, 0x64006400u), whole, whole_zero),
+                                                    pair(and_or(d, 0x00F000F0u, 0x64006400u), part, part_zero),
+                                                    pair(and_or(h, 0x000F000Fu, 0x64006400u), whole, whole_zero),
+                                                    pair(and_or(h, 0x00F000F0u, 0x64006400u), part, part_zero)});
+    }
+    __device__ __forceinline__ bf16x8_t integers(uint32_t d) const { return weights(d); }  // (of set_zero)
+};
 
 // group of the 32 columns that begin at 32 unit
 __device__ __forceinline__ uint32_t group_at(const Int4Args& a, uint32_t unit) {
@@ -172,20 +205,13 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             const uint32_t meta = s.meta[u];
-            ZeroF16 z;
-            vec taken;
-            if constexpr (DT == DK_FP16) {
-                z.set(meta);
-            } else {
-                const __bf16 t = (__bf16)(-16.0f - zero_of(meta));
-                taken = vec{t, t, t, t, t, t, t, t};
-            }
+            I4Group<DT> group;
+            group.set_zero(meta);
             float4_t t = {};
 #pragma unroll
             for (int j = GJ * u; j < GJ * (u + 1); ++j) {
-                const vec w = unpack8<DT>(s.w[j], z), x = *(const vec*)(x_row + 256 * b + 64 * j);
+                const vec w = group.integers(s.w[j]), x = *(const vec*)(x_row + 256 * b + 64 * j);
                 t = I4<DT>::mfma(x, w, t);
-                if constexpr (DT == DK_BF16) t = I4<DT>::mfma(x, taken, t);
             }
             const float scale = scale_of(meta, a.scale_dtype);
 #pragma unroll
@@ -228,12 +254,8 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
 // Tiles of 32 C tokens by 256 rows of the weight (forward) or 256 columns (backward), eight waves of 16 C by 64. The sum
 // goes in steps of 64 terms through a ring of three stages of LDS, filled by loads that go there directly: one wait and
 // one barrier a step, loads two steps ahead. The weight stays in 4 bits up to each wave's registers.
-// W is rounded to the activations' type here. fp16: (code - zero) exact, one packed product. bf16: the pair
-// 1024 + code, as fp16, times scale - (1024 + zero) scale by mixed multiply-adds in fp32 (its constant is within 2^-13 of
-// a scale), then one rounding.
+// W is rounded to the activations' type here, once.
 constexpr int kI4Waves = 8, kI4TileN = 256, kI4Step = 64, kI4Ring = 3;
-
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 // An offset in a stage that every step adds its stage's to: held as it is, or each read's would be formed again.
 __device__ __forceinline__ uint32_t held(uint32_t v) {
@@ -283,53 +305,6 @@ struct I4Tokens {
         for (int i = 0; i < LOADS; ++i)
             bload128_lds(src, stage + 1024 * (wave * LOADS + i),
                          off_if(live && c0 + col[i] < a.x_cols, at[i] + 2 * (uint32_t)c0));
-    }
-};
-
-// scale and zero point as the tiles multiply with them
-template <int DT>
-struct I4Group;
-template <>
-struct I4Group<DK_FP16> {
-    ZeroF16 zero;
-    half2_t scale;
-    __device__ __forceinline__ void set(uint32_t meta, int scale_dtype) {
-        zero.set(meta);
-        const _Float16 s = scale_dtype == DK_FP16 ? __builtin_bit_cast(_Float16, (uint16_t)meta) : (_Float16)I4<DK_BF16>::scale(meta);
-        scale = half2_t{s, s};
-    }
-    // weights of a word's columns 0 .. 7
-    __device__ __forceinline__ half8_t weights(uint32_t d) const {
-        u32x4_t v = __builtin_bit_cast(u32x4_t, unpack8<DK_FP16>(d, zero));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t pair = v[i];  // (a bit_cast of the element itself would take element 0)
-            v[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, pair) * scale);
-        }
-        return __builtin_bit_cast(half8_t, v);
-    }
-};
-template <>
-struct I4Group<DK_BF16> {
-    float whole, whole_zero, part, part_zero;  // of 1024 + code, and of 1024 + 16 code
-    __device__ __forceinline__ void set(uint32_t meta, int scale_dtype) {
-        whole = scale_of(meta, scale_dtype);
-        const float z = zero_of(meta);
-        whole_zero = (-1024.0f - z) * whole;
-        part = whole * 0.0625f;
-        part_zero = (-64.0f - z) * whole;
-    }
-    static __device__ __forceinline__ uint32_t pair(uint32_t v, float by, float plus) {
-        const half2_t h = __builtin_bit_cast(half2_t, v);
-        const float2_t f = float2_t{__builtin_fmaf((float)h[0], by, plus), __builtin_fmaf((float)h[1], by, plus)};
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
-    }
-    __device__ __forceinline__ bf16x8_t weights(uint32_t d) const {
-        const uint32_t h = d >> 8;
-        return __builtin_bit_cast(bf16x8_t, u32x4_t{pair(and_or(d, 0x000F000Fu, 0x64006400u), whole, whole_zero),
-                                                    pair(and_or(d, 0x00F000F0u, 0x64006400u), part, part_zero),
-                                                    pair(and_or(h, 0x000F000Fu, 0x64006400u), whole, whole_zero),
-                                                    pair(and_or(h, 0x00F000F0u, 0x64006400u), part, part_zero)});
     }
 };
 

@@ -178,7 +178,7 @@ def _product(what, backward, x, weight, bias, dtype):
         return x.new_zeros(*x.shape[:-1], cols, dtype=dtype)
     x2 = x if x.dim() == 2 else x.reshape(-1, total)
     m = x2.shape[0]
-    if x2.stride(1) != 1 and total != 1 or (m > 1 and x2.stride(0) >= 2 ** 23):
+    if x2.stride(1) != 1 and total != 1 or (m > 1 and x2.stride(0) >= 2 ** 22):
         x2 = x2.contiguous()
     ldx = x2.stride(0)
     copy = total % 8 != 0 or x2.data_ptr() % 16 != 0 or (m > 1 and ldx % 8 != 0)

@@ -427,8 +427,8 @@ int dk_scaled_rope_bwd(const dk_scaled_rope* d, void* stream);
  * bytes at 16 (16 q + r) hold row r, their 32-bit word j columns 32 j + 8 q + 0 .. 7, column 2 i of these in bits 4 i,
  * 2 i + 1 in bits 16 + 4 i. meta [ceil(n / 16), ceil(k / group), 16]: a row's and group's scale (16 bits, scale_dtype
  * fp16 or bf16) and, from bit 16, the zero point, 0 to 16. Rows from n on: zeros in both; columns from k on: any code. x of x_dtype fp16 or bf16, y of it or fp32; the bias NULL or
- * of bias_dtype. Forward: exact integers times x, group sums in fp32 times the scale, one rounding. Backward: W
- * rounded once to x_dtype, sums in fp32. Sums go in an order that depends on the sizes alone. `copy` = 1: x has rows
+ * of bias_dtype. Forward: exact integers times x, group sums in fp32 times the scale, one rounding. Backward, and forward from 17 tokens on: W
+ * rounded once to x_dtype, sums in fp32. x's row stride: non-negative, below 2^22. Sums go in an order that depends on the sizes alone. `copy` = 1: x has rows
  * that do not start at multiples of 16 bytes or a number of columns that is no multiple of 8; it is then copied to
  * the workspace first. workspace: dk_int4_linear_workspace(..) bytes (0: none). 0 <= m, n < 2^23, m n < 2^37,
  * m k < 2^37, 1 <= k <= 2^20. */
