@@ -61,52 +61,57 @@ def _gate(what, gate, shape):
     raise ValueError(f"{what}: a gate must be [{width}], {tuple(shape)} or {(*shape[:-1], 1)}, not {tuple(gate.shape)}")
 
 
-class _Call:
-    """The checked inputs of a call, and its descriptor."""
+def _inputs(what, x, residual, weight, post_weight, gate, dtype):
+    """The checked inputs of a call: (device, x, residual (rows of one stride), their addresses and row strides, weight,
+    post weight and gate with address and type, type codes of x, stream and y, width)."""
+    dev = gpu_input(what, x)
+    same_gpu(what, dev, residual, weight, post_weight, gate)
+    shape = x.shape
+    xc = sc = yc = DTYPES.get(x.dtype)
+    if xc is None or not shape or not 1 <= shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"{what}: x must be [.., W] with W from 1 to {MAX_WIDTH}, fp16, bf16 or fp32")
+    width = shape[-1]
+    r_at = ldr = 0
+    if residual is not None:
+        sc = DTYPES.get(residual.dtype)
+        if residual.shape != shape or sc not in (xc, 2):
+            raise ValueError(f"{what}: the residual must have x's shape, and x's type or fp32")
+        residual, ldr = _rows(residual, width)
+        r_at = residual.data_ptr()
+    if dtype is not None:
+        yc = DTYPES.get(dtype)
+        if yc not in (xc, 2):
+            raise ValueError(f"{what}: y must be of x's type or fp32")
+    x, ldx = _rows(x, width)
+    return (dev, x, residual, x.data_ptr(), r_at, ldx, ldr, _weight(what, "weight", weight, width),
+            _weight(what, "post_weight", post_weight, width), _gate(what, gate, shape), xc, sc, yc, width)
 
-    __slots__ = ("dev", "x", "residual", "weight", "post", "gate", "codes", "lds", "rows", "width", "scale", "eps", "keep")
 
-    def __init__(self, what, x, residual, weight, post_weight, gate, scale, eps, dtype):
-        self.dev = gpu_input(what, x)
-        same_gpu(what, self.dev, residual, weight, post_weight, gate)
-        xc = DTYPES.get(x.dtype)
-        if xc is None or x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
-            raise ValueError(f"{what}: x must be [.., W] with W from 1 to {MAX_WIDTH}, fp16, bf16 or fp32")
-        width = x.shape[-1]
-        sc = yc = xc
-        if residual is not None:
-            sc = DTYPES.get(residual.dtype)
-            if residual.shape != x.shape or sc not in (xc, 2):
-                raise ValueError(f"{what}: the residual must have x's shape, and x's type or fp32")
-        if dtype is not None:
-            yc = DTYPES.get(dtype)
-            if yc not in (xc, 2):
-                raise ValueError(f"{what}: y must be of x's type or fp32")
-        x2, ldx = _rows(x, width)
-        r2, ldr = (None, 0) if residual is None else _rows(residual, width)
-        self.weight, self.post = _weight(what, "weight", weight, width), _weight(what, "post_weight", post_weight, width)
-        self.gate = _gate(what, gate, x.shape)
-        self.x, self.residual, self.codes, self.lds = x2, r2, (xc, sc, yc), (ldx, ldr)
-        self.rows, self.width, self.scale, self.eps = x.numel() // width, width, scale, eps
+def _like(t, contiguous, dtype):
+    """An empty tensor of t's shape with packed rows."""
+    return torch.empty_like(t) if contiguous and t.dtype == dtype else t.new_empty(t.shape, dtype=dtype)
 
-    def pack(self, gh=0, gy=0, h=0, y=0, dx=0, dres=0, dgate=0, dw=0, dpw=0, ldgh=0, ldgy=0):
-        _, w, wc = self.weight
-        _, pw, pc = self.post
-        _, g, gc, kind, ldg = self.gate
-        r = self.residual
-        return ResidualNorm.PACK.pack(self.x.data_ptr(), 0 if r is None else r.data_ptr(), gh, gy, h, y, dx, dres, dgate,
-                                      w, pw, g, dw, dpw, *self.lds, ldgh, ldgy, ldg, self.rows, self.width, *self.codes,
-                                      wc, pc, gc, kind, self.scale, self.eps, 0)
+
+def _forward(what, x, residual, weight, post_weight, gate, scale, eps, dtype, keep_h):
+    dev, x2, r2, x_at, r_at, ldx, ldr, w, pw, g, xc, sc, yc, width = _inputs(what, x, residual, weight, post_weight, gate,
+                                                                           dtype)
+    packed = x.is_contiguous()
+    h = y = None
+    if keep_h:
+        h = _like(x, packed, x.dtype if residual is None else residual.dtype)
+    if weight is not None:
+        y = _like(x, packed, dtype or x.dtype)
+    desc = ResidualNorm.PACK.pack(x_at, r_at, 0, 0, 0 if h is None else h.data_ptr(), 0 if y is None else y.data_ptr(), 0, 0, 0,
+                                  w[1], pw[1], g[1], 0, 0, ldx, ldr, 0, 0, g[4], x.numel() // width, width, xc, sc, yc,
+                                  w[2], pw[2], g[2], g[3], scale, eps, 0)
+    call_on(dev, lib().dk_residual_norm_fwd, desc)
+    return h, y
 
 
 def residual_norm_forward(x, residual, weight, post_weight=None, gate=None, residual_scale=1.0, eps=1e-6, dtype=None):
     """(h, y) of x [.., W] and residual (the same shape; None: no stream). h is of the residual's type (x's without
     one), y of `dtype` (x's type, the default, or fp32), None without a weight."""
-    c = _Call("residual_norm_forward", x, residual, weight, post_weight, gate, residual_scale, eps, dtype)
-    h = x.new_empty(x.shape, dtype=x.dtype if residual is None else residual.dtype)
-    y = None if weight is None else x.new_empty(x.shape, dtype=dtype)
-    call_on(c.dev, lib().dk_residual_norm_fwd, c.pack(h=h.data_ptr(), y=0 if y is None else y.data_ptr()))
-    return h, y
+    return _forward("residual_norm_forward", x, residual, weight, post_weight, gate, residual_scale, eps, dtype, True)
 
 
 def residual_norm_backward(grad_h, grad_y, x, residual, weight, post_weight=None, gate=None, residual_scale=1.0, eps=1e-6,
@@ -115,36 +120,42 @@ def residual_norm_backward(grad_h, grad_y, x, residual, weight, post_weight=None
     y (None only without a weight) and the same inputs; None for an input that was None. dweight, dpost_weight and
     the gradient of a channel gate are fp32 [W]; without param_grads these three are None."""
     what = "residual_norm_backward"
-    c = _Call(what, x, residual, weight, post_weight, gate, residual_scale, eps, None if grad_y is None else grad_y.dtype)
-    same_gpu(what, c.dev, grad_h, grad_y)
+    dev, x2, r2, x_at, r_at, ldx, ldr, w, pw, g, xc, sc, yc, width = _inputs(
+        what, x, residual, weight, post_weight, gate, None if grad_y is None else grad_y.dtype)
+    same_gpu(what, dev, grad_h, grad_y)
     if (grad_y is None) != (weight is None) or (grad_y is not None and grad_y.shape != x.shape):
         raise ValueError(f"{what}: grad_y of x's shape where there is a weight, and only there")
     h_dtype = x.dtype if residual is None else residual.dtype
-    gh, ldgh, gy, ldgy = None, 0, None, 0
+    gh_at = ldgh = gy_at = ldgy = 0
     if grad_h is not None:
         if grad_h.shape != x.shape or grad_h.dtype != h_dtype:
             raise ValueError(f"{what}: grad_h must have h's shape and type")
-        gh, ldgh = _rows(grad_h, c.width)
+        grad_h, ldgh = _rows(grad_h, width)
+        gh_at = grad_h.data_ptr()
     if grad_y is not None:
-        gy, ldgy = _rows(grad_y, c.width)
-    dx = x.new_empty(x.shape)
-    dres = None if residual is None else x.new_empty(x.shape, dtype=h_dtype)
-    kind = c.gate[3]
-    dgate = None
-    if kind == _CHANNEL:
-        dgate = x.new_empty(c.width, dtype=torch.float32) if param_grads else None
-    elif kind != _NONE:
-        dgate = x.new_empty(gate.shape, dtype=gate.dtype)
-    dw = x.new_empty(c.width, dtype=torch.float32) if param_grads and weight is not None else None
-    dpw = x.new_empty(c.width, dtype=torch.float32) if param_grads and post_weight is not None else None
-    at = [0 if t is None else t.data_ptr() for t in (gh, gy, dres, dgate, dw, dpw)]
-    desc = c.pack(gh=at[0], gy=at[1], dx=dx.data_ptr(), dres=at[2], dgate=at[3], dw=at[4], dpw=at[5], ldgh=ldgh, ldgy=ldgy)
-    need, work = 0, None
-    if dw is not None or dpw is not None or (kind == _CHANNEL and dgate is not None):
+        grad_y, ldgy = _rows(grad_y, width)
+        gy_at = grad_y.data_ptr()
+    packed, rows, kind = x.is_contiguous(), x.numel() // width, g[3]
+    dx = _like(x, packed, x.dtype)
+    dres = None if residual is None else _like(x, packed, h_dtype)
+    dgate = None if kind in (_NONE, _CHANNEL) else x.new_empty(gate.shape, dtype=gate.dtype)
+    # the gradients that are sums over the rows: weight, post weight, channel gate
+    wanted = (weight is not None, post_weight is not None, kind == _CHANNEL) if param_grads else (False,) * 3
+    count = sum(wanted)
+    work, need, dw, dpw = None, 0, None, None
+    if count:
+        sums = iter(x.new_empty(count, width, dtype=torch.float32).unbind())
+        dw, dpw, channel = (next(sums) if want else None for want in wanted)
+        dgate = channel if kind == _CHANNEL else dgate
+    desc = ResidualNorm.PACK.pack(x_at, r_at, gh_at, gy_at, 0, 0, dx.data_ptr(), 0 if dres is None else dres.data_ptr(),
+                                  0 if dgate is None else dgate.data_ptr(), w[1], pw[1], g[1],
+                                  0 if dw is None else dw.data_ptr(), 0 if dpw is None else dpw.data_ptr(), ldx, ldr, ldgh,
+                                  ldgy, g[4], rows, width, xc, sc, yc, w[2], pw[2], g[2], kind, residual_scale, eps, 0)
+    if count:
         need = lib().dk_residual_norm_bwd_workspace(desc)
         # a tensor of its own a call: graphs and streams share none
         work = x.new_empty(need, dtype=torch.uint8) if need > 0 else None
-    call_on(c.dev, lib().dk_residual_norm_bwd, desc, None if work is None else work.data_ptr(), max(need, 0))
+    call_on(dev, lib().dk_residual_norm_bwd, desc, None if work is None else work.data_ptr(), max(need, 0))
     return dx, dres, dw, dpw, dgate
 
 
@@ -201,11 +212,9 @@ class _RmsNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, eps, dtype):
-        c = _Call("rms_norm", x, None, weight, None, None, 1.0, eps, dtype)
         if weight is None:
             raise ValueError("rms_norm: needs a weight")
-        y = x.new_empty(x.shape, dtype=dtype)
-        call_on(c.dev, lib().dk_residual_norm_fwd, c.pack(y=y.data_ptr()))
+        _, y = _forward("rms_norm", x, None, weight, None, None, 1.0, eps, dtype, False)
         ctx.save_for_backward(x, weight)
         ctx.eps = eps
         return y

@@ -386,7 +386,7 @@ def scaled_frequencies(rotary_dim, base=10000.0, scaling=None, length=None, devi
 def _scaled_rope(what, entry, q, k, batch, tokens, heads, d, q_strides, k_strides, positions, inv_freq, layout, factor,
                  shapes):
     dev = q.device
-    same_gpu(what, dev, k, positions, inv_freq)
+    same_gpu(what, dev, positions, inv_freq)
     code = _QK_TYPES.get(q.dtype)
     if code is None or k.dtype != q.dtype:
         raise ValueError(f"{what}: q and k must both be fp16 or both bf16")
@@ -412,13 +412,17 @@ def _scaled_rope(what, entry, q, k, batch, tokens, heads, d, q_strides, k_stride
 
 def _token_major(what, t, heads):
     """(t, B, T, D, strides of batch, token and head) of a [B, T, H * D] or [T, H * D] tensor."""
-    if t.dim() not in (2, 3) or heads < 1 or t.shape[-1] % heads or t.shape[-1] == 0:
-        raise ValueError(f"{what}: q and k must be [B, T, H * D] or [T, H * D], here H = {heads}, not {tuple(t.shape)}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1 or min(t.stride()) < 0:
+    shape = t.shape
+    if len(shape) not in (2, 3) or heads < 1 or shape[-1] % heads or shape[-1] == 0:
+        raise ValueError(f"{what}: q and k must be [B, T, H * D] or [T, H * D], here H = {heads}, not {tuple(shape)}")
+    strides = t.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
         t = t.contiguous()
-    b, n = (1, t.shape[0]) if t.dim() == 2 else t.shape[:2]
-    d = t.shape[-1] // heads
-    return t, b, n, d, (t.stride(0) if t.dim() == 3 else 0, t.stride(-2), d)
+        strides = t.stride()
+    d = shape[-1] // heads
+    if len(shape) == 2:
+        return t, 1, shape[0], d, (0, strides[0], d)
+    return t, shape[0], shape[1], d, (strides[0], strides[1], d)
 
 
 def scaled_rope_forward(q, k, positions, inv_freq, n_heads, n_kv_heads, layout="half", factor=1.0):
