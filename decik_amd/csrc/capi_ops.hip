@@ -136,6 +136,13 @@ bool int4_sizes(int64_t m, int64_t n, int64_t k) {
     return m >= 0 && n >= 0 && m < most && n < most && k >= 1 && k <= (int64_t(1) << 20) && m * n < area && m * k < area;
 }
 
+// workspace of a call: partial sums, then room for x with aligned rows (few tokens take it as it is)
+int64_t int4_bytes(const Int4Plan& p, bool copy, int64_t m, int64_t sum, int64_t* partial) {
+    const int64_t sums = (p.partial_bytes + 15) / 16 * 16;
+    if (partial != nullptr) *partial = sums;
+    return sums + (copy && !p.few ? m * ((sum + 7) / 8 * 16) : 0);
+}
+
 const char* const kInt4Sizes = "dk_int4_linear: 0 <= m, n < 2^23, m n < 2^37, m k < 2^37, 1 <= k <= 2^20";
 
 bool rows_fit(int64_t ld, int heads, int d) { return ld >= (int64_t)heads * d; }
@@ -549,8 +556,7 @@ int64_t dk_int4_linear_workspace(int backward, int copy, int64_t m, int64_t n, i
         return -1;
     }
     if (m == 0 || n == 0) return 0;
-    const int64_t sum = backward ? n : k;
-    return (int4_plan(m, n, k, backward != 0).partial_bytes + 15) / 16 * 16 + (copy ? m * ((sum + 7) / 8 * 16) : 0);
+    return int4_bytes(int4_plan(m, n, k, backward != 0), copy != 0, m, backward ? n : k, nullptr);
 }
 
 int dk_int4_linear_plan(int backward, int64_t m, int64_t n, int64_t k, int32_t* out) {
@@ -591,7 +597,8 @@ int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const 
     if (!copy && (sum % 8 != 0 || !aligned_to(x, 16) || (m > 1 && ldx % 8 != 0)))
         return dk_fail("dk_int4_linear: without copy x needs 16-byte aligned rows of a multiple of 8 columns");
     const Int4Plan p = int4_plan(m, n, k, backward != 0);
-    const int64_t partial = (p.partial_bytes + 15) / 16 * 16, need = partial + (copy ? m * ((sum + 7) / 8 * 16) : 0);
+    int64_t partial = 0;
+    const int64_t need = int4_bytes(p, copy != 0, m, sum, &partial);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16)))
         return dk_fail("dk_int4_linear: workspace too small (dk_int4_linear_workspace)");
     Int4Args a{};
@@ -601,7 +608,8 @@ int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const 
     a.bias = bias;
     a.y = y;
     a.partials = static_cast<float*>(workspace);
-    a.padded = copy ? reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + partial) : nullptr;
+    a.padded = copy && !p.few ? reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(workspace) + partial) : nullptr;
+    a.loose = copy && p.few;
     a.ldx = m > 1 ? ldx : 0;
     a.ldy = ldy;
     a.m = (int32_t)m;

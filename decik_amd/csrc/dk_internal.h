@@ -353,7 +353,7 @@ struct ScaledRopeArgs {
 hipError_t launch_scaled_rope(ScaledRopeArgs a, int dtype, hipStream_t s);
 
 // Products with weights of 4-bit integers (int4_linear.hip).
-constexpr int kInt4FewM = 16;  // forward launches of so few tokens stream the weight to registers
+constexpr int kInt4FewM = 32, kInt4FewSmallM = 64;  // forward launches of so few tokens stream the weight to registers
 constexpr int kInt4FewLds = 155648;  // and keep at most so many bytes of the tokens in LDS
 struct Int4Args {
     const void* x;       // [m, k], backward dy [m, n]: 16-byte aligned rows, or `padded` set
@@ -367,6 +367,7 @@ struct Int4Args {
     int32_t m, n, k, kblocks, x_cols, groups, group_units, scale_dtype, bias_dtype, y_dtype;
     uint32_t group_mul;
     int32_t blocks, blocks_per_split, splits, m_tiles, n_tiles, shares;
+    bool loose;  // few tokens: rows of x that start anywhere, or k is no multiple of eight
 };
 struct Int4Plan {
     bool few;

@@ -144,11 +144,13 @@ __device__ __forceinline__ void store_out(const Int4Args& a, int64_t at, float v
 }
 
 // ---- forward, few tokens -------------------------------------------------------------------------
-// Up to 16 tokens. The NW waves of a work-group are NW / a.shares tiles of 16 rows by a.shares shares of the split's
+// Tokens by 16 (blockIdx.z). The NW waves of a work-group are NW / a.shares tiles of 16 rows by a.shares shares of the split's
 // columns, whose sums meet in LDS; each streams its share of the weight to registers, P blocks ahead. The tokens' columns
 // of the split are kept in LDS: from the caches with each block they cost the address unit four loads for the
 // weight's one, and the L2 as much traffic as the weight from four tokens on ([3584, 18944] at 16 tokens: 22 us that
 // way). GJ: the 32-column units a scale is constant over (4, 2 or 1).
+typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
+typedef u16x8_t u16x8_loose_t __attribute__((aligned(2)));
 constexpr int kI4RowPad = 64;  // bytes behind a token's row in LDS: neighbouring rows start in other banks
 
 // (whole loads of a wave)
@@ -166,6 +168,7 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
     const int per = (blocks + a.shares - 1) / a.shares, b0 = share * per;  // blocks of the split
     const int b1 = wave / a.shares < tiles && tile < a.n_tiles ? min(blocks, b0 + per) : 0;
 
+    const int m0 = 16 * blockIdx.z, toks = min(16, a.m - m0);
     const rsrc_t wr = make_rsrc(a.w + ((int64_t)tile * a.kblocks + first) * kI4Tile, (uint32_t)(blocks * kI4Tile));
     const rsrc_t mr = make_rsrc(a.meta + (int64_t)tile * a.groups * 16, (uint32_t)(a.groups * 64));
     struct Stage {
@@ -186,19 +189,37 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
     // the tokens' rows, zeros behind their columns
     const int pitch = blocks * 256 + kI4RowPad;
     {
-        const rsrc_t xr = make_rsrc((const uint16_t*)a.x, (uint32_t)(((a.m - 1) * a.ldx + a.x_cols) * 2));
-        const int chunks = pitch / 16, total = a.m * chunks, cols = a.x_cols - first * kI4Block;
-        for (int i = 64 * wave; i < total; i += 64 * NW) {
-            const int row = (i + lane) / chunks, c = 8 * (i + lane - row * chunks);
-            bload128_lds(xr, smem + 16 * i,
-                         off_if(row < a.m && c < cols, (uint32_t)(row * a.ldx + first * kI4Block + c) * 2));
+        const uint16_t* const x = (const uint16_t*)a.x + m0 * a.ldx;
+        const int chunks = pitch / 16, total = toks * chunks, c0 = first * kI4Block;
+        if (!a.loose) {
+            const rsrc_t xr = make_rsrc(x, (uint32_t)(((toks - 1) * a.ldx + a.k) * 2));
+            for (int i = 64 * wave; i < total; i += 64 * NW) {
+                const int row = (i + lane) / chunks, c = c0 + 8 * (i + lane - row * chunks);
+                bload128_lds(xr, smem + 16 * i,
+                             off_if(row < toks && c < min(a.k, c0 + blocks * kI4Block), (uint32_t)(row * a.ldx + c) * 2));
+            }
+        } else {
+            // rows that start anywhere, or end inside eight columns
+            for (int i = threadIdx.x; i < total; i += 64 * NW) {
+                const int row = i / chunks, c = c0 + 8 * (i - row * chunks), left = min(a.k, c0 + blocks * kI4Block) - c;
+                u16x8_t v = {};
+                const uint16_t* const p = x + row * a.ldx + c;
+                if (left >= 8) {
+                    v = *(const u16x8_loose_t*)p;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < left) v[e] = p[e];
+                }
+                *(u16x8_t*)(smem + 16 * i) = v;
+            }
         }
     }
 #pragma unroll
     for (int p = 0; p < P; ++p) fetch(st[p], b0 + p);
     wait_vmcnt<P>();  // the tokens, and of the weight (and its scales) some
     lds_barrier();
-    const uint8_t* const x_row = smem + (r < a.m ? r : 0) * pitch + 16 * q;  // (other rows' results are not stored)
+    const uint8_t* const x_row = smem + (r < toks ? r : 0) * pitch + 16 * q;  // (other rows' results are not stored)
 
     float4_t acc = {};
     const auto compute = [&](const Stage& s, int b) {
@@ -237,7 +258,7 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
     for (int i = 0; i < 4; ++i) sums[wave][i][lane] = acc[i];
     __syncthreads();
     for (int e = threadIdx.x; e < tiles * 256; e += 64 * NW) {
-        const int t = e >> 8, l = e & 63, m = 4 * (l >> 4) + ((e >> 6) & 3), n = 16 * (blockIdx.x * tiles + t) + (l & 15);
+        const int t = e >> 8, l = e & 63, m = m0 + 4 * (l >> 4) + ((e >> 6) & 3), n = 16 * (blockIdx.x * tiles + t) + (l & 15);
         if (m >= a.m || n >= a.n) continue;
         float v = 0.0f;
         for (int w = 0; w < a.shares; ++w) v += sums[t * a.shares + w][(e >> 6) & 3][l];
@@ -772,12 +793,10 @@ __global__ __launch_bounds__(256) void int4_rows_kernel(const uint16_t* __restri
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
         const int64_t row = i / (ld / 8);
         const int c = (int)(i - row * (ld / 8)) * 8;
-        typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
-        typedef u16x8_t loose __attribute__((aligned(2)));
         u16x8_t v = {};
         const uint16_t* const p = x + row * ldx + c;
         if (c + 8 <= cols) {
-            v = *(const loose*)p;
+            v = *(const u16x8_loose_t*)p;
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -792,10 +811,14 @@ __global__ __launch_bounds__(256) void int4_rows_kernel(const uint16_t* __restri
 Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
     Int4Plan p{};
     const int64_t blocks = (k + kI4Block - 1) / kI4Block;
-    if (!backward && m <= kInt4FewM) {
+    // Tokens by 16 with the weight streamed to registers for each: up to 32 (18944 x 3584: 30 us, as the tiles), up to 64
+    // on small weights, whose tiles are all start and end ([2057] x 1121 at 37 tokens: 12.8 us and 3.9 for the join).
+    const bool small = n * ((k + 7) / 8 * 8) <= (int64_t(1) << 23);
+    if (!backward && std::getenv("DECIK_INT4_PLAN") == nullptr && m <= (small ? kInt4FewSmallM : kInt4FewM)) {
         p.few = true;
         p.tokens = 16;
-        p.m_tiles = 1;
+        p.m_tiles = (int)((m + 15) / 16);
+        const int toks = m < 16 ? (int)m : 16;
         p.n_tiles = (int)((n + 15) / 16);
         // Splits where the tokens' columns do not fit the LDS. Where they take much of it and there are more row tiles than CUs,
         // work-groups of 16 waves with as many tiles as one round of the CUs needs; else one tile a work-group, four or eight
@@ -803,9 +826,9 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
         // 1 token 11.1, 11.0, 13.6, 11.0; at 16 30.4, 24.7, 26.4, 14.1; [8960] x 1536 at 1 token 4.8, 5.2, 6.9, 4.8; at 16 6.3,
         // 6.7, 8.3, 5.6; [4096] x 4096 at 4 tokens 5.9, 5.3, 5.3, 5.3.
         p.splits = 1;
-        while (few_x_bytes((int)m, (int)((blocks + p.splits - 1) / p.splits)) > kInt4FewLds) ++p.splits;
-        const int x_bytes = few_x_bytes((int)m, (int)((blocks + p.splits - 1) / p.splits));
-        const int64_t groups = (int64_t)p.n_tiles * p.splits;
+        while (few_x_bytes(toks, (int)((blocks + p.splits - 1) / p.splits)) > kInt4FewLds) ++p.splits;
+        const int x_bytes = few_x_bytes(toks, (int)((blocks + p.splits - 1) / p.splits));
+        const int64_t groups = (int64_t)p.n_tiles * p.splits * p.m_tiles;
         if (x_bytes > 32768 && groups > 256) {
             const int64_t tiles = (groups + 255) / 256;
             p.waves = 16;
@@ -865,10 +888,10 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
 template <int DT, int GJ, int NW, int P>
 static hipError_t launch_ahead(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
     const int tiles = NW / p.shares;
-    const size_t sums = NW * 4 * 64 * sizeof(float), x = few_x_bytes(a.m, p.steps_per_split), lds = sums > x ? sums : x;
+    const size_t sums = NW * 4 * 64 * sizeof(float), x = few_x_bytes(a.m < 16 ? a.m : 16, p.steps_per_split), lds = sums > x ? sums : x;
     if (lds > 65536)
         if (hipError_t e = allow_dynamic_lds((const void*)int4_few_kernel<DT, GJ, NW, P>, kInt4FewLds)) return e;
-    hipLaunchKernelGGL((int4_few_kernel<DT, GJ, NW, P>), dim3((a.n_tiles + tiles - 1) / tiles, a.splits), dim3(64 * NW), lds, s, a);
+    hipLaunchKernelGGL((int4_few_kernel<DT, GJ, NW, P>), dim3((a.n_tiles + tiles - 1) / tiles, a.splits, p.m_tiles), dim3(64 * NW), lds, s, a);
     return hipGetLastError();
 }
 

@@ -429,8 +429,8 @@ int dk_scaled_rope_bwd(const dk_scaled_rope* d, void* stream);
  * fp16 or bf16) and, from bit 16, the zero point, 0 to 16. Rows from n on: zeros in both; columns from k on: any code. x of x_dtype fp16 or bf16, y of it or fp32; the bias NULL or
  * of bias_dtype. Forward: exact integers times x, group sums in fp32 times the scale, one rounding. Backward, and forward from 17 tokens on: W
  * rounded once to x_dtype, sums in fp32. x's row stride: non-negative, below 2^22. Sums go in an order that depends on the sizes alone. `copy` = 1: x has rows
- * that do not start at multiples of 16 bytes or a number of columns that is no multiple of 8; it is then copied to
- * the workspace first. workspace: dk_int4_linear_workspace(..) bytes (0: none). 0 <= m, n < 2^23, m n < 2^37,
+ * that do not start at multiples of 16 bytes or a number of columns that is no multiple of 8; where
+ * more than a few tokens come it is then copied to the workspace first. workspace: dk_int4_linear_workspace(..) bytes (0: none). 0 <= m, n < 2^23, m n < 2^37,
  * m k < 2^37, 1 <= k <= 2^20. */
 int64_t dk_int4_linear_workspace(int backward, int copy, int64_t m, int64_t n, int64_t k);
 int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, const uint32_t* meta,

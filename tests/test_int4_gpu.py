@@ -151,7 +151,7 @@ def test_refusals_of_weights():
 # tokens, rows, columns: each form and what lies around its edges
 FORWARD = [(1, 1, 1), (1, 17, 128), (2, 100, 129), (15, 333, 1121), (16, 48, 4096), (16, 48, 8961), (1, 8200, 2100), (3, 16500, 640), (1, 8200, 30),
            (16, 4200, 1100), (9, 8209, 2100), (16, 18944, 1121), (16, 70000, 1030), (16, 40, 18944), (13, 3600, 9728), (7, 257, 70000),
-           (17, 40, 640), (31, 257, 5000), (32, 3000, 2049), (33, 70, 512), (64, 300, 4100), (65, 256, 128), (65, 3, 130), (128, 255, 1000),
+           (17, 40, 640), (31, 257, 5000), (32, 3000, 2049), (29, 4200, 9000), (33, 70, 512), (64, 300, 4100), (40, 3000, 4100), (65, 256, 128), (65, 3, 130), (128, 255, 1000),
            (129, 257, 4096), (300, 700, 1121), (830, 1536, 1536), (257, 1000, 31), (2000, 3000, 1121), (600, 20000, 300)]
 BACKWARD = [(1, 1, 1), (1, 128, 17), (2, 129, 300), (16, 1121, 333), (32, 640, 256), (33, 1000, 257), (64, 4096, 128), (65, 31, 600), (128, 2057, 1121),
             (129, 300, 513), (300, 1121, 700), (830, 1536, 1536), (37, 2057, 1121), (50, 200, 600)]
@@ -197,6 +197,8 @@ def test_every_form_for_few_tokens_is_tested():
     assert few >= {(4, 4), (8, 8), (16, 8), (16, 5), (16, 3), (16, 1)}
     assert {p["splits"] > 1 for p in plans if p["waves"] == 8} == {p["splits"] > 1 for p in plans if p["waves"] == 16} == {True, False}
     assert {p["tile_tokens"] for p in plans if not p["waves"]} == {64, 128, 256}
+    # more than 16 tokens: on any weight up to 32, on small ones up to 64
+    assert any(p["waves"] and m > 32 for (m, _, _), p in zip(FORWARD, plans)) and not launch_plan(False, 33, 8192, 4096)["waves"]
 
 
 @pytest.mark.gpu

@@ -114,7 +114,7 @@ def test_rope_empty():
 
 # ---- 4-bit linears -------------------------------------------------------------------------------
 
-def lin(back=0, x=P, dt=0, ldx=64, w=P, meta=P, group=32, sdt=0, bias=None, bdt=0, y=P, ydt=0, ldy=64, m=40, n=64, k=64, copy=0, work=None,
+def lin(back=0, x=P, dt=0, ldx=64, w=P, meta=P, group=32, sdt=0, bias=None, bdt=0, y=P, ydt=0, ldy=64, m=100, n=64, k=64, copy=0, work=None,
         wb=0):
     return _lib.lib().dk_int4_linear(back, x, dt, ldx, w, meta, group, sdt, bias, bdt, y, ydt, ldy, m, n, k, copy, work, wb, None)
 
@@ -140,7 +140,8 @@ def test_linear_workspace_and_empty():
     L = _lib.lib()
     assert L.dk_int4_linear_workspace(0, 0, -1, 8, 8) == -1 and L.dk_int4_linear_workspace(0, 0, 5, 8, 0) == -1
     assert L.dk_int4_linear_workspace(0, 0, 0, 8, 8) == 0 and L.dk_int4_linear_workspace(0, 0, 5, 64, 64) == 0
-    assert L.dk_int4_linear_workspace(0, 1, 5, 64, 63) == 5 * 64 * 2 and L.dk_int4_linear_workspace(1, 1, 5, 65, 64) == 5 * 72 * 2
+    assert L.dk_int4_linear_workspace(0, 1, 100, 64, 63) == 100 * 64 * 2 and L.dk_int4_linear_workspace(1, 1, 5, 65, 64) == 5 * 72 * 2
+    assert L.dk_int4_linear_workspace(0, 1, 5, 64, 63) == 0  # few tokens are read as they are
     plan = (ctypes.c_int32 * 4)()
     assert L.dk_int4_linear_plan(0, 16, 64, 18944, plan) == 0 and plan[3] > 1
     need = L.dk_int4_linear_workspace(0, 0, 16, 64, 18944)
