@@ -7,10 +7,14 @@
 // Angles are kept in turns as 64-bit fixed-point fractions (turn_fraction), so that whole turns drop out exactly: at
 // position 2^20 within 2^-33 radians, where an fp32 product of position and frequency would be off by 2^-5.
 // A work-group takes a few tokens, forms each of their R / 2 cosines and sines once, in LDS, and turns all heads with
-// them; a thread has one to four items in flight. An item is 16 elements, two 16-byte loads (halves with R and D
+// them; a thread has one or two items in flight. An item is 16 elements, two 16-byte loads (halves with R and D
 // multiples of 16: both elements of eight pairs), or eight: with pairs whole, with halves of any even R and their
 // partners loaded beside them (lines that the work-group reads anyway). Sizes of D that are no multiple of eight go
 // pair by pair.
+//
+// Bound: HBM (q and k in and out): 8192 tokens of 28 + 4 heads of 128, bf16, 26.7 us either way with q and k from memory
+// (5.0 TB/s; a large copy reaches 5.2). Three sequences of 683 tokens, 9 + 3 heads of 80, a quarter turned, 7.4 us and 16
+// single tokens 3.7: a launch and two memory round trips.
 #include "elem.h"
 
 namespace dk {
@@ -182,7 +186,7 @@ static void launch_items(const ScaledRopeArgs& a, bool many, hipStream_t s) {
     const dim3 grid((a.rows + a.tpw - 1) / a.tpw), threads(kScaledThreads);
     const size_t lds = (size_t)a.tpw * (a.r / 2) * sizeof(float2_t);
     if (many)
-        hipLaunchKernelGGL((scaled_rope_kernel<DT, MODE, 4>), grid, threads, lds, s, a);
+        hipLaunchKernelGGL((scaled_rope_kernel<DT, MODE, 2>), grid, threads, lds, s, a);
     else
         hipLaunchKernelGGL((scaled_rope_kernel<DT, MODE, 1>), grid, threads, lds, s, a);
 }
@@ -202,15 +206,16 @@ hipError_t launch_scaled_rope(ScaledRopeArgs a, int dtype, hipStream_t s) {
                      : a.pairs                                   ? PAIRS8
                      : a.d % 16 == 0 && a.r % 16 == 0 && a.r > 0 ? HALF16
                                                                  : HALF8;
-    // Tokens a work-group: about four items a thread where the tokens are enough for two work-groups a CU, else one
-    // token, so that few tokens spread over the CUs; at most 32 KB of tables.
+    // Tokens a work-group: about two items a thread where the tokens are enough for two work-groups a CU, else one
+    // token, so that few tokens spread over the CUs; at most 32 KB of tables. (8192 tokens of 28 + 4 heads of 128, bf16: 26.7
+    // us; four items a thread 30.9, of which two in flight at a time 28.5, eight items 30.8.)
     const int64_t items = (int64_t)(a.hq + a.hk) * items_a_head(mode, a.d, a.r);
     const int64_t table = (int64_t)(a.r > 0 ? a.r / 2 : 1) * (int64_t)sizeof(float2_t);
-    int64_t tpw = 4 * kScaledThreads / items;
+    int64_t tpw = 2 * kScaledThreads / items;
     tpw = tpw < 1 ? 1 : tpw > 16 ? 16 : tpw;
     while (tpw > 1 && (a.rows < 512 * tpw || tpw * table > 32768)) tpw /= 2;
     a.tpw = (int32_t)tpw;
-    const bool many = tpw * items > 2 * kScaledThreads;
+    const bool many = tpw * items > kScaledThreads;
     if (dtype == DK_FP16)
         launch_mode<DK_FP16>(a, mode, many, s);
     else
