@@ -311,6 +311,11 @@ def axes_rope(q, k, positions, inv_freq, sections, n_heads, n_kv_heads, interlea
 
 
 LAYOUTS = ("half", "pairs")
+# kinds of scaled_frequencies and the keys that each uses
+_SCALINGS = {"default": (), "linear": ("factor",), "ntk": ("factor",), "dynamic": ("factor",),
+             "yarn": ("factor", "beta_fast", "beta_slow", "attention_factor"),
+             "llama3": ("factor", "low_freq_factor", "high_freq_factor"),
+             "longrope": ("factor", "short_factor", "long_factor", "attention_factor")}
 
 
 def scaled_frequencies(rotary_dim, base=10000.0, scaling=None, length=None, device=None):
@@ -328,13 +333,20 @@ def scaled_frequencies(rotary_dim, base=10000.0, scaling=None, length=None, devi
                the number of turns
       longrope short_factor, long_factor (a divisor a frequency; the second where `length` is longer than the original),
                original_max_position_embeddings, and factor or attention_factor (sqrt(1 + ln factor / ln original))
-    Computed in 64 bits and rounded once."""
+    Computed in 64 bits and rounded once. A key that its kind does not use is refused: it would change the result
+    elsewhere (original_max_position_embeddings and None values may always be there)."""
     what = "scaled_frequencies"
     r = int(rotary_dim)
     if r < 2 or r % 2:
         raise ValueError(f"{what}: rotary_dim must be even and positive")
     s = dict(scaling or {})
     kind = s.get("rope_type", s.get("type", "default"))
+    if kind not in _SCALINGS:
+        raise ValueError(f"{what}: unknown kind of scaling {kind!r}")
+    unused = sorted(key for key in s if s[key] is not None
+                    and key not in ("rope_type", "type", "original_max_position_embeddings") + _SCALINGS[kind])
+    if unused:
+        raise ValueError(f"{what}: {kind} does not use {', '.join(unused)}")
 
     def given(name):
         if s.get(name) is None:
@@ -378,8 +390,6 @@ def scaled_frequencies(rotary_dim, base=10000.0, scaling=None, length=None, devi
         if attention is None:
             factor = given("factor")
             attention = math.sqrt(1.0 + math.log(factor) / math.log(original)) if factor > 1.0 else 1.0
-    elif kind != "default":
-        raise ValueError(f"{what}: unknown kind of scaling {kind!r}")
     return inv.to(torch.float32).to(device), float(attention)
 
 

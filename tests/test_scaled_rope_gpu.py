@@ -260,6 +260,8 @@ def test_frequency_refusals():
 
     for args, msg in (((7,), "even"), ((0,), "even"), ((8, 1e4, dict(rope_type="other")), "unknown"), ((8, 1e4, dict(rope_type="linear")), "factor"),
                       ((8, 1e4, dict(rope_type="yarn", factor=2.0)), "original"),
+                      ((8, 1e4, dict(rope_type="yarn", factor=2.0, original_max_position_embeddings=8, mscale=0.7)), "mscale"),
+                      ((8, 1e4, dict(factor=2.0)), "factor"),
                       ((8, 1e4, dict(rope_type="longrope", short_factor=[1.0], original_max_position_embeddings=8, factor=2.0)), "divisors")):
         with pytest.raises(ValueError, match=msg):
             scaled_frequencies(*args)
