@@ -2,10 +2,11 @@
 //   W[n, k] = (code[n, k] - zero[n, k / group]) scale[n, k / group]
 //   forward   y[m, n]  = sum over groups g of scale[n, g] (sum over k in g of x[m, k] (code[n, k] - zero[n, g])) + bias[n]
 //   backward  dx[m, k] = sum over n of dy[m, n] W[n, k]
-// on 16x16x32 MFMAs of the activations' type with fp32 sums. The forward's matrix operands are exact, code - zero a small
-// integer, and the scale is applied to a group's fp32 sum: nothing is rounded but the sums and the output. The
-// backward sums over rows, each with its own scale, so there W is rounded once to 16 bits, as the matrix cores take it (at
-// most half a step of the type a weight, of alternating sign along a sum).
+// on 16x16x32 MFMAs of the activations' type with fp32 sums. Few tokens: the matrix operands are exact, code - zero a
+// small integer, and the scale is applied to a group's fp32 sum: nothing is rounded but the sums and the output. Tiles, and
+// the backward, whose sum goes over rows that each have a scale of their own: W is rounded once to 16 bits, as the
+// matrix cores take it (at most half a step of the type a weight, which is what a product with a 16-bit weight has).
+// Against 64 bits at 4096 tokens of [18944] x 3584, bf16: 0.0022 of the outputs' size, of which 0.0017 their own rounding.
 //
 // Layout: tiles of 16 rows by 128 columns in 1024 bytes, a row of tiles after the other, so that a wave's load is one
 // piece of memory and a lane's 16 bytes are its operands of four MFMAs as they lie: the 16 bytes 16 q + r hold row r,

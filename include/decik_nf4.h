@@ -401,7 +401,7 @@ int dk_int8_linear_bwd(const void* dy, int dy_dtype, int64_t lddy, const int8_t*
  * [batch, heads, tokens, head_dim]; backward turns the other way, reads gradients with the same kind of strides and
  * writes packed [batch, tokens, heads * head_dim]. positions: int32 or int64, [tokens] for each batch entry,
  * pos_batch_stride apart (0: shared); angles are exact to 2^-24 turns for positions below 2^28 and frequencies up to
- * 2 pi. dtype fp16 or bf16; 1 <= head_dim <= 1024, rotary_dim even and from 0 to head_dim, 1 to 65536 heads each,
+ * 2 pi. Outputs overlap no input. dtype fp16 or bf16; 1 <= head_dim <= 1024, rotary_dim even and from 0 to head_dim, 1 to 65536 heads each,
  * batch * tokens below 2^24. */
 typedef struct {
     const void* q;
@@ -426,12 +426,14 @@ int dk_scaled_rope_bwd(const dk_scaled_rope* d, void* stream);
  * packed: tiles of 16 rows by 128 columns in 1024 bytes [ceil(n / 16), ceil(k / 128)], 16-byte aligned. Of a tile the 16
  * bytes at 16 (16 q + r) hold row r, their 32-bit word j columns 32 j + 8 q + 0 .. 7, column 2 i of these in bits 4 i,
  * 2 i + 1 in bits 16 + 4 i. meta [ceil(n / 16), ceil(k / group), 16]: a row's and group's scale (16 bits, scale_dtype
- * fp16 or bf16) and, from bit 16, the zero point, 0 to 16. Rows from n on: zeros in both; columns from k on: any code. x of x_dtype fp16 or bf16, y of it or fp32; the bias NULL or
- * of bias_dtype. Forward: exact integers times x, group sums in fp32 times the scale, one rounding. Backward, and forward from 17 tokens on: W
- * rounded once to x_dtype, sums in fp32. x's row stride: non-negative, below 2^22. Sums go in an order that depends on the sizes alone. `copy` = 1: x has rows
- * that do not start at multiples of 16 bytes or a number of columns that is no multiple of 8; where
- * more than a few tokens come it is then copied to the workspace first. workspace: dk_int4_linear_workspace(..) bytes (0: none). 0 <= m, n < 2^23, m n < 2^37,
- * m k < 2^37, 1 <= k <= 2^20. */
+ * fp16 or bf16) and, from bit 16, the zero point, 0 to 16. Rows from n on: zeros in both; columns from k on: any code.
+ * x of x_dtype fp16 or bf16, y of it or fp32; the bias NULL or of bias_dtype. Forward of up to 32 tokens (64 where
+ * n k <= 2^23): exact integers times x, group sums in fp32 times the scale, one rounding. More tokens, and backward: W
+ * rounded once to x_dtype (fp16 keeps it in steps of 2^-24 at least and up to 65504), sums in fp32. Scales are finite.
+ * Sums go in an order that depends on the sizes alone. x's row stride: non-negative, below 2^22. `copy` = 1: x has rows
+ * that do not start at multiples of 16 bytes, or a number of columns that is no multiple of 8; where more than those few
+ * tokens come it is then copied to the workspace first. workspace: dk_int4_linear_workspace(..) bytes (0: none). y overlaps
+ * no input. 0 <= m, n < 2^23, m n < 2^37, m k < 2^37, 1 <= k <= 2^20. */
 int64_t dk_int4_linear_workspace(int backward, int copy, int64_t m, int64_t n, int64_t k);
 int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, const uint32_t* meta,
                    int64_t group, int scale_dtype, const void* bias, int bias_dtype, void* y,
@@ -453,8 +455,8 @@ int dk_int4_linear_plan(int backward, int64_t m, int64_t n, int64_t k, int32_t* 
  * fp32 [width], else of gate_dtype with packed rows), dweight and dpost_weight (fp32 [width], NULL: not wanted).
  * x and dx are of x_dtype; residual, h and their gradients of stream_dtype, y and grad_y of y_dtype: each x's type
  * or DK_FP32. Outputs have packed rows; input rows may have any non-negative stride (elements) and start at any
- * element. 1 <= width <= 16384, rows < 2^31 - 65536. The gradients of the weights and of a channel's gate are
- * added in a fixed order: the same bits every run. */
+ * element; no output overlaps an input or another. 1 <= width <= 16384, rows < 2^31 - 65536. The gradients of the
+ * weights and of a channel's gate are added in a fixed order: the same bits every run. */
 #define DK_GATE_NONE 0
 #define DK_GATE_CHANNEL 1
 #define DK_GATE_TOKEN 2
