@@ -302,18 +302,22 @@ __device__ __forceinline__ void tile_of(const Int4Args& a, int& m_tile, int& n_t
     n_tile = in / rows;
 }
 
-// The activations' part of a stage: rows of 64 terms (128 bytes), and a wave's loads of a step.
+// The activations' part of a stage: rows of 64 terms (128 bytes), and a wave's loads of a step. Steps are fetched in
+// turn: `src` starts at the next one's columns, of which `left` are there (none behind the last).
 template <int C>
 struct I4Tokens {
     static constexpr int TM = 32 * C, BYTES = TM * 128, LOADS = BYTES / 1024 / kI4Waves;
-    rsrc_t src;
+    const uint16_t* from;
+    uint32_t bytes;
+    int left, wave;
     uint32_t at[LOADS];
     int col[LOADS];
-    int wave;
-    __device__ __forceinline__ void set(const Int4Args& a, int m0, int w, int lane) {
+    __device__ __forceinline__ void set(const Int4Args& a, int m0, int c0, int cols, int w, int lane) {
         const int toks = min(TM, a.m - m0);
         wave = w;
-        src = make_rsrc((const uint16_t*)a.x + (int64_t)m0 * a.ldx, (uint32_t)(((toks - 1) * a.ldx + a.x_cols) * 2));
+        from = (const uint16_t*)a.x + (int64_t)m0 * a.ldx + c0;
+        left = min(cols, a.x_cols - c0);
+        bytes = (uint32_t)(((toks - 1) * a.ldx + left) * 2);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int row = 8 * (wave * LOADS + i) + (lane >> 3);
@@ -321,12 +325,18 @@ struct I4Tokens {
             at[i] = off_if(row < toks, (row * (uint32_t)a.ldx + col[i]) * 2);
         }
     }
-    // columns c0 .. c0 + 63 (live: the step exists)
-    __device__ __forceinline__ void fetch(uint8_t* stage, const Int4Args& a, int c0, bool live) const {
+    __device__ __forceinline__ void load(uint8_t* stage, int i) const {
+        bload128_lds(make_rsrc(from, left > 0 ? bytes : 0), stage + 1024 * (wave * LOADS + i), off_if(col[i] < left, at[i]));
+    }
+    __device__ __forceinline__ void turn() {
+        from += kI4Step;
+        bytes -= 2 * kI4Step;
+        left -= kI4Step;
+    }
+    __device__ __forceinline__ void fetch(uint8_t* stage) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            bload128_lds(src, stage + 1024 * (wave * LOADS + i),
-                         off_if(live && c0 + col[i] < a.x_cols, at[i] + 2 * (uint32_t)c0));
+        for (int i = 0; i < LOADS; ++i) load(stage, i);
+        turn();
     }
 };
 
@@ -369,12 +379,12 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
     const int b0 = split * a.blocks_per_split, blocks = min(a.blocks_per_split, a.blocks - b0);
 
     I4Tokens<C> x;
-    x.set(a, m0, wave, lane);
+    x.set(a, m0, b0 * kI4Block, blocks * kI4Block, wave, lane);
     const int tiles = (min(kI4TileN, a.n - n0) + 15) / 16;
     const rsrc_t wr = make_rsrc(a.w + (int64_t)(n0 / 16) * a.kblocks * kI4Tile, (uint32_t)(tiles * a.kblocks * kI4Tile));
     const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(tiles * a.groups * 64));
     uint8_t* const weights = smem + kI4Ring * XB;
-    const auto fetch_x = [&](int h) { x.fetch(smem + (h % kI4Ring) * XB, a, b0 * kI4Block + kI4Step * h, h < 2 * blocks); };
+    const auto fetch_x = [&](int h) { x.fetch(smem + (h % kI4Ring) * XB); };
     const auto fetch_w = [&](int b) {
         uint8_t* const stage = weights + (b % kI4Ring) * WB;
         const bool live = b < blocks;
@@ -573,6 +583,20 @@ struct BackRows<DK_BF16> {
     }
 };
 
+template <int DT, int C>
+constexpr int kI4BackVector = (DT == DK_BF16 ? 80 : 72) / (2 * C);
+
+// order of a part's instructions: V vector ones behind each of M matrix ones, a load every L of them
+template <int M, int V, int L = 1 << 20>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        __builtin_amdgcn_sched_group_barrier(8, 1, 0);
+        if (i % L == 0 && L <= M) __builtin_amdgcn_sched_group_barrier(16, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(2, V, 0);
+    }
+}
+
 constexpr int kI4BackWBytes = kI4Step * 128;  // 64 rows of 256 columns
 template <int DT, int C>
 constexpr int int4_back_stage() {
@@ -596,7 +620,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     const int n_end = min(a.n, n_begin + a.blocks_per_split * kI4Block), steps = (n_end - n_begin + kI4Step - 1) / kI4Step;
 
     I4Tokens<C> x;
-    x.set(a, m0, wave, lane);
+    x.set(a, m0, n_begin, a.blocks_per_split * kI4Block, wave, lane);
     // Words of a stage: row 8 q + i of a step's half lies so that the four rows that a read takes (q = 0 .. 3) use different
     // banks: chunks swap halves of the row by bit 3 of the row, rows swap places in their pair by bit 4.
     const int w_slot = 8 * wave + (lane >> 3), w_row = w_slot ^ ((w_slot >> 4) & 1);
@@ -605,20 +629,23 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     const bool w_live = w_block < (uint32_t)a.kblocks;
     const uint32_t w_at = kI4Tile * ((w_row >> 4) * (uint32_t)a.kblocks + w_block) + 16 * (16 * (w_chunk & 3) + (w_row & 15));
     const uint32_t e_group = min(group_at(a, k0 / 32 + (threadIdx.x >> 6)), (uint32_t)a.groups - 1);
-    const auto fetch = [&](int h) {
-        const int n0 = n_begin + kI4Step * h;
-        const bool live = h < steps;
-        uint8_t* const stage = smem + (h % kI4Ring) * STAGE;
-        x.fetch(stage, a, n0, live);
-        const int tiles = live ? (min(kI4Step, n_end - n0) + 15) / 16 : 0;
-        const rsrc_t wr = make_rsrc(a.w + (int64_t)(n0 / 16) * a.kblocks * kI4Tile, (uint32_t)(tiles * a.kblocks * kI4Tile));
-        bload128_lds(wr, stage + XB + 1024 * wave, off_if(w_live, w_at));
+    // steps are fetched in turn: the next one's tiles and words of the groups, and how many rows are left for them
+    const uint8_t* w_from = a.w + (int64_t)(n_begin / 16) * a.kblocks * kI4Tile;
+    const uint32_t* m_from = a.meta + (int64_t)n_begin * a.groups;
+    int w_left = n_end - n_begin, m_left = w_left;
+    const uint32_t m_at = 64 * (q * (uint32_t)a.groups + e_group) + 4 * r;
+    const auto tiles_of = [](int rows) { return rows <= 0 ? 0 : min(4, (rows + 15) / 16); };
+    const auto fetch_w = [&](uint8_t* stage) {
+        bload128_lds(make_rsrc(w_from, (uint32_t)(tiles_of(w_left) * a.kblocks * kI4Tile)), stage + XB + 1024 * wave, off_if(w_live, w_at));
+        w_from += (int64_t)(4 * kI4Tile) * a.kblocks;
+        w_left -= kI4Step;
     };
     const auto fetch_meta = [&](int h) {
-        const int n0 = n_begin + kI4Step * h, tiles = h < steps ? (min(kI4Step, n_end - n0) + 15) / 16 : 0;
-        const rsrc_t mr = make_rsrc(a.meta + (int64_t)n0 * a.groups, (uint32_t)(tiles * a.groups * 64));
-        bload32_lds(mr, raw + (h & 3) * kI4Entries + 64 * wave, 64 * (q * (uint32_t)a.groups + e_group) + 4 * r);
+        bload32_lds(make_rsrc(m_from, (uint32_t)(tiles_of(m_left) * a.groups * 64)), raw + (h & 3) * kI4Entries + 64 * wave, m_at);
+        m_from += (int64_t)kI4Step * a.groups;
+        m_left -= kI4Step;
     };
+    const auto stage_of = [&](int h) { return smem + (h % kI4Ring) * STAGE; };
     const auto table = [&](int h) { return (meta_t*)(smem + (h % kI4Ring) * STAGE + XB + kI4BackWBytes); };
 
     float4_t acc[C][4];
@@ -684,39 +711,45 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     };
     constexpr int GROUP = I4Tokens<C>::LOADS + 2;
     fetch_meta(0);
-    fetch_meta(1);
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-        fetch_meta(i + 2 < 4 ? i + 2 : 3);
-        fetch(i);
+        fetch_meta(i + 1);
+        x.fetch(stage_of(i));
+        fetch_w(stage_of(i));
     }
     wait_vmcnt<2 * GROUP>();
     keep(0);
-    keep(1);
     lds_barrier();
     uint32_t at = 0;
     read_x(0, 0);
     read_w(0, 0);
     unpack(0);
     for (int h = 0; h < steps; ++h) {
-#pragma unroll
-        for (int part = 0; part < 4; ++part) {
-            const bool last = part == 3, turns = part & 1;  // turns: the 32 terms' last part
-            if (last) {
-                wait_vmcnt<GROUP>();  // all but the newest step's
-                lds_barrier();
-                keep(h + 2);
-                fetch_meta(h + 4);
-                fetch(h + 3);
-                at = at == 2 * STAGE ? 0 : at + STAGE;
-                read_x(at, 0);
-            } else {
-                read_x(at, part + 1);
-            }
-            if (turns) read_w(at, last ? 0 : 1);
-            multiply(part);
-            if (turns) unpack(last ? 0 : 1);
-        }
+        read_x(at, 1);
+        read_w(at, 1);
+        multiply(0);
+        keep(h + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        read_x(at, 2);
+        multiply(1);
+        unpack(1);
+        interleave<2 * C, kI4BackVector<DT, C>>();
+        __builtin_amdgcn_sched_barrier(0);
+        read_x(at, 3);
+        multiply(2);
+        wait_vmcnt<GROUP>();  // all but the newest step's
+        lds_barrier();
+        at = at == 2 * STAGE ? 0 : at + STAGE;
+        read_w(at, 0);
+        read_x(at, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(3);
+        unpack(0);
+        fetch_meta(h + 4);
+        x.fetch(stage_of(h + 3));
+        fetch_w(stage_of(h + 3));
+        interleave<2 * C, kI4BackVector<DT, C>, (2 * C > GROUP ? 2 * C / GROUP : 1)>();
+        __builtin_amdgcn_sched_barrier(0);
     }
     wait_vmcnt<0>();
 
