@@ -449,9 +449,9 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
         fetch_x(i);
-        fetch_w(i);
+        if (i < 2) fetch_w(i);
     }
-    wait_vmcnt<2 * GROUP>();
+    wait_vmcnt<2 * GROUP - WLOADS>();
     lds_barrier();
     uint32_t xs = 0, ws = 0, next_ws = 0;
     read_raw(0);
@@ -464,12 +464,12 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
                 wait_vmcnt<GROUP>();  // all but the newest step's and the newest block's
                 lds_barrier();
                 fetch_x(2 * b + (v >> 2) + 3);
-                if (v == 7) fetch_w(b + 3);
                 xs = xs == 2 * XB ? 0 : xs + XB;
                 read_x(xs, 0);
             } else {
                 read_x(xs, (v & 3) + 1);
             }
+            if (v == 0) fetch_w(b + 2);  // (its stage is free since the barrier before)
             multiply(v);
             if (v == 7) ws = next_ws;
             if (v & 1) unpack(ws, ((v >> 1) + 1) & 3);
