@@ -145,6 +145,9 @@ __device__ __forceinline__ void store_out(const Int4Args& a, int64_t at, float v
 }
 
 // ---- forward, few tokens -------------------------------------------------------------------------
+// Bound: the weight's bytes and the latency of a launch's phases. [18944] x 3584 from memory, fp16: 1 token 10.9 us (34 MB and
+// 1.2 MB of groups' words, 3.3 TB/s; the first kernel 19), 16 tokens 14.9, 32 tokens 22; [3584] x 18944 at 16 tokens, bf16,
+// 17.5 and 3.9 for the join of two splits (first 31): there the unpacking, 32 vector instructions an MFMA, weighs as much.
 // Tokens by 16 (blockIdx.z). The NW waves of a work-group are NW / a.shares tiles of 16 rows by a.shares shares of the split's
 // columns, whose sums meet in LDS; each streams its share of the weight to registers, P blocks ahead. The tokens' columns
 // of the split are kept in LDS: from the caches with each block they cost the address unit four loads for the
@@ -273,11 +276,18 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
 }
 
 // ---- tiles ---------------------------------------------------------------------------------------
-// Tiles of 32 C tokens by 256 rows of the weight (forward) or 256 columns (backward), eight waves of 16 C by 64. The sum
+// Bound: the matrix cores' and vector units' cycles and the loads' issue between them. 4096 tokens of [18944] x 3584, bf16:
+// forward 475 us (1.17 PFLOP/s, matrix cores busy 51% of all cycles; the first kernel 1479), backward 540 to 580 (1.0
+// PFLOP/s, 42%; first 1364), where a library product of the same sizes with a 16-bit weight takes 537 to 547. 830 tokens of
+// [8960] x 1536, fp16: forward 33 to 40 us (245 work-groups of 12 blocks), backward 42 and 7 for the join of six splits.
+// Tiles of 32 C tokens by 256 rows of the weight (forward) or 256 columns (backward), eight waves: with 256 tokens of 128 by
+// 64, with fewer of all tokens by 32, so that no weight is unpacked twice (kI4Across: waves along the tokens). The sum
 // goes in steps of 64 terms through a ring of three stages of LDS, filled by loads that go there directly: one wait and
 // one barrier a step, loads two steps ahead. The weight stays in 4 bits up to each wave's registers.
 // W is rounded to the activations' type here, once.
 constexpr int kI4Waves = 8, kI4TileN = 256, kI4Step = 64, kI4Ring = 3;
+template <int C>
+constexpr int kI4Across = C == 8 ? 2 : 1;
 
 // An offset in a stage that every step adds its stage's to: held as it is, or each read's would be formed again.
 __device__ __forceinline__ uint32_t held(uint32_t v) {
@@ -340,18 +350,19 @@ struct I4Tokens {
     }
 };
 
-template <int DT>
-__device__ __forceinline__ void put4(const Int4Args& a, int64_t at, float4_t v, int left) {
+// N neighbouring outputs, of which `left` are there
+template <int DT, int N>
+__device__ __forceinline__ void put(void* y, int64_t at, float __attribute__((ext_vector_type(N))) v, int left) {
     typedef typename Elem<DT>::type E;
-    typedef E vec4 __attribute__((ext_vector_type(4)));
-    typedef vec4 loose4 __attribute__((aligned(sizeof(E))));
+    typedef E vec_n __attribute__((ext_vector_type(N)));
+    typedef vec_n loose_n __attribute__((aligned(sizeof(E))));
     asm("" : "+v"(v));
-    if (left >= 4) {
-        *(loose4*)((E*)a.y + at) = __builtin_convertvector(v, vec4);
+    if (left >= N) {
+        *(loose_n*)((E*)y + at) = __builtin_convertvector(v, vec_n);
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < left) ((E*)a.y)[at + e] = (E)v[e];
+        for (int e = 0; e < N; ++e)
+            if (e < left) ((E*)y)[at + e] = (E)v[e];
     }
 }
 
@@ -360,14 +371,16 @@ constexpr int kI4WBytes = kI4TileN * 64;
 template <int C, int GJ>
 constexpr size_t int4_tile_lds() {
     constexpr size_t ring = kI4Ring * (I4Tokens<C>::BYTES + kI4WBytes + 4 / GJ * kI4TileN * 4);
-    constexpr size_t out = kI4Waves * (C < 4 ? 16 * C : 64) * 72 * 2;
+    constexpr size_t out = kI4Waves * 64 * (32 * kI4Across<C> + 8) * 2;
     return ring > out ? ring : out;
 }
 
 template <int DT, int C, int GJ>
 __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4Args a) {
     typedef typename I4<DT>::vec vec;
-    constexpr int UNITS = 4 / GJ, R = 4, XB = I4Tokens<C>::BYTES, WB = kI4WBytes + UNITS * kI4TileN * 4;
+    // a wave: F times 16 tokens by R times 16 rows
+    constexpr int WM = kI4Across<C>, F = 2 * C / WM, R = 2 * WM;
+    constexpr int UNITS = 4 / GJ, XB = I4Tokens<C>::BYTES, WB = kI4WBytes + UNITS * kI4TileN * 4;
     constexpr int METAS = UNITS == 4 ? 2 : 1, WLOADS = 2 + METAS;  // a wave's loads of a block
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -375,7 +388,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
     int mt, nt, split;
     tile_of(a, mt, nt, split);
     const int m0 = mt * 32 * C, n0 = nt * kI4TileN;
-    const int wm = (wave & 1) * 16 * C, wn = (wave >> 1) * 64;
+    const int wm = wave % WM * 16 * F, wn = wave / WM * 16 * R;
     const int b0 = split * a.blocks_per_split, blocks = min(a.blocks_per_split, a.blocks - b0);
 
     I4Tokens<C> x;
@@ -401,15 +414,15 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
         }
     };
 
-    float4_t acc[R][C];
+    float4_t acc[R][F];
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int c = 0; c < C; ++c) acc[i][c] = float4_t{};
+        for (int c = 0; c < F; ++c) acc[i][c] = float4_t{};
 
     // A step is four parts: each 32 terms by half of the tokens. Operands of a part are read in the one before, across
     // the steps too: the wait and the barrier of a step come before its last part, when all of it has been read.
-    constexpr int H = C / 2;
+    constexpr int H = F / 2;
     vec xv[2][H], wv[2][R];
     u32x4_t raw[R];
     I4Group<DT> group[R];
@@ -490,7 +503,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
             if (n >= a.n) continue;
             const float bias = a.splits == 1 && a.bias != nullptr ? load_any(a.bias, a.bias_dtype, n) : 0.0f;
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+            for (int c = 0; c < F; ++c)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int m = m0 + wm + 16 * c + 4 * q + e;
@@ -503,12 +516,12 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
         }
         return;
     }
-    // 16-bit outputs leave as pieces of 16 bytes: up to 64 tokens of the wave's 64 rows at a time through LDS
-    constexpr int PART = C < 4 ? C : 4;
+    // 16-bit outputs leave as pieces of 16 bytes: 64 tokens of the wave's rows at a time through LDS
+    constexpr int PART = 4, PITCH = 16 * R + 8, PIECES = 2 * R;  // of a token
     typedef typename Elem<DT>::type E;
-    E* const mine = (E*)smem + wave * 16 * PART * 72;
+    E* const mine = (E*)smem + wave * 16 * PART * PITCH;
 #pragma unroll
-    for (int part = 0; part < C / PART; ++part) {
+    for (int part = 0; part < F / PART; ++part) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const int n = n0 + wn + 16 * i + r;
@@ -517,15 +530,16 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
             for (int c = 0; c < PART; ++c)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    store1<DT>(mine + (16 * c + 4 * q + e) * 72 + 16 * i + r, acc[i][part * PART + c][e] + bias);
+                    store1<DT>(mine + (16 * c + 4 * q + e) * PITCH + 16 * i + r, acc[i][part * PART + c][e] + bias);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int s = 0; s < 2 * PART; ++s) {
-            const int row = 8 * s + (lane >> 3), m = m0 + wm + 16 * PART * part + row, n = n0 + wn + 8 * (lane & 7);
+        for (int s = 0; s < PIECES; ++s) {
+            const int row = 64 / PIECES * s + lane / PIECES, piece = 8 * (lane % PIECES);
+            const int m = m0 + wm + 16 * PART * part + row, n = n0 + wn + piece;
             if (m >= a.m || n >= a.n) continue;
-            const E* const from = mine + row * 72 + 8 * (lane & 7);
+            const E* const from = mine + row * PITCH + piece;
             E* const to = (E*)a.y + (int64_t)m * a.ldy + n;
             if (n + 8 <= a.n) {
                 *(typename Elem<DT>::loose*)to = *(const typename Elem<DT>::vec*)from;
@@ -541,9 +555,9 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
 }
 
 // ---- backward ------------------------------------------------------------------------------------
-// The weight's layout is the forward's. Lanes r and r + 8 of an MFMA operand hold columns j and j + 4 of the
-// same word (j = 0 .. 3: four MFMAs), each of its eight rows' words; the bytes with those columns of two rows' words, joined in
-// one register, unpack to pairs along the rows. Rows' scales and zero points go through tables of 64 rows by the tile's eight units
+// The weight's layout is the forward's. Lanes of an MFMA operand that share a word hold different columns of it, each of
+// its eight rows' words: with 64 columns a wave lanes r and r + 8 four each (as many MFMAs), with 32 lanes 4 q' to 4 q' + 3
+// two. The bytes with those columns of two rows' words, joined in one register, unpack to pairs along the rows. Rows' scales and zero points go through tables of 64 rows by the tile's eight units
 // of 32 columns: their words come a step before the step's other loads, and the threads (an entry each) make the tables
 // of the next step.
 constexpr int kI4BackUnits = 8, kI4Entries = kI4BackUnits * kI4Step;
@@ -584,9 +598,12 @@ struct BackRows<DK_BF16> {
 };
 
 template <int DT, int C>
-constexpr int kI4BackVector = (DT == DK_BF16 ? 80 : 72) / (2 * C);
+constexpr int kI4BackVector = (C == 8 ? (DT == DK_BF16 ? 80 : 72) : (DT == DK_BF16 ? 48 : 40)) / (2 * C);
 
-// order of a part's instructions: V vector ones behind each of M matrix ones, a load every L of them
+// Order of a part's instructions: V vector ones behind each of M matrix ones, a load every L of them. Issued at once, the
+// loads of eight waves and the arithmetic of their addresses hold up the matrix instructions behind them: 4096 tokens of
+// [18944] x 3584, bf16, 641 us that way, 542 spread. (The forward has no registers left for it: ordered so it spills, 570
+// us for 485.)
 template <int M, int V, int L = 1 << 20>
 __device__ __forceinline__ void interleave() {
 #pragma unroll
@@ -607,6 +624,8 @@ template <int DT, int C>
 __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4Args a) {
     typedef typename I4<DT>::vec vec;
     typedef typename BackRows<DT>::elem meta_t;
+    // a wave: F times 16 tokens by J times 16 columns
+    constexpr int WM = kI4Across<C>, F = 2 * C / WM, J = 2 * WM;
     constexpr int XB = I4Tokens<C>::BYTES, STAGE = int4_back_stage<DT, C>();
     extern __shared__ __attribute__((aligned(32))) uint8_t smem[];
     uint32_t* const raw = (uint32_t*)(smem + kI4Ring * STAGE);  // four steps' words of the groups
@@ -615,7 +634,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     int mt, kt, split;
     tile_of(a, mt, kt, split);
     const int m0 = mt * 32 * C, k0 = kt * 256;
-    const int wm = (wave & 1) * 16 * C, wk = wave >> 1;  // the wave's 64 columns: half wk & 1 of block wk >> 1
+    const int wm = wave % WM * 16 * F, wk = wave / WM;  // the wave's columns: 16 J wk and on
     const int n_begin = split * a.blocks_per_split * kI4Block;
     const int n_end = min(a.n, n_begin + a.blocks_per_split * kI4Block), steps = (n_end - n_begin + kI4Step - 1) / kI4Step;
 
@@ -648,20 +667,20 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     const auto stage_of = [&](int h) { return smem + (h % kI4Ring) * STAGE; };
     const auto table = [&](int h) { return (meta_t*)(smem + (h % kI4Ring) * STAGE + XB + kI4BackWBytes); };
 
-    float4_t acc[C][4];
+    float4_t acc[F][J];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < F; ++c)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[c][j] = float4_t{};
+        for (int j = 0; j < J; ++j) acc[c][j] = float4_t{};
 
-    // this lane's word of a row: word 4 q' + j' of its block with j' = 2 (wk & 1) + (r & 1), q' = (r >> 1) & 3
-    const int unit = 4 * (wk >> 1) + 2 * (wk & 1) + (r & 1), chunk = 4 * (wk >> 1) + ((r >> 1) & 3);
-    const int word = 2 * (wk & 1) + (r & 1);
-    // its bytes: of each half of two rows' words, the one that holds its four columns
-    const uint32_t pick = r < 8 ? 0x06040200u : 0x07050301u;
+    // This lane's word of a row is word `word` of chunk 4 (unit / 4) + qw, its columns 8 qw + own and on of the unit. Its
+    // bytes: of each half of two rows' words, the one that holds its columns, of which two begin at bit `low`.
+    const int unit = WM == 2 ? 2 * wk + (r & 1) : wk, qw = WM == 2 ? (r >> 1) & 3 : r >> 2, word = unit & 3;
+    const int chunk = 4 * (unit >> 2) + qw, own = WM == 2 ? 4 * (r >> 3) : 2 * (r & 3), low = 4 * (r & 1);
+    const uint32_t pick = own < 4 ? 0x06040200u : 0x07050301u;
     // the parts of a step as in the forward
-    constexpr int H = C / 2;
-    vec xv[2][H], wv[2][4];
+    constexpr int H = F / 2;
+    vec xv[2][H], wv[2][J];
     uint32_t d[8];
     BackRows<DT> rows;
     const uint32_t x_off[2] = {held((wm + r) * 128 + 16 * (q ^ chunk_key(r))), held((wm + r) * 128 + 16 * ((4 + q) ^ chunk_key(r)))};
@@ -684,22 +703,25 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
         rows.zero = *(const decltype(rows.zero)*)(t + kI4Table * sizeof(meta_t));
     };
     const auto unpack = [&](int s) {
-        uint32_t w[4][4];
+        uint32_t w[J][4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             // nibbles of row 2 p: columns 0 2 1 3, then of row 2 p + 1
-            const uint32_t v = __builtin_amdgcn_perm(d[2 * p + 1], d[2 * p], pick);
+            uint32_t v = __builtin_amdgcn_perm(d[2 * p + 1], d[2 * p], pick);
+            if constexpr (WM == 1) v >>= low;
             w[0][p] = rows.pair(and_or(v, 0x000F000Fu, 0x64006400u), p);
             w[1][p] = rows.pair(and_or(v >> 8, 0x000F000Fu, 0x64006400u), p);
-            w[2][p] = rows.pair(and_or(v >> 4, 0x000F000Fu, 0x64006400u), p);
-            w[3][p] = rows.pair(and_or(v >> 12, 0x000F000Fu, 0x64006400u), p);
+            if constexpr (WM == 2) {
+                w[2][p] = rows.pair(and_or(v >> 4, 0x000F000Fu, 0x64006400u), p);
+                w[3][p] = rows.pair(and_or(v >> 12, 0x000F000Fu, 0x64006400u), p);
+            }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) wv[s][j] = __builtin_bit_cast(vec, u32x4_t{w[j][0], w[j][1], w[j][2], w[j][3]});
+        for (int j = 0; j < J; ++j) wv[s][j] = __builtin_bit_cast(vec, u32x4_t{w[j][0], w[j][1], w[j][2], w[j][3]});
     };
     const auto multiply = [&](int part) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int c = 0; c < H; ++c) {
                 float4_t& t = acc[H * (part & 1) + c][j];
@@ -753,25 +775,25 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     }
     wait_vmcnt<0>();
 
-    // lane: tokens wm + 16 c + 4 q + e, four columns
-    const int k = k0 + 128 * (wk >> 1) + 32 * word + 8 * ((r >> 1) & 3) + 4 * (r >> 3), left = a.k - k;
+    // lane: tokens wm + 16 c + 4 q + e, J columns
+    typedef float out_t __attribute__((ext_vector_type(J)));
+    const int k = k0 + 32 * unit + 8 * qw + own, left = a.k - k;
     if (left <= 0) return;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < F; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int m = m0 + wm + 16 * c + 4 * q + e;
             if (m >= a.m) continue;
-            const float4_t v = float4_t{acc[c][0][e], acc[c][1][e], acc[c][2][e], acc[c][3][e]};
-            if (a.splits > 1) {
-                Int4Args p = a;
-                p.y = a.partials;
-                put4<DK_FP32>(p, split * a.slab + (int64_t)m * a.k + k, v, left);
-            } else if (a.y_dtype == DK_FP32) {
-                put4<DK_FP32>(a, (int64_t)m * a.ldy + k, v, left);
-            } else {
-                put4<DT>(a, (int64_t)m * a.ldy + k, v, left);
-            }
+            out_t v;
+#pragma unroll
+            for (int j = 0; j < J; ++j) v[j] = acc[c][j][e];
+            if (a.splits > 1)
+                put<DK_FP32, J>(a.partials, split * a.slab + (int64_t)m * a.k + k, v, left);
+            else if (a.y_dtype == DK_FP32)
+                put<DK_FP32, J>(a.y, (int64_t)m * a.ldy + k, v, left);
+            else
+                put<DT, J>(a.y, (int64_t)m * a.ldy + k, v, left);
         }
 }
 
@@ -812,11 +834,11 @@ __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a, int co
         v = v + bias;
         const int64_t at = m * a.ldy + n;
         if (a.y_dtype == DK_FP32)
-            put4<DK_FP32>(a, at, v, left);
+            put<DK_FP32, 4>(a.y, at, v, left);
         else if (a.y_dtype == DK_BF16)
-            put4<DK_BF16>(a, at, v, left);
+            put<DK_BF16, 4>(a.y, at, v, left);
         else
-            put4<DK_FP16>(a, at, v, left);
+            put<DK_FP16, 4>(a.y, at, v, left);
     }
 }
 
