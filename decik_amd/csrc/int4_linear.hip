@@ -897,12 +897,12 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
         p.partial_bytes = p.splits > 1 ? (int64_t)p.splits * m * n * 4 : 0;
         return p;
     }
-    // Tokens a tile (256, 128 or 64) and splits of the sum: the least estimate of the time. A round of the
-    // CUs takes the times below a block of 128 terms (measured at 4096 and 830 tokens, fp16; tiles of 64 tokens run two
-    // work-groups a CU), a split's partial sums go to memory and back at about 5 TB/s, their join takes a launch.
-    // Measured against the choice: [830, 8960] x 1536 forward 36 us (256 tokens 46, 64 tokens 45), backward 49 in six
-    // splits of 128 tokens (8 of 256: 53, 3 of 64: 71); [512, 4096] x 4096 forward 41 in four splits of 128 (two of 64: 45,
-    // eight of 256: 47).
+    // Tokens a tile (256, 128 or 64) and splits of the sum: the least estimate of the time. A round of the CUs takes the times
+    // below for a block of 128 terms and for its start and end (tiles of 64 tokens run two work-groups a CU, one alone
+    // takes less), a split's partial sums go to memory and back, their join takes a launch. Fitted to 1300 timed plans of 70
+    // products (fp16, 64 to 4096 tokens, weights from [512] x 3584 to [18944] x 3584): estimates are off by 6%, the chosen
+    // plan by 0.4% of the best one's time at the mean and 5% at most. Measured against the choice: [830, 8960] x 1536
+    // forward 29 us (tiles of 64 tokens 33, of 256 45), backward 42 in six splits of 128 (10 of 256: 47, 6 of 64: 48).
     // (Tuning hook, read on every call: DECIK_INT4_PLAN = "tokens,splits" forces a plan.)
     const int64_t cols = backward ? k : n, steps = backward ? (n + kI4Block - 1) / kI4Block : blocks;
     p.n_tiles = (int)((cols + kI4TileN - 1) / kI4TileN);
@@ -919,14 +919,20 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
             if (forced_tokens != 0) want = forced_splits;
             if (want > 1 && (want > steps / 2 || tiles * want > 1024) && forced_tokens == 0) break;
             const int64_t per = (steps + want - 1) / want, splits = (steps + per - 1) / per, groups = tiles * splits;
-            double block = 0.0;  // us of a block of 128 terms, over all rounds
+            // us of a block, of a round's start and end
+            struct Time {
+                double block, ends;
+            };
+            const Time of256 = backward ? Time{2.94, 7.3} : Time{2.74, 4.6}, of128 = backward ? Time{1.88, 4.1} : Time{1.53, 3.5};
+            const Time of64 = backward ? Time{2.40, 4.1} : Time{1.85, 2.1}, alone64 = backward ? Time{1.40, 4.1} : Time{1.10, 2.1};
+            const auto round = [&](Time t) { return t.block * (double)per + t.ends; };
+            double cost = splits > 1 ? 3.8 + (double)(splits * m * cols) * 8 / (backward ? 8.4e6 : 6.1e6) : 0.0;
             if (tokens > 64) {
-                block = (double)((groups + 255) / 256) * (tokens == 256 ? 3.7 : 2.7);
+                cost += (double)((groups + 255) / 256) * round(tokens == 256 ? of256 : of128);
             } else {
                 const int64_t rest = groups % 512;
-                block = (double)(groups / 512) * 3.3 + (rest == 0 ? 0.0 : rest <= 256 ? 2.2 : 3.3);
+                cost += (double)(groups / 512) * round(of64) + (rest == 0 ? 0.0 : round(rest <= 256 ? alone64 : of64));
             }
-            const double cost = block * (double)per + (splits > 1 ? 4.0 + (double)(splits * m * cols) * 8 / 5e6 : 0.0);
             if (best == 0.0 || cost < best) {
                 best = cost;
                 p.tokens = tokens;
