@@ -7,8 +7,11 @@ Python API (the `solution` package name is kept as an alias, see solution/__init
 - lora.py    LoRA r=16 with the A.B term fused into the GEMM epilogues; q/k/v in one launch
 - swiglu.py  SwiGLU forward/backward kernels
 - dropout.py dropout from a counter-based generator, masks never stored
-- rope.py    q/k RoPE; RMS norms of q and k heads with the rotation; positions with several axes
+- rope.py    q/k RoPE; RMS norms of q and k heads with the rotation; positions with several axes; part of
+             each head turned, in halves or pairs, by frequencies stretched for long contexts
+- norm.py    the residual stream between two blocks: norm, gate, scaled residual and the next norm in one pass
 - int8.py    linears in 8-bit integers with scales per token and channel
+- int4.py    linears in 4-bit integers with a scale and a zero point a group
 - quant.py   bitsandbytes-layout NF4 quantizer and QuantState stand-in (no bitsandbytes needed)
 
 apply() installs the patches the reference installs for this path (solution/__init__.py:30-51):

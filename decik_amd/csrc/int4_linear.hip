@@ -277,9 +277,11 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
 
 // ---- tiles ---------------------------------------------------------------------------------------
 // Bound: the matrix cores' and vector units' cycles and the loads' issue between them. 4096 tokens of [18944] x 3584, bf16:
-// forward 475 us (1.17 PFLOP/s, matrix cores busy 51% of all cycles; the first kernel 1479), backward 540 to 580 (1.0
-// PFLOP/s, 42%; first 1364), where a library product of the same sizes with a 16-bit weight takes 537 to 547. 830 tokens of
-// [8960] x 1536, fp16: forward 33 to 40 us (245 work-groups of 12 blocks), backward 42 and 7 for the join of six splits.
+// forward 475 to 510 us (1.1 to 1.17 PFLOP/s, matrix cores busy 51% of all cycles; the first kernel 1479), backward 540 to
+// 595 (1.0 PFLOP/s, 42%; first 1364), where a library product of the same sizes with a 16-bit weight takes 537 to 547. 830
+// tokens of [8960] x 1536, fp16: forward 28 to 34 us (245 work-groups of 12 blocks; such a library product 29), backward 41
+// with the join of six splits (45), 40 + 7 from memory. Waves of 64 by 64 in the smaller tiles, as in the largest, unpack
+// each weight twice: 34 and 43.5 us.
 // Tiles of 32 C tokens by 256 rows of the weight (forward) or 256 columns (backward), eight waves: with 256 tokens of 128 by
 // 64, with fewer of all tokens by 32, so that no weight is unpacked twice (kI4Across: waves along the tokens). The sum
 // goes in steps of 64 terms through a ring of three stages of LDS, filled by loads that go there directly: one wait and

@@ -16,6 +16,13 @@
 // to one of two LDS slots in turn, and a slot is written again only after the other's barrier. The sums of
 // the weights' gradients leave as a slab a work-group, added in work-group order by a second launch: no atomics, the
 // same bits every run.
+//
+// Bound: HBM at many rows. 8192 x 3584, bf16, both norms and a channel's gate: forward 40.7 us (235 MB, 5.8 TB/s; a large
+// copy reaches 5.2), backward 73 (352 MB, 4.8 TB/s) and 4.7 for the join of the slabs; first forms 49 and 119. What took them
+// there: waits by count past the stores (every load and store unconditional), weights held in registers, FULL without the
+// optional parts' tests, DPP sums and one barrier a reduction, float8 arithmetic without conversions in between.
+// Against it: two passes of 256 threads 45.0 and 75.9; twice as many work-groups in the backward 74.9 and 8.4 for the
+// join. 830 x 1536, fp16 with an fp32 stream, 6 + 9 + 5 us, 16 rows of 3584 3.7: launches and memory round trips.
 #include "elem.h"
 
 namespace dk {
