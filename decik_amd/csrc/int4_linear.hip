@@ -869,9 +869,11 @@ __global__ __launch_bounds__(256) void int4_rows_kernel(const uint16_t* __restri
 Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
     Int4Plan p{};
     const int64_t blocks = (k + kI4Block - 1) / kI4Block;
-    // Tokens by 16 with the weight streamed to registers for each: up to 32 (18944 x 3584: 30 us, as the tiles), up to 64
-    // on small weights, whose tiles are all start and end ([2057] x 1121 at 37 tokens: 12.8 us and 3.9 for the join).
-    const bool small = n * ((k + 7) / 8 * 8) <= (int64_t(1) << 23);
+    // Tokens by 16 with the weight streamed to registers for each: up to 32, up to 64 on weights whose tiles are mostly start
+    // and end. us, streamed and by the best tiles, fp16 / bf16: [18944] x 3584 at 32 tokens 19.8 and 20.7 / 26.1 and 21.2,
+    // [3584] x 18944 18.6 and 22.1 / 23.1 and 22.4; at 64 [4096] x 4096 9.6 and 16.7 / 11.5 and 17.1, [8960] x 1536 12.2 and
+    // 15.3 / 15.2 and 15.5, [5120] x 5120, past the bound, 18.3 and 18.7 / 22.8 and 19.5.
+    const bool small = n * ((k + 7) / 8 * 8) <= (int64_t(1) << 24);
     if (!backward && std::getenv("DECIK_INT4_PLAN") == nullptr && m <= (small ? kInt4FewSmallM : kInt4FewM)) {
         p.few = true;
         p.tokens = 16;
@@ -879,7 +881,8 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
         const int toks = m < 16 ? (int)m : 16;
         p.n_tiles = (int)((n + 15) / 16);
         // Splits where the tokens' columns do not fit the LDS. Where they take much of it and there are more row tiles than CUs,
-        // work-groups of 16 waves with as many tiles as one round of the CUs needs; else one tile a work-group, four or eight
+        // work-groups of 16 waves with as many tiles as one round of the CUs needs (over all tokens and splits: [4096] x 4096
+        // at 48 tokens 16.0 us with three tiles, a round and two work-groups, 9.4 with four); else one tile a work-group, four or eight
         // waves sharing its columns. us, in turn with four waves, eight, sixteen sharing and the choice: [18944] x 3584 at
         // 1 token 11.1, 11.0, 13.6, 11.0; at 16 30.4, 24.7, 26.4, 14.1; [8960] x 1536 at 1 token 4.8, 5.2, 6.9, 4.8; at 16 6.3,
         // 6.7, 8.3, 5.6; [4096] x 4096 at 4 tokens 5.9, 5.3, 5.3, 5.3.
@@ -888,9 +891,10 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
         const int x_bytes = few_x_bytes(toks, (int)((blocks + p.splits - 1) / p.splits));
         const int64_t groups = (int64_t)p.n_tiles * p.splits * p.m_tiles;
         if (x_bytes > 32768 && groups > 256) {
-            const int64_t tiles = (groups + 255) / 256;
+            int tiles = 2;
+            while (tiles < 16 && (p.n_tiles + tiles - 1) / tiles * (int64_t)(p.splits * p.m_tiles) > 256) ++tiles;
             p.waves = 16;
-            p.shares = tiles < 16 ? 16 / (int)tiles : 1;
+            p.shares = 16 / tiles;
         } else {
             p.waves = p.shares = p.n_tiles >= 512 && blocks <= 16 ? 4 : 8;
         }

@@ -3,7 +3,7 @@
 A frozen weight [N, K] is held as codes 0 .. 15 with a scale (fp16 or bf16) and, where asked, a zero point for every `group`
 columns of a row, about a quarter of fp16's bytes; zero points are 8 where none are given:
   W[n, k] = (code[n, k] - zero[n, k // group]) * scale[n, k // group]
-  forward:  y = x . W^T + bias. Up to 32 tokens (64 on small weights) stream the weight to registers: the integers times
+  forward:  y = x . W^T + bias. Up to 32 tokens (64 on weights of up to 2^24) stream the weight to registers: the integers times
             x exactly, each group's sum in fp32 times its scale, rounded once. More go by tiles, with W rounded once to x's
             type (at most half a step of it a weight; fp16 keeps W in steps of 2^-24 at least) and sums in fp32
   backward: dX = dY . W by tiles, W rounded once to dY's type, sums in fp32
