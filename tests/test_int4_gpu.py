@@ -152,7 +152,8 @@ def test_refusals_of_weights():
 FORWARD = [(1, 1, 1), (1, 17, 128), (2, 100, 129), (15, 333, 1121), (16, 48, 4096), (16, 48, 8961), (1, 8200, 2100), (3, 16500, 640), (1, 8200, 30),
            (16, 4200, 1100), (9, 8209, 2100), (16, 18944, 1121), (16, 70000, 1030), (16, 40, 18944), (13, 3600, 9728), (7, 257, 70000),
            (17, 40, 640), (31, 257, 5000), (32, 3000, 2049), (29, 4200, 9000), (33, 70, 512), (64, 300, 4100), (40, 3000, 4100), (65, 256, 128), (65, 3, 130), (128, 255, 1000),
-           (129, 257, 4096), (300, 700, 1121), (830, 1536, 1536), (257, 1000, 31), (2000, 3000, 1121), (600, 20000, 300)]
+           (129, 257, 4096), (300, 700, 1121), (830, 1536, 1536), (257, 1000, 31), (2000, 3000, 1121), (600, 20000, 300),
+           (48, 4100, 3000), (33, 5000, 3301), (64, 8190, 1540), (64, 1500, 9000), (64, 4200, 4100)]
 BACKWARD = [(1, 1, 1), (1, 128, 17), (2, 129, 300), (16, 1121, 333), (32, 640, 256), (33, 1000, 257), (64, 4096, 128), (65, 31, 600), (128, 2057, 1121),
             (129, 300, 513), (300, 1121, 700), (830, 1536, 1536), (37, 2057, 1121), (50, 200, 600)]
 
