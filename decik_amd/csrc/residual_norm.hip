@@ -361,12 +361,20 @@ static int norm_threads(int width) {
     return ((width + per - 1) / per + kWave - 1) / kWave * kWave;
 }
 
-// Work-groups: as many as the CUs hold at once, each with several rows where there are many.
+// Work-groups: as many as the CUs hold at once, each with several rows where there are many. In the backward each leaves a
+// slab, which costs as much as a third of a row to four fifths: up to four rows a work-group once there are enough for
+// the CUs. (us of the backward and its join at one, two, three, four rows: 830 x 1536 fp16 with an fp32 stream 15.1, 12.7, 12.6,
+// 13.4; 512 x 3584 13.0, 11.0, 11.4, 11.0; 2048 x 1536 23.1, 21.2, 21.6, 20.1; 128 x 3584 9.6, 10.7, 11.8, 13.1; and
+// 1024 x 8192, of which a CU holds one work-group, 39.5 with two a CU, 31.4 with one.)
 int residual_norm_groups(int64_t rows, int width, bool backward) {
     const int waves = norm_threads(width) / kWave;
-    const int64_t per_cu = backward ? (waves > 8 ? 1 : 16 / waves) : (24 + waves - 1) / waves;
-    const int64_t want = per_cu * 256;
-    return (int)(rows < want ? rows : want);
+    if (!backward) {
+        const int64_t want = (24 + waves - 1) / waves * 256;
+        return (int)(rows < want ? rows : want);
+    }
+    const int64_t want = (norm_passes(width) > 1 ? 1 : 16 / waves) * 256, each = (rows + 191) / 256;
+    const int64_t few = each <= 1 ? rows : (rows + (each < 4 ? each : 4) - 1) / (each < 4 ? each : 4);
+    return (int)(few < want ? few : want);
 }
 
 template <int XT, int ST, int YT, int V, int MODE, bool BWD>
