@@ -22,7 +22,8 @@
 // there: waits by count past the stores (every load and store unconditional), weights held in registers, FULL without the
 // optional parts' tests, DPP sums and one barrier a reduction, float8 arithmetic without conversions in between.
 // Against it: two passes of 256 threads 45.0 and 75.9; twice as many work-groups in the backward 74.9 and 8.4 for the
-// join. 830 x 1536, fp16 with an fp32 stream, 6 + 9 + 5 us, 16 rows of 3584 3.7: launches and memory round trips.
+// join. 830 x 1536, fp16 with an fp32 stream, 6 + 10 + 4 us, 16 rows of 3584 3.7: launches and memory round trips. Rows past
+// 8192 columns are read without the next one in flight: 2048 x 16384 back 189 us, 2.4 times its bytes' time.
 #include "elem.h"
 
 namespace dk {
@@ -364,7 +365,8 @@ static int norm_threads(int width) {
 // Work-groups: as many as the CUs hold at once, each with several rows where there are many. In the backward each leaves a
 // slab, which costs as much as a third of a row to four fifths: up to four rows a work-group once there are enough for
 // the CUs. (us of the backward and its join at one, two, three, four rows: 830 x 1536 fp16 with an fp32 stream 15.1, 12.7, 12.6,
-// 13.4; 512 x 3584 13.0, 11.0, 11.4, 11.0; 2048 x 1536 23.1, 21.2, 21.6, 20.1; 128 x 3584 9.6, 10.7, 11.8, 13.1; and
+// 13.4; 512 x 3584 13.0, 11.0, 11.4, 11.0; 2048 x 1536 23.1, 21.2, 21.6, 20.1; 128 x 3584 9.6, 10.7, 11.8, 13.1; 333 x 1121
+// from memory 12.4, 13.5; and
 // 1024 x 8192, of which a CU holds one work-group, 39.5 with two a CU, 31.4 with one.)
 int residual_norm_groups(int64_t rows, int width, bool backward) {
     const int waves = norm_threads(width) / kWave;
@@ -372,7 +374,7 @@ int residual_norm_groups(int64_t rows, int width, bool backward) {
         const int64_t want = (24 + waves - 1) / waves * 256;
         return (int)(rows < want ? rows : want);
     }
-    const int64_t want = (norm_passes(width) > 1 ? 1 : 16 / waves) * 256, each = (rows + 191) / 256;
+    const int64_t want = (norm_passes(width) > 1 ? 1 : 16 / waves) * 256, each = (rows + 127) / 256;
     const int64_t few = each <= 1 ? rows : (rows + (each < 4 ? each : 4) - 1) / (each < 4 ? each : 4);
     return (int)(few < want ? few : want);
 }
