@@ -15,9 +15,11 @@
 // row r of its operand. `meta` holds groups' words, a scale (low 16 bits) and a zero point (next byte), by tile rows, groups
 // and the tile's 16 rows.
 // From pairs to operands: 0x6400 | q is 1024 + q as fp16, 0x6400 | 16 q is 1024 + 16 q. fp16: one packed subtraction or
-// multiply-add leaves q - zero, exactly, one packed product the weight. bf16: mixed multiply-adds give (1024 + q) scale -
-// (1024 + zero) scale in fp32, and one conversion a pair rounds: a scale has 11 bits at most, so both products are
-// exact and the difference is scale (q - zero) without any error (with 1 for the scale, q - zero).
+// multiply-add leaves q - zero, exactly, one packed product the weight. bf16, and fp16 with bf16 scales (rounded to fp16 before
+// the product, a scale below 2^-17 would be off by up to fifteen half steps in a weight, one past 65504 no number): mixed multiply-adds
+// give (1024 + q) scale - (1024 + zero) scale in fp32, and one conversion a pair rounds: a scale has 11 bits at most, so both
+// products are exact and the difference is scale (q - zero) without any error (with 1 for the scale, q - zero). us, fp16 with fp16
+// and with bf16 scales: 4096 tokens of [18944] x 3584 forward 460 and 480, backward 485 and 530.
 #include <cstdio>
 #include <cstdlib>
 
@@ -66,11 +68,21 @@ __device__ __forceinline__ float scale_of(uint32_t meta, int scale_dtype) {
 
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
-// Constants of a row's group, and operands of a word's columns 0 .. 7: the integers code - zero, or the weights.
+// Which weights are formed in fp32 and rounded at the end: bf16 ones, and fp16 ones with bf16 scales.
+constexpr bool i4_wide(int dt, int scale_dtype) { return dt == DK_BF16 || scale_dtype == DK_BF16; }
+
+// two weights as operands of type DT
 template <int DT>
+__device__ __forceinline__ uint32_t narrow(float a, float b) {
+    if constexpr (DT == DK_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{a, b}, bf16x2_t));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{a, b}, half2_t));
+}
+
+// Constants of a row's group, and operands of a word's columns 0 .. 7: the integers code - zero, or the weights.
+template <int DT, bool WIDE = i4_wide(DT, DT)>
 struct I4Group;
 template <>
-struct I4Group<DK_FP16> {
+struct I4Group<DK_FP16, false> {
     half2_t whole, part, scale;  // -(1024 + zero), -(64 + zero)
     __device__ __forceinline__ void set_zero(uint32_t meta) {
         const _Float16 z = (_Float16)zero_of(meta);
@@ -78,9 +90,9 @@ struct I4Group<DK_FP16> {
         whole = half2_t{a, a};
         part = half2_t{b, b};
     }
-    __device__ __forceinline__ void set(uint32_t meta, int scale_dtype) {
+    __device__ __forceinline__ void set(uint32_t meta, int) {
         set_zero(meta);
-        const _Float16 s = scale_dtype == DK_FP16 ? __builtin_bit_cast(_Float16, (uint16_t)meta) : (_Float16)I4<DK_BF16>::scale(meta);
+        const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)meta);
         scale = half2_t{s, s};
     }
     __device__ __forceinline__ half2_t even(uint32_t v) const {
@@ -98,8 +110,9 @@ struct I4Group<DK_FP16> {
         return join(even(d) * scale, odd(d) * scale, even(d >> 8) * scale, odd(d >> 8) * scale);
     }
 };
-template <>
-struct I4Group<DK_BF16> {
+template <int DT>
+struct I4Group<DT, true> {
+    typedef typename I4<DT>::vec vec;
     float whole, whole_zero, part, part_zero;  // of 1024 + code, and of 1024 + 16 code
     __device__ __forceinline__ void set_scale(uint32_t meta, float s) {
         const float z = zero_of(meta);
@@ -113,20 +126,21 @@ struct I4Group<DK_BF16> {
         asm("" : "+v"(one));  // a factor: a product by 1 is made a conversion and a sum
         set_scale(meta, one);
     }
-    __device__ __forceinline__ void set(uint32_t meta, int scale_dtype) { set_scale(meta, scale_of(meta, scale_dtype)); }
+    __device__ __forceinline__ void set(uint32_t meta, int scale_dtype) {
+        set_scale(meta, scale_of(meta, DT == DK_FP16 ? DK_BF16 : scale_dtype));
+    }
     static __device__ __forceinline__ uint32_t pair(uint32_t v, float by, float plus) {
         const half2_t h = __builtin_bit_cast(half2_t, v);
-        const float2_t f = float2_t{__builtin_fmaf((float)h[0], by, plus), __builtin_fmaf((float)h[1], by, plus)};
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
+        return narrow<DT>(__builtin_fmaf((float)h[0], by, plus), __builtin_fmaf((float)h[1], by, plus));
     }
-    __device__ __forceinline__ bf16x8_t weights(uint32_t d) const {
+    __device__ __forceinline__ vec weights(uint32_t d) const {
         const uint32_t h = d >> 8;
-        return __builtin_bit_cast(bf16x8_t, u32x4_t{pair(and_or(d, 0x000F000Fu, 0x64006400u), whole, whole_zero),
-                                                    pair(and_or(d, 0x00F000F0u, 0x64006400u), part, part_zero),
-                                                    pair(and_or(h, 0x000F000Fu, 0x64006400u), whole, whole_zero),
-                                                    pair(and_or(h, 0x00F000F0u, 0x64006400u), part, part_zero)});
+        return __builtin_bit_cast(vec, u32x4_t{pair(and_or(d, 0x000F000Fu, 0x64006400u), whole, whole_zero),
+                                               pair(and_or(d, 0x00F000F0u, 0x64006400u), part, part_zero),
+                                               pair(and_or(h, 0x000F000Fu, 0x64006400u), whole, whole_zero),
+                                               pair(and_or(h, 0x00F000F0u, 0x64006400u), part, part_zero)});
     }
-    __device__ __forceinline__ bf16x8_t integers(uint32_t d) const { return weights(d); }  // (of set_zero)
+    __device__ __forceinline__ vec integers(uint32_t d) const { return weights(d); }  // (of set_zero)
 };
 
 // group of the 32 columns that begin at 32 unit
@@ -377,7 +391,7 @@ constexpr size_t int4_tile_lds() {
     return ring > out ? ring : out;
 }
 
-template <int DT, int C, int GJ>
+template <int DT, bool WIDE, int C, int GJ>
 __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4Args a) {
     typedef typename I4<DT>::vec vec;
     // a wave: F times 16 tokens by R times 16 rows
@@ -427,7 +441,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
     constexpr int H = F / 2;
     vec xv[2][H], wv[2][R];
     u32x4_t raw[R];
-    I4Group<DT> group[R];
+    I4Group<DT, WIDE> group[R];
     const uint32_t x_off[2] = {held((wm + r) * 128 + 16 * (q ^ chunk_key(r))), held((wm + r) * 128 + 16 * ((4 + q) ^ chunk_key(r)))};
     const uint32_t w_off = held(kI4Ring * XB + wn * 64 + 16 * lane);
     const uint32_t g_off = held(kI4Ring * XB + kI4WBytes + 4 * (wn + r));
@@ -447,7 +461,11 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_tile_kernel(const Int4A
         const uint8_t* const at = smem + (g_off + ws);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            if (j % GJ == 0) group[i].set(*(const uint32_t*)(at + 4 * (kI4TileN * (j / GJ) + 16 * i)), a.scale_dtype);
+            if (j % GJ == 0) {
+                group[i].set(*(const uint32_t*)(at + 4 * (kI4TileN * (j / GJ) + 16 * i)), a.scale_dtype);
+                // (else fp16's rows are set at once, early, and 256 tokens spill)
+                if constexpr (DT == DK_FP16) __builtin_amdgcn_sched_barrier(0);
+            }
             wv[j & 1][i] = group[i].weights(raw[i][j]);
         }
     };
@@ -566,14 +584,14 @@ constexpr int kI4BackUnits = 8, kI4Entries = kI4BackUnits * kI4Step;
 // a unit's rows in a table: padded, so that the two units that a wave reads use different banks
 constexpr int kI4Unit = kI4Step + 32, kI4Table = kI4BackUnits * kI4Unit;
 
-template <int DT>
+template <int DT, bool WIDE>
 struct BackRows;  // of the eight rows of a lane
 template <>
-struct BackRows<DK_FP16> {
+struct BackRows<DK_FP16, false> {
     typedef _Float16 elem;
     half8_t scale, zero;  // -(1024 + zero)
-    static __device__ __forceinline__ void keep(elem* table, int e, uint32_t meta, int scale_dtype) {
-        table[e] = (elem)scale_of(meta, scale_dtype);
+    static __device__ __forceinline__ void keep(elem* table, int e, uint32_t meta, int) {
+        table[e] = __builtin_bit_cast(_Float16, (uint16_t)meta);
         table[kI4Table + e] = (elem)(-1024.0f - zero_of(meta));
     }
     // weights of rows 2 p and 2 p + 1: 1024 + code
@@ -582,25 +600,24 @@ struct BackRows<DK_FP16> {
         return __builtin_bit_cast(uint32_t, w * half2_t{scale[2 * p], scale[2 * p + 1]});
     }
 };
-template <>
-struct BackRows<DK_BF16> {
+template <int DT>
+struct BackRows<DT, true> {
     typedef float elem;
     float8_t scale, zero;  // -(1024 + zero) scale
     static __device__ __forceinline__ void keep(elem* table, int e, uint32_t meta, int scale_dtype) {
-        const float s = scale_of(meta, scale_dtype);
+        const float s = scale_of(meta, DT == DK_FP16 ? DK_BF16 : scale_dtype);
         table[e] = s;
         table[kI4Table + e] = (-1024.0f - zero_of(meta)) * s;
     }
     __device__ __forceinline__ uint32_t pair(uint32_t v, int p) const {
         const half2_t h = __builtin_bit_cast(half2_t, v);
-        const float2_t f = float2_t{__builtin_fmaf((float)h[0], scale[2 * p], zero[2 * p]),
-                                    __builtin_fmaf((float)h[1], scale[2 * p + 1], zero[2 * p + 1])};
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
+        return narrow<DT>(__builtin_fmaf((float)h[0], scale[2 * p], zero[2 * p]),
+                          __builtin_fmaf((float)h[1], scale[2 * p + 1], zero[2 * p + 1]));
     }
 };
 
-template <int DT, int C>
-constexpr int kI4BackVector = (C == 8 ? (DT == DK_BF16 ? 80 : 72) : (DT == DK_BF16 ? 48 : 40)) / (2 * C);
+template <bool WIDE, int C>
+constexpr int kI4BackVector = (C == 8 ? (WIDE ? 80 : 72) : (WIDE ? 48 : 40)) / (2 * C);
 
 // Order of a part's instructions: V vector ones behind each of M matrix ones, a load every L of them. Issued at once, the
 // loads of eight waves and the arithmetic of their addresses hold up the matrix instructions behind them: 4096 tokens of
@@ -617,18 +634,18 @@ __device__ __forceinline__ void interleave() {
 }
 
 constexpr int kI4BackWBytes = kI4Step * 128;  // 64 rows of 256 columns
-template <int DT, int C>
+template <int DT, bool WIDE, int C>
 constexpr int int4_back_stage() {
-    return I4Tokens<C>::BYTES + kI4BackWBytes + 2 * kI4Table * (int)sizeof(typename BackRows<DT>::elem);
+    return I4Tokens<C>::BYTES + kI4BackWBytes + 2 * kI4Table * (int)sizeof(typename BackRows<DT, WIDE>::elem);
 }
 
-template <int DT, int C>
+template <int DT, bool WIDE, int C>
 __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4Args a) {
     typedef typename I4<DT>::vec vec;
-    typedef typename BackRows<DT>::elem meta_t;
+    typedef typename BackRows<DT, WIDE>::elem meta_t;
     // a wave: F times 16 tokens by J times 16 columns
     constexpr int WM = kI4Across<C>, F = 2 * C / WM, J = 2 * WM;
-    constexpr int XB = I4Tokens<C>::BYTES, STAGE = int4_back_stage<DT, C>();
+    constexpr int XB = I4Tokens<C>::BYTES, STAGE = int4_back_stage<DT, WIDE, C>();
     extern __shared__ __attribute__((aligned(32))) uint8_t smem[];
     uint32_t* const raw = (uint32_t*)(smem + kI4Ring * STAGE);  // four steps' words of the groups
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -684,7 +701,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
     constexpr int H = F / 2;
     vec xv[2][H], wv[2][J];
     uint32_t d[8];
-    BackRows<DT> rows;
+    BackRows<DT, WIDE> rows;
     const uint32_t x_off[2] = {held((wm + r) * 128 + 16 * (q ^ chunk_key(r))), held((wm + r) * 128 + 16 * ((4 + q) ^ chunk_key(r)))};
     // (row 8 q + i lies at 8 q + i ^ bit 4 of it, which is bit 1 of q)
     const uint32_t w_off = XB + 8 * q * 128 + 16 * (chunk ^ ((q & 1) << 2)) + 4 * word, swap = 128 * ((q >> 1) & 1);
@@ -731,7 +748,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
             }
     };
     const auto keep = [&](int h) {  // (a wave's own words)
-        BackRows<DT>::keep(table(h), kI4Unit * wave + lane, raw[(h & 3) * kI4Entries + threadIdx.x], a.scale_dtype);
+        BackRows<DT, WIDE>::keep(table(h), kI4Unit * wave + lane, raw[(h & 3) * kI4Entries + threadIdx.x], a.scale_dtype);
     };
     constexpr int GROUP = I4Tokens<C>::LOADS + 2;
     fetch_meta(0);
@@ -757,7 +774,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
         read_x(at, 2);
         multiply(1);
         unpack(1);
-        interleave<2 * C, kI4BackVector<DT, C>>();
+        interleave<2 * C, kI4BackVector<WIDE, C>>();
         __builtin_amdgcn_sched_barrier(0);
         read_x(at, 3);
         multiply(2);
@@ -772,7 +789,7 @@ __global__ __launch_bounds__(64 * kI4Waves, 2) void int4_back_kernel(const Int4A
         fetch_meta(h + 4);
         x.fetch(stage_of(h + 3));
         fetch_w(stage_of(h + 3));
-        interleave<2 * C, kI4BackVector<DT, C>, (2 * C > GROUP ? 2 * C / GROUP : 1)>();
+        interleave<2 * C, kI4BackVector<WIDE, C>, (2 * C > GROUP ? 2 * C / GROUP : 1)>();
         __builtin_amdgcn_sched_barrier(0);
     }
     wait_vmcnt<0>();
@@ -970,44 +987,44 @@ static hipError_t launch_few(const Int4Args& a, const Int4Plan& p, hipStream_t s
     return launch_ahead<DT, GJ, NW, 4>(a, p, s);
 }
 
-template <int DT, int C, int GJ>
+template <int DT, bool WIDE, int C, int GJ>
 static hipError_t launch_tile(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
     constexpr size_t lds = int4_tile_lds<C, GJ>();
-    if (hipError_t e = allow_dynamic_lds((const void*)int4_tile_kernel<DT, C, GJ>, lds)) return e;
-    hipLaunchKernelGGL((int4_tile_kernel<DT, C, GJ>), dim3(p.m_tiles * p.n_tiles * p.splits), dim3(64 * kI4Waves), lds, s, a);
+    if (hipError_t e = allow_dynamic_lds((const void*)int4_tile_kernel<DT, WIDE, C, GJ>, lds)) return e;
+    hipLaunchKernelGGL((int4_tile_kernel<DT, WIDE, C, GJ>), dim3(p.m_tiles * p.n_tiles * p.splits), dim3(64 * kI4Waves), lds, s, a);
     return hipGetLastError();
 }
 
-template <int DT, int GJ>
+template <int DT, bool WIDE, int GJ>
 static hipError_t launch_forward(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
     if (p.few) {
         if (p.waves == 16) return launch_few<DT, GJ, 16>(a, p, s);
         if (p.waves == 8) return launch_few<DT, GJ, 8>(a, p, s);
         return launch_few<DT, GJ, 4>(a, p, s);
     }
-    if (p.tokens == 256) return launch_tile<DT, 8, GJ>(a, p, s);
-    if (p.tokens == 128) return launch_tile<DT, 4, GJ>(a, p, s);
-    return launch_tile<DT, 2, GJ>(a, p, s);
+    if (p.tokens == 256) return launch_tile<DT, WIDE, 8, GJ>(a, p, s);
+    if (p.tokens == 128) return launch_tile<DT, WIDE, 4, GJ>(a, p, s);
+    return launch_tile<DT, WIDE, 2, GJ>(a, p, s);
 }
 
-template <int DT, int C>
+template <int DT, bool WIDE, int C>
 static hipError_t launch_back(const Int4Args& a, const Int4Plan& p, hipStream_t s) {
-    constexpr size_t lds = kI4Ring * int4_back_stage<DT, C>() + 4 * kI4Entries * sizeof(uint32_t);
-    if (hipError_t e = allow_dynamic_lds((const void*)int4_back_kernel<DT, C>, lds)) return e;
-    hipLaunchKernelGGL((int4_back_kernel<DT, C>), dim3(p.m_tiles * p.n_tiles * p.splits), dim3(64 * kI4Waves), lds, s, a);
+    constexpr size_t lds = kI4Ring * int4_back_stage<DT, WIDE, C>() + 4 * kI4Entries * sizeof(uint32_t);
+    if (hipError_t e = allow_dynamic_lds((const void*)int4_back_kernel<DT, WIDE, C>, lds)) return e;
+    hipLaunchKernelGGL((int4_back_kernel<DT, WIDE, C>), dim3(p.m_tiles * p.n_tiles * p.splits), dim3(64 * kI4Waves), lds, s, a);
     return hipGetLastError();
 }
 
-template <int DT>
+template <int DT, bool WIDE>
 static hipError_t launch_typed(const Int4Args& a, const Int4Plan& p, bool backward, hipStream_t s) {
     if (backward) {
-        if (p.tokens == 64) return launch_back<DT, 2>(a, p, s);
-        if (p.tokens == 128) return launch_back<DT, 4>(a, p, s);
-        return launch_back<DT, 8>(a, p, s);
+        if (p.tokens == 64) return launch_back<DT, WIDE, 2>(a, p, s);
+        if (p.tokens == 128) return launch_back<DT, WIDE, 4>(a, p, s);
+        return launch_back<DT, WIDE, 8>(a, p, s);
     }
-    if (a.group_units % 4 == 0) return launch_forward<DT, 4>(a, p, s);
-    if (a.group_units % 2 == 0) return launch_forward<DT, 2>(a, p, s);
-    return launch_forward<DT, 1>(a, p, s);
+    if (a.group_units % 4 == 0) return launch_forward<DT, WIDE, 4>(a, p, s);
+    if (a.group_units % 2 == 0) return launch_forward<DT, WIDE, 2>(a, p, s);
+    return launch_forward<DT, WIDE, 1>(a, p, s);
 }
 
 hipError_t launch_int4(Int4Args a, const Int4Plan& p, int dtype, bool backward, hipStream_t s) {
@@ -1031,7 +1048,9 @@ hipError_t launch_int4(Int4Args a, const Int4Plan& p, int dtype, bool backward, 
         a.ldx = ld;
         if (hipError_t e = hipGetLastError()) return e;
     }
-    hipError_t e = dtype == DK_FP16 ? launch_typed<DK_FP16>(a, p, backward, s) : launch_typed<DK_BF16>(a, p, backward, s);
+    hipError_t e = dtype == DK_BF16            ? launch_typed<DK_BF16, true>(a, p, backward, s)
+                   : a.scale_dtype == DK_FP16 ? launch_typed<DK_FP16, false>(a, p, backward, s)
+                                              : launch_typed<DK_FP16, true>(a, p, backward, s);
     if (e != hipSuccess || p.splits == 1) return e;
     hipLaunchKernelGGL(int4_join_kernel, dim3((cols + 1023) / 1024, a.m < 4096 ? a.m : 4096), dim3(256), 0, s, a, cols);
     return hipGetLastError();
