@@ -591,9 +591,8 @@ int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const 
     if (x == nullptr || packed == nullptr || meta == nullptr) return dk_fail("dk_int4_linear: null pointer");
     if (!aligned_to(packed, 16) || !aligned_to(meta, 4))
         return dk_fail("dk_int4_linear: packed must be 16-byte aligned, meta 4-byte aligned");
-    // (256 rows of x lie within a buffer of 2^31 bytes)
-    if (m > 1 && (ldx < 0 || ldx >= (int64_t(1) << 22)))
-        return dk_fail("dk_int4_linear: x's row stride must be non-negative and below 2^22");
+    if (m > 1 && (ldx < 0 || ldx >= (sum < kInt4LongRow ? 1 : 2) * kInt4LongRow))
+        return dk_fail("dk_int4_linear: x's row stride must be non-negative and below 2^22 (2^23 where a row has 2^22 elements)");
     if (!copy && (sum % 8 != 0 || !aligned_to(x, 16) || (m > 1 && ldx % 8 != 0)))
         return dk_fail("dk_int4_linear: without copy x needs 16-byte aligned rows of a multiple of 8 columns");
     const Int4Plan p = int4_plan(m, n, k, backward != 0);

@@ -355,6 +355,9 @@ hipError_t launch_scaled_rope(ScaledRopeArgs a, int dtype, hipStream_t s);
 // Products with weights of 4-bit integers (int4_linear.hip).
 constexpr int kInt4FewM = 32, kInt4FewSmallM = 64;  // forward launches of so few tokens stream the weight to registers
 constexpr int kInt4FewLds = 155648;  // and keep at most so many bytes of the tokens in LDS
+// Rows of x this long, which only a backward has, go by tiles of 64 tokens: the rows of a tile, up to twice as far apart, lie in a
+// buffer of less than 2^31 bytes, behind which masked loads point (off_if). Up to here 256 do.
+constexpr int64_t kInt4LongRow = int64_t(1) << 22;
 struct Int4Args {
     const void* x;       // [m, k], backward dy [m, n]: 16-byte aligned rows, or `padded` set
     const uint8_t* w;      // tiles of 16 rows by 128 columns [ceil(n / 16), kblocks, 1024]

@@ -928,14 +928,15 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
     // forward 29 us (tiles of 64 tokens 33, of 256 45), backward 42 in six splits of 128 (10 of 256: 47, 6 of 64: 48).
     // (Tuning hook, read on every call: DECIK_INT4_PLAN = "tokens,splits" forces a plan.)
     const int64_t cols = backward ? k : n, steps = backward ? (n + kI4Block - 1) / kI4Block : blocks;
+    const int most = (backward ? n : k) < kInt4LongRow ? 256 : 64;
     p.n_tiles = (int)((cols + kI4TileN - 1) / kI4TileN);
     int forced_tokens = 0, forced_splits = 0;
     if (const char* v = std::getenv("DECIK_INT4_PLAN"))
         if (std::sscanf(v, "%d,%d", &forced_tokens, &forced_splits) != 2 || forced_splits < 1 || forced_splits > steps ||
-            (forced_tokens != 256 && forced_tokens != 128 && forced_tokens != 64))
+            (forced_tokens != 256 && forced_tokens != 128 && forced_tokens != 64) || forced_tokens > most)
             forced_tokens = 0;
     double best = 0.0;
-    for (int tokens = 256; tokens >= 64; tokens /= 2) {
+    for (int tokens = most; tokens >= 64; tokens /= 2) {
         if (forced_tokens != 0 && tokens != forced_tokens) continue;
         const int64_t m_tiles = (m + tokens - 1) / tokens, tiles = m_tiles * p.n_tiles;
         for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {

@@ -430,10 +430,10 @@ int dk_scaled_rope_bwd(const dk_scaled_rope* d, void* stream);
  * x of x_dtype fp16 or bf16, y of it or fp32; the bias NULL or of bias_dtype. Forward of up to 32 tokens (64 where
  * n k <= 2^24): exact integers times x, group sums in fp32 times the scale, one rounding. More tokens, and backward: W
  * rounded once to x_dtype (fp16 keeps it in steps of 2^-24 at least and up to 65504), sums in fp32. Scales are finite.
- * Sums go in an order that depends on the sizes alone. x's row stride: non-negative, below 2^22. `copy` = 1: x has rows
- * that do not start at multiples of 16 bytes, or a number of columns that is no multiple of 8; where more than those few
- * tokens come it is then copied to the workspace first. workspace: dk_int4_linear_workspace(..) bytes (0: none). y overlaps
- * no input. 0 <= m, n < 2^23, m n < 2^37, m k < 2^37, 1 <= k <= 2^20. */
+ * Sums go in an order that depends on the sizes alone. x's row stride: non-negative, below 2^22 (2^23 backward where
+ * n >= 2^22). `copy` = 1: x has rows that do not start at multiples of 16 bytes, or a number of columns that is no
+ * multiple of 8; where more than those few tokens come it is then copied to the workspace first. workspace:
+ * dk_int4_linear_workspace(..) bytes (0: none). y overlaps no input. 0 <= m, n < 2^23, m n < 2^37, m k < 2^37, 1 <= k <= 2^20. */
 int64_t dk_int4_linear_workspace(int backward, int copy, int64_t m, int64_t n, int64_t k);
 int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, const uint32_t* meta,
                    int64_t group, int scale_dtype, const void* bias, int bias_dtype, void* y,
