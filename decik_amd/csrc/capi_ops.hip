@@ -468,6 +468,8 @@ int dk_residual_norm_bwd(const dk_residual_norm* d, void* workspace, int64_t wor
     if (int rc = residual_norm_common(d, &a)) return rc;
     if (int rc = residual_norm_sums(d, &a)) return rc;
     if (a.rows == 0 && a.nslabs == 0) return 0;
+    // (the join of the sums reads a channel's gate, without rows too)
+    if (a.gate_kind == DK_GATE_CHANNEL && a.gate == nullptr) return dk_fail("dk_residual_norm_bwd: null gate");
     if (a.rows > 0) {
         if (d->dx == nullptr) return dk_fail("dk_residual_norm_bwd: null pointer");
         if ((d->weight != nullptr) != (d->grad_y != nullptr))
