@@ -121,7 +121,7 @@ def quantize_int4(w, group=128, symmetric=False, scale_dtype=None):
     n, k = w.shape
     groups = -(-k // group)
     width = min(group, k)  # (one group where it is longer than a row)
-    v = torch.zeros((n, groups * width), device=w.device)
+    v = torch.zeros((n, groups * width), dtype=torch.float32, device=w.device)
     v[:, :k] = w
     v = v.view(n, groups, width)
     if symmetric:
