@@ -16,10 +16,11 @@
 // and the tile's 16 rows.
 // From pairs to operands: 0x6400 | q is 1024 + q as fp16, 0x6400 | 16 q is 1024 + 16 q. fp16: one packed subtraction or
 // multiply-add leaves q - zero, exactly, one packed product the weight. bf16, and fp16 with bf16 scales (rounded to fp16 before
-// the product, a scale below 2^-17 would be off by up to fifteen half steps in a weight, one past 65504 no number): mixed multiply-adds
-// give (1024 + q) scale - (1024 + zero) scale in fp32, and one conversion a pair rounds: a scale has 11 bits at most, so both
-// products are exact and the difference is scale (q - zero) without any error (with 1 for the scale, q - zero). us, fp16 with fp16
-// and with bf16 scales: 4096 tokens of [18944] x 3584 forward 460 and 480, backward 485 and 530.
+// the product, a scale below 2^-17 would be off by up to fifteen half steps in a weight, one past 65504 no number): mixed
+// multiply-adds give (1024 + q) scale - (1024 + zero) scale in fp32, and one conversion a pair rounds: a scale has 11 bits at
+// most and is below 2^117, so both products are exact and the difference is scale (q - zero) without any error (with 1 for the
+// scale, q - zero). us, fp16 with fp16 and with bf16 scales: 4096 tokens of [18944] x 3584 forward 460 and 480, backward 485
+// and 530.
 #include <cstdio>
 #include <cstdlib>
 

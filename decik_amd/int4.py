@@ -71,8 +71,8 @@ _SHIFTS = (0, 16, 4, 20, 8, 24, 12, 28)
 
 
 def int4_weight(codes, scales, zeros=None, group=128):
-    """Int4Weight of codes [N, K] (uint8, 0 to 15), scales [N, ceil(K / group)] (fp16 or bf16) and zero points of the
-    same shape (uint8, 0 to 16; None: 8). group: a multiple of 32. On any device; the layout is made once."""
+    """Int4Weight of codes [N, K] (uint8, 0 to 15), scales [N, ceil(K / group)] (fp16 or bf16, below 2^117) and zero points of
+    the same shape (uint8, 0 to 16; None: 8). group: a multiple of 32. On any device; the layout is made once."""
     what = "int4_weight"
     group = int(group)
     if group < 32 or group % 32 or group > 2 ** 20:
@@ -90,6 +90,8 @@ def int4_weight(codes, scales, zeros=None, group=128):
             raise ValueError(f"{what}: codes, scales and zeros must be on one device")
     if n and (int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 16)):
         raise ValueError(f"{what}: codes must be 0 to 15, zeros 0 to 16")
+    if n and not float(scales.detach().abs().max()) < 2.0 ** 117:
+        raise ValueError(f"{what}: scales must be numbers below 2^117")
     tiles, blocks = -(-n // ROWS), -(-k // BLOCK)
     cols = torch.zeros((tiles * ROWS, blocks * BLOCK), dtype=torch.uint8, device=codes.device)
     cols[:n, :k] = codes

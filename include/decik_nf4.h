@@ -429,7 +429,7 @@ int dk_scaled_rope_bwd(const dk_scaled_rope* d, void* stream);
  * fp16 or bf16) and, from bit 16, the zero point, 0 to 16. Rows from n on: zeros in both; columns from k on: any code.
  * x of x_dtype fp16 or bf16, y of it or fp32; the bias NULL or of bias_dtype. Forward of up to 32 tokens (64 where
  * n k <= 2^24): exact integers times x, group sums in fp32 times the scale, one rounding. More tokens, and backward: W
- * rounded once to x_dtype (fp16 keeps it in steps of 2^-24 at least and up to 65504), sums in fp32. Scales are finite.
+ * rounded once to x_dtype (fp16 keeps it in steps of 2^-24 at least and up to 65504), sums in fp32. Scales: below 2^117.
  * Sums go in an order that depends on the sizes alone. x's row stride: non-negative, below 2^22 (2^23 backward where
  * n >= 2^22). `copy` = 1: x has rows that do not start at multiples of 16 bytes, or a number of columns that is no
  * multiple of 8; where more than those few tokens come it is then copied to the workspace first. workspace:
