@@ -119,7 +119,13 @@ def residual_norm_backward(grad_h, grad_y, x, residual, weight, post_weight=None
     """(dx, dresidual, dweight, dpost_weight, dgate) of residual_norm_forward from the gradients of h (None: zeros) and
     y (None only without a weight) and the same inputs; None for an input that was None. dweight, dpost_weight and
     the gradient of a channel gate are fp32 [W]; without param_grads these three are None."""
-    what = "residual_norm_backward"
+    return _backward("residual_norm_backward", grad_h, grad_y, x, residual, weight, post_weight, gate, residual_scale, eps,
+                     (param_grads, param_grads, param_grads), True)
+
+
+def _backward(what, grad_h, grad_y, x, residual, weight, post_weight, gate, residual_scale, eps, sums_of, gate_grad):
+    """residual_norm_backward with the sums over the rows that are asked for (weight, post weight, channel gate) and, where
+    asked for, the gradient of another gate."""
     dev, x2, r2, x_at, r_at, ldx, ldr, w, pw, g, xc, sc, yc, width = _inputs(
         what, x, residual, weight, post_weight, gate, None if grad_y is None else grad_y.dtype)
     same_gpu(what, dev, grad_h, grad_y)
@@ -138,9 +144,9 @@ def residual_norm_backward(grad_h, grad_y, x, residual, weight, post_weight=None
     packed, rows, kind = x.is_contiguous(), x.numel() // width, g[3]
     dx = _like(x, packed, x.dtype)
     dres = None if residual is None else _like(x, packed, h_dtype)
-    dgate = None if kind in (_NONE, _CHANNEL) else x.new_empty(gate.shape, dtype=gate.dtype)
+    dgate = x.new_empty(gate.shape, dtype=gate.dtype) if kind in (_TOKEN, _ELEMENT) and gate_grad else None
     # the gradients that are sums over the rows: weight, post weight, channel gate
-    wanted = (weight is not None, post_weight is not None, kind == _CHANNEL) if param_grads else (False,) * 3
+    wanted = [asked and there for asked, there in zip(sums_of, (weight is not None, post_weight is not None, kind == _CHANNEL))]
     count = sum(wanted)
     work, need, dw, dpw = None, 0, None, None
     if count:
@@ -181,9 +187,8 @@ class _ResidualNorm(torch.autograd.Function):
             if weight is not None:
                 # nothing reached y: the norm before the next block drops out
                 grads_w, weight = torch.zeros_like(weight), None
-        params = any(ctx.needs_input_grad[i] for i in (2, 3)) or (ctx.needs_input_grad[4] and gate is not None)
-        dx, dres, dw, dpw, dgate = residual_norm_backward(grad_h, grad_y, x, residual, weight, post_weight, gate, ctx.scale,
-                                                          ctx.eps, params)
+        dx, dres, dw, dpw, dgate = _backward("residual_norm", grad_h, grad_y, x, residual, weight, post_weight, gate, ctx.scale,
+                                             ctx.eps, ctx.needs_input_grad[2:5], ctx.needs_input_grad[4])
         if grad_y is None:
             dw = grads_w
         elif dw is not None:
