@@ -4,8 +4,9 @@
 //   forward: (a c - b s, b c + a s)        back: (a c + b s, b c - a s)
 // in fp32, one rounding at the end. Token-major in and head-major out, or, back, the other way round.
 //
-// Angles are kept in turns as 64-bit fixed-point fractions (turn_fraction), so that whole turns drop out exactly: at
-// position 2^20 within 2^-33 radians, where an fp32 product of position and frequency would be off by 2^-5.
+// Angles are formed in turns as 64-bit fixed-point fractions (turn_fraction), so that whole turns drop out exactly, and reach
+// sincospif as fp32 half turns: within 2^-24 turns at positions below 2^28, where an fp32 product of position and frequency
+// is off by 2^-5 radians at 2^20 already.
 // A work-group takes a few tokens, forms each of their R / 2 cosines and sines once, in LDS, and turns all heads with
 // them; a thread has one or two items in flight. An item is 16 elements, two 16-byte loads (halves with R and D
 // multiples of 16: both elements of eight pairs), or eight: with pairs whole, with halves of any even R and their
