@@ -161,8 +161,10 @@ __device__ __forceinline__ void store_out(const Int4Args& a, int64_t at, float v
 
 // ---- forward, few tokens -------------------------------------------------------------------------
 // Bound: the weight's bytes and the latency of a launch's phases. [18944] x 3584 from memory, fp16: 1 token 10.9 us (34 MB and
-// 1.2 MB of groups' words, 3.3 TB/s; the first kernel 19), 16 tokens 14.9, 32 tokens 22; [3584] x 18944 at 16 tokens, bf16,
-// 17.5 and 3.9 for the join of two splits (first 31): there the unpacking, 32 vector instructions an MFMA, weighs as much.
+// 1.2 MB of groups' words, 3.3 TB/s; the first kernel 19), 16 tokens 14.9, 32 tokens 22. [3584] x 18944: 1 to 4 tokens
+// 11.6 (bf16 13.8: its unpacking, 32 vector instructions an MFMA); 8, 12 and 16 tokens in two, three and four splits 14.7 (16.7)
+// all three, as each of some 224 work-groups has 150 KB of tokens to bring to LDS before its first product, and 3.9 for the join,
+// a launch and two round trips (first 31 in all).
 // Tokens by 16 (blockIdx.z). The NW waves of a work-group are NW / a.shares tiles of 16 rows by a.shares shares of the split's
 // columns, whose sums meet in LDS; each streams its share of the weight to registers, P blocks ahead. The tokens' columns
 // of the split are kept in LDS: from the caches with each block they cost the address unit four loads for the
@@ -292,9 +294,9 @@ __global__ __launch_bounds__(64 * NW) void int4_few_kernel(const Int4Args a) {
 
 // ---- tiles ---------------------------------------------------------------------------------------
 // Bound: the matrix cores' and vector units' cycles and the loads' issue between them. 4096 tokens of [18944] x 3584, bf16:
-// forward 475 to 510 us (1.1 to 1.17 PFLOP/s, matrix cores busy 51% of all cycles; the first kernel 1479), backward 540 to
+// forward 470 to 510 us (1.1 to 1.18 PFLOP/s, matrix cores busy 51% of all cycles; the first kernel 1479), backward 540 to
 // 595 (1.0 PFLOP/s, 42%; first 1364), where a library product of the same sizes with a 16-bit weight takes 537 to 547. 830
-// tokens of [8960] x 1536, fp16: forward 28 to 34 us (245 work-groups of 12 blocks; such a library product 29), backward 41
+// tokens of [8960] x 1536, fp16: forward 27 to 31 us (245 work-groups of 12 blocks; such a library product 29), backward 40
 // with the join of six splits (45), 40 + 7 from memory. Waves of 64 by 64 in the smaller tiles, as in the largest, unpack
 // each weight twice: 34 and 43.5 us.
 // Tiles of 32 C tokens by 256 rows of the weight (forward) or 256 columns (backward), eight waves: with 256 tokens of 128 by
@@ -888,7 +890,8 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
     Int4Plan p{};
     const int64_t blocks = (k + kI4Block - 1) / kI4Block;
     // Tokens by 16 with the weight streamed to registers for each: up to 32, up to 64 on weights whose tiles are mostly start
-    // and end. us, streamed and by the best tiles, fp16 / bf16: [18944] x 3584 at 32 tokens 19.8 and 20.7 / 26.1 and 21.2,
+    // and end. For both types, although tiles would take bf16 less time past 16 tokens of large weights: streamed, no weight is
+    // rounded. us, streamed and by the best tiles, fp16 / bf16: [18944] x 3584 at 32 tokens 19.8 and 20.7 / 26.1 and 21.2,
     // [3584] x 18944 18.6 and 22.1 / 23.1 and 22.4; at 64 [4096] x 4096 9.6 and 16.7 / 11.5 and 17.1, [8960] x 1536 12.2 and
     // 15.3 / 15.2 and 15.5, [5120] x 5120, past the bound, 18.3 and 18.7 / 22.8 and 19.5.
     const bool small = n * ((k + 7) / 8 * 8) <= (int64_t(1) << 24);
@@ -924,8 +927,9 @@ Int4Plan int4_plan(int64_t m, int64_t n, int64_t k, bool backward) {
     // Tokens a tile (256, 128 or 64) and splits of the sum: the least estimate of the time. A round of the CUs takes the times
     // below for a block of 128 terms and for its start and end (tiles of 64 tokens run two work-groups a CU, one alone
     // takes less), a split's partial sums go to memory and back, their join takes a launch. Fitted to 1300 timed plans of 70
-    // products (fp16, 64 to 4096 tokens, weights from [512] x 3584 to [18944] x 3584): estimates are off by 6%, the chosen
-    // plan by 0.4% of the best one's time at the mean and 5% at most. Measured against the choice: [830, 8960] x 1536
+    // products (fp16, 64 to 4096 tokens, weights from [512] x 3584 to [18944] x 3584), launches included: estimates are off by 10%
+    // forward and 8% backward at the mean, 44% at most ([830, 8960] x 1536 forward 22 us for 29), mostly too low; the
+    // chosen plan is off the best one's time by 0.4% at the mean and 5% at most. Measured against the choice: [830, 8960] x 1536
     // forward 29 us (tiles of 64 tokens 33, of 256 45), backward 42 in six splits of 128 (10 of 256: 47, 6 of 64: 48).
     // (Tuning hook, read on every call: DECIK_INT4_PLAN = "tokens,splits" forces a plan.)
     const int64_t cols = backward ? k : n, steps = backward ? (n + kI4Block - 1) / kI4Block : blocks;

@@ -5,7 +5,8 @@ columns of a row, about a quarter of fp16's bytes; zero points are 8 where none 
   W[n, k] = (code[n, k] - zero[n, k // group]) * scale[n, k // group]
   forward:  y = x . W^T + bias. Up to 32 tokens (64 on weights of up to 2^24) stream the weight to registers: the integers times
             x exactly, each group's sum in fp32 times its scale, rounded once. More go by tiles, with W rounded once to x's
-            type (at most half a step of it a weight; fp16 keeps W in steps of 2^-24 at least) and sums in fp32
+            type (at most half a step of it a weight; fp16 keeps W in steps of 2^-24 at least) and sums in fp32; where W is
+            not to be rounded, call it on up to 32 tokens at a time
   backward: dX = dY . W by tiles, W rounded once to dY's type, sums in fp32
 quantize_int4 makes such a weight from values, int4_weight from codes, scales and zero points that a checkpoint holds;
 both lay the codes out once for the kernels (Int4Weight). Sums are added in an order that depends on the sizes alone.

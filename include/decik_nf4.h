@@ -441,7 +441,8 @@ int dk_int4_linear(int backward, const void* x, int x_dtype, int64_t ldx, const 
                    int64_t workspace_bytes, void* stream);
 /* Diagnostic, host-only: out[0] = tokens a tile, out[1] = waves of a work-group that streams the weight to registers (0:
  * tiles of 256 rows or columns), out[2] = those that share a row's columns, out[3] = splits of the sum. Returns 0, or
- * nonzero on bad sizes. DECIK_INT4_PLAN = "tokens,splits" (64, 128 or 256 tokens; read on every call) forces the tiles'. */
+ * nonzero on bad sizes. DECIK_INT4_PLAN = "tokens,splits" (64, 128 or 256 tokens, only 64 where a row of
+ * dy has 2^22 elements; read on every call) forces the tiles'. */
 int dk_int4_linear_plan(int backward, int64_t m, int64_t n, int64_t k, int32_t* out);
 
 /* ---- the residual stream between two blocks, no counterpart in the reference --------------- */

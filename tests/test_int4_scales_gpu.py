@@ -69,6 +69,21 @@ def test_few_tokens_round_no_weight(m, dtype, scale_dtype, device):
 
 
 @pytest.mark.gpu
+def test_pieces_of_few_tokens_round_no_weight(device):
+    """What a caller does with more tokens where W is not to be rounded."""
+    from decik_amd.int4 import int4_linear_forward, launch_plan
+
+    n, k, m = 4200, 4100, 100
+    weight, w = weight_of(n, k, 128, spread(n, k, 128, F16, -24, 11.9, 1), 1, device)
+    cols = torch.arange(m) * 41 % k
+    x = ones_at(cols, k, F16, device)
+    assert launch_plan(False, 32, n, k)["waves"] and not launch_plan(False, m, n, k)["waves"]
+    exact = w[:, cols].t().float()
+    assert torch.equal(torch.cat([int4_linear_forward(p, weight, None, F32) for p in x.split(32)]), exact)
+    assert torch.equal(int4_linear_forward(x, weight, None, F32), w[:, cols].t().half().float())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [40, 300])
 def test_zero_weights_under_scales_past_fp16(m, device):
     """Codes that are their zero points stand for 0 under any scale: what a scale of 1 gives."""

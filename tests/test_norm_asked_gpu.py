@@ -9,16 +9,16 @@ from test_norm_gpu import EPS, F16, F32, gate_of, make
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("gate", ["none", "channel", "token", "element"])
-@pytest.mark.parametrize("asked", [(0,), (1,), (2,), (3,), (4,), (0, 1), (2, 4), (0, 3), (0, 1, 2, 3, 4)])
-def test_only_what_is_asked_for(gate, asked, device, monkeypatch):
+ASKED = [(0,), (1,), (2,), (3,), (4,), (0, 1), (2, 4), (0, 3), (0, 1, 2, 3, 4)]
+
+
+@pytest.mark.parametrize("asked,gate", [(a, g) for a in ASKED for g in ("none", "channel", "token", "element") if (a, g) != ((4,), "none")])
+def test_only_what_is_asked_for(asked, gate, device, monkeypatch):
     from decik_amd import _lib, norm
 
     b, t, width = 2, 19, 320
     inputs = [make((b, t, width), F16, device, 1), make((b, t, width), F32, device, 2), make((width,), F32, device, 3),
               make((width,), F32, device, 4), gate_of(gate, (b, t, width), F32, device)]
-    if gate == "none" and asked == (4,):
-        pytest.skip("nothing is asked for")
     leaves = [v.clone().requires_grad_() if i in asked and v is not None else v for i, v in enumerate(inputs)]
     h, y = norm.residual_norm(*leaves, 0.5, EPS)
     gh, gy = make(h.shape, F32, device, 5), make(y.shape, F16, device, 6)
